@@ -30,7 +30,7 @@ import torch
 
 from . import ops
 from .feed import PackedSignal
-from .lib import GPU_CAPTURE_LOCK, AdamWCfg
+from .lib import AdamWCfg, capture_section
 from .ops import (NS_GEMM_ATOMIC32, NS_GEMM_COLSUM_A, NS_GEMM_DROP_A, NS_GEMM_GELU, NS_GEMM_GELU_SAVE_GRAD, NS_GEMM_MUL_P16, NS_GEMM_TN,
                   rowmap)
 
@@ -1292,7 +1292,7 @@ class MegWhisperEngine:
         def cut_here(lo, hi):
             end((lo, hi))
             begin()
-        with GPU_CAPTURE_LOCK:      # no other thread of this package touches the GPU API while the capture is open
+        with capture_section():     # no other thread of this package touches the GPU API, no graph is garbage-collected while the capture is open
             begin()
             try:
                 self.zero_grad()

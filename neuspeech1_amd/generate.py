@@ -22,7 +22,7 @@ import numpy as np
 import torch
 
 from . import ops
-from .lib import GPU_CAPTURE_LOCK
+from .lib import capture_section
 from .ops import rowmap
 
 F16, F32 = torch.float16, torch.float32
@@ -360,7 +360,9 @@ class Generator:
                     for _ in range(2):
                         if as_list:
                             gs, gt = ops.LaunchList(), ops.LaunchList()
-                            gs.keep = gt.keep = ws       # the session's tensors are what the recorded raw addresses point into
+                            # the session's tensors are what the recorded raw addresses point into (not the session itself: it holds this
+                            # list, and a cycle would leave its captured graphs to the cyclic collector: see lib.capture_section)
+                            gs.keep = gt.keep = (ws["t"], ws["sb"])
                             with ops.recording(gs):
                                 select(cur, ctr)
                             with ops.recording(gt):
@@ -369,7 +371,7 @@ class Generator:
                             gs, gt = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
                             # thread-local capture mode + the package's capture lock: other host threads (the data feed's
                             # loader thread synchronizes, allocates and copies on its own stream) must not invalidate this
-                            with GPU_CAPTURE_LOCK:
+                            with capture_section():
                                 with torch.cuda.graph(gs, capture_error_mode="thread_local"):
                                     select(cur, ctr)
                                 with torch.cuda.graph(gt, capture_error_mode="thread_local"):

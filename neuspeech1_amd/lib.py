@@ -21,8 +21,26 @@ class NeuSpeechHipError(RuntimeError):
 # package around its GPU API calls (the data feed's loader thread: device synchronize, pinned / device allocations, copies).
 # HIP invalidates an open capture when another thread synchronizes the device or allocates meanwhile, thread-local capture
 # mode notwithstanding (seen on ROCm 7.0/7.2: hipErrorStreamCaptureInvalidated at the first captured launch).
+import contextlib  # noqa: E402
+import gc  # noqa: E402
 import threading  # noqa: E402
 GPU_CAPTURE_LOCK = threading.RLock()
+
+
+@contextlib.contextmanager
+def capture_section():
+    """Everything between begin and end of a hipGraph capture runs inside this: GPU_CAPTURE_LOCK held, Python's cyclic collector off.
+    torch's ~CUDAGraph synchronizes the device on ROCm, which fails while this thread captures; the check throws inside a destructor and
+    ends the process.  A graph that only a reference cycle kept alive is destroyed whenever the collector happens to run -- the Python
+    allocations of a capture are enough to start it -- so collection waits until the capture is closed."""
+    with GPU_CAPTURE_LOCK:
+        was = gc.isenabled()
+        gc.disable()
+        try:
+            yield
+        finally:
+            if was:
+                gc.enable()
 
 ABI_VERSION = 3      # ns_version() of the library this binding was written against (3: ns_zero_spans / ns_add_i32)
 

@@ -518,3 +518,22 @@ def test_token_ids_exact_at_273_channels_and_large_v2_width(dev, tag, name, nb, 
                    make_rescore(dims, torch.from_numpy(x), 4, **kw))
     else:
         check_greedy_up_to_fp16_ties(out, g[name], g[name + "_margin"], 4, dims.pad_id)
+
+
+def test_no_garbage_collection_runs_while_a_decode_graph_is_captured(setup, monkeypatch):
+    """a CUDAGraph that only a reference cycle keeps alive is destroyed when the cyclic collector runs, and torch's destructor
+    synchronizes the device: inside an open capture that ends the process (neuspeech1_amd.lib.capture_section)"""
+    import gc
+    from neuspeech1_amd import ops
+    from neuspeech1_amd.generate import Generator
+    g, dims, gen, x, prompt = setup
+    real, seen = ops.add_i32, []
+
+    def add_i32(*a, **k):
+        if torch.cuda.is_current_stream_capturing():
+            seen.append(gc.isenabled())
+        return real(*a, **k)
+    monkeypatch.setattr(ops, "add_i32", add_i32)
+    g2 = Generator(gen.eng, use_graph=True, graph_min_steps=0)
+    g2.generate(x, prompt, num_beams=1, max_new_tokens=20, suppress_tokens=(dims.eos_id,))
+    assert g2.last_loop_mode == "graphs" and seen and not any(seen) and gc.isenabled()
