@@ -335,6 +335,83 @@ int ns_cross_entropy(const void* logits16, const int64_t* labels, int rows, int 
 int ns_argmax_rows(const void* logits16, int rows, int V, int ldv, int64_t* out, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Training losses over the vocabulary beside ns_cross_entropy.  Element types:
+ * ---------------------------------------------------------------------- */
+typedef enum { NS_F16 = 0, NS_BF16 = 1, NS_F32 = 2 } ns_dtype;
+
+/* The LM head AND its loss (utils/load_model.py:1047-1054: proj_out, then
+ * CrossEntropyLoss) without the (rows, vocab) logits, and the gradients of both:
+ *     z = h w^T,  loss = mean over valid rows of
+ *         (1 - alpha) (lse(z) - z[label]) + alpha T^2 KL(softmax(top / T) || softmax(z / T))
+ * h (rows, d), w (vocab, d), dh, dw of `dtype` (NS_F16 / NS_BF16), row strides in
+ * elements, multiples of 8; tensors start on 16 bytes; d a multiple of 8.
+ *  - labels int64; a label outside [0, vocab) (-100) drops the row from both terms:
+ *    row_loss 0, dh 0, whatever h holds there.
+ *  - k = 0 (or alpha = 0): hard labels alone.  k > 0: the teacher's list per row,
+ *    top_vals (rows, ld_top) fp32 logits and top_idx int32 tokens; a token outside
+ *    [0, vocab) is no entry, entries that name a token twice add up, the softmax is
+ *    over the entries there are, and a row without one (or with -inf alone) keeps
+ *    the hard term only.
+ *  - row_loss fp32 (rows), *loss_dev, *nvalid_dev (rows with a label).
+ *  - dh (or NULL) and dw (or NULL): gradients of loss_scale x loss; loss_scale_dev
+ *    may be NULL (1).  dw_f32: dw is fp32; dw_add (fp32 only): added to what is there.
+ *  - workspace: ns_linear_ce_workspace_bytes(d) bytes (host-only call: sizes, k,
+ *    alpha, temperature, ldw and whether dh / dw are set decide), 16-B aligned,
+ *    free again when the call's work has run; it holds at most 256 MiB of dz at a
+ *    time (one piece of the vocabulary) plus fp32 partial sums of dh.
+ *  - the same inputs give the same bits (no atomics).  dh, dw must not overlap h, w. */
+typedef struct {
+  const void *h, *w;
+  const int64_t* labels;
+  const float* top_vals;
+  const int32_t* top_idx;
+  float *row_loss, *loss_dev;
+  int* nvalid_dev;
+  const float* loss_scale_dev;
+  void *dh, *dw;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t ldh, ldw, lddh, lddw, ld_top;
+  int32_t rows, vocab, d, k, dtype, dw_f32, dw_add;
+  float temperature, alpha;
+} ns_linear_ce_desc;
+int ns_linear_cross_entropy(const ns_linear_ce_desc* d, void* stream);
+size_t ns_linear_ce_workspace_bytes(const ns_linear_ce_desc* d);   /* 0: sizes that the call refuses */
+
+/* Distillation from a teacher's top logits over logits that exist (rows, ldz) of
+ * `dtype` (any ns_dtype): the loss of ns_linear_cross_entropy at z = logits, and
+ * dlogits (or NULL; may be the logits themselves).  Rows may start at any element;
+ * columns [vocab, ldz) are neither read nor written.  labels NULL (alpha = 1 only):
+ * every row counts. */
+typedef struct {
+  const void* logits;
+  const int64_t* labels;
+  const float* top_vals;
+  const int32_t* top_idx;
+  float *row_loss, *loss_dev;
+  int* nvalid_dev;
+  const float* loss_scale_dev;
+  void* dlogits;
+  int64_t ldz, lddz, ld_top;
+  int32_t rows, vocab, k, dtype;
+  float temperature, alpha;
+} ns_distill_desc;
+int ns_distill_topk(const ns_distill_desc* d, void* stream);
+
+/* The teacher's side: the k largest logits of each row, largest first, equal ones
+ * by the lowest token; vals fp32, idx int32 (rows, ldo), lse (or NULL): the row's
+ * log-sum-exp (fp32).  A NaN ranks above +inf. */
+typedef struct {
+  const void* logits;
+  float* vals;
+  int32_t* idx;
+  float* lse;
+  int64_t ldz, ldo;
+  int32_t rows, vocab, k, dtype;
+} ns_topk_desc;
+int ns_topk_logits(const ns_topk_desc* d, void* stream);
+
+/* ------------------------------------------------------------------------
  * Optimizer tail of one training step on the flat fp32 trainable buffer
  * (HF Trainer defaults configured at finetune.py:231-253): grad-norm + inf
  * check -> [skip if inf] unscale, clip to max_grad_norm, AdamW, LR schedule,

@@ -1,0 +1,889 @@
+// ns_linear_cross_entropy: the LM head and its loss in one call, without the (rows, vocabulary) logits.
+//
+//   z = h W^T                                       h (N, d) hidden states, W (V, d) the head
+//   CE_i = lse(z_i) - z_i[label_i]
+//   KL_i = sum_k p_ik (log p_ik - (z_i[idx_ik] / T - lse(z_i / T))),      p_i = softmax of the teacher's top logits / T
+//   loss = mean over the rows with a label of (1 - alpha) CE_i + alpha T^2 KL_i
+//   dz_i = g [ w1 softmax(z_i) + w2 softmax(z_i / T) - w1 onehot(label_i) - w2 sum_k p_ik onehot(idx_ik) ],   w1 = 1 - alpha, w2 = alpha T
+//   dh = dz W,  dW = dz^T h,                        g = loss_scale / rows with a label
+//
+// The logits pass twice through the registers of a 256 x 256 tile and are never stored: a first pass keeps the running maximum and sum of
+// every row (fp32, one pair per row and 256 columns, joined by ll_rows_kernel), a second one forms dz of one PIECE of the vocabulary, rounds
+// it to the operands' type and leaves it in a workspace of at most LL_PIECE_BYTES (it stays in the 256-MiB last-level cache), from where the two products
+// dh += dz W and dW = dz^T h take it.  4 products instead of 3 (the logits are formed again) against 4 N V bytes written and read three times.
+//   * Rows without a label are packed away first: they cost nothing, and an infinity or NaN in a masked row reaches neither loss nor gradient.
+//   * A row's sparse terms (its label, the teacher's list) are no part of the dense epilogue: their logits are gathered as dot products in fp32
+//     and their cells of dz are written afterwards from those.
+//   * dz in the operands' type: fp16 cells carry a factor 2^s (exact; taken out in fp32 at the end), so that a probability of 1 / V does
+//     not fall among the subnormals; a probability below 2^-29 of full scale is a subnormal, below 2^-40 zero.  bf16 has the range of fp32.
+//     The label's cell is rounded once, after the subtraction.
+//   * Sums over the vocabulary (dh) and over the rows (dW) stay in fp32 MFMA accumulators / fp32 slabs added in a fixed order: no atomics,
+//     the same bits every time.
+// The 256 x 256 main loop is ns_gemm_p8.hip's four-phase LDS-DMA ring (see there: two wave groups one barrier interval apart), here for both
+// 16-bit types and with a second operand that may be K-major (W for dh, dz for dW): such a region holds 64 k-rows of 256 B and its fragments are
+// read transposed by ds_read_b64_tr_b16.
+#include "ns_common.h"
+
+namespace {
+
+constexpr int BM = 256, BN = 256, BK = 64, NTH = 512;
+constexpr int REGION = 128 * 128;            // 16 KiB
+constexpr int BUF = 4 * REGION;              // 64 KiB
+constexpr int RA0 = 0, RA1 = 1, RB0 = 2, RB1 = 3;
+constexpr int LDH = BN * 2 + 16;             // epilogue: bytes per staged 16-bit row
+constexpr int LL_LDS = BM * LDH > 2 * BUF ? BM * LDH : 2 * BUF;
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr size_t LL_PIECE_BYTES = 256u << 20;
+constexpr int LL_MAX_K = 256;
+constexpr uint32_t OUT = 0x80000000u;        // a buffer offset past every resource: the hardware returns zeros
+
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef unsigned short ushort4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v lds_s4;
+
+struct tf16 {
+  typedef half_t e;
+  typedef half8 v8;
+  static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+struct tbf16 {
+  typedef __bf16 e;
+  typedef bf8 v8;
+  static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <class E> __device__ __forceinline__ ushort4v cvt4(float a, float b, float c, float d) {
+  typedef E e4 __attribute__((ext_vector_type(4)));
+  const e4 r = {(E)a, (E)b, (E)c, (E)d};
+  return __builtin_bit_cast(ushort4v, r);
+}
+
+// A DMA piece in asm: behind the builtin hipcc waits for every piece in flight (vmcnt(0)) before a transposed LDS read, which it takes to alias
+// them; the ring's own counted waits order the two.  The instruction has no register result.
+__device__ __forceinline__ void ll_dma16(ns_u4v rsrc, uint32_t voff, int soff, uint32_t lds_dst) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(voff), "s"(rsrc), "s"(soff), "s"(lds_dst) : "memory");
+}
+__device__ __forceinline__ ns_u4v ll_rsrc(const void* base) {
+  const uint64_t a = (uint64_t)base;
+  return ns_u4v{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)), OUT, 0x00020000u};
+}
+
+#define LL_BARRIER()                            \
+  do {                                          \
+    asm volatile("" ::: "memory");              \
+    __builtin_amdgcn_s_barrier();               \
+    asm volatile("" ::: "memory");              \
+  } while (0)
+
+// One 256 x 256 tile, C = A B over `K`: A rows are K-contiguous; B is K-contiguous (BT = false: rows n) or K-major (BT = true: rows k).
+// a_base / b_base: first element of the tile's operand (row m0 / row n0, or column n0 of k-row 0); ld in elements, extents from there < 2 GiB.
+// kA / kB: valid k of each operand (chunks / k-rows past them are zeros); b_rows: valid rows n (BT = false) or columns n (BT = true), a multiple of 8 when BT.
+// SWAP = false: a lane owns 4 consecutive n of row m = l15 (acc[..][reg]); SWAP = true: 4 consecutive m of column n = l15.
+template <class T, bool BT, bool SWAP>
+__device__ __forceinline__ void ll_tile(f32x4 (&acc)[2][4][2][2], char* smem, const void* a_base, int lda, int kA,
+                                        const void* b_base, int ldb, int kB, int b_rows, int K) {
+  typedef typename T::v8 v8;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  const int l15 = lane & 15, lg = lane >> 4;
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[a][i][b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // DMA sources: wave w fills region bytes [2048 w, 2048 w + 2048) as two 1-KiB pieces.  K-contiguous: 8 rows x 128 B, chunk c of region row r
+  // holds source chunk c ^ ((r >> 1) & 7).  K-major: 4 k-rows x 256 B, the 32-B windows of k-row r are permuted by g(r) = (r & 3) | ((r >> 3) & 1) << 2:
+  // the eight row segments that half a wave reads transposed (four k-rows of two 16-lane groups, 8 k-rows apart) lie in eight different windows.
+  uint32_t a_off[2][2], b_off[2][2];
+  int a_k[2], b_k[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int rr = 16 * wave + 8 * j + (lane >> 3);
+    const int ch = (lane & 7) ^ ((rr >> 1) & 7);
+    a_k[j] = ch * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int arow = ((rr >> 6) << 7) + h * 64 + (rr & 63);
+      a_off[h][j] = (uint32_t)(arow * lda + ch * 8) * 2u;
+      if (!BT) {
+        const int brow = ((rr >> 5) << 6) + h * 32 + (rr & 31);
+        b_off[h][j] = brow < b_rows ? (uint32_t)(brow * ldb + ch * 8) * 2u : OUT;
+      }
+    }
+    b_k[j] = ch * 8;
+    if (BT) {
+      const int kr = 8 * wave + 4 * j + (lane >> 4);
+      const int g = (kr & 3) | (((kr >> 3) & 1) << 2);
+      const int col = ((lane & 15) ^ (g << 1)) * 8;        // region column 0 .. 127
+      b_k[j] = kr;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int n = ((col >> 5) << 6) + h * 32 + (col & 31);
+        b_off[h][j] = n < b_rows ? (uint32_t)(kr * ldb + n) * 2u : OUT;
+      }
+    }
+  }
+  const ns_u4v rsrc_a = ll_rsrc(a_base), rsrc_b = ll_rsrc(b_base);
+  const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)smem;
+  auto stage = [&](int tt, int region, int buf) __attribute__((always_inline)) {
+    const int k0 = tt * BK, h = region & 1;
+    const bool isb = region >= 2;
+    const int klen = (isb ? kB : kA) - k0;
+    const int soff = isb ? (BT ? k0 * ldb * 2 : k0 * 2) : k0 * 2;
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_base + buf * BUF + region * REGION + wave * 2048);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const bool ok = (isb ? b_k[j] : a_k[j]) < klen;
+      const uint32_t off = isb ? b_off[h][j] : a_off[h][j];
+      // (a tile past the end asks for nothing: offset and scalar offset must not wrap around together)
+      ll_dma16(isb ? rsrc_b : rsrc_a, ok ? off : OUT, klen > 0 ? soff : 0, dst + j * 1024);
+    }
+  };
+  const int fsw = ((lg ^ (l15 >> 1)) & 7) << 4;
+  const int a_rd = (wm * 64 + l15) * 128 + fsw;
+  const int q = l15 >> 2, pp = l15 & 3;
+  const int b_rd = BT ? (8 * lg + q) * 256 + (((wn * 2) ^ (q | ((lg & 1) << 2))) << 5) + pp * 8 : (wn * 32 + l15) * 128 + fsw;
+
+  v8 af[4][2], bq[2][2][2];
+  auto read_a = [&](int buf, int ah) __attribute__((always_inline)) {
+    const char* st = smem + buf * BUF + (ah ? RA1 : RA0) * REGION;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) af[mt][ks] = *(const v8*)(st + ((a_rd ^ (ks << 6)) + mt * 2048));
+  };
+  auto read_b = [&](int buf, int bh) __attribute__((always_inline)) {
+    const char* st = smem + buf * BUF + (bh ? RB1 : RB0) * REGION;
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (!BT) {
+          bq[bh][nt][ks] = *(const v8*)(st + ((b_rd ^ (ks << 6)) + nt * 2048));
+        } else {
+          const char* const at = st + ((b_rd ^ (nt << 5)) + ks * 8192);
+          const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at);
+          const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 1024));
+          const short8v r = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          bq[bh][nt][ks] = __builtin_bit_cast(v8, r);
+        }
+      }
+  };
+  auto mma = [&](int ah, int bh) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+          acc[ah][mt][bh][nt] = SWAP ? T::mma(af[mt][ks], bq[bh][nt][ks], acc[ah][mt][bh][nt]) : T::mma(bq[bh][nt][ks], af[mt][ks], acc[ah][mt][bh][nt]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+#define LL_RUN(AH, BH)                                      \
+  do {                                                      \
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");        \
+    LL_BARRIER();                                           \
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      \
+    __builtin_amdgcn_sched_barrier(0);                      \
+    mma(AH, BH);                                            \
+    __builtin_amdgcn_sched_barrier(0);                      \
+    LL_BARRIER();                                           \
+  } while (0)
+  auto tile = [&](int t, int b) __attribute__((always_inline)) {
+    read_b(b, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    read_a(b, 0);
+    stage(t + 1, RB1, b ^ 1);
+    LL_RUN(0, 0);
+    read_b(b, 1);
+    stage(t + 1, RA1, b ^ 1);
+    LL_RUN(0, 1);
+    read_a(b, 1);
+    stage(t + 2, RA0, b);
+    LL_RUN(1, 1);
+    stage(t + 2, RB0, b);
+    LL_RUN(1, 0);
+  };
+  const int nsteps = (K + BK - 1) / BK;
+  stage(0, RA0, 0); stage(0, RB0, 0); stage(0, RB1, 0); stage(0, RA1, 0);
+  stage(1, RA0, 1); stage(1, RB0, 1);
+  asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  LL_BARRIER();
+  if (wm == 1) LL_BARRIER();        // group 1 runs one barrier interval behind group 0
+  for (int t = 0; t < nsteps; t += 2) {
+    tile(t, 0);
+    tile(t + 1, 1);
+  }
+  if (wm == 0) LL_BARRIER();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last zero chunks must not land on what the epilogue stages
+  LL_BARRIER();
+#undef LL_RUN
+}
+
+// linear tile index of this workgroup: XCD x (= block % 8) owns a contiguous run of the `total` live tiles; -1: no tile
+__device__ __forceinline__ int ll_pos(int total) {
+  const int bid = blockIdx.x;
+  if (bid >= total) return -1;
+  const int q = total >> 3, r = total & 7, xcd = bid & 7, idx = bid >> 3;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+}
+
+// ------------------------------------------------------------------------------------------------ rows with a label, in order
+// order[i] = i-th row with a label, inv[row] = its place or -1, *nvalid; ignored rows get their zero loss here
+__global__ __launch_bounds__(1024) void ll_compact_kernel(const int64_t* __restrict__ labels, int rows, int V, int* __restrict__ order,
+                                                          int* __restrict__ inv, int* __restrict__ lab, float* __restrict__ row_loss, int* __restrict__ nvalid) {
+  __shared__ int sh[17];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int base = 0;
+  for (int r0 = 0; r0 < rows; r0 += 1024) {
+    const int row = r0 + tid;
+    const int64_t l = row < rows ? labels[row] : -1;
+    const bool ok = l >= 0 && l < V;
+    const uint64_t m = __ballot(ok);
+    if (lane == 0) sh[wave] = __popcll(m);
+    __syncthreads();
+    int before = base, all = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) before += sh[w];
+      all += sh[w];
+    }
+    const int at = before + __popcll(m & ((1ull << lane) - 1ull));
+    if (row < rows) {
+      inv[row] = ok ? at : -1;
+      if (ok) { order[at] = row; lab[at] = (int)l; }
+      else row_loss[row] = 0.f;
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (tid == 0) *nvalid = base;
+}
+
+// hp[i] = h[order[i]], columns [d, dp) and rows [nvalid, next multiple of 256) zero; zk[i][e] = h_i . W[token e], e = 0 .. k - 1 the teacher's
+// list, e = k the label.  One wave per row; products in fp32, added over the lanes' partial sums.
+template <class T>
+__global__ __launch_bounds__(256) void ll_pack_kernel(const void* __restrict__ h_, int64_t ldh, const void* __restrict__ w_, int64_t ldw, int d, int dp, int V,
+                                                      const int* __restrict__ order, const int* __restrict__ lab, const int32_t* __restrict__ top_idx,
+                                                      int64_t ld_top, int k, const int* __restrict__ nvalid, void* __restrict__ hp_, float* __restrict__ zk) {
+  typedef typename T::v8 v8;
+  typedef typename T::e E;
+  const int lane = threadIdx.x & 63, i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int nv = *nvalid;
+  if (i >= (nv + BM - 1) / BM * BM) return;
+  E* const dst = (E*)hp_ + (int64_t)i * dp;
+  if (i >= nv) {
+    for (int c = lane * 8; c < dp; c += 512) *(uint4*)(dst + c) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int row = order[i];
+  const E* const src = (const E*)h_ + row * ldh;
+  for (int c = lane * 8; c < dp; c += 512) *(uint4*)(dst + c) = c < d ? *(const uint4*)(src + c) : make_uint4(0, 0, 0, 0);
+  for (int e = 0; e <= k; ++e) {
+    const int tok = e == k ? lab[i] : top_idx[row * ld_top + e];
+    float s = 0.f;
+    if (tok >= 0 && tok < V) {
+      const E* const wr = (const E*)w_ + tok * ldw;
+      for (int c = lane * 8; c < d; c += 512) {
+        const v8 a = *(const v8*)(src + c), b = *(const v8*)(wr + c);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) s += (float)a[x] * (float)b[x];
+      }
+    }
+    s = ns_wave_sum(s);
+    if (lane == 0) zk[(int64_t)i * (k + 1) + e] = s;
+  }
+}
+
+// hT[c][i] = hp[i][c], 64 x 64 tiles through LDS
+__global__ __launch_bounds__(256) void ll_transpose_kernel(const uint16_t* __restrict__ hp, int dp, const int* __restrict__ nvalid, uint16_t* __restrict__ hT, int ldt) {
+  __shared__ uint16_t t[64][66];
+  const int i0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  if (i0 >= (*nvalid + 63) / 64 * 64) return;
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  for (int r = y; r < 64; r += 4) t[r][x] = hp[(int64_t)(i0 + r) * dp + c0 + x];
+  __syncthreads();
+  for (int r = y; r < 64; r += 4) hT[(int64_t)(c0 + r) * ldt + i0 + x] = t[x][r];
+}
+
+// ------------------------------------------------------------------------------------------------ the logits' tiles
+struct LogitsArgs {
+  const void* hp; const void* w; int64_t ldw;
+  int dp, d, V, col0, tiles_n, R;        // R: packed rows the buffers are laid out for (a multiple of 256)
+  const int* nvalid;
+  float c1, c2;                          // log2(e) / temperature of the softmaxes
+  float *pm, *p1, *p2;                   // (tiles_n, R): maximum, sum of exp2((z - max) c1), the same with c2
+  const float *La, *Lb;                  // (R): base-2 log-sum-exp minus log2 of the weight and of 2^s
+  void* G; int ldg;
+  const int* lab; const float* zk;       // FIX: the label's cell of dz is put right in the staged tile
+  float wlab;                            // w1 2^s
+};
+
+template <class T, bool GRAD, bool DUAL, bool FIX>
+__global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  typedef typename T::e E;
+  const int nv = *p.nvalid;
+  const int tiles_m = (nv + BM - 1) / BM;
+  const int pos = ll_pos(tiles_m * p.tiles_n);
+  if (pos < 0) return;
+  // eight row tiles by the columns: the 32 workgroups of an XCD that run together read 8 + 4 operand tiles instead of 1 + 32
+  constexpr int GM = 8;
+  const int grp = pos / (GM * p.tiles_n), rem = pos - grp * GM * p.tiles_n;
+  const int gm = min(GM, tiles_m - grp * GM);
+  const int tm = grp * GM + rem % gm, tn = rem / gm;
+  const int m0 = tm * BM, n0 = p.col0 + tn * BN;
+  f32x4 acc[2][4][2][2];
+  ll_tile<T, false, false>(acc, smem, (const E*)p.hp + (int64_t)m0 * p.dp, p.dp, p.dp, (const E*)p.w + (int64_t)n0 * p.ldw, (int)p.ldw, p.d,
+                           min(BN, p.V - n0), p.d);
+  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  const bool edge = n0 + BN > p.V;
+  if (!GRAD) {
+    // a lane holds 16 of the wave's 64 columns of 8 rows; the row's other lanes are 16 and 32 apart, its other columns in the waves of equal wm
+    float* const sm = (float*)smem;
+#pragma unroll
+    for (int ah = 0; ah < 2; ++ah)
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        float z[16];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float v = acc[ah][mt][b >> 1][b & 1][r];
+            if (edge && n0 + wn * 64 + b * 16 + 4 * lg + r >= p.V) v = -INFINITY;
+            z[b * 4 + r] = v;
+            mx = fmaxf(mx, v);
+          }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float ms = mx == -INFINITY ? 0.f : mx;     // a strip past the vocabulary: sums of zeros
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          s1 += __builtin_amdgcn_exp2f((z[x] - ms) * p.c1);
+          if (DUAL) s2 += __builtin_amdgcn_exp2f((z[x] - ms) * p.c2);
+        }
+        s1 += __shfl_xor(s1, 16, 64);
+        s1 += __shfl_xor(s1, 32, 64);
+        if (DUAL) { s2 += __shfl_xor(s2, 16, 64); s2 += __shfl_xor(s2, 32, 64); }
+        if (lg == 0) {
+          const int row = wm * 128 + ah * 64 + mt * 16 + l15;
+          sm[wn * 256 + row] = mx;
+          sm[1024 + wn * 256 + row] = s1;
+          if (DUAL) sm[2048 + wn * 256 + row] = s2;
+        }
+      }
+    __syncthreads();
+    if (tid < 256) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, sm[w * 256 + tid]);
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float dm = sm[w * 256 + tid] - mx;
+        s1 += sm[1024 + w * 256 + tid] * __builtin_amdgcn_exp2f(dm * p.c1);
+        if (DUAL) s2 += sm[2048 + w * 256 + tid] * __builtin_amdgcn_exp2f(dm * p.c2);
+      }
+      const int64_t o = (int64_t)tn * p.R + m0 + tid;
+      p.pm[o] = mx;
+      p.p1[o] = s1;
+      if (DUAL) p.p2[o] = s2;
+    }
+    return;
+  }
+  // ---- dz of this tile: exponentials in place, one rounding, staged as rows of 256 columns, stored 512 B a row
+#pragma unroll
+  for (int ah = 0; ah < 2; ++ah)
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const int rl = wm * 128 + ah * 64 + mt * 16 + l15;
+      const float la = p.La[m0 + rl], lb = DUAL ? p.Lb[m0 + rl] : 0.f;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const f32x4 a = acc[ah][mt][b >> 1][b & 1];
+        const int cl = wn * 64 + b * 16 + 4 * lg;
+        float g[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          g[r] = __builtin_amdgcn_exp2f(a[r] * p.c1 - la);
+          if (DUAL) g[r] += __builtin_amdgcn_exp2f(a[r] * p.c2 - lb);
+          if (edge && n0 + cl + r >= p.V) g[r] = 0.f;
+        }
+        *(ushort4v*)(smem + rl * LDH + cl * 2) = cvt4<E>(g[0], g[1], g[2], g[3]);
+      }
+    }
+  __syncthreads();
+  if (FIX) {
+    if (tid < 256) {
+      const int i = m0 + tid;
+      const int c = i < nv ? p.lab[i] - n0 : -1;
+      if (c >= 0 && c < BN) *(E*)(smem + tid * LDH + c * 2) = (E)(__builtin_amdgcn_exp2f(p.zk[i] * p.c1 - p.La[i]) - p.wlab);
+    }
+    __syncthreads();
+  }
+  char* const G = (char*)p.G + ((int64_t)m0 * p.ldg + tn * BN) * 2;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int rl = (tid >> 5) + 16 * i, cg = tid & 31;
+    *(uint4*)(G + (int64_t)rl * p.ldg * 2 + cg * 16) = *(const uint4*)(smem + rl * LDH + cg * 16);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ rows: log-sum-exp, losses, weights
+struct RowArgs {
+  const float *pm, *p1, *p2;
+  int tiles_n, R, k, V;
+  float c1, c2, invT, w1, w2, lw1, lw2, kd;     // lw*: log2(w* 2^s), -inf for a zero weight; kd: alpha T^2
+  int dual, soft_only;                          // one softmax: p1 is at temperature T when only soft targets count
+  const int* nvalid; const int* order;
+  const float* zk; const float* top_vals; const int32_t* top_idx; int64_t ld_top;
+  float *La, *Lb, *pk, *row_loss, *packed_loss;
+};
+
+// 16 rows per workgroup, 16 threads per row
+__global__ __launch_bounds__(256) void ll_rows_kernel(const RowArgs p) {
+  __shared__ float sm[3][16][17];
+  const int nv = *p.nvalid, i0 = blockIdx.x * 16;
+  if (i0 >= (nv + BM - 1) / BM * BM) return;
+  {
+    const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
+    float mx = -INFINITY, s1 = 0.f, s2 = 0.f;
+    for (int t = q; t < p.tiles_n; t += 16) {
+      const int64_t o = (int64_t)t * p.R + i0 + r;
+      const float m = p.pm[o];
+      const float nm = fmaxf(mx, m);
+      const float f = __builtin_amdgcn_exp2f((mx - nm) * p.c1), g = __builtin_amdgcn_exp2f((m - nm) * p.c1);
+      s1 = s1 * (mx == -INFINITY ? 0.f : f) + p.p1[o] * g;
+      if (p.dual) s2 = s2 * (mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mx - nm) * p.c2)) + p.p2[o] * __builtin_amdgcn_exp2f((m - nm) * p.c2);
+      mx = nm;
+    }
+    sm[0][r][q] = mx; sm[1][r][q] = s1; sm[2][r][q] = s2;
+  }
+  __syncthreads();
+  const int r = threadIdx.x >> 4, q = threadIdx.x & 15, i = i0 + r;
+  float mx = sm[0][r][q];
+  const float own = mx;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+  float s1 = own == -INFINITY ? 0.f : sm[1][r][q] * __builtin_amdgcn_exp2f((own - mx) * p.c1);
+  float s2 = own == -INFINITY ? 0.f : sm[2][r][q] * __builtin_amdgcn_exp2f((own - mx) * p.c2);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
+  const bool live = i < nv;
+  if (!live) {                      // padding rows of the last tile: no probability
+    if (q == 0) { p.La[i] = INFINITY; if (p.Lb) p.Lb[i] = INFINITY; }
+    return;
+  }
+  const int row = p.order[i];
+  float loss = 0.f;
+  bool soft = false;
+  if (p.k > 0) {
+    // the teacher's distribution over the entries that name a token; a list without any leaves the hard label alone
+    const float* const tv = p.top_vals + row * p.ld_top;
+    const int32_t* const ti = p.top_idx + row * p.ld_top;
+    float tm = -INFINITY;
+    for (int e = q; e < p.k; e += 16) if (ti[e] >= 0 && ti[e] < p.V) tm = fmaxf(tm, tv[e] * p.invT);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor(tm, o, 64));
+    soft = tm > -INFINITY;
+    float ts = 0.f;
+    for (int e = q; e < p.k; e += 16) if (soft && ti[e] >= 0 && ti[e] < p.V) ts += expf(tv[e] * p.invT - tm);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) ts += __shfl_xor(ts, o, 64);
+    const float lt = logf(ts), inv = 1.f / ts;
+    const float lq = mx * p.invT + logf(p.dual ? s2 : s1);      // lse(z / T)  (one softmax: it is the one at T)
+    float kl = 0.f;
+    for (int e = q; e < p.k; e += 16) {
+      float pr = 0.f;
+      if (soft && ti[e] >= 0 && ti[e] < p.V) {
+        const float lp = tv[e] * p.invT - tm;
+        pr = expf(lp) * inv;
+        if (pr > 0.f) kl += pr * ((lp - lt) - (p.zk[(int64_t)i * (p.k + 1) + e] * p.invT - lq));
+      }
+      p.pk[(int64_t)i * p.k + e] = pr;
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) kl += __shfl_xor(kl, o, 64);
+    if (soft) loss += p.kd * kl;
+  }
+  if (q == 0) {
+    if (!p.soft_only) loss += p.w1 * ((mx - p.zk[(int64_t)i * (p.k + 1) + p.k]) + logf(s1));
+    const float l1 = mx * p.c1 + log2f(s1);
+    if (p.dual) {
+      p.La[i] = l1 - p.lw1;
+      p.Lb[i] = soft ? mx * p.c2 + log2f(s2) - p.lw2 : INFINITY;
+    } else if (p.k > 0) {
+      // one softmax carries both weights (T = 1), or the soft weight alone
+      const float w = (p.soft_only ? 0.f : p.w1) + (soft ? p.w2 : 0.f);
+      p.La[i] = w > 0.f ? l1 - (p.lw1 + log2f(w)) : INFINITY;      // (lw1 is log2(2^s) here)
+    } else {
+      p.La[i] = l1 - p.lw1;
+    }
+    p.row_loss[row] = loss;
+    p.packed_loss[i] = loss;
+  }
+}
+
+__global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__ packed_loss, const int* __restrict__ nvalid, float* __restrict__ loss) {
+  __shared__ float sh[16];
+  const int nv = *nvalid;
+  float s = 0.f;
+  for (int i = threadIdx.x; i < nv; i += 1024) s += packed_loss[i];
+  s = ns_wave_sum(s);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.f;
+    for (int w = 0; w < 16; ++w) s += sh[w];
+    *loss = s / (float)max(nv, 1);
+  }
+}
+
+// the sparse cells of dz in one piece: one wave per row, each token written once whatever number of entries name it
+template <class E>
+__global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ nvalid, const int* __restrict__ order, const int* __restrict__ lab,
+                                                       const int32_t* __restrict__ top_idx, int64_t ld_top, int k, const float* __restrict__ zk,
+                                                       const float* __restrict__ pk, const float* __restrict__ La, const float* __restrict__ Lb, float c1, float c2,
+                                                       float w1s, float w2s, int col0, int cols, int V, E* __restrict__ G, int ldg) {
+  __shared__ int sidx[4][LL_MAX_K + 1];
+  __shared__ float sp[4][LL_MAX_K];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = blockIdx.x * 4 + wave;
+  const int nv = *nvalid;
+  const bool live = i < nv;
+  if (live) {
+    const int row = order[i];
+    for (int e = lane; e <= k; e += 64) {
+      const int t = e == k ? lab[i] : top_idx[row * ld_top + e];
+      sidx[wave][e] = t >= 0 && t < V ? t : -1;
+      if (e < k) sp[wave][e] = pk[(int64_t)i * k + e];
+    }
+  }
+  __syncthreads();
+  if (!live) return;
+  const float la = La[i], lb = Lb ? Lb[i] : INFINITY;
+  for (int e = lane; e <= k; e += 64) {
+    const int t = sidx[wave][e], c = t - col0;
+    if (t < 0 || c < 0 || c >= cols) continue;
+    float soft = 0.f;
+    bool first = true;
+    for (int o = 0; o < k; ++o)
+      if (sidx[wave][o] == t) { soft += sp[wave][o]; first = first && o >= e; }
+    if (!first) continue;                                   // an earlier entry of the list names the same token: that one writes
+    const float z = zk[(int64_t)i * (k + 1) + e];
+    float v = __builtin_amdgcn_exp2f(z * c1 - la);
+    if (Lb) v += __builtin_amdgcn_exp2f(z * c2 - lb);
+    v -= w2s * soft;
+    if (t == lab[i]) v -= w1s;
+    G[(int64_t)i * ldg + c] = (E)v;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ dh += dz W,  dW = dz^T h
+struct DhArgs {
+  const void* G; const void* w; int64_t ldw;
+  int ldg, col0, cols, V, d, R, splits, chunk, add;
+  const int* nvalid;
+  float* slab;                      // (splits, R, d)
+};
+
+template <class T>
+__global__ __launch_bounds__(NTH) void ll_dh_kernel(const DhArgs p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  typedef typename T::e E;
+  const int tiles_m = (*p.nvalid + BM - 1) / BM, tiles_d = (p.d + BN - 1) / BN;
+  const int tiles = tiles_m * tiles_d;
+  const int pos = ll_pos(tiles * p.splits);
+  if (pos < 0) return;
+  const int split = pos / tiles, t = pos - split * tiles;
+  const int tm = t / tiles_d, td = t - tm * tiles_d;
+  const int m0 = tm * BM, n0 = td * BN;
+  const int k0 = split * p.chunk, kn = min(p.chunk, p.cols - k0);          // (a split past the end leaves its zeros)
+  f32x4 acc[2][4][2][2];
+  ll_tile<T, true, false>(acc, smem, (const E*)p.G + (int64_t)m0 * p.ldg + k0, p.ldg, kn,
+                          (const E*)p.w + (int64_t)(p.col0 + k0) * p.ldw + n0, (int)p.ldw, min(kn, p.V - p.col0 - k0), min(BN, p.d - n0), max(kn, 0));
+  const int lane = threadIdx.x & 63, l15 = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  float* const out = p.slab + ((int64_t)split * p.R + m0) * p.d + n0;
+#pragma unroll
+  for (int ah = 0; ah < 2; ++ah)
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int rl = wm * 128 + ah * 64 + mt * 16 + l15, cl = wn * 64 + b * 16 + 4 * lg;
+        if (n0 + cl >= p.d) continue;
+        f32x4* const at = (f32x4*)(out + (int64_t)rl * p.d + cl);
+        f32x4 v = acc[ah][mt][b >> 1][b & 1];
+        if (p.add) v += *at;
+        *at = v;
+      }
+}
+
+// dh[row] = g 2^-s sum of the slabs, zero for a row without a label
+template <class E>
+__global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict__ slab, int splits, int R, int d, int rows, const int* __restrict__ inv,
+                                                        const int* __restrict__ nvalid, const float* __restrict__ loss_scale, float unscale, E* __restrict__ dh, int64_t lddh) {
+  const int per = d / 8;
+  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int row = (int)(x / per), c = (int)(x - (int64_t)row * per) * 8;
+  if (row >= rows) return;
+  const int i = inv[row];
+  typedef E e8 __attribute__((ext_vector_type(8)));
+  e8 o;
+  if (i < 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (E)0.f;
+  } else {
+    const float gs = (loss_scale ? *loss_scale : 1.f) / (float)max(*nvalid, 1) * unscale;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+    for (int s = 0; s < splits; ++s) {
+      const float* const q = slab + ((int64_t)s * R + i) * d + c;
+      a += *(const f32x4*)q;
+      b += *(const f32x4*)(q + 4);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { o[e] = (E)(a[e] * gs); o[4 + e] = (E)(b[e] * gs); }
+  }
+  *(e8*)(dh + row * lddh + c) = o;
+}
+
+struct DwArgs {
+  const void* hT; int ldt;
+  const void* G; int ldg, col0, tiles_v, V, d;
+  const int* nvalid; const float* loss_scale;
+  float unscale;
+  void* dw; int64_t lddw; int f32, add;
+};
+
+template <class T>
+__global__ __launch_bounds__(NTH) void ll_dw_kernel(const DwArgs p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  typedef typename T::e E;
+  const int tiles_d = (p.d + BM - 1) / BM;
+  const int pos = ll_pos(tiles_d * p.tiles_v);
+  if (pos < 0) return;
+  const int tv = pos / tiles_d, td = pos - tv * tiles_d;
+  const int m0 = td * BM, n0 = tv * BN;                    // columns of h, columns of dz (= rows of W)
+  const int nv = *p.nvalid, K = (nv + BK - 1) / BK * BK;
+  f32x4 acc[2][4][2][2];
+  ll_tile<T, true, true>(acc, smem, (const E*)p.hT + (int64_t)m0 * p.ldt, p.ldt, K, (const E*)p.G + n0, p.ldg, K, BN, K);
+  const float gs = (p.loss_scale ? *p.loss_scale : 1.f) / (float)max(nv, 1) * p.unscale;
+  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  // a lane owns 4 consecutive columns of h (m) of one row of W (n)
+  const int v0 = p.col0 + n0;
+  if (p.f32) {
+    float* const out = (float*)p.dw + (int64_t)v0 * p.lddw + m0;
+#pragma unroll
+    for (int ah = 0; ah < 2; ++ah)
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int cl = wm * 128 + ah * 64 + mt * 16 + 4 * lg, rl = wn * 64 + b * 16 + l15;
+          if (m0 + cl >= p.d || v0 + rl >= p.V) continue;
+          f32x4* const at = (f32x4*)(out + (int64_t)rl * p.lddw + cl);
+          f32x4 v = acc[ah][mt][b >> 1][b & 1] * gs;
+          if (p.add) v += *at;
+          *at = v;
+        }
+    return;
+  }
+  // 16-bit: staged as rows of W, stored (or added to what is there, in fp32) 512 B a row
+#pragma unroll
+  for (int ah = 0; ah < 2; ++ah)
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int cl = wm * 128 + ah * 64 + mt * 16 + 4 * lg, rl = wn * 64 + b * 16 + l15;
+        const f32x4 v = acc[ah][mt][b >> 1][b & 1] * gs;
+        *(ushort4v*)(smem + rl * LDH + cl * 2) = cvt4<E>(v[0], v[1], v[2], v[3]);
+      }
+  __syncthreads();
+  const int cg = tid & 31;
+  if (m0 + cg * 8 >= p.d) return;
+  typedef typename T::v8 v8;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int rl = (tid >> 5) + 16 * i;
+    if (v0 + rl >= p.V) continue;
+    *(v8*)((E*)p.dw + (int64_t)(v0 + rl) * p.lddw + m0 + cg * 8) = *(const v8*)(smem + rl * LDH + cg * 16);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+struct Plan {
+  int R, dp, dt, tiles_n, piece_tiles, pieces, splits, chunk;
+  size_t order, inv, lab, hp, hT, zk, pk, pm, p1, p2, La, Lb, ploss, G, slab, total;
+};
+
+bool dual_of(const ns_linear_ce_desc* d) { return d->k > 0 && d->alpha > 0.f && d->alpha < 1.f && d->temperature != 1.f; }
+
+Plan plan_of(const ns_linear_ce_desc* d) {
+  Plan p;
+  p.R = (d->rows > 0 ? d->rows + BM - 1 : BM) / BM * BM;
+  p.dp = (d->d + BK - 1) / BK * BK;
+  p.dt = (d->d + BM - 1) / BM * BM;
+  p.tiles_n = (d->vocab + BN - 1) / BN;
+  const bool grad = d->dh || d->dw;
+  // pieces: the 16-bit dz of one piece fits LL_PIECE_BYTES, and a k-range of the head stays addressable with 32-bit byte offsets
+  int64_t most = (int64_t)(LL_PIECE_BYTES / ((size_t)p.R * BN * 2));
+  const int64_t by_ld = ((int64_t)0x7FF00000 / 2 / (d->ldw > d->d ? d->ldw : d->d)) / BN;
+  if (most > by_ld) most = by_ld;
+  if (most < 1) most = 1;
+  p.pieces = (int)((p.tiles_n + most - 1) / most);
+  p.piece_tiles = (p.tiles_n + p.pieces - 1) / p.pieces;
+  p.pieces = (p.tiles_n + p.piece_tiles - 1) / p.piece_tiles;
+  // dh: (row tile, column tile, split of the piece's vocabulary): about one workgroup per CU, splits of 512 tokens at least
+  const int tiles = (p.R / BM) * ((d->d + BN - 1) / BN);
+  p.splits = 256 / tiles;
+  if (p.splits < 1) p.splits = 1;
+  if (p.splits > p.piece_tiles / 2) p.splits = p.piece_tiles / 2 > 0 ? p.piece_tiles / 2 : 1;
+  p.chunk = ((p.piece_tiles * BN + p.splits - 1) / p.splits + BK - 1) / BK * BK;
+  size_t at = 0;
+  auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
+  p.order = take((size_t)d->rows * 4);
+  p.inv = take((size_t)d->rows * 4);
+  p.lab = take((size_t)d->rows * 4);
+  p.hp = take((size_t)p.R * p.dp * 2);
+  p.hT = d->dw ? take((size_t)p.dt * p.R * 2) : 0;
+  p.zk = take((size_t)p.R * (d->k + 1) * 4);
+  p.pk = take((size_t)p.R * d->k * 4);
+  p.pm = take((size_t)p.tiles_n * p.R * 4);
+  p.p1 = take((size_t)p.tiles_n * p.R * 4);
+  p.p2 = dual_of(d) ? take((size_t)p.tiles_n * p.R * 4) : 0;
+  p.La = take((size_t)p.R * 4);
+  p.Lb = take((size_t)p.R * 4);
+  p.ploss = take((size_t)p.R * 4);
+  p.G = grad ? take((size_t)p.R * p.piece_tiles * BN * 2) : 0;
+  p.slab = d->dh ? take((size_t)p.splits * p.R * d->d * 4) : 0;
+  p.total = at;
+  return p;
+}
+
+bool ll_sizes_ok(const ns_linear_ce_desc* d) {
+  return d->rows >= 0 && d->rows <= (1 << 21) && d->vocab > 0 && d->vocab <= (1 << 28) && d->d > 0 && d->d % 8 == 0 && d->d <= (1 << 16) && d->k >= 0 && d->k <= LL_MAX_K;
+}
+
+template <class T>
+int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
+  typedef typename T::e E;
+  char* const ws = (char*)d->workspace;
+  int *order = (int*)(ws + p.order), *inv = (int*)(ws + p.inv), *lab = (int*)(ws + p.lab);
+  float *zk = (float*)(ws + p.zk), *pk = (float*)(ws + p.pk), *La = (float*)(ws + p.La), *Lb = (float*)(ws + p.Lb), *ploss = (float*)(ws + p.ploss);
+  const bool dual = dual_of(d), soft_only = d->k > 0 && d->alpha == 1.f, grad = d->dh || d->dw;
+  const float alpha = d->k > 0 ? d->alpha : 0.f, T_ = d->k > 0 ? d->temperature : 1.f;
+  const float w1 = 1.f - alpha, w2 = alpha * T_;
+  // fp16 cells of dz: |w1 + w2| <= 2^x  =>  2^s with s = 15 - x keeps them below 2^15
+  int s = 0;
+  if (d->dtype == NS_F16) {
+    s = 15;
+    for (float b = 1.f; b < w1 + w2; b *= 2.f) --s;
+  }
+  const float up = ldexpf(1.f, s);
+  static ns_dev_once once;
+  if (!ns_dyn_lds_once(once, {(const void*)ll_logits_kernel<T, false, false, false>, (const void*)ll_logits_kernel<T, false, true, false>,
+                              (const void*)ll_logits_kernel<T, true, false, true>, (const void*)ll_logits_kernel<T, true, false, false>,
+                              (const void*)ll_logits_kernel<T, true, true, false>, (const void*)ll_dh_kernel<T>, (const void*)ll_dw_kernel<T>}, LL_LDS, "ns_linear_cross_entropy"))
+    return NS_ERR_HIP;
+  hipLaunchKernelGGL(ll_compact_kernel, dim3(1), dim3(1024), 0, st, d->labels, d->rows, d->vocab, order, inv, lab, d->row_loss, d->nvalid_dev);
+  hipLaunchKernelGGL(ll_pack_kernel<T>, dim3(p.R / 4), dim3(256), 0, st, d->h, d->ldh, d->w, d->ldw, d->d, p.dp, d->vocab, order, lab, d->top_idx, d->ld_top, d->k,
+                     d->nvalid_dev, (void*)(ws + p.hp), zk);
+  if (d->dw)
+    hipLaunchKernelGGL(ll_transpose_kernel, dim3(p.R / 64, p.dp / 64), dim3(256), 0, st, (const uint16_t*)(ws + p.hp), p.dp, d->nvalid_dev, (uint16_t*)(ws + p.hT), p.R);
+  LogitsArgs a = {};
+  a.hp = ws + p.hp; a.w = d->w; a.ldw = d->ldw; a.dp = p.dp; a.d = d->d; a.V = d->vocab; a.col0 = 0; a.tiles_n = p.tiles_n; a.R = p.R; a.nvalid = d->nvalid_dev;
+  a.c1 = soft_only ? LOG2E / T_ : LOG2E;
+  a.c2 = LOG2E / T_;
+  a.pm = (float*)(ws + p.pm); a.p1 = (float*)(ws + p.p1); a.p2 = (float*)(ws + p.p2);
+  a.La = La; a.Lb = Lb; a.G = ws + p.G; a.ldg = p.piece_tiles * BN; a.lab = lab; a.zk = zk; a.wlab = w1 * up;
+  const dim3 all(p.R / BM * p.tiles_n);
+  if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, false, true, false>), all, dim3(NTH), LL_LDS, st, a);
+  else hipLaunchKernelGGL((ll_logits_kernel<T, false, false, false>), all, dim3(NTH), LL_LDS, st, a);
+  RowArgs r = {};
+  r.pm = a.pm; r.p1 = a.p1; r.p2 = a.p2; r.tiles_n = p.tiles_n; r.R = p.R; r.k = d->k; r.V = d->vocab;
+  r.c1 = a.c1; r.c2 = a.c2; r.invT = 1.f / T_; r.w1 = w1; r.w2 = w2; r.kd = alpha * T_ * T_;
+  r.lw1 = (d->k > 0 && !dual) ? (float)s : log2f(w1) + (float)s;
+  r.lw2 = log2f(w2) + (float)s;
+  r.dual = dual; r.soft_only = soft_only; r.nvalid = d->nvalid_dev; r.order = order; r.zk = zk; r.top_vals = d->top_vals; r.top_idx = d->top_idx; r.ld_top = d->ld_top;
+  r.La = La; r.Lb = dual ? Lb : nullptr; r.pk = pk; r.row_loss = d->row_loss; r.packed_loss = ploss;
+  hipLaunchKernelGGL(ll_rows_kernel, dim3(p.R / 16), dim3(256), 0, st, r);
+  hipLaunchKernelGGL(ll_mean_kernel, dim3(1), dim3(1024), 0, st, ploss, d->nvalid_dev, d->loss_dev);
+  if (grad) {
+    for (int pc = 0; pc < p.pieces; ++pc) {
+      a.col0 = pc * p.piece_tiles * BN;
+      a.tiles_n = p.tiles_n - pc * p.piece_tiles < p.piece_tiles ? p.tiles_n - pc * p.piece_tiles : p.piece_tiles;
+      const dim3 grid(p.R / BM * a.tiles_n);
+      if (d->k == 0) hipLaunchKernelGGL((ll_logits_kernel<T, true, false, true>), grid, dim3(NTH), LL_LDS, st, a);
+      else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, true, true, false>), grid, dim3(NTH), LL_LDS, st, a);
+      else hipLaunchKernelGGL((ll_logits_kernel<T, true, false, false>), grid, dim3(NTH), LL_LDS, st, a);
+      if (d->k > 0)
+        hipLaunchKernelGGL(ll_cells_kernel<E>, dim3(p.R / 4), dim3(256), 0, st, d->nvalid_dev, order, lab, d->top_idx, d->ld_top, d->k, zk, pk, La, dual ? Lb : nullptr,
+                           a.c1, a.c2, w1 * up, w2 * up, a.col0, a.tiles_n * BN, d->vocab, (E*)a.G, a.ldg);
+      if (d->dh) {
+        DhArgs q = {};
+        q.G = a.G; q.w = d->w; q.ldw = d->ldw; q.ldg = a.ldg; q.col0 = a.col0; q.cols = a.tiles_n * BN; q.V = d->vocab; q.d = d->d; q.R = p.R;
+        q.splits = p.splits; q.chunk = p.chunk; q.add = pc > 0; q.nvalid = d->nvalid_dev; q.slab = (float*)(ws + p.slab);
+        hipLaunchKernelGGL(ll_dh_kernel<T>, dim3(p.R / BM * ((d->d + BN - 1) / BN) * p.splits), dim3(NTH), LL_LDS, st, q);
+      }
+      if (d->dw) {
+        DwArgs q = {};
+        q.hT = ws + p.hT; q.ldt = p.R; q.G = a.G; q.ldg = a.ldg; q.col0 = a.col0; q.tiles_v = a.tiles_n; q.V = d->vocab; q.d = d->d; q.nvalid = d->nvalid_dev;
+        q.loss_scale = d->loss_scale_dev; q.unscale = 1.f / up; q.dw = d->dw; q.lddw = d->lddw; q.f32 = d->dw_f32; q.add = d->dw_add;
+        hipLaunchKernelGGL(ll_dw_kernel<T>, dim3(p.dt / BM * a.tiles_n), dim3(NTH), LL_LDS, st, q);
+      }
+    }
+    if (d->dh)
+      hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)(((int64_t)d->rows * (d->d / 8) + 255) / 256)), dim3(256), 0, st, (const float*)(ws + p.slab), p.splits, p.R,
+                         d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh, d->lddh);
+  }
+  NS_CHECK_LAUNCH("ns_linear_cross_entropy");
+  return NS_OK;
+}
+
+}  // namespace
+
+extern "C" size_t ns_linear_ce_workspace_bytes(const ns_linear_ce_desc* d) {
+  if (!d || !ll_sizes_ok(d)) return 0;
+  ns_linear_ce_desc c = *d;
+  if (c.alpha == 0.f) c.k = 0;       // the hard labels alone: the teacher's list is not read
+  return plan_of(&c).total;
+}
+
+extern "C" int ns_linear_cross_entropy(const ns_linear_ce_desc* desc, void* stream) {
+  NS_CHECK_ARG(desc, "ns_linear_cross_entropy: null descriptor");
+  ns_linear_ce_desc c = *desc;
+  ns_linear_ce_desc* const d = &c;
+  NS_CHECK_ARG(d->w && d->loss_dev && d->nvalid_dev && (d->rows == 0 || (d->h && d->labels && d->row_loss)), "ns_linear_cross_entropy: null pointer");
+  NS_CHECK_ARG(ll_sizes_ok(d), "ns_linear_cross_entropy: bad sizes rows=%d vocab=%d d=%d k=%d (d a multiple of 8, k <= %d)", d->rows, d->vocab, d->d, d->k, LL_MAX_K);
+  NS_CHECK_ARG(d->dtype == NS_F16 || d->dtype == NS_BF16, "ns_linear_cross_entropy: dtype %d (NS_F16 or NS_BF16)", d->dtype);
+  const int64_t lds[] = {d->ldh, d->ldw, d->dh ? d->lddh : d->ldh, d->dw ? d->lddw : d->ldw};
+  for (int64_t ld : lds) NS_CHECK_ARG(ld >= d->d && ld % 8 == 0 && ld < (1 << 21), "ns_linear_cross_entropy: row stride %lld (a multiple of 8, >= d, < 2^21)", (long long)ld);
+  for (const void* q : {d->h, d->w, (const void*)d->dh, (const void*)d->dw, (const void*)d->workspace})
+    NS_CHECK_ARG(((size_t)q & 15) == 0, "ns_linear_cross_entropy: a tensor does not start on 16 bytes");
+  NS_CHECK_ARG(d->k == 0 || (d->top_vals && d->top_idx && d->ld_top >= d->k), "ns_linear_cross_entropy: the teacher's list needs values, tokens and a row stride >= k");
+  NS_CHECK_ARG(d->k == 0 || (d->temperature >= 1e-3f && d->temperature <= 1e3f && d->alpha >= 0.f && d->alpha <= 1.f),
+               "ns_linear_cross_entropy: temperature %g in [1e-3, 1e3], alpha %g in [0, 1]", (double)d->temperature, (double)d->alpha);
+  NS_CHECK_ARG(!d->dw_add || d->dw_f32, "ns_linear_cross_entropy: only an fp32 weight gradient is added to");
+  if (d->alpha == 0.f) d->k = 0;     // the hard labels alone: the teacher's list is not read
+  const Plan p = plan_of(d);
+  NS_CHECK_ARG(d->workspace && d->workspace_bytes >= p.total, "ns_linear_cross_entropy: workspace of %zu bytes, %zu needed", d->workspace_bytes, p.total);
+  NS_CHECK_ARG((int64_t)(p.R / BM) * p.tiles_n < (1ll << 31) && (int64_t)d->rows * (d->d / 8) < (1ll << 38), "ns_linear_cross_entropy: too many tiles");
+  return d->dtype == NS_F16 ? ll_launch<tf16>(d, p, (hipStream_t)stream) : ll_launch<tbf16>(d, p, (hipStream_t)stream);
+}

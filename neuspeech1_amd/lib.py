@@ -177,6 +177,36 @@ class LoraBwdDesc(C.Structure):
     ]
 
 
+NS_F16, NS_BF16, NS_F32 = 0, 1, 2
+
+
+class LinearCeDesc(C.Structure):
+    _fields_ = [
+        ("h", C.c_void_p), ("w", C.c_void_p), ("labels", C.c_void_p), ("top_vals", C.c_void_p), ("top_idx", C.c_void_p),
+        ("row_loss", C.c_void_p), ("loss_dev", C.c_void_p), ("nvalid_dev", C.c_void_p), ("loss_scale_dev", C.c_void_p),
+        ("dh", C.c_void_p), ("dw", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("ldh", C.c_int64), ("ldw", C.c_int64), ("lddh", C.c_int64), ("lddw", C.c_int64), ("ld_top", C.c_int64),
+        ("rows", C.c_int32), ("vocab", C.c_int32), ("d", C.c_int32), ("k", C.c_int32), ("dtype", C.c_int32),
+        ("dw_f32", C.c_int32), ("dw_add", C.c_int32), ("temperature", C.c_float), ("alpha", C.c_float),
+    ]
+
+
+class DistillDesc(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("labels", C.c_void_p), ("top_vals", C.c_void_p), ("top_idx", C.c_void_p),
+        ("row_loss", C.c_void_p), ("loss_dev", C.c_void_p), ("nvalid_dev", C.c_void_p), ("loss_scale_dev", C.c_void_p),
+        ("dlogits", C.c_void_p), ("ldz", C.c_int64), ("lddz", C.c_int64), ("ld_top", C.c_int64),
+        ("rows", C.c_int32), ("vocab", C.c_int32), ("k", C.c_int32), ("dtype", C.c_int32),
+        ("temperature", C.c_float), ("alpha", C.c_float),
+    ]
+
+
+class TopkDesc(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("vals", C.c_void_p), ("idx", C.c_void_p), ("lse", C.c_void_p),
+                ("ldz", C.c_int64), ("ldo", C.c_int64),
+                ("rows", C.c_int32), ("vocab", C.c_int32), ("k", C.c_int32), ("dtype", C.c_int32)]
+
+
 class BeamDesc(C.Structure):
     _fields_ = [
         ("top_vals", C.c_void_p), ("top_idx", C.c_void_p),
@@ -231,6 +261,10 @@ SIGNATURES = {
     "ns_attn_bwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "ns_cross_entropy": (C.c_int, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "ns_argmax_rows": (C.c_int, [_vp, _i, _i, _i, _vp, _vp]),
+    "ns_linear_cross_entropy": (C.c_int, [C.POINTER(LinearCeDesc), _vp]),
+    "ns_linear_ce_workspace_bytes": (_sz, [C.POINTER(LinearCeDesc)]),
+    "ns_distill_topk": (C.c_int, [C.POINTER(DistillDesc), _vp]),
+    "ns_topk_logits": (C.c_int, [C.POINTER(TopkDesc), _vp]),
     "ns_attn_decode": (C.c_int, [C.POINTER(AttnDecodeDesc), _vp]),
     "ns_attn_fewq": (C.c_int, [C.POINTER(AttnFewqDesc), _vp]),
     "ns_vt_pack": (C.c_int, [_vp, _i, _vp, _i, _i, _i, _i, _vp]),

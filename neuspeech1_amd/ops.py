@@ -11,7 +11,7 @@ from .lib import (AdamWCfg, AttnDesc, CastJob, GemmDesc, RowMap, NS_GEMM_ATOMIC3
                   NS_GEMM_GELU, NS_GEMM_GELU_SAVE_GRAD, NS_GEMM_MUL_P16, NS_GEMM_TN)
 
 __all__ = ["gemm", "rowmap", "ptr", "layernorm_fwd", "layernorm_bwd", "signal_pack", "feed_pack", "embed_pos", "attn_fwd",
-           "attn_bwd", "cross_entropy", "dgelu_mul", "colsum", "argmax_rows", "grad_norm", "adamw_step", "cast_jobs", "make_cast_jobs",
+           "attn_bwd", "cross_entropy", "linear_cross_entropy", "linear_ce_workspace_bytes", "distill_topk", "topk_logits", "dgelu_mul", "colsum", "argmax_rows", "grad_norm", "adamw_step", "cast_jobs", "make_cast_jobs",
            "NS_GEMM_GELU", "NS_GEMM_DGELU", "NS_GEMM_TN", "NS_GEMM_ATOMIC32", "NS_GEMM_DROP_A", "NS_GEMM_GELU_SAVE_GRAD",
            "NS_GEMM_MUL_P16", "NS_GEMM_COLSUM_A"]
 
@@ -329,6 +329,202 @@ def cross_entropy(logits16, labels, rows, V, ldv, row_loss, dlogits16, nvalid_de
     _work("cross_entropy", 0.0, rows * V * (2.0 + (2.0 if dlogits16 is not None else 0.0)))
     _call("ns_cross_entropy", ptr(logits16), ptr(labels), rows, V, ldv, ptr(row_loss), ptr(dlogits16),
                                       ptr(nvalid_dev), ptr(loss_scale_dev), ptr(loss_dev))
+
+
+# ---- losses over the vocabulary.  Shapes and types come from the tensors; what the kernels cannot take is refused here with a ValueError.
+_DTYPES = {torch.float16: L.NS_F16, torch.bfloat16: L.NS_BF16, torch.float32: L.NS_F32}
+
+
+def _need(ok, what: str):
+    if not ok:
+        raise ValueError(what)
+
+
+def _matrix(name, t, rows=None, cols=None, dtypes=None) -> int:
+    """row stride (elements) of a 2-D tensor with unit column stride"""
+    _need(isinstance(t, torch.Tensor) and t.dim() == 2, f"{name}: a 2-D tensor")
+    _need((rows is None or t.shape[0] == rows) and (cols is None or t.shape[1] == cols),
+          f"{name}: shape {tuple(t.shape)}, expected ({'any' if rows is None else rows}, {'any' if cols is None else cols})")
+    _need(dtypes is None or t.dtype in dtypes, f"{name}: dtype {t.dtype}, expected one of {dtypes}")
+    _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{name}: columns must be contiguous (strides {t.stride()})")
+    _need(t.shape[0] <= 1 or t.stride(0) >= t.shape[1], f"{name}: rows overlap (strides {t.stride()})")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vector(name, t, n, dtype):
+    _need(isinstance(t, torch.Tensor) and t.dtype == dtype and t.numel() == n and t.is_contiguous(), f"{name}: a contiguous tensor of {n} {dtype}")
+
+
+def _span(t):
+    """[first, last) byte address that a tensor's elements occupy"""
+    if t.numel() == 0:
+        return (0, 0)
+    return (t.data_ptr(), t.data_ptr() + (sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1) * t.element_size())
+
+
+def _apart(name, out, *ins):
+    a = _span(out)
+    for what, t in ins:
+        b = _span(t)
+        _need(a[1] <= b[0] or b[1] <= a[0], f"{name} overlaps {what}")
+
+
+def _on_one_gpu(*named):
+    dev = None
+    for name, t in named:
+        if t is None:
+            continue
+        _need(t.is_cuda, f"{name}: on {t.device}, expected a GPU")
+        dev = t.device if dev is None else dev
+        _need(t.device == dev, f"{name}: on {t.device}, the others are on {dev}")
+    return dev
+
+
+def _targets(rows, vocab, labels, row_loss, loss, nvalid, loss_scale, top_vals, top_idx, temperature, alpha):
+    """the arguments that both losses share -> k, row stride of the teacher's list"""
+    if labels is not None:
+        _vector("labels", labels, rows, torch.int64)
+    _vector("row_loss", row_loss, rows, torch.float32)
+    _vector("loss", loss, 1, torch.float32)
+    _vector("nvalid", nvalid, 1, torch.int32)
+    if loss_scale is not None:
+        _vector("loss_scale", loss_scale, 1, torch.float32)
+    if top_vals is None and top_idx is None:
+        _need(alpha == 0.0, f"alpha {alpha}: soft targets need top_vals and top_idx")
+        return 0, 0
+    _need(top_vals is not None and top_idx is not None, "top_vals and top_idx come together")
+    lt = _matrix("top_vals", top_vals, rows, None, (torch.float32,))
+    k = top_vals.shape[1]
+    li = _matrix("top_idx", top_idx, rows, k, (torch.int32,))
+    _need(rows <= 1 or lt == li, f"top_vals and top_idx: different row strides ({lt}, {li})")
+    _need(1 <= k <= 256, f"top_vals: {k} entries a row, 1 to 256 are supported")
+    _need(1e-3 <= temperature <= 1e3, f"temperature {temperature}: expected 1e-3 to 1e3")
+    _need(0.0 <= alpha <= 1.0, f"alpha {alpha}: expected 0 to 1")
+    return k, lt
+
+
+def _linear_ce_desc(h, weight, labels, row_loss, loss, nvalid, dh, dweight, loss_scale, top_vals, top_idx, temperature, alpha, accumulate):
+    d = L.LinearCeDesc()
+    ldh = _matrix("h", h, None, None, (torch.float16, torch.bfloat16))
+    rows, width = h.shape
+    ldw = _matrix("weight", weight, None, width, (h.dtype,))
+    vocab = weight.shape[0]
+    _need(vocab >= 1, "weight: no rows")
+    _need(width >= 8 and width % 8 == 0 and width <= 1 << 16, f"h: {width} columns, a multiple of 8 up to 65536 is supported")
+    _need(rows <= 1 << 21, f"h: {rows} rows, up to {1 << 21} are supported")
+    k, ldt = _targets(rows, vocab, labels, row_loss, loss, nvalid, loss_scale, top_vals, top_idx, temperature, alpha)
+    for name, t, ld in (("h", h, ldh), ("weight", weight, ldw)):
+        _need(ld % 8 == 0 and ld < 1 << 21 and t.data_ptr() % 16 == 0, f"{name}: rows must start on 16 bytes (row stride {ld} elements, below {1 << 21})")
+    d.ldh, d.ldw, d.ld_top = ldh, ldw, ldt
+    if dh is not None:
+        d.lddh = _matrix("dh", dh, rows, width, (h.dtype,))
+        _need(d.lddh % 8 == 0 and d.lddh < 1 << 21 and dh.data_ptr() % 16 == 0, f"dh: rows must start on 16 bytes (row stride {d.lddh} elements)")
+        _apart("dh", dh, ("h", h), ("weight", weight))
+    if dweight is not None:
+        d.lddw = _matrix("dweight", dweight, vocab, width, (h.dtype, torch.float32))
+        _need(d.lddw % 8 == 0 and d.lddw < 1 << 21 and dweight.data_ptr() % 16 == 0, f"dweight: rows must start on 16 bytes (row stride {d.lddw} elements)")
+        _apart("dweight", dweight, ("h", h), ("weight", weight))
+        if dh is not None:
+            _apart("dweight", dweight, ("dh", dh))
+        d.dw_f32 = int(dweight.dtype == torch.float32)
+    _need(not accumulate or (dweight is not None and d.dw_f32), "accumulate: adds to a float32 dweight only")
+    d.dw_add = int(accumulate)
+    d.h, d.w, d.labels, d.top_vals, d.top_idx = ptr(h), ptr(weight), ptr(labels), ptr(top_vals), ptr(top_idx)
+    d.row_loss, d.loss_dev, d.nvalid_dev, d.loss_scale_dev = ptr(row_loss), ptr(loss), ptr(nvalid), ptr(loss_scale)
+    d.dh, d.dw = ptr(dh), ptr(dweight)
+    if rows == 0 and dh is not None:
+        d.dh = 0                                  # nothing to write
+    d.rows, d.vocab, d.d, d.k, d.dtype = rows, vocab, width, k, _DTYPES[h.dtype]
+    d.temperature, d.alpha = temperature, alpha
+    return d
+
+
+def linear_ce_workspace_bytes(h, weight, labels, *, row_loss, loss, nvalid, dh=None, dweight=None, loss_scale=None, top_vals=None, top_idx=None,
+                              temperature=1.0, alpha=0.0, accumulate=False) -> int:
+    """workspace of linear_cross_entropy for these arguments"""
+    return int(L.load().ns_linear_ce_workspace_bytes(C.byref(_linear_ce_desc(h, weight, labels, row_loss, loss, nvalid, dh, dweight, loss_scale, top_vals,
+                                                                             top_idx, float(temperature), float(alpha), accumulate))))
+
+
+def linear_cross_entropy(h, weight, labels, *, row_loss, loss, nvalid, dh=None, dweight=None, loss_scale=None, top_vals=None, top_idx=None,
+                         temperature=1.0, alpha=0.0, accumulate=False, workspace=None):
+    """The LM head and its loss without the logits (ns_linear_cross_entropy): z = h weight^T is formed in tiles, once for the losses and, when dh
+    or dweight is given, once more for dz.
+
+    h (rows, d), weight (vocab, d): float16 or bfloat16; labels (rows) int64, outside [0, vocab) = the row is ignored.  Written: row_loss (rows) and
+    loss (1) float32, nvalid (1) int32, dh like h, dweight like weight or float32 (`accumulate`: added to a float32 one): gradients of
+    loss_scale x loss.  top_vals / top_idx (rows, k): a teacher's top logits and tokens (topk_logits), mixed in by `alpha` at `temperature`:
+    loss = mean of (1 - alpha) CE + alpha T^2 KL.
+    workspace: a uint8 tensor of linear_ce_workspace_bytes(...) (default: allocated for the call, on the current stream).  A captured graph keeps
+    the default's memory in its own pool; two graphs that may run at the same time must not share an explicit one."""
+    d = _linear_ce_desc(h, weight, labels, row_loss, loss, nvalid, dh, dweight, loss_scale, top_vals, top_idx, float(temperature), float(alpha), accumulate)
+    dev = _on_one_gpu(("h", h), ("weight", weight), ("labels", labels), ("row_loss", row_loss), ("loss", loss), ("nvalid", nvalid), ("dh", dh),
+                      ("dweight", dweight), ("loss_scale", loss_scale), ("top_vals", top_vals), ("top_idx", top_idx), ("workspace", workspace))
+    need = int(L.load().ns_linear_ce_workspace_bytes(C.byref(d)))
+    if workspace is None:
+        _need(getattr(_tls, "rec", None) is None, "a recorded launch list replays raw addresses: pass a workspace that outlives it")
+        workspace = torch.empty(need, device=dev, dtype=torch.uint8)
+    _need(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.numel() >= need and workspace.data_ptr() % 16 == 0,
+          f"workspace: {need} contiguous bytes of uint8 that start on 16 bytes")
+    d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    if STEP_PROFILE is not None:
+        n, v, w = d.rows, d.vocab, d.d
+        _work("linear_cross_entropy", 2.0 * n * v * w * (1 + (dh is not None) + (dweight is not None)),
+              2.0 * (n * w + v * w) + (2.0 * n * w if dh is not None else 0.0) + ((4.0 if d.dw_f32 else 2.0) * v * w if dweight is not None else 0.0))
+    with torch.cuda.device(dev):
+        _call("ns_linear_cross_entropy", C.byref(d))
+
+
+def distill_topk(logits, labels, top_vals, top_idx, *, row_loss, loss, nvalid, temperature=1.0, alpha=1.0, dlogits=None, loss_scale=None):
+    """Distillation from a teacher's top logits over logits that exist (ns_distill_topk): loss = mean of (1 - alpha) CE + alpha T^2 KL and, with
+    dlogits, the gradient of loss_scale x loss with respect to the logits (like logits; may be the logits themselves).
+
+    logits (rows, vocab) float16, bfloat16 or float32, rows at any stride (a [:, :vocab] view of a padded buffer: the padding is not
+    touched); labels as in linear_cross_entropy, or None with alpha = 1: every row counts; top_vals / top_idx (rows, k) float32 / int32, k <= 256."""
+    d = L.DistillDesc()
+    d.ldz = _matrix("logits", logits, None, None, tuple(_DTYPES))
+    rows, vocab = logits.shape
+    _need(vocab >= 1, "logits: no columns")
+    _need(labels is not None or alpha == 1.0, f"alpha {alpha}: the hard term needs labels")
+    _need(top_vals is not None and alpha > 0.0, "top_vals, top_idx and alpha > 0: without them this is cross_entropy")
+    d.k, d.ld_top = _targets(rows, vocab, labels, row_loss, loss, nvalid, loss_scale, top_vals, top_idx, temperature, alpha)
+    if dlogits is not None:
+        d.lddz = _matrix("dlogits", dlogits, rows, vocab, (logits.dtype,))
+        if not (dlogits.data_ptr() == logits.data_ptr() and d.lddz == d.ldz):
+            _apart("dlogits", dlogits, ("logits", logits))
+    dev = _on_one_gpu(("logits", logits), ("labels", labels), ("top_vals", top_vals), ("top_idx", top_idx), ("row_loss", row_loss), ("loss", loss),
+                      ("nvalid", nvalid), ("dlogits", dlogits), ("loss_scale", loss_scale))
+    d.logits, d.labels, d.top_vals, d.top_idx = ptr(logits), ptr(labels), ptr(top_vals), ptr(top_idx)
+    d.row_loss, d.loss_dev, d.nvalid_dev, d.loss_scale_dev, d.dlogits = ptr(row_loss), ptr(loss), ptr(nvalid), ptr(loss_scale), ptr(dlogits)
+    d.rows, d.vocab, d.dtype, d.temperature, d.alpha = rows, vocab, _DTYPES[logits.dtype], float(temperature), float(alpha)
+    _work("distill_topk", 0.0, logits.element_size() * rows * vocab * (2.0 if dlogits is not None else 1.0) + 8.0 * rows * d.k)
+    with torch.cuda.device(dev):
+        _call("ns_distill_topk", C.byref(d))
+
+
+def topk_logits(logits, k, *, vals, idx, lse=None):
+    """A teacher's lists (ns_topk_logits): the k (<= 256) largest logits of each row, largest first, equal ones by the lowest token.
+
+    logits (rows, vocab) float16, bfloat16 or float32, rows at any stride; vals (rows, k) float32, idx (rows, k) int32, lse (rows) float32: the
+    row's log-sum-exp."""
+    d = L.TopkDesc()
+    d.ldz = _matrix("logits", logits, None, None, tuple(_DTYPES))
+    rows, vocab = logits.shape
+    _need(isinstance(k, int) and 1 <= k <= 256 and k <= vocab, f"k {k}: expected 1 to {min(256, vocab)}")
+    d.ldo = _matrix("vals", vals, rows, k, (torch.float32,))
+    ldi = _matrix("idx", idx, rows, k, (torch.int32,))
+    _need(rows <= 1 or ldi == d.ldo, f"vals and idx: different row strides ({d.ldo}, {ldi})")
+    if lse is not None:
+        _vector("lse", lse, rows, torch.float32)
+    dev = _on_one_gpu(("logits", logits), ("vals", vals), ("idx", idx), ("lse", lse))
+    for name, t in (("vals", vals), ("idx", idx), ("lse", lse)):
+        if t is not None:
+            _apart(name, t, ("logits", logits))
+    d.logits, d.vals, d.idx, d.lse = ptr(logits), ptr(vals), ptr(idx), ptr(lse)
+    d.rows, d.vocab, d.k, d.dtype = rows, vocab, k, _DTYPES[logits.dtype]
+    _work("topk_logits", 0.0, logits.element_size() * rows * vocab + 8.0 * rows * k)
+    with torch.cuda.device(dev):
+        _call("ns_topk_logits", C.byref(d))
 
 
 def argmax_rows(logits16, rows, V, ldv, out):

@@ -1,0 +1,478 @@
+"""GPU: linear_cross_entropy, distill_topk and topk_logits against their definitions in 64 bits (tests/vocab_loss_ref.py derives the tolerances)."""
+import math
+
+import pytest
+import torch
+
+from tests import vocab_loss_ref as R
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from neuspeech1_amd import ops as o
+    return o
+
+
+def gen(seed, dev):
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    return g
+
+
+def make_linear(dev, rows, d, v, dtype, seed=0, ignored=0.3, k=0, sharp=1.0):
+    g = gen(seed + 1000 * rows + d, dev)
+    w = (torch.randn(v, d, generator=g, device=dev) * 2.0 * d ** -0.5).to(dtype)
+    labels = torch.randint(0, v, (rows,), generator=g, device=dev)
+    h = (torch.randn(rows, d, generator=g, device=dev) + sharp * w[labels].float()).to(dtype)
+    off = torch.rand(rows, generator=g, device=dev) < ignored
+    labels = torch.where(off, -100, labels)
+    if rows > 4:
+        labels[1], labels[2] = v, -1           # out of range: ignored as well
+    return h, w, labels, (make_lists(dev, g, rows, v, k, labels) if k else (None, None))
+
+
+def make_lists(dev, g, rows, v, k, labels):
+    tv = torch.randn(rows, k, generator=g, device=dev) * 3
+    ti = torch.randint(0, v, (rows, k), generator=g, device=dev, dtype=torch.int32)        # (repeats happen and add up)
+    if k > 1:
+        ti[:, 1] = torch.where((labels >= 0) & (labels < v), labels, 0).int()
+        ti[::3, k - 1] = ti[::3, 0]            # the same token twice
+        ti[::4, k // 2] = -1                   # an absent entry
+    if rows > 6:
+        ti[5] = -1                             # no list at all
+        tv[6] = float("-inf")
+        tv[3, 0] = float("-inf")
+        ti[4, :] = v + 3                       # tokens outside the vocabulary
+    return tv, ti
+
+
+def outputs(dev, rows):
+    return dict(row_loss=torch.full((rows,), 7.0, device=dev), loss=torch.full((1,), 7.0, device=dev), nvalid=torch.full((1,), 7, device=dev, dtype=torch.int32))
+
+
+def close(got, want, tol, what):
+    got = got.double()
+    bad = ~((got - want).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), bad.numel(), float((got - want).abs()[bad].max()), float(tol[bad].min()), bad.nonzero()[:4].tolist())
+
+
+def check_linear(ops, dev, h, w, labels, lists=(None, None), temp=1.0, alpha=0.0, scale=None, grad="hw", dw_dtype=None, **kw):
+    rows, d = h.shape
+    o = outputs(dev, rows)
+    dh = torch.full_like(h, 3.0) if "h" in grad else None
+    dw = torch.full_like(w, 3.0, dtype=dw_dtype or w.dtype) if "w" in grad else None
+    sc = None if scale is None else torch.tensor([scale], device=dev)
+    more = dict(top_vals=lists[0], top_idx=lists[1], temperature=temp, alpha=alpha) if lists[0] is not None else {}
+    ops.linear_cross_entropy(h, w, labels, dh=dh, dweight=dw, loss_scale=sc, **o, **more, **kw)
+    torch.cuda.synchronize()
+    ref = R.linear(h, w, labels, 1.0 if scale is None else scale, dw_dtype, temp, alpha, *lists)
+    assert int(o["nvalid"]) == ref["nvalid"]
+    close(o["row_loss"], ref["row_loss"], ref["row_tol"], "row_loss")
+    close(o["loss"], ref["loss"].reshape(1), ref["loss_tol"].reshape(1), "loss")
+    if dh is not None:
+        close(dh, ref["dh"], ref["dh_tol"], "dh")
+    if dw is not None:
+        close(dw, ref["dw"], ref["dw_tol"], "dw")
+    return o, dh, dw
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,d,v", [(1, 8, 1), (1, 64, 300), (3, 72, 7), (5, 8, 257), (64, 64, 256), (65, 136, 511), (255, 256, 1000), (257, 264, 1001),
+                                      (300, 512, 2600), (700, 776, 513)])
+def test_linear_cross_entropy(ops, dev, dtype, rows, d, v):
+    h, w, labels, _ = make_linear(dev, rows, d, v, dtype)
+    check_linear(ops, dev, h, w, labels)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,d,v,k", [(1, 64, 300, 5), (9, 72, 50, 1), (130, 128, 1000, 64), (300, 256, 777, 256), (40, 64, 40, 40)])
+@pytest.mark.parametrize("temp,alpha", [(1.0, 0.5), (2.0, 0.5), (3.5, 1.0), (1.0, 1.0), (0.5, 0.25), (2.0, 0.0)])
+def test_linear_cross_entropy_with_a_teacher(ops, dev, dtype, rows, d, v, k, temp, alpha):
+    h, w, labels, lists = make_linear(dev, rows, d, v, dtype, seed=1, k=k)
+    check_linear(ops, dev, h, w, labels, lists, temp, alpha)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("grad,dw_dtype", [("", None), ("h", None), ("w", None), ("w", F32), ("hw", F32)])
+def test_linear_cross_entropy_gradients_on_request(ops, dev, dtype, grad, dw_dtype):
+    h, w, labels, _ = make_linear(dev, 90, 192, 700, dtype, seed=2)
+    check_linear(ops, dev, h, w, labels, grad=grad, dw_dtype=dw_dtype, scale=512.0)
+
+
+def test_linear_cross_entropy_adds_to_a_float32_weight_gradient(ops, dev):
+    h, w, labels, _ = make_linear(dev, 90, 192, 700, BF16, seed=3)
+    o = outputs(dev, 90)
+    base = torch.randn(700, 192, device=dev)
+    dw = base.clone()
+    ops.linear_cross_entropy(h, w, labels, dweight=dw, accumulate=True, **o)
+    ref = R.linear(h, w, labels, dw_dtype=F32)
+    close(dw, ref["dw"] + base.double(), ref["dw_tol"] + 2 * R.U32 * (ref["dw"].abs() + base.double().abs()), "dw")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_linear_cross_entropy_in_two_pieces_of_the_vocabulary(ops, dev, dtype):
+    rows, d, v = 2049, 64, 60001
+    h, w, labels, lists = make_linear(dev, rows, d, v, dtype, seed=4, ignored=0.0, k=3)
+    check_linear(ops, dev, h, w, labels, lists, 2.0, 0.5)
+
+
+def test_rows_without_a_label_are_not_read(ops, dev):
+    """infinities and NaN in masked rows reach neither loss nor gradients; their gradient is zero"""
+    h, w, labels, lists = make_linear(dev, 300, 128, 600, BF16, seed=5, k=9)
+    off = ~((labels >= 0) & (labels < 600))
+    h[off] = float("nan")
+    h[off.nonzero()[::2, 0]] = float("inf")
+    lists[0][off] = float("nan")
+    o, dh, dw = check_linear(ops, dev, h, w, labels, lists, 2.0, 0.5)
+    assert (dh[off] == 0).all() and (o["row_loss"][off] == 0).all() and torch.isfinite(dw).all()
+
+
+@pytest.mark.parametrize("rows", [0, 1, 70])
+def test_no_row_has_a_label(ops, dev, rows):
+    h = torch.full((rows, 64), float("nan"), device=dev, dtype=F16)
+    w = torch.randn(300, 64, device=dev).half()
+    labels = torch.full((rows,), -100, device=dev, dtype=torch.int64)
+    o = outputs(dev, rows)
+    dh, dw = torch.full_like(h, 3.0), torch.full_like(w, 3.0)
+    ops.linear_cross_entropy(h, w, labels, dh=dh, dweight=dw, **o)
+    assert int(o["nvalid"]) == 0 and float(o["loss"]) == 0 and (o["row_loss"] == 0).all() and (dh == 0).all() and (dw == 0).all()
+
+
+def test_strided_operands_and_what_lies_beside_them(ops, dev):
+    g = gen(6, dev)
+    rows, d, v = 130, 72, 301
+    hb = torch.full((rows, 136), float("nan"), device=dev, dtype=F16)
+    wb = torch.full((v + 3, 200), float("inf"), device=dev, dtype=F16)
+    h, w = hb[:, 64:136], wb[2:v + 2, 8:80]
+    h.copy_(torch.randn(rows, d, generator=g, device=dev))
+    w.copy_(torch.randn(v, d, generator=g, device=dev) * 0.2)
+    labels = torch.randint(0, v, (rows,), generator=g, device=dev)
+    o = outputs(dev, rows)
+    dhb = torch.full((rows + 2, 96), 5.0, device=dev, dtype=F16)
+    dwb = torch.full((v + 2, 80), 5.0, device=dev, dtype=F32)
+    dh, dw = dhb[1:rows + 1, 16:88], dwb[1:v + 1, 8:80]
+    ops.linear_cross_entropy(h, w, labels, dh=dh, dweight=dw, **o)
+    ref = R.linear(h, w, labels, dw_dtype=F32)
+    close(dh, ref["dh"], ref["dh_tol"], "dh")
+    close(dw, ref["dw"], ref["dw_tol"], "dw")
+    close(o["row_loss"], ref["row_loss"], ref["row_tol"], "row_loss")
+    for buf, view in ((dhb, dh), (dwb, dw)):
+        view.fill_(5.0)
+        assert (buf == 5.0).all()
+
+
+def test_large_logits(ops, dev):
+    """logits of hundreds: the softmax is one-hot, every exponential stays finite"""
+    h, w, labels, _ = make_linear(dev, 70, 64, 500, BF16, seed=7, sharp=0.0)
+    check_linear(ops, dev, h * 64, w * 4, labels)
+
+
+def test_same_inputs_give_the_same_bits_and_workspaces_are_not_shared(ops, dev):
+    """repeated, interleaved with another call, on another stream and with a caller's workspace: equal bits; nothing past the workspace is written"""
+    h, w, labels, lists = make_linear(dev, 600, 256, 3001, F16, seed=8, k=20)
+    h2, w2, labels2, _ = make_linear(dev, 500, 128, 900, F16, seed=9)
+    kw = dict(top_vals=lists[0], top_idx=lists[1], temperature=2.0, alpha=0.5)
+
+    def once(**more):
+        o = outputs(dev, 600)
+        dh, dw = torch.empty_like(h), torch.empty_like(w)
+        ops.linear_cross_entropy(h, w, labels, dh=dh, dweight=dw, **o, **kw, **more)
+        return [o["row_loss"], o["loss"], dh, dw]
+    a = once()
+    o2 = outputs(dev, 500)
+    ops.linear_cross_entropy(h2, w2, labels2, dh=torch.empty_like(h2), **o2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b = once()
+    c = once()
+    need = ops.linear_ce_workspace_bytes(h, w, labels, dh=torch.empty_like(h), dweight=torch.empty_like(w), **outputs(dev, 600), **kw)
+    ws = torch.full((need + 4096,), 0xA5, device=dev, dtype=torch.uint8)
+    e = once(workspace=ws[:need])
+    torch.cuda.synchronize()
+    assert (ws[need:] == 0xA5).all()
+    for other in (b, c, e):
+        for x, y in zip(a, other):
+            assert torch.equal(x, y)
+    with pytest.raises(ValueError, match="workspace"):
+        once(workspace=ws[:need - 256])
+
+
+def test_captured_graphs_replay_with_new_data(ops, dev):
+    """two graphs, replayed several times between eager calls, against eager results"""
+    sets = [make_linear(dev, 260, 128, 1200, BF16, seed=s, k=6) for s in (10, 11, 12)]
+    h, w, labels = (t.clone() for t in sets[0][:3])
+    tv, ti = (t.clone() for t in sets[0][3])
+
+    def bufs():
+        return dict(outputs(dev, 260), dh=torch.empty_like(h), dweight=torch.empty_like(w))
+
+    def call(b):
+        ops.linear_cross_entropy(h, w, labels, top_vals=tv, top_idx=ti, temperature=2.0, alpha=0.5, **b)
+
+    def call_hard(b):
+        ops.linear_cross_entropy(h, w, labels, **b)
+    eager, ga, gb = bufs(), bufs(), bufs()
+    call(eager)
+    torch.cuda.synchronize()
+    from neuspeech1_amd.lib import capture_section
+    graphs = []
+    for fn, b in ((call, ga), (call_hard, gb)):
+        g = torch.cuda.CUDAGraph()
+        with capture_section(), torch.cuda.graph(g, capture_error_mode="thread_local"):
+            fn(b)
+        graphs.append(g)
+    for hh, ww, ll, (a, i) in sets + sets[:1]:
+        h.copy_(hh), w.copy_(ww), labels.copy_(ll), tv.copy_(a), ti.copy_(i)
+        for fn, g, b in ((call, graphs[0], ga), (call_hard, graphs[1], gb)):
+            fn(eager)
+            want = {n: t.clone() for n, t in eager.items()}
+            g.replay()
+            torch.cuda.synchronize()
+            for n in want:
+                assert torch.equal(b[n], want[n]), n
+
+
+def test_gradients_against_differences_of_the_loss(ops, dev):
+    """central differences of the kernel's own loss along random directions.  h is a multiple of 2^-5 and the step 2^-4 times directions of -1, 0, 1:
+    the moved h is exact.  The loss along a line has a third derivative below 2 r^3 a row, r = the range of the logits' change per step."""
+    g = gen(13, dev)
+    rows, d, v, eps = 40, 64, 200, 2.0 ** -4
+    w = (torch.randn(v, d, generator=g, device=dev) * 0.25).half()
+    h = (torch.randn(rows, d, generator=g, device=dev) * 32).round().div(32).half()
+    labels = torch.randint(0, v, (rows,), generator=g, device=dev)
+    tv, ti = make_lists(dev, g, rows, v, 7, labels)
+    kw = dict(top_vals=tv, top_idx=ti, temperature=2.0, alpha=0.5)
+    dh = torch.empty_like(h)
+    ops.linear_cross_entropy(h, w, labels, dh=dh, loss_scale=torch.tensor([256.0], device=dev), **outputs(dev, rows), **kw)
+    ref = R.linear(h, w, labels, 256.0, None, 2.0, 0.5, tv, ti)
+    for _ in range(4):
+        u = torch.randint(-1, 2, (rows, d), generator=g, device=dev).half()
+        f = []
+        for s in (1, -1):
+            o = outputs(dev, rows)
+            ops.linear_cross_entropy(h + s * eps * u, w, labels, **o, **kw)
+            f.append(o["row_loss"].double())
+        slope = (f[0] - f[1]) / (2 * eps)
+        line = u.double() @ w.double().t()
+        r = line.amax(1) - line.amin(1)
+        got = (dh.double() / 256.0 * rows * u.double()).sum(1)
+        tol = eps ** 2 / 6 * 2 * r ** 3 + ref["row_tol"] * 1.5 / eps + (ref["dh_tol"] / 256.0 * rows).sum(1)
+        assert ((slope - got).abs() <= tol).all()
+        assert float((slope - got).abs().mean()) < 0.05 * float(got.abs().mean())
+
+
+# ------------------------------------------------------------------------------------------------ distillation over logits
+def make_logits(dev, rows, v, dtype, seed, pad=0, first=0, ignored=0.3, k=5):
+    g = gen(seed, dev)
+    buf = (torch.randn(rows, v + pad + first, generator=g, device=dev) * 3).to(dtype)
+    z = buf[:, first:first + v]
+    labels = torch.randint(0, v, (rows,), generator=g, device=dev)
+    labels = torch.where(torch.rand(rows, generator=g, device=dev) < ignored, -100, labels)
+    return buf, z, labels, make_lists(dev, g, rows, v, k, labels)
+
+
+def check_distill(ops, dev, z, labels, lists, temp, alpha, dz=None, scale=None):
+    rows, v = z.shape
+    zd = z.double()
+    o = outputs(dev, rows)
+    sc = None if scale is None else torch.tensor([scale], device=dev)
+    ops.distill_topk(z, labels, *lists, temperature=temp, alpha=alpha, dlogits=dz, loss_scale=sc, **o)
+    torch.cuda.synchronize()
+    valid = torch.ones(rows, dtype=torch.bool, device=dev) if labels is None else (labels >= 0) & (labels < v)
+    ref = R.losses(torch.where(valid.unsqueeze(1), zd, torch.zeros_like(zd)), torch.zeros((), dtype=torch.float64, device=dev), labels, temp, alpha, *lists)
+    assert int(o["nvalid"]) == ref["nvalid"]
+    close(o["row_loss"], ref["row_loss"], ref["row_tol"], "row_loss")
+    close(o["loss"], ref["loss"].reshape(1), ref["loss_tol"].reshape(1), "loss")
+    if dz is not None:
+        gs = (scale or 1.0) / ref["n"]
+        U = R.half_step(z.dtype)
+        want = ref["cell"] * gs
+        small = {F16: 2.0 ** -25, BF16: 2.0 ** -126, F32: 2.0 ** -126}[z.dtype]
+        close(dz, want, (ref["cell_err"] * gs + 4 * R.U32 * want.abs()) * (1 + U) + U * want.abs() + small, "dlogits")
+    return o
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,v,pad,first,k", [(1, 1, 0, 0, 1), (7, 9, 0, 0, 3), (9, 1000, 24, 0, 8), (8, 1001, 2, 3, 33), (3, 2050, 1, 1, 256), (5, 9001, 0, 0, 64),
+                                                (2, 33003, 5, 2, 12), (3, 51865, 103, 0, 64), (2, 70001, 0, 0, 20)])
+@pytest.mark.parametrize("temp,alpha", [(2.0, 0.5), (1.0, 0.5), (4.0, 1.0)])
+def test_distill_topk(ops, dev, dtype, rows, v, pad, first, k, temp, alpha):
+    buf, z, labels, lists = make_logits(dev, rows, v, dtype, rows + v, pad, first, k=k)
+    ob = torch.full_like(buf, 5.0)
+    dz = ob[:, first:first + v]
+    check_distill(ops, dev, z, labels, lists, temp, alpha, dz, scale=64.0)
+    dz.fill_(5.0)
+    assert (ob == 5.0).all()                                   # columns beside the view are left as they were
+    other = torch.full((rows, v + 9), 5.0, device=dev, dtype=dtype)[:, 3:v + 3]      # another alignment than the logits'
+    check_distill(ops, dev, z, labels, lists, temp, alpha, other)
+    check_distill(ops, dev, z, labels, lists, temp, alpha)     # the loss alone
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("v", [300, 5000, 66000])
+def test_distill_topk_in_place(ops, dev, dtype, v):
+    buf, z, labels, lists = make_logits(dev, 9, v, dtype, 21, 1, 0, k=9)
+    out = torch.empty_like(z)
+    ops.distill_topk(z, labels, *lists, temperature=2.0, alpha=0.5, dlogits=out, **outputs(dev, 9))
+    keep = buf[:, v:].clone()
+    ops.distill_topk(z, labels, *lists, temperature=2.0, alpha=0.5, dlogits=z, **outputs(dev, 9))
+    assert torch.equal(z, out) and torch.equal(buf[:, v:], keep)
+
+
+def test_distill_topk_without_labels_and_with_masked_rows(ops, dev):
+    buf, z, labels, lists = make_logits(dev, 20, 700, F32, 22, k=4)
+    check_distill(ops, dev, z, None, lists, 2.0, 1.0, torch.empty_like(z))
+    off = labels < 0
+    z[off] = float("nan")
+    lists[0][off] = float("nan")
+    dz = torch.empty_like(z)
+    o = check_distill(ops, dev, z, labels, lists, 2.0, 0.5, dz)
+    assert (dz[off] == 0).all() and (o["row_loss"][off] == 0).all()
+    labels.fill_(-100)
+    o = check_distill(ops, dev, z, labels, lists, 2.0, 0.5, dz)
+    assert (dz == 0).all() and float(o["loss"]) == 0
+    o = outputs(dev, 0)
+    ops.distill_topk(z[:0], labels[:0], lists[0][:0], lists[1][:0], alpha=0.5, dlogits=dz[:0], **o)
+    assert float(o["loss"]) == 0 and int(o["nvalid"]) == 0
+
+
+def test_distill_topk_with_masked_logits(ops, dev):
+    """student logits of -inf and of the type's lowest value: finite losses where the targets do not name them, zero probability there"""
+    buf, z, labels, lists = make_logits(dev, 6, 900, F16, 23, ignored=0.0, k=5)
+    named = torch.zeros(6, 900, dtype=torch.bool, device=dev)
+    named.scatter_(1, lists[1].clamp(0, 899).long(), True)
+    named.scatter_(1, labels.clamp(0, 899).unsqueeze(1), True)
+    z[:, ::3] = torch.where(named[:, ::3], z[:, ::3], float("-inf"))
+    z[:, 1::3] = torch.where(named[:, 1::3], z[:, 1::3], torch.finfo(F16).min)
+    dz = torch.empty_like(z)
+    o = outputs(dev, 6)
+    ops.distill_topk(z, labels, *lists, temperature=2.0, alpha=0.5, dlogits=dz, **o)
+    ref = R.losses(z.double(), torch.zeros((), dtype=torch.float64, device=dev), labels, 2.0, 0.5, *lists)
+    fin = torch.isfinite(ref["row_loss"])
+    assert torch.isfinite(o["row_loss"][fin]).all() and fin.any() and torch.isfinite(dz[fin]).all()
+    assert ((o["row_loss"].double() - ref["row_loss"]).abs()[fin] <= 1e-4).all()      # (z of -65504 in the tolerance's |z| would say nothing)
+    assert (dz[:, ::3][~named[:, ::3]] == 0).all() and (dz[:, 1::3][~named[:, 1::3]] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ the teacher's lists
+def ref_topk(z, k):
+    z = z.double()
+    key = torch.where(torch.isnan(z), torch.full_like(z, float("inf")), z)
+    nan = torch.isnan(z)
+    vals, idx = [], []
+    for r in range(z.shape[0]):
+        order = sorted(range(z.shape[1]), key=lambda c: (not bool(nan[r, c]), -float(key[r, c]), c)) if z.shape[1] <= 600 else None
+        if order is None:
+            order = torch.sort(z[r] + 0.0, descending=True, stable=True).indices[:k].tolist()
+        idx.append(order[:k])
+        vals.append([float(z[r, c]) for c in order[:k]])
+    return torch.tensor(vals, dtype=torch.float64), torch.tensor(idx)
+
+
+def check_topk(ops, dev, z, k):
+    rows, v = z.shape
+    vals = torch.empty(rows, k, device=dev)
+    idx = torch.empty(rows, k, device=dev, dtype=torch.int32)
+    lse = torch.empty(rows, device=dev)
+    ops.topk_logits(z, k, vals=vals, idx=idx, lse=lse)
+    rv, ri = ref_topk(z.cpu(), k)
+    assert torch.equal(idx.cpu().long(), ri)
+    assert torch.equal(torch.nan_to_num(vals.cpu().double(), nan=1e30), torch.nan_to_num(rv, nan=1e30))
+    want = torch.logsumexp(z.double(), 1)
+    fin = torch.isfinite(want)
+    close(lse[fin], want[fin], (160 + 8 * z.double().abs().amax(1)[fin].clamp(min=1)) * R.U32, "lse")
+    return vals, idx, lse
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,v,pad,first,k", [(1, 1, 0, 0, 1), (4, 9, 0, 0, 9), (5, 257, 3, 1, 256), (3, 1000, 0, 0, 128), (3, 2050, 1, 2, 7), (2, 9001, 0, 0, 256),
+                                                (2, 33003, 5, 3, 100), (3, 51865, 103, 0, 64), (2, 70001, 1, 0, 33)])
+def test_topk_logits(ops, dev, dtype, rows, v, pad, first, k):
+    g = gen(v + k, dev)
+    z = (torch.randn(rows, v + pad + first, generator=g, device=dev) * 3).to(dtype)[:, first:first + v]
+    check_topk(ops, dev, z, k)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("v", [500, 9001, 51865])
+def test_topk_logits_of_equal_values(ops, dev, dtype, v):
+    """rows of one value, of two values, of the lowest value and -inf, of zeros of both signs: lowest tokens first, and the long way round the buffer"""
+    z = torch.zeros(6, v, device=dev, dtype=dtype)
+    z[0] = 1.5
+    z[1] = 1.0
+    z[1, 5::7] = 2.0
+    z[2] = float("-inf")
+    z[2, 3] = torch.finfo(dtype).min
+    z[3, ::2] = -0.0
+    z[4] = torch.arange(v, device=dev).remainder(5).to(dtype)
+    z[5] = 3.0
+    z[5, v - 20:] = 4.0
+    check_topk(ops, dev, z, 64)
+
+
+def test_topk_logits_with_infinities_and_nan(ops, dev):
+    z = torch.randn(3, 400, device=dev)
+    z[0, 100], z[0, 50] = float("inf"), float("inf")
+    z[1, 7], z[1, 300], z[1, 2] = float("nan"), -float("nan"), float("inf")
+    z[2] = float("-inf")
+    vals, idx, lse = check_topk(ops, dev, z, 5)
+    assert idx[1, :3].tolist() == [7, 300, 2] and lse[0] == float("inf") and torch.isnan(lse[1]) and lse[2] == float("-inf")
+
+
+# ------------------------------------------------------------------------------------------------ together
+def test_teacher_lists_distil_a_student_head(ops, dev):
+    """a teacher's logits -> its lists -> the student's head without logits, and over logits: the same loss and, through the head, the same gradient;
+    a captured step learns: replays equal eager calls"""
+    g = gen(31, dev)
+    rows, d, v, k = 200, 128, 1500, 32
+    teacher = (torch.randn(rows, v + 20, generator=g, device=dev) * 3).half()[:, :v]
+    h, w, labels, _ = make_linear(dev, rows, d, v, F16, seed=32)
+    tv, ti = torch.empty(rows, k, device=dev), torch.empty(rows, k, device=dev, dtype=torch.int32)
+    lse = torch.empty(rows, device=dev)
+    ops.topk_logits(teacher, k, vals=tv, idx=ti, lse=lse)
+    scale = torch.tensor([256.0], device=dev)
+    a, b = outputs(dev, rows), outputs(dev, rows)
+    dh, dw = torch.empty_like(h), torch.empty_like(w)
+    ops.linear_cross_entropy(h, w, labels, top_vals=tv, top_idx=ti, temperature=2.0, alpha=0.5, dh=dh, dweight=dw, loss_scale=scale, **a)
+    z = h.float() @ w.float().t()
+    dz = torch.empty_like(z)
+    ops.distill_topk(z, labels, tv, ti, temperature=2.0, alpha=0.5, dlogits=dz, loss_scale=scale, **b)
+    ref = R.linear(h, w, labels, 256.0, None, 2.0, 0.5, tv, ti)
+    close(a["row_loss"], ref["row_loss"], ref["row_tol"], "row_loss, linear")
+    close(b["row_loss"], ref["row_loss"], ref["row_tol"], "row_loss, logits")
+    close(dh, ref["dh"], ref["dh_tol"], "dh")
+    close(dw, ref["dw"], ref["dw_tol"], "dw")
+    close(dz.double() @ w.double(), ref["dh"], ref["dh_tol"], "dz W")
+    # hard labels alone: ops.cross_entropy over fp16 logits is the same loss up to the logits' rounding (2^-11 of |z| <= 32)
+    hard = outputs(dev, rows)
+    ops.linear_cross_entropy(h, w, labels, **hard)
+    z16 = torch.zeros(rows, (v + 7) // 8 * 8, device=dev, dtype=F16)
+    z16[:, :v] = z
+    old = outputs(dev, rows)
+    ops.cross_entropy(z16, labels, rows, v, z16.shape[1], old["row_loss"], None, old["nvalid"], None, old["loss"])
+    assert int(old["nvalid"]) == int(hard["nvalid"])
+    assert float((old["row_loss"] - hard["row_loss"]).abs().max()) <= 2 * 2.0 ** -11 * float(z.abs().max()) + 1e-4
+    from neuspeech1_amd.lib import capture_section
+    graph = torch.cuda.CUDAGraph()
+    got = [torch.empty_like(t) for t in (dh, dw, dz)]
+    c, e = outputs(dev, rows), outputs(dev, rows)
+    torch.cuda.synchronize()
+    with capture_section(), torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        ops.topk_logits(teacher, k, vals=tv, idx=ti, lse=lse)
+        ops.linear_cross_entropy(h, w, labels, top_vals=tv, top_idx=ti, temperature=2.0, alpha=0.5, dh=got[0], dweight=got[1], loss_scale=scale, **c)
+        ops.distill_topk(z, labels, tv, ti, temperature=2.0, alpha=0.5, dlogits=got[2], loss_scale=scale, **e)
+    for step in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(got + [c["row_loss"], e["row_loss"]], (dh, dw, dz, a["row_loss"], b["row_loss"])):
+            assert torch.equal(x, y)
+        w.sub_((dw.float() / 256).half())                       # the student learns; the graph reads the new weight
+        z.copy_(h.float() @ w.float().t())
+        ops.linear_cross_entropy(h, w, labels, top_vals=tv, top_idx=ti, temperature=2.0, alpha=0.5, dh=dh, dweight=dw, loss_scale=scale, **a)
+        ops.distill_topk(z, labels, tv, ti, temperature=2.0, alpha=0.5, dlogits=dz, loss_scale=scale, **b)
+        torch.cuda.synchronize()
+    assert math.isfinite(float(a["loss"]))
