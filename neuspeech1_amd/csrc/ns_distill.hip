@@ -16,65 +16,64 @@ constexpr int DT_MAX_K = 256;
 
 template <class E> struct vec { static constexpr int N = 16 / (int)sizeof(E); typedef E t __attribute__((ext_vector_type(16 / sizeof(E)))); };
 
-// A row's elements as 16-B chunks: chunk c holds the elements [c N - sh, (c + 1) N - sh); the first and the last one may be ragged.
+// A row as 16-B chunks from its first 16-B boundary, plus at most one element per thread from its ragged ends: threads 0 .. take the elements before
+// the boundary, threads 64 .. those behind the last whole chunk (extra_j: this thread's, or -1).
 template <class E, int NC, int NT>
 struct row_view {
   typedef typename vec<E>::t V;
   static constexpr int N = vec<E>::N;
   const E* p;
-  int n, sh, chunks;
-  V reg[NC > 0 ? NC : 1];
-  __device__ __forceinline__ void init(const E* row, int len) {
-    p = row; n = len;
-    sh = (int)(((size_t)row & 15) / sizeof(E));
-    chunks = (n + sh + N - 1) / N;
-  }
-  __device__ __forceinline__ V fetch(int c) const {
-    const int j = c * N - sh;
-    V v;
-    if (j >= 0 && j + N <= n) {
-      v = *(const V*)(p + j);
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = j + e >= 0 && j + e < n ? p[j + e] : (E)(-INFINITY);
-    }
-    return v;
+  const ns_u4v* body;
+  int head, chunks, extra_j;
+  float extra;
+  ns_u4v reg[NC > 0 ? NC : 1];
+  __device__ __forceinline__ void init(const E* row, int n) {
+    p = row;
+    head = min(n, (int)((0 - (size_t)row) & 15) / (int)sizeof(E));
+    chunks = (n - head) / N;
+    body = (const ns_u4v*)(row + head);
+    const int tail = n - head - chunks * N, t = threadIdx.x;
+    extra_j = t < head ? t : (t >= 64 && t - 64 < tail ? head + chunks * N + t - 64 : -1);
+    extra = -INFINITY;
   }
   __device__ __forceinline__ void load() {
     if (NC > 0) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int c = threadIdx.x + i * NT;
-        if (c < chunks) reg[i] = fetch(c);
-        else {
-#pragma unroll
-          for (int e = 0; e < N; ++e) reg[i][e] = (E)(-INFINITY);
-        }
-      }
+      for (int i = 0; i < NC; ++i)
+        if ((int)threadIdx.x + i * NT < chunks) reg[i] = body[threadIdx.x + i * NT];
     }
+    if (extra_j >= 0) extra = (float)p[extra_j];
   }
-  // f(first element index of the chunk, chunk); elements outside the row are -inf
-  template <class F> __device__ __forceinline__ void each(F f) const {
+  // f(chunk index, chunk).  The empty asm keeps hipcc from carrying the CONVERTED elements of one sweep over to the next (64 more registers per 8 chunks:
+  // it spilled them).
+  template <class F> __device__ __forceinline__ void each(F f) {
     if (NC > 0) {
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        const int c = threadIdx.x + i * NT;
-        if (c < chunks) f(c * N - sh, reg[i]);
+        if ((int)threadIdx.x + i * NT < chunks) {
+          asm volatile("" : "+v"(reg[i]));
+          f((int)threadIdx.x + i * NT, __builtin_bit_cast(V, reg[i]));
+        }
       }
     } else {
-      for (int c = threadIdx.x; c < chunks; c += NT) f(c * N - sh, fetch(c));
+      again(f);
     }
+  }
+  template <class F> __device__ __forceinline__ void again(F f) const {      // from memory
+#pragma unroll 1
+    for (int c = threadIdx.x; c < chunks; c += NT) f(c, __builtin_bit_cast(V, body[c]));
   }
 };
 
-template <int NT> __device__ __forceinline__ float block_max(float v, float* sh) {
-  v = ns_wave_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = sh[0];
+// sum / maximum over NW neighbouring lanes, one per wave's entry
+template <int NW, class T> __device__ __forceinline__ T over_waves(T v) {
 #pragma unroll
-  for (int i = 1; i < NT / 64; ++i) v = fmaxf(v, sh[i]);
+  for (int o = NW / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+template <int NW> __device__ __forceinline__ float max_over_waves(float v) {
+#pragma unroll
+  for (int o = NW / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
   return v;
 }
 template <int NT> __device__ __forceinline__ float block_sum(float v, float* sh) {
@@ -82,24 +81,26 @@ template <int NT> __device__ __forceinline__ float block_sum(float v, float* sh)
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = sh[0];
+  return over_waves<NT / 64>(sh[threadIdx.x & (NT / 64 - 1)]);
+}
+__device__ __forceinline__ int wave_sum_int(int v) {
 #pragma unroll
-  for (int i = 1; i < NT / 64; ++i) v += sh[i];
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
 template <int NT> __device__ __forceinline__ int block_count(int v, int* sh) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  v = wave_sum_int(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = sh[0];
-#pragma unroll
-  for (int i = 1; i < NT / 64; ++i) v += sh[i];
-  return v;
+  return over_waves<NT / 64>(sh[threadIdx.x & (NT / 64 - 1)]);
 }
+// a maximum to subtract: an infinite one is left in place of the difference (-inf: every exponential is zero; +inf: the sum becomes infinite)
+__device__ __forceinline__ float finite_or_zero(float m) { return fabsf(m) == INFINITY ? 0.f : m; }
 
 // ------------------------------------------------------------------------------------------------ the student
+constexpr int DT_COUNT_HERE = 4;      // labels per thread that a row's workgroup counts itself (64 KB of L2 reads under its own row's loads) instead of a launch
+
 __global__ __launch_bounds__(1024) void dt_count_kernel(const int64_t* __restrict__ labels, int rows, int V, int* __restrict__ nvalid) {
   __shared__ int sh[16];
   int c = 0;
@@ -120,41 +121,55 @@ __global__ __launch_bounds__(1024) void dt_mean_kernel(const float* __restrict__
 struct DistillArgs {
   const void* z; int64_t ldz;
   const int64_t* labels; const float* tv; const int32_t* ti; int64_t ldt;
-  int V, k, dual, soft_only;
+  int rows, V, k, soft_only, count_here;
   float T, w1, w2, kd;
   float* row_loss; void* dz; int64_t lddz;
-  const int* nvalid; const float* loss_scale;
+  int* nvalid; const float* loss_scale;
 };
 
-template <class E, int NC, int NT>
-__global__ __launch_bounds__(NT) void distill_kernel(const DistillArgs p) {
-  __shared__ float sh[16];
+// DUAL: two softmaxes (0 < alpha < 1 at T != 1), else one, at T when only soft targets count.
+// Per logit: a conversion and a maximum, then an fma, an exponential (a quarter-rate instruction) and an addition per softmax, and the same again for the
+// gradient: with DUAL ~30 issue slots, 26 k cycles of a CU a row of 51 865 against the 20 k that the row's 208 KB take at the copy rate.
+template <class E, int NC, int NT, bool DUAL>
+__global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_kernel(const DistillArgs p) {
+  constexpr int NW = NT / 64;
+  __shared__ float sh[3][NW];
+  __shared__ int shc[NW];
   __shared__ int sidx[DT_MAX_K + 1];
   __shared__ float sp[DT_MAX_K], sz[DT_MAX_K + 1];
   typedef row_view<E, NC, NT> RV;
-  const int row = blockIdx.x, tid = threadIdx.x;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t lab64 = p.labels ? p.labels[row] : -1;
   const bool has = lab64 >= 0 && lab64 < p.V;
   E* const out = p.dz ? (E*)p.dz + row * p.lddz : nullptr;
   RV r;
   r.init((const E*)p.z + row * p.ldz, p.V);
   const bool same = out && (((size_t)out ^ (size_t)r.p) & 15) == 0;
-  auto put = [&](int j, typename RV::V v) __attribute__((always_inline)) {
-    if (same && j >= 0 && j + RV::N <= p.V) {
-      *(typename RV::V*)(out + j) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < RV::N; ++e)
-        if (j + e >= 0 && j + e < p.V) out[j + e] = v[e];
-    }
-  };
-  if (p.labels && !has) {                  // an ignored row: never read, zero gradient
+  ns_u4v* const obody = (ns_u4v*)(out + r.head);
+  const bool dead = p.labels && !has;      // an ignored row: its logits are not read, its gradient is zero
+  if (dead) {
     if (tid == 0) p.row_loss[row] = 0.f;
     if (out) {
-      typename RV::V zero;
-#pragma unroll
-      for (int e = 0; e < RV::N; ++e) zero[e] = (E)0.f;
-      for (int c = tid; c < r.chunks; c += NT) put(c * RV::N - r.sh, zero);
+      if (same) {
+        for (int c = tid; c < r.chunks; c += NT) obody[c] = ns_u4v{0, 0, 0, 0};
+        if (r.extra_j >= 0) out[r.extra_j] = (E)0.f;
+      } else {
+        for (int j = tid; j < p.V; j += NT) out[j] = (E)0.f;
+      }
+    }
+    if (!(p.count_here && row == 0)) return;
+  }
+  int live = 0;
+  if (p.count_here)
+    for (int i = tid; i < p.rows; i += NT) live += !p.labels || (p.labels[i] >= 0 && p.labels[i] < p.V);
+  if (dead) {                              // (row 0 alone: it writes the count)
+    live = wave_sum_int(live);
+    if (lane == 0) shc[wave] = live;
+    __syncthreads();
+    if (tid == 0) {
+      int n = 0;
+      for (int w = 0; w < NW; ++w) n += shc[w];
+      *p.nvalid = n;
     }
     return;
   }
@@ -168,61 +183,92 @@ __global__ __launch_bounds__(NT) void distill_kernel(const DistillArgs p) {
     if (e < p.k) sp[e] = ok ? p.tv[row * p.ldt + e] / p.T : -INFINITY;
   }
   const float c1 = p.soft_only ? LOG2E / p.T : LOG2E, c2 = LOG2E / p.T;
+  // every wave's maximum and sums relative to it, joined over the workgroup
   float mx = -INFINITY;
-  r.each([&](int j, typename RV::V v) __attribute__((always_inline)) {
+  r.each([&](int, typename RV::V v) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < RV::N; ++e) mx = fmaxf(mx, (float)v[e]);
   });
-  mx = block_max<NT>(mx, sh);
+  mx = ns_wave_max(fmaxf(mx, r.extra));
   float s1 = 0.f, s2 = 0.f;
-  r.each([&](int j, typename RV::V v) __attribute__((always_inline)) {
+  {
+    const float m = finite_or_zero(mx);      // (subtracted first: a maximum near the type's lowest value times c would overflow)
+    auto add = [&](float x) __attribute__((always_inline)) {
+      s1 += __builtin_amdgcn_exp2f((x - m) * c1);
+      if (DUAL) s2 += __builtin_amdgcn_exp2f((x - m) * c2);
+    };
+    r.each([&](int, typename RV::V v) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < RV::N; ++e) {
-      const float x = (float)v[e] - mx;
-      s1 += __builtin_amdgcn_exp2f(x * c1);
-      if (p.dual) s2 += __builtin_amdgcn_exp2f(x * c2);
-    }
-  });
-  s1 = block_sum<NT>(s1, sh);
-  if (p.dual) s2 = block_sum<NT>(s2, sh);
-  // the teacher's distribution and the row's loss
-  float tm = -INFINITY;
-  for (int e = tid; e < p.k; e += NT) tm = fmaxf(tm, sp[e]);
-  tm = block_max<NT>(tm, sh);
-  const bool soft = tm > -INFINITY;        // a list that names no token leaves the hard label alone
-  float ts = 0.f;
-  for (int e = tid; e < p.k; e += NT) ts += soft ? expf(sp[e] - tm) : 0.f;
-  ts = block_sum<NT>(ts, sh);
-  const float lt = logf(ts), its = 1.f / ts, lq = mx / p.T + logf(p.dual ? s2 : s1);
-  float kl = 0.f;
-  for (int e = tid; e < p.k; e += NT) {
-    const float lp = sp[e] - tm;
-    const float pr = soft ? expf(lp) * its : 0.f;
-    if (pr > 0.f) kl += pr * ((lp - lt) - (sz[e] / p.T - lq));
-    sp[e] = pr;
+      for (int e = 0; e < RV::N; ++e) add((float)v[e]);
+    });
+    add(r.extra);
   }
-  kl = block_sum<NT>(kl, sh);              // (also: every sp[] is final)
-  if (tid == 0) {
-    float loss = soft ? p.kd * kl : 0.f;
-    if (!p.soft_only) loss += p.w1 * ((mx - sz[p.k]) + logf(s1));
-    p.row_loss[row] = loss;
+  s1 = ns_wave_sum(s1);
+  if (DUAL) s2 = ns_wave_sum(s2);
+  if (p.count_here) live = wave_sum_int(live);
+  if (lane == 0) { sh[0][wave] = mx; sh[1][wave] = s1; sh[2][wave] = s2; shc[wave] = live; }
+  __syncthreads();                         // also: sz[] has been read from z by everyone who reads it
+  const int ent = lane & (NW - 1);
+  const float wm = sh[0][ent];
+  mx = max_over_waves<NW>(wm);
+  const float ms = finite_or_zero(mx), dm = wm == -INFINITY ? -INFINITY : finite_or_zero(wm) - ms;      // (a wave without elements, or of -inf: no part)
+  s1 = over_waves<NW>(sh[1][ent] * __builtin_amdgcn_exp2f(dm * c1));
+  if (DUAL) s2 = over_waves<NW>(sh[2][ent] * __builtin_amdgcn_exp2f(dm * c2));
+  live = over_waves<NW>(shc[ent]);
+  if (p.count_here) { if (row == 0 && tid == 0) *p.nvalid = live; }
+  else live = *p.nvalid;
+  // the teacher's distribution: every wave forms its maximum, the first one the row's loss and the probabilities
+  float tm = -INFINITY;
+  for (int e = lane; e < p.k; e += 64) tm = fmaxf(tm, sp[e]);
+  tm = ns_wave_max(tm);
+  const bool soft = tm > -INFINITY;        // a list that names no token leaves the hard label alone
+  __syncthreads();                         // every wave has read sp[] before the first one turns it into probabilities
+  if (wave == 0) {
+    float ts = 0.f;
+    for (int e = lane; e < p.k; e += 64) ts += soft ? expf(sp[e] - tm) : 0.f;
+    ts = ns_wave_sum(ts);
+    const float lt = logf(ts), its = 1.f / ts, lq = ms / p.T + logf(DUAL ? s2 : s1);
+    float kl = 0.f;
+    for (int e = lane; e < p.k; e += 64) {
+      const float lp = sp[e] - tm;
+      const float pr = soft ? expf(lp) * its : 0.f;
+      if (pr > 0.f) kl += pr * ((lp - lt) - (sz[e] / p.T - lq));
+      sp[e] = pr;
+    }
+    kl = ns_wave_sum(kl);
+    if (lane == 0) {
+      float loss = soft ? p.kd * kl : 0.f;
+      if (!p.soft_only) loss += p.w1 * ((ms - sz[p.k]) + logf(s1));
+      p.row_loss[row] = loss;
+    }
   }
   if (!out) return;
-  const float gs = (p.loss_scale ? *p.loss_scale : 1.f) / (float)max(*p.nvalid, 1);
+  // the gradient's weights ride in the exponents: g w 2^((z - m) c) / s = 2^((z - m) c - (log2 s - log2(g w))); a weight of zero is an exponent of -inf
+  const float gs = (p.loss_scale ? *p.loss_scale : 1.f) / (float)max(live, 1);
   const float w2 = soft ? p.w2 : 0.f;
-  const float f1 = (p.dual ? p.w1 : (p.soft_only ? 0.f : p.w1) + w2) / s1, f2 = p.dual ? w2 / s2 : 0.f;
-  __syncthreads();                         // sz[] has been read from z by everyone who reads it; dz may be z itself
+  const float f1 = fabsf(gs) * (DUAL ? p.w1 : (p.soft_only ? 0.f : p.w1) + w2), f2 = fabsf(gs) * w2;
+  const float a1 = log2f(s1) - log2f(f1), a2 = DUAL ? log2f(s2) - log2f(f2) : 0.f;
+  const float sign = gs < 0.f ? -1.f : 1.f;
   auto grad = [&](float z) __attribute__((always_inline)) {
-    float g = f1 * __builtin_amdgcn_exp2f((z - mx) * c1);
-    if (p.dual) g += f2 * __builtin_amdgcn_exp2f((z - mx) * c2);
-    return g;
+    const float x = z - ms;
+    float g = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c1, -a1));
+    if (DUAL) g += __builtin_amdgcn_exp2f(__builtin_fmaf(x, c2, -a2));
+    return g * sign;
   };
-  r.each([&](int j, typename RV::V v) __attribute__((always_inline)) {
-    typename RV::V o;
+  if (same) {
+    r.each([&](int c, typename RV::V v) __attribute__((always_inline)) {
+      typename RV::V o;
 #pragma unroll
-    for (int e = 0; e < RV::N; ++e) o[e] = (E)(grad((float)v[e]) * gs);
-    put(j, o);
-  });
+      for (int e = 0; e < RV::N; ++e) o[e] = (E)grad((float)v[e]);
+      obody[c] = __builtin_bit_cast(ns_u4v, o);
+    });
+  } else {
+    r.again([&](int c, typename RV::V v) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < RV::N; ++e) out[r.head + c * RV::N + e] = (E)grad((float)v[e]);
+    });
+  }
+  if (r.extra_j >= 0) out[r.extra_j] = (E)grad(r.extra);
   // the sparse cells, each token once whatever number of entries name it, behind the dense stores
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -234,95 +280,136 @@ __global__ __launch_bounds__(NT) void distill_kernel(const DistillArgs p) {
     for (int o = 0; o < p.k; ++o)
       if (sidx[o] == t) { q += sp[o]; first = first && o >= e; }
     if (!first) continue;
-    float g = grad(sz[e]) - w2 * q;
-    if (has && t == (int)lab64) g -= p.w1;
-    out[t] = (E)(g * gs);
+    float g = grad(sz[e]) - gs * w2 * q;
+    if (has && t == (int)lab64) g -= gs * p.w1;
+    out[t] = (E)g;
   }
 }
 
 // ------------------------------------------------------------------------------------------------ the teacher
-// The k largest of a row: (1) every thread's largest element; (2) the k-th largest of those, rounded down to its 16 leading bits, is a bound
-// that at least k elements reach and, unless many elements are equal or one thread's chunks hold many of the largest, not many more; (3) the elements that
-// reach it are collected and ordered by (value, lowest token first).  If more than CAP reach it, the k-th largest value itself is found bit by bit, then
-// the token below which enough elements EQUAL to it lie: exactly k elements remain.  A NaN ranks above +inf.
-template <class E> __device__ __forceinline__ uint32_t order_key(E x) {
-  const float f = (float)x + 0.f;                             // -0 ranks as +0
+// The k largest of a row.  Every thread's largest element is put into one of BINS equal bins between the smallest and the largest of those; the bin
+// that the k-th largest of them falls into is a bound that at least k elements reach and few more: the elements in that bin or above it are collected
+// (only in chunks whose own maximum reaches it) and ordered by (value, lowest token first).  If more than CAP reach it -- rows of equal values -- or
+// the row holds an infinity or a NaN, the k-th largest value is found bit by bit over all elements, then the token below which enough elements EQUAL to it
+// lie: exactly k remain.  A NaN ranks above +inf.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const float f = x + 0.f;                             // -0 ranks as +0
   const uint32_t u = __float_as_uint(f);
   if (f != f) return 0xFFFFFFFFu;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
 template <class E, int NC, int NT>
-__global__ __launch_bounds__(NT) void topk_row_kernel(const E* __restrict__ z, int64_t ldz, int V, int k, float* __restrict__ vals, int32_t* __restrict__ idx,
-                                                      int64_t ldo, float* __restrict__ lse) {
-  constexpr int CAP = 2048;
+__global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void topk_row_kernel(const E* __restrict__ z, int64_t ldz, int V, int k,
+                                                                                              float* __restrict__ vals, int32_t* __restrict__ idx,
+                                                                                              int64_t ldo, float* __restrict__ lse) {
+  constexpr int CAP = 1024, BINS = 256, NW = NT / 64;
   __shared__ uint64_t cand[CAP];
-  __shared__ int shi[16];
-  __shared__ float sh[16];
-  __shared__ int count;
+  __shared__ int hist[BINS];
+  __shared__ int shi[NW];
+  __shared__ float sh[3][NW];
+  __shared__ int count, bound_bin;
   typedef row_view<E, NC, NT> RV;
-  const int row = blockIdx.x, tid = threadIdx.x;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   RV r;
   r.init(z + row * ldz, V);
   r.load();
-  uint32_t best = 0;                                          // below every element's key
-  float mx = -INFINITY;
-  r.each([&](int j, typename RV::V v) __attribute__((always_inline)) {
-#pragma unroll
-    for (int e = 0; e < RV::N; ++e)
-      if (j + e >= 0 && j + e < V) { mx = fmaxf(mx, (float)v[e]); best = max(best, order_key(v[e])); }
-  });
-  if (lse) {
-    const float m = block_max<NT>(mx, sh);
-    float s = 0.f;
-    const float ms = fabsf(m) == INFINITY ? 0.f : m;          // (an infinite maximum is the answer: the sum becomes 0 or infinite)
-    r.each([&](int j, typename RV::V v) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < RV::N; ++e) s += __builtin_amdgcn_exp2f(((float)v[e] - ms) * LOG2E);
-    });
-    s = block_sum<NT>(s, sh);
-    if (tid == 0) lse[row] = ms + logf(s);
-  }
-  // (2) the bound: leading 16 bits of the k-th largest thread maximum (0, i.e. everything, when fewer threads hold elements)
-  uint32_t bound = 0;
-  for (int b = 31; b >= 16; --b) {
-    const uint32_t t = bound | (1u << b);
-    if (block_count<NT>(best >= t, shi) >= k) bound = t;
-  }
+  for (int b = tid; b < BINS; b += NT) hist[b] = 0;
   if (tid == 0) count = 0;
-  __syncthreads();
-  auto collect = [&](auto take) __attribute__((always_inline)) {
-    r.each([&](int j, typename RV::V v) __attribute__((always_inline)) {
+  const bool some = tid < r.chunks || r.extra_j >= 0;         // this thread holds elements
+  float mx = -INFINITY;
+  r.each([&](int, typename RV::V v) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < RV::N; ++e) {
-        if (j + e < 0 || j + e >= V) continue;
-        const uint32_t key = order_key(v[e]);
-        if (!take(key, j + e)) continue;
-        const int at = atomicAdd(&count, 1);
-        if (at < CAP) cand[at] = ((uint64_t)key << 32) | (uint32_t)~(j + e);
+    for (int e = 0; e < RV::N; ++e) mx = fmaxf(mx, (float)v[e]);
+  });
+  mx = fmaxf(mx, r.extra);
+  const float wmx = ns_wave_max(mx);
+  const float wmn = -ns_wave_max(some ? -mx : -INFINITY);
+  float s = 0.f;
+  {
+    const float m = finite_or_zero(wmx);
+    r.each([&](int, typename RV::V v) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < RV::N; ++e) s += __builtin_amdgcn_exp2f(((float)v[e] - m) * LOG2E);
+    });
+    s += __builtin_amdgcn_exp2f((r.extra - m) * LOG2E);
+    s = ns_wave_sum(s);
+  }
+  if (lane == 0) { sh[0][wave] = wmx; sh[1][wave] = wmn; sh[2][wave] = s; }
+  __syncthreads();
+  const int ent = lane & (NW - 1);
+  const float wm = sh[0][ent];
+  const float hi = max_over_waves<NW>(wm), lo = -max_over_waves<NW>(-sh[1][ent]);
+  const float ms = finite_or_zero(hi);
+  s = over_waves<NW>(sh[2][ent] * (wm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((finite_or_zero(wm) - ms) * LOG2E)));
+  if (lse && tid == 0) lse[row] = ms + logf(s);
+  // a bin is a monotone function of the value: rounding keeps the order.  (hi == lo: one bin.)
+  const bool plain = s == s && fabsf(hi) < INFINITY && fabsf(lo) < INFINITY;
+  const float scale = hi > lo ? (float)(BINS - 1) / (hi - lo) : 0.f;
+  auto bin = [&](float x) __attribute__((always_inline)) { return x >= lo ? min((int)((x - lo) * scale), BINS - 1) : -1; };
+  int n = CAP + 1;
+  if (plain && scale < INFINITY) {
+    if (some) atomicAdd(&hist[bin(mx)], 1);
+    __syncthreads();
+    if (wave == 0) {                                          // the highest bin that, with those above it, holds k thread maxima (-1: fewer than k threads)
+      int own[4], sum = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) { own[b] = hist[lane * 4 + b]; sum += own[b]; }
+      int above = 0;                                          // in the bins of higher lanes
+      int run = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_down(run, o, 64);
+        run += lane + o < 64 ? t : 0;
+      }
+      above = run - sum;
+      int at = -1;
+#pragma unroll
+      for (int b = 3; b >= 0; --b) {
+        above += own[b];
+        if (at < 0 && above >= k) at = lane * 4 + b;
+      }
+      at = (int)ns_wave_max((float)at);
+      if (lane == 0) bound_bin = at;
+    }
+    __syncthreads();
+    const int bb = bound_bin;
+    auto offer = [&](float x, int at) __attribute__((always_inline)) {
+      if (bin(x) < bb) return;
+      const int to = atomicAdd(&count, 1);
+      if (to < CAP) cand[to] = ((uint64_t)order_key(x) << 32) | (uint32_t)~at;
+    };
+    r.each([&](int c, typename RV::V v) __attribute__((always_inline)) {
+      float cm = (float)v[0];
+#pragma unroll
+      for (int e = 1; e < RV::N; ++e) cm = fmaxf(cm, (float)v[e]);
+      if (bin(cm) >= bb) {
+#pragma unroll
+        for (int e = 0; e < RV::N; ++e) offer((float)v[e], r.head + c * RV::N + e);
       }
     });
-  };
-  collect([&](uint32_t key, int) { return key >= bound; });
-  __syncthreads();
-  int n = count;
+    if (r.extra_j >= 0) offer(r.extra, r.extra_j);
+    __syncthreads();
+    n = count;
+  }
   if (n > CAP) {
     auto reach = [&](auto take) __attribute__((always_inline)) {
-      int c = 0;
-      r.each([&](int j, typename RV::V v) __attribute__((always_inline)) {
+      int c = r.extra_j >= 0 && take(order_key(r.extra), r.extra_j) ? 1 : 0;
+      r.again([&](int at, typename RV::V v) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < RV::N; ++e)
-          if (j + e >= 0 && j + e < V) c += take(order_key(v[e]), j + e);
+        for (int e = 0; e < RV::N; ++e) c += take(order_key((float)v[e]), r.head + at * RV::N + e);
       });
       return block_count<NT>(c, shi);
     };
     uint32_t kth = 0;
+#pragma unroll 1
     for (int b = 31; b >= 0; --b) {
       const uint32_t t = kth | (1u << b);
       if (reach([&](uint32_t key, int) { return key >= t; }) >= k) kth = t;
     }
     const int more = reach([&](uint32_t key, int) { return key > kth; });
     int upto = 0;                                             // the largest bound below which fewer than k - more equal elements lie
+#pragma unroll 1
     for (int b = 30; b >= 0; --b) {
       const int t = upto | (1 << b);
       if (reach([&](uint32_t key, int at) { return key == kth && at < t; }) < k - more) upto = t;
@@ -330,16 +417,28 @@ __global__ __launch_bounds__(NT) void topk_row_kernel(const E* __restrict__ z, i
     __syncthreads();
     if (tid == 0) count = 0;
     __syncthreads();
-    collect([&](uint32_t key, int at) { return key > kth || (key == kth && at <= upto); });
+    auto keep = [&](float x, int at) __attribute__((always_inline)) {
+      const uint32_t key = order_key(x);
+      if (key > kth || (key == kth && at <= upto)) cand[atomicAdd(&count, 1)] = ((uint64_t)key << 32) | (uint32_t)~at;
+    };
+    r.again([&](int c, typename RV::V v) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < RV::N; ++e) keep((float)v[e], r.head + c * RV::N + e);
+    });
+    if (r.extra_j >= 0) keep(r.extra, r.extra_j);
     __syncthreads();
-    n = count;
+    n = count;                                                // exactly k
   }
-  // (3) each candidate's place is the number of candidates above it
-  for (int c = tid; c < n; c += NT) {
+  // each candidate's place is the number of candidates above it: eight lanes a candidate
+  const int sub = tid & 7;
+  for (int c = tid >> 3; c < n; c += NT / 8) {
     const uint64_t me = cand[c];
     int above = 0;
-    for (int o = 0; o < n; ++o) above += cand[o] > me;
-    if (above < k) {
+    for (int o = sub; o < n; o += 8) above += cand[o] > me;
+    above += __shfl_xor(above, 1, 64);
+    above += __shfl_xor(above, 2, 64);
+    above += __shfl_xor(above, 4, 64);
+    if (sub == 0 && above < k) {
       const int t = (int)~(uint32_t)me;
       vals[row * ldo + above] = (float)r.p[t];
       idx[row * ldo + above] = t;
@@ -349,19 +448,25 @@ __global__ __launch_bounds__(NT) void topk_row_kernel(const E* __restrict__ z, i
 
 template <class E, template <class, int, int> class Launch, class... A>
 void by_length(int V, A... a) {
-  // threads and registers by the row's length: one access per thread up to 256 accesses, then 1024 threads with as many as the row needs
-  const int chunks = V / vec<E>::N + 2;
-  constexpr int F = sizeof(E) == 4 ? 2 : 1;      // an access holds half as many fp32 elements: twice the accesses cover the same rows
+  // threads and registers by the row's length: one or two accesses a thread on 256 threads, then 1024 threads with as many as the row needs; up to seven
+  // (28 registers) two workgroups share a CU, so that one loads while the other computes
+  const int chunks = V / vec<E>::N;
   if (chunks <= 256) Launch<E, 1, 256>::go(a...);
   else if (chunks <= 512) Launch<E, 2, 256>::go(a...);
-  else if (chunks <= 1024 * 2) Launch<E, 2, 1024>::go(a...);
-  else if (chunks <= 1024 * 4 * F) Launch<E, 4 * F, 1024>::go(a...);
-  else if (chunks <= 1024 * 8 * F) Launch<E, 8 * F, 1024>::go(a...);
+  else if (chunks <= 2 * 1024) Launch<E, 2, 1024>::go(a...);
+  else if (chunks <= 4 * 1024) Launch<E, 4, 1024>::go(a...);
+  else if (chunks <= 7 * 1024) Launch<E, 7, 1024>::go(a...);
+  else if (sizeof(E) == 4 && chunks <= 14 * 1024) Launch<E, sizeof(E) == 4 ? 14 : 0, 1024>::go(a...);
   else Launch<E, 0, 1024>::go(a...);
 }
 
 template <class E, int NC, int NT> struct distill_go {
-  static void go(const DistillArgs& a, int rows, hipStream_t st) { hipLaunchKernelGGL((distill_kernel<E, NC, NT>), dim3(rows), dim3(NT), 0, st, a); }
+  static void go(DistillArgs a, bool dual, hipStream_t st) {
+    a.count_here = a.rows <= DT_COUNT_HERE * NT;
+    if (!a.count_here) hipLaunchKernelGGL(dt_count_kernel, dim3(1), dim3(1024), 0, st, a.labels, a.rows, a.V, a.nvalid);
+    if (dual) hipLaunchKernelGGL((distill_kernel<E, NC, NT, true>), dim3(a.rows), dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((distill_kernel<E, NC, NT, false>), dim3(a.rows), dim3(NT), 0, st, a);
+  }
 };
 template <class E, int NC, int NT> struct topk_go {
   static void go(const ns_topk_desc* d, hipStream_t st) {
@@ -385,17 +490,18 @@ extern "C" int ns_distill_topk(const ns_distill_desc* d, void* stream) {
                (double)d->temperature, (double)d->alpha);
   NS_CHECK_ARG(d->labels || d->alpha == 1.f || d->rows == 0, "ns_distill_topk: alpha %g < 1 needs labels", (double)d->alpha);
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(dt_count_kernel, dim3(1), dim3(1024), 0, st, d->labels, d->rows, d->vocab, d->nvalid_dev);
   if (d->rows > 0) {
     DistillArgs a = {};
-    a.z = d->logits; a.ldz = d->ldz; a.labels = d->labels; a.tv = d->top_vals; a.ti = d->top_idx; a.ldt = d->ld_top; a.V = d->vocab; a.k = d->k;
+    a.z = d->logits; a.ldz = d->ldz; a.labels = d->labels; a.tv = d->top_vals; a.ti = d->top_idx; a.ldt = d->ld_top; a.rows = d->rows; a.V = d->vocab; a.k = d->k;
     a.soft_only = d->alpha == 1.f;
-    a.dual = !a.soft_only && d->temperature != 1.f;
+    const bool dual = !a.soft_only && d->temperature != 1.f;
     a.T = d->temperature; a.w1 = 1.f - d->alpha; a.w2 = d->alpha * d->temperature; a.kd = d->alpha * d->temperature * d->temperature;
     a.row_loss = d->row_loss; a.dz = d->dlogits; a.lddz = d->lddz; a.nvalid = d->nvalid_dev; a.loss_scale = d->loss_scale_dev;
-    if (d->dtype == NS_F16) by_length<half_t, distill_go>(d->vocab, a, d->rows, st);
-    else if (d->dtype == NS_BF16) by_length<__bf16, distill_go>(d->vocab, a, d->rows, st);
-    else by_length<float, distill_go>(d->vocab, a, d->rows, st);
+    if (d->dtype == NS_F16) by_length<half_t, distill_go>(d->vocab, a, dual, st);
+    else if (d->dtype == NS_BF16) by_length<__bf16, distill_go>(d->vocab, a, dual, st);
+    else by_length<float, distill_go>(d->vocab, a, dual, st);
+  } else {
+    hipLaunchKernelGGL(dt_count_kernel, dim3(1), dim3(1024), 0, st, d->labels, 0, d->vocab, d->nvalid_dev);
   }
   hipLaunchKernelGGL(dt_mean_kernel, dim3(1), dim3(1024), 0, st, d->row_loss, d->rows, d->nvalid_dev, d->loss_dev);
   NS_CHECK_LAUNCH("ns_distill_topk");
