@@ -332,110 +332,140 @@ def cross_entropy(logits16, labels, rows, V, ldv, row_loss, dlogits16, nvalid_de
 
 
 # ---- losses over the vocabulary.  Shapes and types come from the tensors; what the kernels cannot take is refused here with a ValueError.
+# (These calls take ~10 us of GPU time at the small end: messages are only formatted when something is refused, attributes read once.)
 _DTYPES = {torch.float16: L.NS_F16, torch.bfloat16: L.NS_BF16, torch.float32: L.NS_F32}
+_HALF_TYPES = (torch.float16, torch.bfloat16)
+_F32_ONLY, _I32_ONLY = (torch.float32,), (torch.int32,)
 
 
-def _need(ok, what: str):
-    if not ok:
-        raise ValueError(what)
-
-
-def _matrix(name, t, rows=None, cols=None, dtypes=None) -> int:
-    """row stride (elements) of a 2-D tensor with unit column stride"""
-    _need(isinstance(t, torch.Tensor) and t.dim() == 2, f"{name}: a 2-D tensor")
-    _need((rows is None or t.shape[0] == rows) and (cols is None or t.shape[1] == cols),
-          f"{name}: shape {tuple(t.shape)}, expected ({'any' if rows is None else rows}, {'any' if cols is None else cols})")
-    _need(dtypes is None or t.dtype in dtypes, f"{name}: dtype {t.dtype}, expected one of {dtypes}")
-    _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{name}: columns must be contiguous (strides {t.stride()})")
-    _need(t.shape[0] <= 1 or t.stride(0) >= t.shape[1], f"{name}: rows overlap (strides {t.stride()})")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _matrix(name, t, rows, cols, dtypes):
+    """(rows, columns, row stride in elements) of a 2-D tensor with unit column stride; rows / cols: what they have to be (None: any)"""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise ValueError(f"{name}: a 2-D tensor")
+    n, m = t.shape
+    if (rows is not None and n != rows) or (cols is not None and m != cols):
+        raise ValueError(f"{name}: shape {(n, m)}, expected ({'any' if rows is None else rows}, {'any' if cols is None else cols})")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: dtype {t.dtype}, expected one of {tuple(dtypes)}")
+    ld, one = t.stride()
+    if m > 1 and one != 1:
+        raise ValueError(f"{name}: columns must be contiguous (strides {t.stride()})")
+    if n <= 1:
+        return n, m, m
+    if ld < m:
+        raise ValueError(f"{name}: rows overlap (strides {t.stride()})")
+    return n, m, ld
 
 
 def _vector(name, t, n, dtype):
-    _need(isinstance(t, torch.Tensor) and t.dtype == dtype and t.numel() == n and t.is_contiguous(), f"{name}: a contiguous tensor of {n} {dtype}")
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.numel() == n and t.is_contiguous()):
+        raise ValueError(f"{name}: a contiguous tensor of {n} {dtype}")
+    return t.data_ptr()
 
 
-def _span(t):
-    """[first, last) byte address that a tensor's elements occupy"""
-    if t.numel() == 0:
-        return (0, 0)
-    return (t.data_ptr(), t.data_ptr() + (sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1) * t.element_size())
+def _apart(name, a, na, *others):
+    """[a, a + na) bytes against (what, first byte, bytes) of the others"""
+    for what, b, nb in others:
+        if na > 0 and nb > 0 and a < b + nb and b < a + na:
+            raise ValueError(f"{name} overlaps {what}")
 
 
-def _apart(name, out, *ins):
-    a = _span(out)
-    for what, t in ins:
-        b = _span(t)
-        _need(a[1] <= b[0] or b[1] <= a[0], f"{name} overlaps {what}")
+def _extent(n, m, ld, size):
+    return ((n - 1) * ld + m) * size if n > 0 and m > 0 else 0
 
 
-def _on_one_gpu(*named):
+def _one_gpu(*tensors) -> int:
+    """ordinal of the GPU that all of them are on; None entries are skipped"""
     dev = None
-    for name, t in named:
-        if t is None:
-            continue
-        _need(t.is_cuda, f"{name}: on {t.device}, expected a GPU")
-        dev = t.device if dev is None else dev
-        _need(t.device == dev, f"{name}: on {t.device}, the others are on {dev}")
+    for t in tensors:
+        if t is not None:
+            d = t.get_device()
+            if d != dev:
+                if d < 0:
+                    raise ValueError(f"a tensor is on {t.device}, expected a GPU")
+                if dev is not None:
+                    raise ValueError(f"a tensor is on {t.device}, the others are on cuda:{dev}")
+                dev = d
     return dev
 
 
-def _targets(rows, vocab, labels, row_loss, loss, nvalid, loss_scale, top_vals, top_idx, temperature, alpha):
-    """the arguments that both losses share -> k, row stride of the teacher's list"""
+def _call_on(dev: int, name, d):
+    """launch on the current stream of GPU `dev`, whatever device is current"""
+    if dev == torch.cuda.current_device():
+        _call(name, C.byref(d))
+    else:
+        with torch.cuda.device(dev):
+            _call(name, C.byref(d))
+
+
+def _targets(d, rows, labels, row_loss, loss, nvalid, loss_scale, top_vals, top_idx, temperature, alpha):
+    """the arguments that both losses share, checked and written into the descriptor"""
     if labels is not None:
-        _vector("labels", labels, rows, torch.int64)
-    _vector("row_loss", row_loss, rows, torch.float32)
-    _vector("loss", loss, 1, torch.float32)
-    _vector("nvalid", nvalid, 1, torch.int32)
+        d.labels = _vector("labels", labels, rows, torch.int64)
+    d.row_loss = _vector("row_loss", row_loss, rows, torch.float32)
+    d.loss_dev = _vector("loss", loss, 1, torch.float32)
+    d.nvalid_dev = _vector("nvalid", nvalid, 1, torch.int32)
     if loss_scale is not None:
-        _vector("loss_scale", loss_scale, 1, torch.float32)
+        d.loss_scale_dev = _vector("loss_scale", loss_scale, 1, torch.float32)
+    d.rows, d.temperature, d.alpha = rows, temperature, alpha
     if top_vals is None and top_idx is None:
-        _need(alpha == 0.0, f"alpha {alpha}: soft targets need top_vals and top_idx")
-        return 0, 0
-    _need(top_vals is not None and top_idx is not None, "top_vals and top_idx come together")
-    lt = _matrix("top_vals", top_vals, rows, None, (torch.float32,))
-    k = top_vals.shape[1]
-    li = _matrix("top_idx", top_idx, rows, k, (torch.int32,))
-    _need(rows <= 1 or lt == li, f"top_vals and top_idx: different row strides ({lt}, {li})")
-    _need(1 <= k <= 256, f"top_vals: {k} entries a row, 1 to 256 are supported")
-    _need(1e-3 <= temperature <= 1e3, f"temperature {temperature}: expected 1e-3 to 1e3")
-    _need(0.0 <= alpha <= 1.0, f"alpha {alpha}: expected 0 to 1")
-    return k, lt
+        if alpha != 0.0:
+            raise ValueError(f"alpha {alpha}: soft targets need top_vals and top_idx")
+        return
+    if top_vals is None or top_idx is None:
+        raise ValueError("top_vals and top_idx come together")
+    _, k, ld = _matrix("top_vals", top_vals, rows, None, _F32_ONLY)
+    _, _, li = _matrix("top_idx", top_idx, rows, k, _I32_ONLY)
+    if ld != li:
+        raise ValueError(f"top_vals and top_idx: different row strides ({ld}, {li})")
+    if not 1 <= k <= 256:
+        raise ValueError(f"top_vals: {k} entries a row, 1 to 256 are supported")
+    if not 1e-3 <= temperature <= 1e3:
+        raise ValueError(f"temperature {temperature}: expected 1e-3 to 1e3")
+    if not 0.0 <= alpha <= 1.0:
+        raise ValueError(f"alpha {alpha}: expected 0 to 1")
+    d.k, d.ld_top, d.top_vals, d.top_idx = k, ld, top_vals.data_ptr(), top_idx.data_ptr()
+
+
+def _head_operand(name, t, rows, cols, dtypes):
+    n, m, ld = _matrix(name, t, rows, cols, dtypes)
+    if m % 8 or not 8 <= m <= 1 << 16:
+        raise ValueError(f"{name}: {m} columns, a multiple of 8 up to 65536 is supported")
+    at = t.data_ptr()
+    if ld % 8 or ld >= 1 << 21 or at % 16:
+        raise ValueError(f"{name}: rows must start on 16 bytes (row stride {ld} elements, below {1 << 21})")
+    return n, m, ld, at
 
 
 def _linear_ce_desc(h, weight, labels, row_loss, loss, nvalid, dh, dweight, loss_scale, top_vals, top_idx, temperature, alpha, accumulate):
     d = L.LinearCeDesc()
-    ldh = _matrix("h", h, None, None, (torch.float16, torch.bfloat16))
-    rows, width = h.shape
-    ldw = _matrix("weight", weight, None, width, (h.dtype,))
-    vocab = weight.shape[0]
-    _need(vocab >= 1, "weight: no rows")
-    _need(width >= 8 and width % 8 == 0 and width <= 1 << 16, f"h: {width} columns, a multiple of 8 up to 65536 is supported")
-    _need(rows <= 1 << 21, f"h: {rows} rows, up to {1 << 21} are supported")
-    k, ldt = _targets(rows, vocab, labels, row_loss, loss, nvalid, loss_scale, top_vals, top_idx, temperature, alpha)
-    for name, t, ld in (("h", h, ldh), ("weight", weight, ldw)):
-        _need(ld % 8 == 0 and ld < 1 << 21 and t.data_ptr() % 16 == 0, f"{name}: rows must start on 16 bytes (row stride {ld} elements, below {1 << 21})")
-    d.ldh, d.ldw, d.ld_top = ldh, ldw, ldt
-    if dh is not None:
-        d.lddh = _matrix("dh", dh, rows, width, (h.dtype,))
-        _need(d.lddh % 8 == 0 and d.lddh < 1 << 21 and dh.data_ptr() % 16 == 0, f"dh: rows must start on 16 bytes (row stride {d.lddh} elements)")
-        _apart("dh", dh, ("h", h), ("weight", weight))
-    if dweight is not None:
-        d.lddw = _matrix("dweight", dweight, vocab, width, (h.dtype, torch.float32))
-        _need(d.lddw % 8 == 0 and d.lddw < 1 << 21 and dweight.data_ptr() % 16 == 0, f"dweight: rows must start on 16 bytes (row stride {d.lddw} elements)")
-        _apart("dweight", dweight, ("h", h), ("weight", weight))
+    rows, width, d.ldh, d.h = _head_operand("h", h, None, None, _HALF_TYPES)
+    dtype = h.dtype
+    vocab, _, d.ldw, d.w = _head_operand("weight", weight, None, width, (dtype,))
+    if vocab < 1:
+        raise ValueError("weight: no rows")
+    if rows > 1 << 21:
+        raise ValueError(f"h: {rows} rows, up to {1 << 21} are supported")
+    if labels is None:
+        raise ValueError("labels: a tensor, -100 for a row that does not count")
+    d.vocab, d.d, d.dtype = vocab, width, _DTYPES[dtype]
+    _targets(d, rows, labels, row_loss, loss, nvalid, loss_scale, top_vals, top_idx, temperature, alpha)
+    if dh is not None or dweight is not None:
+        taken = (("h", d.h, _extent(rows, width, d.ldh, 2)), ("weight", d.w, _extent(vocab, width, d.ldw, 2)))
         if dh is not None:
-            _apart("dweight", dweight, ("dh", dh))
-        d.dw_f32 = int(dweight.dtype == torch.float32)
-    _need(not accumulate or (dweight is not None and d.dw_f32), "accumulate: adds to a float32 dweight only")
-    d.dw_add = int(accumulate)
-    d.h, d.w, d.labels, d.top_vals, d.top_idx = ptr(h), ptr(weight), ptr(labels), ptr(top_vals), ptr(top_idx)
-    d.row_loss, d.loss_dev, d.nvalid_dev, d.loss_scale_dev = ptr(row_loss), ptr(loss), ptr(nvalid), ptr(loss_scale)
-    d.dh, d.dw = ptr(dh), ptr(dweight)
-    if rows == 0 and dh is not None:
-        d.dh = 0                                  # nothing to write
-    d.rows, d.vocab, d.d, d.k, d.dtype = rows, vocab, width, k, _DTYPES[h.dtype]
-    d.temperature, d.alpha = temperature, alpha
+            _, _, d.lddh, at = _head_operand("dh", dh, rows, width, (dtype,))
+            size = _extent(rows, width, d.lddh, 2)
+            _apart("dh", at, size, *taken)
+            taken += (("dh", at, size),)
+            d.dh = at if rows else 0              # (no rows: nothing to write)
+        if dweight is not None:
+            _, _, d.lddw, d.dw = _head_operand("dweight", dweight, vocab, width, (dtype, torch.float32))
+            d.dw_f32 = int(dweight.dtype == torch.float32)
+            _apart("dweight", d.dw, _extent(vocab, width, d.lddw, 4 if d.dw_f32 else 2), *taken)
+    if accumulate:
+        if dweight is None or not d.dw_f32:
+            raise ValueError("accumulate: adds to a float32 dweight only")
+        d.dw_add = 1
     return d
 
 
@@ -458,21 +488,20 @@ def linear_cross_entropy(h, weight, labels, *, row_loss, loss, nvalid, dh=None, 
     workspace: a uint8 tensor of linear_ce_workspace_bytes(...) (default: allocated for the call, on the current stream).  A captured graph keeps
     the default's memory in its own pool; two graphs that may run at the same time must not share an explicit one."""
     d = _linear_ce_desc(h, weight, labels, row_loss, loss, nvalid, dh, dweight, loss_scale, top_vals, top_idx, float(temperature), float(alpha), accumulate)
-    dev = _on_one_gpu(("h", h), ("weight", weight), ("labels", labels), ("row_loss", row_loss), ("loss", loss), ("nvalid", nvalid), ("dh", dh),
-                      ("dweight", dweight), ("loss_scale", loss_scale), ("top_vals", top_vals), ("top_idx", top_idx), ("workspace", workspace))
-    need = int(L.load().ns_linear_ce_workspace_bytes(C.byref(d)))
+    dev = _one_gpu(h, weight, labels, row_loss, loss, nvalid, dh, dweight, loss_scale, top_vals, top_idx, workspace)
+    need = L.load().ns_linear_ce_workspace_bytes(C.byref(d))
     if workspace is None:
-        _need(getattr(_tls, "rec", None) is None, "a recorded launch list replays raw addresses: pass a workspace that outlives it")
-        workspace = torch.empty(need, device=dev, dtype=torch.uint8)
-    _need(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.numel() >= need and workspace.data_ptr() % 16 == 0,
-          f"workspace: {need} contiguous bytes of uint8 that start on 16 bytes")
+        if getattr(_tls, "rec", None) is not None:
+            raise ValueError("a recorded launch list replays raw addresses: pass a workspace that outlives it")
+        workspace = torch.empty(need, device=h.device, dtype=torch.uint8)
+    elif not (workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.numel() >= need and workspace.data_ptr() % 16 == 0):
+        raise ValueError(f"workspace: {need} contiguous bytes of uint8 that start on 16 bytes")
     d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel()
     if STEP_PROFILE is not None:
         n, v, w = d.rows, d.vocab, d.d
         _work("linear_cross_entropy", 2.0 * n * v * w * (1 + (dh is not None) + (dweight is not None)),
               2.0 * (n * w + v * w) + (2.0 * n * w if dh is not None else 0.0) + ((4.0 if d.dw_f32 else 2.0) * v * w if dweight is not None else 0.0))
-    with torch.cuda.device(dev):
-        _call("ns_linear_cross_entropy", C.byref(d))
+    _call_on(dev, "ns_linear_cross_entropy", d)
 
 
 def distill_topk(logits, labels, top_vals, top_idx, *, row_loss, loss, nvalid, temperature=1.0, alpha=1.0, dlogits=None, loss_scale=None):
@@ -482,24 +511,25 @@ def distill_topk(logits, labels, top_vals, top_idx, *, row_loss, loss, nvalid, t
     logits (rows, vocab) float16, bfloat16 or float32, rows at any stride (a [:, :vocab] view of a padded buffer: the padding is not
     touched); labels as in linear_cross_entropy, or None with alpha = 1: every row counts; top_vals / top_idx (rows, k) float32 / int32, k <= 256."""
     d = L.DistillDesc()
-    d.ldz = _matrix("logits", logits, None, None, tuple(_DTYPES))
-    rows, vocab = logits.shape
-    _need(vocab >= 1, "logits: no columns")
-    _need(labels is not None or alpha == 1.0, f"alpha {alpha}: the hard term needs labels")
-    _need(top_vals is not None and alpha > 0.0, "top_vals, top_idx and alpha > 0: without them this is cross_entropy")
-    d.k, d.ld_top = _targets(rows, vocab, labels, row_loss, loss, nvalid, loss_scale, top_vals, top_idx, temperature, alpha)
+    rows, vocab, d.ldz = _matrix("logits", logits, None, None, _DTYPES)
+    if vocab < 1:
+        raise ValueError("logits: no columns")
+    if labels is None and alpha != 1.0:
+        raise ValueError(f"alpha {alpha}: the hard term needs labels")
+    if top_vals is None or not alpha > 0.0:
+        raise ValueError("top_vals, top_idx and alpha > 0: without them this is cross_entropy")
+    _targets(d, rows, labels, row_loss, loss, nvalid, loss_scale, top_vals, top_idx, float(temperature), float(alpha))
+    d.logits, d.vocab, d.dtype = logits.data_ptr(), vocab, _DTYPES[logits.dtype]
     if dlogits is not None:
-        d.lddz = _matrix("dlogits", dlogits, rows, vocab, (logits.dtype,))
-        if not (dlogits.data_ptr() == logits.data_ptr() and d.lddz == d.ldz):
-            _apart("dlogits", dlogits, ("logits", logits))
-    dev = _on_one_gpu(("logits", logits), ("labels", labels), ("top_vals", top_vals), ("top_idx", top_idx), ("row_loss", row_loss), ("loss", loss),
-                      ("nvalid", nvalid), ("dlogits", dlogits), ("loss_scale", loss_scale))
-    d.logits, d.labels, d.top_vals, d.top_idx = ptr(logits), ptr(labels), ptr(top_vals), ptr(top_idx)
-    d.row_loss, d.loss_dev, d.nvalid_dev, d.loss_scale_dev, d.dlogits = ptr(row_loss), ptr(loss), ptr(nvalid), ptr(loss_scale), ptr(dlogits)
-    d.rows, d.vocab, d.dtype, d.temperature, d.alpha = rows, vocab, _DTYPES[logits.dtype], float(temperature), float(alpha)
-    _work("distill_topk", 0.0, logits.element_size() * rows * vocab * (2.0 if dlogits is not None else 1.0) + 8.0 * rows * d.k)
-    with torch.cuda.device(dev):
-        _call("ns_distill_topk", C.byref(d))
+        _, _, d.lddz = _matrix("dlogits", dlogits, rows, vocab, (logits.dtype,))
+        d.dlogits = dlogits.data_ptr()
+        if d.dlogits != d.logits or d.lddz != d.ldz:
+            size = logits.element_size()
+            _apart("dlogits", d.dlogits, _extent(rows, vocab, d.lddz, size), ("logits", d.logits, _extent(rows, vocab, d.ldz, size)))
+    dev = _one_gpu(logits, labels, top_vals, top_idx, row_loss, loss, nvalid, dlogits, loss_scale)
+    if STEP_PROFILE is not None:
+        _work("distill_topk", 0.0, logits.element_size() * rows * vocab * (2.0 if dlogits is not None else 1.0) + 8.0 * rows * d.k)
+    _call_on(dev, "ns_distill_topk", d)
 
 
 def topk_logits(logits, k, *, vals, idx, lse=None):
@@ -508,23 +538,24 @@ def topk_logits(logits, k, *, vals, idx, lse=None):
     logits (rows, vocab) float16, bfloat16 or float32, rows at any stride; vals (rows, k) float32, idx (rows, k) int32, lse (rows) float32: the
     row's log-sum-exp."""
     d = L.TopkDesc()
-    d.ldz = _matrix("logits", logits, None, None, tuple(_DTYPES))
-    rows, vocab = logits.shape
-    _need(isinstance(k, int) and 1 <= k <= 256 and k <= vocab, f"k {k}: expected 1 to {min(256, vocab)}")
-    d.ldo = _matrix("vals", vals, rows, k, (torch.float32,))
-    ldi = _matrix("idx", idx, rows, k, (torch.int32,))
-    _need(rows <= 1 or ldi == d.ldo, f"vals and idx: different row strides ({d.ldo}, {ldi})")
+    rows, vocab, d.ldz = _matrix("logits", logits, None, None, _DTYPES)
+    if not (isinstance(k, int) and 1 <= k <= 256 and k <= vocab):
+        raise ValueError(f"k {k}: expected 1 to {min(256, vocab)}")
+    _, _, d.ldo = _matrix("vals", vals, rows, k, _F32_ONLY)
+    _, _, ldi = _matrix("idx", idx, rows, k, _I32_ONLY)
+    if ldi != d.ldo:
+        raise ValueError(f"vals and idx: different row strides ({d.ldo}, {ldi})")
     if lse is not None:
-        _vector("lse", lse, rows, torch.float32)
-    dev = _on_one_gpu(("logits", logits), ("vals", vals), ("idx", idx), ("lse", lse))
-    for name, t in (("vals", vals), ("idx", idx), ("lse", lse)):
-        if t is not None:
-            _apart(name, t, ("logits", logits))
-    d.logits, d.vals, d.idx, d.lse = ptr(logits), ptr(vals), ptr(idx), ptr(lse)
+        d.lse = _vector("lse", lse, rows, torch.float32)
+    dev = _one_gpu(logits, vals, idx, lse)
+    d.logits, d.vals, d.idx = logits.data_ptr(), vals.data_ptr(), idx.data_ptr()
+    z = ("logits", d.logits, _extent(rows, vocab, d.ldz, logits.element_size()))
+    _apart("vals", d.vals, _extent(rows, k, d.ldo, 4), z)
+    _apart("idx", d.idx, _extent(rows, k, d.ldo, 4), z)
     d.rows, d.vocab, d.k, d.dtype = rows, vocab, k, _DTYPES[logits.dtype]
-    _work("topk_logits", 0.0, logits.element_size() * rows * vocab + 8.0 * rows * k)
-    with torch.cuda.device(dev):
-        _call("ns_topk_logits", C.byref(d))
+    if STEP_PROFILE is not None:
+        _work("topk_logits", 0.0, logits.element_size() * rows * vocab + 8.0 * rows * k)
+    _call_on(dev, "ns_topk_logits", d)
 
 
 def argmax_rows(logits16, rows, V, ldv, out):

@@ -36,6 +36,7 @@ BAD_LINEAR = [
     (dict(weight=torch.zeros(50, 24, dtype=F16)), "weight"),
     (dict(weight=torch.zeros(50, 16, dtype=BF16)), "weight"),
     (dict(weight=torch.zeros(0, 16, dtype=F16)), "no rows"),
+    (dict(labels=None), "labels"),
     (dict(labels=torch.zeros(6, dtype=torch.int32)), "labels"),
     (dict(labels=torch.zeros(5, dtype=torch.int64)), "labels"),
     (dict(labels=torch.zeros(12, dtype=torch.int64)[::2]), "labels"),
@@ -137,7 +138,7 @@ def test_workspace_rule():
 
 
 def test_a_recorded_launch_list_needs_the_callers_workspace(monkeypatch):
-    monkeypatch.setattr(ops, "_on_one_gpu", lambda *a: torch.device("cpu"))
+    monkeypatch.setattr(ops, "_one_gpu", lambda *a: 0)
     a = linear_args()
     with ops.recording(ops.LaunchList()):
         with pytest.raises(ValueError, match="workspace"):
