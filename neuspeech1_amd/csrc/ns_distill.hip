@@ -227,12 +227,12 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
     float ts = 0.f;
     for (int e = lane; e < p.k; e += 64) ts += soft ? expf(sp[e] - tm) : 0.f;
     ts = ns_wave_sum(ts);
-    const float lt = logf(ts), its = 1.f / ts, lq = ms / p.T + logf(DUAL ? s2 : s1);
+    const float lt = logf(ts), its = 1.f / ts, ls = logf(DUAL ? s2 : s1);
     float kl = 0.f;
     for (int e = lane; e < p.k; e += 64) {
       const float lp = sp[e] - tm;
       const float pr = soft ? expf(lp) * its : 0.f;
-      if (pr > 0.f) kl += pr * ((lp - lt) - (sz[e] / p.T - lq));
+      if (pr > 0.f) kl += pr * ((lp - lt) - ((sz[e] - ms) / p.T - ls));
       sp[e] = pr;
     }
     kl = ns_wave_sum(kl);

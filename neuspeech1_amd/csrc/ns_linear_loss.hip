@@ -448,19 +448,25 @@ struct RowArgs {
   int tiles_n, R, k, V;
   float c1, c2, invT, w1, w2, lw1, lw2, kd;     // lw*: log2(w* 2^s), -inf for a zero weight; kd: alpha T^2
   int dual, soft_only;                          // one softmax: p1 is at temperature T when only soft targets count
-  const int* nvalid; const int* order;
+  const int* nvalid; const int *order, *lab;
+  const float* z; int64_t ldz;                  // the few-row path's logits (or NULL: the gathered ones)
+  float* loss;
   const float* zk; const float* top_vals; const int32_t* top_idx; int64_t ld_top;
   float *La, *Lb, *pk, *row_loss, *packed_loss;
 };
 
-// 16 rows per workgroup, 16 threads per row
-__global__ __launch_bounds__(256) void ll_rows_kernel(const RowArgs p) {
-  __shared__ float sm[3][16][17];
-  const int nv = *p.nvalid, i0 = blockIdx.x * 16;
-  if (i0 >= (nv + BM - 1) / BM * BM) return;
+// 16 threads per row; one workgroup of 1024 threads (the few-row path) also takes the mean
+template <int NT>
+__global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
+  constexpr int RB = NT / 16;
+  __shared__ float sm[3][RB][17];
+  __shared__ float all[RB];
+  const int nv = *p.nvalid, i0 = blockIdx.x * RB;
+  if (NT == 256 && i0 >= (nv + BM - 1) / BM * BM) return;
   {
-    const int r = threadIdx.x & 15, q = threadIdx.x >> 4;
+    const int r = threadIdx.x & (RB - 1), q = threadIdx.x / RB;
     float mx = -INFINITY, s1 = 0.f, s2 = 0.f;
+#pragma unroll 4
     for (int t = q; t < p.tiles_n; t += 16) {
       const int64_t o = (int64_t)t * p.R + i0 + r;
       const float m = p.pm[o];
@@ -483,12 +489,14 @@ __global__ __launch_bounds__(256) void ll_rows_kernel(const RowArgs p) {
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
   const bool live = i < nv;
+  float loss = 0.f;
   if (!live) {                      // padding rows of the last tile: no probability
     if (q == 0) { p.La[i] = INFINITY; if (p.Lb) p.Lb[i] = INFINITY; }
-    return;
+    if (NT == 256) return;
   }
+  if (live) {
   const int row = p.order[i];
-  float loss = 0.f;
+  auto logit = [&](int e, int tok) __attribute__((always_inline)) { return p.z ? p.z[(int64_t)i * p.ldz + tok] : p.zk[(int64_t)i * (p.k + 1) + e]; };
   bool soft = false;
   if (p.k > 0) {
     // the teacher's distribution over the entries that name a token; a list without any leaves the hard label alone
@@ -504,14 +512,14 @@ __global__ __launch_bounds__(256) void ll_rows_kernel(const RowArgs p) {
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) ts += __shfl_xor(ts, o, 64);
     const float lt = logf(ts), inv = 1.f / ts;
-    const float lq = mx * p.invT + logf(p.dual ? s2 : s1);      // lse(z / T)  (one softmax: it is the one at T)
+    const float ls = logf(p.dual ? s2 : s1);      // lse(z / T) - max / T  (one softmax: it is the one at T)
     float kl = 0.f;
     for (int e = q; e < p.k; e += 16) {
       float pr = 0.f;
       if (soft && ti[e] >= 0 && ti[e] < p.V) {
         const float lp = tv[e] * p.invT - tm;
         pr = expf(lp) * inv;
-        if (pr > 0.f) kl += pr * ((lp - lt) - (p.zk[(int64_t)i * (p.k + 1) + e] * p.invT - lq));
+        if (pr > 0.f) kl += pr * ((lp - lt) - ((logit(e, ti[e]) - mx) * p.invT - ls));
       }
       p.pk[(int64_t)i * p.k + e] = pr;
     }
@@ -520,7 +528,7 @@ __global__ __launch_bounds__(256) void ll_rows_kernel(const RowArgs p) {
     if (soft) loss += p.kd * kl;
   }
   if (q == 0) {
-    if (!p.soft_only) loss += p.w1 * ((mx - p.zk[(int64_t)i * (p.k + 1) + p.k]) + logf(s1));
+    if (!p.soft_only) loss += p.w1 * ((mx - logit(p.k, p.lab[i])) + logf(s1));
     const float l1 = mx * p.c1 + log2f(s1);
     if (p.dual) {
       p.La[i] = l1 - p.lw1;
@@ -533,7 +541,16 @@ __global__ __launch_bounds__(256) void ll_rows_kernel(const RowArgs p) {
       p.La[i] = l1 - p.lw1;
     }
     p.row_loss[row] = loss;
-    p.packed_loss[i] = loss;
+    if (NT == 256) p.packed_loss[i] = loss;
+  }
+  }
+  if (NT == 1024) {
+    if (q == 0) all[r] = live ? loss : 0.f;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      const float s = ns_wave_sum(all[threadIdx.x]);
+      if (threadIdx.x == 0) *p.loss = s / (float)max(nv, 1);
+    }
   }
 }
 
@@ -618,47 +635,72 @@ __global__ __launch_bounds__(NTH) void ll_dh_kernel(const DhArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 2, wn = wave & 3;
   float* const out = p.slab + ((int64_t)split * p.R + m0) * p.d + n0;
+  // eight 16-B loads in flight before the first addition (a load, an addition and a store at a time cost a memory latency each)
 #pragma unroll
   for (int ah = 0; ah < 2; ++ah)
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
+    for (int mp = 0; mp < 4; mp += 2) {
+      f32x4 old[2][4];
+      if (p.add) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int rl = wm * 128 + ah * 64 + mt * 16 + l15, cl = wn * 64 + b * 16 + 4 * lg;
-        if (n0 + cl >= p.d) continue;
-        f32x4* const at = (f32x4*)(out + (int64_t)rl * p.d + cl);
-        f32x4 v = acc[ah][mt][b >> 1][b & 1];
-        if (p.add) v += *at;
-        *at = v;
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int rl = wm * 128 + ah * 64 + (mp + m) * 16 + l15, cl = wn * 64 + b * 16 + 4 * lg;
+            if (n0 + cl < p.d) old[m][b] = *(const f32x4*)(out + (int64_t)rl * p.d + cl);
+          }
       }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int rl = wm * 128 + ah * 64 + (mp + m) * 16 + l15, cl = wn * 64 + b * 16 + 4 * lg;
+          if (n0 + cl >= p.d) continue;
+          f32x4 v = acc[ah][mp + m][b >> 1][b & 1];
+          if (p.add) v += old[m][b];
+          *(f32x4*)(out + (int64_t)rl * p.d + cl) = v;
+        }
+    }
 }
 
-// dh[row] = g 2^-s sum of the slabs, zero for a row without a label
+// dh[row] = g 2^-s sum of the slabs (in their order), zero for a row without a label.  A workgroup takes 64 columns of a row with 16 threads of 4 columns,
+// and 16 groups of slabs side by side: with one token and 203 slabs a single chain of loads took 28 us
 template <class E>
 __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict__ slab, int splits, int R, int d, int rows, const int* __restrict__ inv,
                                                         const int* __restrict__ nvalid, const float* __restrict__ loss_scale, float unscale, E* __restrict__ dh, int64_t lddh) {
-  const int per = d / 8;
-  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int row = (int)(x / per), c = (int)(x - (int64_t)row * per) * 8;
-  if (row >= rows) return;
-  const int i = inv[row];
-  typedef E e8 __attribute__((ext_vector_type(8)));
-  e8 o;
-  if (i < 0) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = (E)0.f;
-  } else {
-    const float gs = (loss_scale ? *loss_scale : 1.f) / (float)max(*nvalid, 1) * unscale;
-    f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-    for (int s = 0; s < splits; ++s) {
-      const float* const q = slab + ((int64_t)s * R + i) * d + c;
-      a += *(const f32x4*)q;
-      b += *(const f32x4*)(q + 4);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { o[e] = (E)(a[e] * gs); o[4 + e] = (E)(b[e] * gs); }
+  typedef E e4 __attribute__((ext_vector_type(4)));
+  __shared__ f32x4 sm[16][16];
+  const int groups = splits >= 16 ? 16 : splits >= 4 ? 4 : 1;             // slab groups; the rest of the 16 lanes-of-16 take further column blocks
+  const int sub = threadIdx.x >> 4, g = sub & (groups - 1), blk = sub / groups;
+  const int per = (d + 63) / 64, nblk = 16 / groups;
+  const int64_t x = (int64_t)blockIdx.x * nblk + blk;
+  const int row = (int)(x / per), c = (int)(x - (int64_t)row * per) * 64 + (threadIdx.x & 15) * 4;
+  const bool in = row < rows && c < d;
+  const int i = in ? inv[row] : -1;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+  if (i >= 0) {
+    const int per_g = (splits + groups - 1) / groups, s1 = min(splits, (g + 1) * per_g);
+#pragma unroll 4
+    for (int s = g * per_g; s < s1; ++s) a += *(const f32x4*)(slab + ((int64_t)s * R + i) * d + c);
   }
-  *(e8*)(dh + row * lddh + c) = o;
+  if (groups > 1) {
+    sm[sub][threadIdx.x & 15] = a;
+    __syncthreads();
+    if (g == 0)
+      for (int o = 1; o < groups; ++o) a += sm[sub + o][threadIdx.x & 15];
+  }
+  if (!in || g != 0) return;
+  const float gs = (loss_scale ? *loss_scale : 1.f) / (float)max(*nvalid, 1) * unscale;
+  e4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = (E)(i < 0 ? 0.f : a[e] * gs);
+  *(e4*)(dh + row * lddh + c) = o;
+}
+template <class E> void launch_dh_out(const float* slab, int splits, int R, int d, int rows, const int* inv, const int* nvalid, const float* loss_scale, float unscale, E* dh,
+                                      int64_t lddh, hipStream_t st) {
+  const int nblk = splits >= 16 ? 1 : splits >= 4 ? 4 : 16;
+  const int64_t items = (int64_t)rows * ((d + 63) / 64);
+  hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)((items + nblk - 1) / nblk)), dim3(256), 0, st, slab, splits, R, d, rows, inv, nvalid, loss_scale, unscale, dh, lddh);
 }
 
 struct DwArgs {
@@ -727,8 +769,339 @@ __global__ __launch_bounds__(NTH) void ll_dw_kernel(const DwArgs p) {
   }
 }
 
+// ------------------------------------------------------------------------------------------------ few rows
+// Up to LL_FEW_ROWS rows: the time is W's bytes, read once for the logits and once more for dh (dW is written once).  No 256-row tiles, no packing, and
+// the logits of so few rows (N V fp32, 13 MB at 64) ARE kept, in the workspace: nothing is formed twice.
+//   ll_few_logits  a workgroup takes 256 rows of W, a wave 32 of them, straight from memory into MFMA operands (16 B per lane and 32 columns, four steps ahead)
+//   ll_rows        as for many rows, one workgroup for all of them, and the mean
+//   ll_few_grad    a workgroup takes 256 tokens: dz of those (rows x 256, in LDS, sparse cells put right there), then 64 columns of W at a time by LDS-DMA,
+//                  three chunks in flight: dh's part of these tokens, and the tokens' rows of dW
+// Rows with a label are found by every workgroup itself: one ballot over at most 64 labels.
+constexpr int LL_FEW_ROWS = 64;
+
+// this wave's view: number of rows with a label; src = original row of packed row `lane` (or -1)
+__device__ __forceinline__ int few_rows(const int64_t* labels, int rows, int V, int lane, int& src) {
+  const int64_t l = lane < rows ? labels[lane] : -1;
+  const bool ok = l >= 0 && l < V;
+  const uint64_t m = __ballot(ok);
+  const int n = __popcll(m);
+  // the lane-th set bit of m: binary search over prefix counts
+  int pos = 0;
+#pragma unroll
+  for (int b = 32; b > 0; b >>= 1) {
+    const uint64_t low = pos + b >= 64 ? m : m & ((1ull << (pos + b)) - 1ull);
+    if (__popcll(low) <= lane) pos += b;
+  }
+  src = lane < n ? pos : -1;
+  return n;
+}
+
+struct FewArgs {
+  const void* h; int64_t ldh; const void* w; int64_t ldw;
+  const int64_t* labels;
+  int rows, d, V, tiles_n;
+  float c1, c2;
+  float* z; int64_t ldz;            // (16 MT, tiles_n 256)
+  float *pm, *p1, *p2; int R;       // (tiles_n, R)
+  int *order, *inv, *lab, *nvalid; float* row_loss;
+  // gradient
+  const float *La, *Lb, *pk; const int32_t* top_idx; int64_t ld_top; int k;
+  float w1s, w2s, unscale;
+  const float* loss_scale;
+  float* slab;                      // (tiles_n, 16 MT, d)
+  void* dw; int64_t lddw; int f32, add, dh;
+};
+
+template <class T, int MT, bool DUAL>
+__global__ __launch_bounds__(512) void ll_few_logits_kernel(const FewArgs p) {
+  typedef typename T::e E;
+  typedef typename T::v8 v8;
+  __shared__ float sm[3][8][16 * MT];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, lg = lane >> 4;
+  int src;
+  const int nv = few_rows(p.labels, p.rows, p.V, lane, src);
+  if (blockIdx.x == 0 && wave == 0) {
+    if (lane < p.rows) {
+      const int64_t l = p.labels[lane];
+      const bool ok = l >= 0 && l < p.V;
+      const uint64_t m = __ballot(ok);
+      p.inv[lane] = ok ? __popcll(m & ((1ull << lane) - 1ull)) : -1;
+      if (!ok) p.row_loss[lane] = 0.f;
+    }
+    if (src >= 0) { p.order[lane] = src; p.lab[lane] = (int)p.labels[src]; }
+    if (lane == 0) *p.nvalid = nv;
+  }
+  const int n0 = blockIdx.x * 256, v0 = n0 + wave * 32;
+  const E* wr[2];
+  bool wok[2];
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+    const int v = v0 + f * 16 + l15;
+    wok[f] = v < p.V;
+    wr[f] = (const E*)p.w + (int64_t)(wok[f] ? v : p.V - 1) * p.ldw;
+  }
+  const E* hr[MT];
+  bool hok[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int s_ = __shfl(src, m * 16 + l15, 64);
+    hok[m] = s_ >= 0;
+    hr[m] = (const E*)p.h + (int64_t)(s_ >= 0 ? s_ : 0) * p.ldh;
+  }
+  const v8 zero = {};
+  f32x4 acc[2][MT];
+#pragma unroll
+  for (int f = 0; f < 2; ++f)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[f][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  v8 wf[2][4][2];
+  auto fetch = [&](v8 (&to)[4][2], int k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s_ = 0; s_ < 4; ++s_)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const int k = k0 + s_ * 32 + 8 * lg;
+        to[s_][f] = k < p.d ? *(const v8*)(wr[f] + k) : zero;
+      }
+  };
+  auto mul = [&](v8 (&a)[4][2], int k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s_ = 0; s_ < 4; ++s_) {
+      const int k = k0 + s_ * 32 + 8 * lg;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const v8 b = hok[m] && k < p.d ? *(const v8*)(hr[m] + k) : zero;
+#pragma unroll
+        for (int f = 0; f < 2; ++f) acc[f][m] = T::mma(a[s_][f], b, acc[f][m]);
+      }
+    }
+  };
+  fetch(wf[0], 0);
+  for (int k0 = 0; k0 < p.d; k0 += 256) {
+    fetch(wf[1], k0 + 128);
+    mul(wf[0], k0);
+    fetch(wf[0], k0 + 256);
+    mul(wf[1], k0 + 128);
+  }
+  // a lane holds 4 neighbouring tokens of 16 MT rows, twice
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = m * 16 + l15;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      if (hok[m]) *(f32x4*)(p.z + (int64_t)r * p.ldz + v0 + f * 16 + 4 * lg) = acc[f][m];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (v0 + f * 16 + 4 * lg + e >= p.V) acc[f][m][e] = -INFINITY;
+        mx = fmaxf(mx, acc[f][m][e]);
+      }
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float ms = mx == -INFINITY ? 0.f : mx;
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s1 += __builtin_amdgcn_exp2f((acc[f][m][e] - ms) * p.c1);
+        if (DUAL) s2 += __builtin_amdgcn_exp2f((acc[f][m][e] - ms) * p.c2);
+      }
+    s1 += __shfl_xor(s1, 16, 64);
+    s1 += __shfl_xor(s1, 32, 64);
+    if (DUAL) { s2 += __shfl_xor(s2, 16, 64); s2 += __shfl_xor(s2, 32, 64); }
+    if (lg == 0) { sm[0][wave][r] = mx; sm[1][wave][r] = s1; if (DUAL) sm[2][wave][r] = s2; }
+  }
+  __syncthreads();
+  if (tid < 16 * MT) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) mx = fmaxf(mx, sm[0][w][tid]);
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const float dm = sm[0][w][tid] - mx;
+      s1 += sm[1][w][tid] * __builtin_amdgcn_exp2f(dm * p.c1);
+      if (DUAL) s2 += sm[2][w][tid] * __builtin_amdgcn_exp2f(dm * p.c2);
+    }
+    const int64_t o = (int64_t)blockIdx.x * p.R + tid;
+    p.pm[o] = mx;
+    p.p1[o] = s1;
+    if (DUAL) p.p2[o] = s2;
+  }
+}
+
+constexpr int FG_LD = 256 * 2 + 16;          // bytes per staged row of dz
+constexpr int FW_BYTES = 256 * 128;          // a chunk of W: 256 tokens x 64 columns
+constexpr int FH_LD = 64 * 2 + 16;           // bytes per staged row of h (64 columns)
+template <int MT> constexpr int few_lds() { return 3 * FW_BYTES + 16 * MT * FG_LD + (MT < 2 ? 32 : 16 * MT) * FH_LD; }
+
+// grid (tiles_n, column groups).  K of dW is the rows, padded to 32 with zeros.
+template <class T, int MT, bool DUAL>
+__global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  typedef typename T::e E;
+  typedef typename T::v8 v8;
+  constexpr int KR = MT < 2 ? 32 : 16 * MT;            // rows of h in LDS
+  char* const gs_ = smem + 3 * FW_BYTES;
+  char* const hs = gs_ + 16 * MT * FG_LD;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, lg = lane >> 4;
+  const int n0 = blockIdx.x * 256;
+  const int chunks = (p.d + 63) / 64, per = (chunks + gridDim.y - 1) / gridDim.y;
+  const int c_begin = blockIdx.y * per, c_end = min(chunks, c_begin + per);
+  // W by LDS-DMA: wave w fills rows [32 w, 32 w + 32) of a chunk in four pieces of 8 rows x 128 B.  The 32-B windows of row r are permuted by
+  // f(r) = bit 1 | bit 3 << 1, so that the eight row segments of half a transposed read lie in different banks (even and odd rows already do).
+  const ns_u4v rsrc = ll_rsrc((const E*)p.w + (int64_t)n0 * p.ldw);
+  const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)smem;
+  uint32_t off[4];
+  int col[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = 32 * wave + 8 * j + (lane >> 3), f = ((r >> 1) & 1) | (((r >> 3) & 1) << 1);
+    col[j] = ((lane & 7) ^ (f << 1)) * 8;
+    off[j] = n0 + r < p.V ? (uint32_t)(r * (int)p.ldw + col[j]) * 2u : OUT;
+  }
+  auto stage = [&](int c) __attribute__((always_inline)) {
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_base + (c % 3) * FW_BYTES + wave * 4096);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ll_dma16(rsrc, c < c_end && c * 64 + col[j] < p.d ? off[j] : OUT, c < c_end ? c * 128 : 0, dst + j * 1024);
+  };
+  int src;
+  const int nv = few_rows(p.labels, p.rows, p.V, lane, src);
+  if (p.dh) { stage(c_begin); stage(c_begin + 1); }
+  // dz of these 256 tokens
+  for (int x = tid; x < 16 * MT * 64; x += 512) {
+    const int r = x >> 6, c = (x & 63) * 4;
+    float g[4] = {0.f, 0.f, 0.f, 0.f};
+    if (r < nv) {
+      const f32x4 z = *(const f32x4*)(p.z + (int64_t)r * p.ldz + n0 + c);
+      const float la = p.La[r], lb = DUAL ? p.Lb[r] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        g[e] = __builtin_amdgcn_exp2f(z[e] * p.c1 - la);
+        if (DUAL) g[e] += __builtin_amdgcn_exp2f(z[e] * p.c2 - lb);
+        if (n0 + c + e >= p.V) g[e] = 0.f;
+      }
+    }
+    *(ushort4v*)(gs_ + r * FG_LD + c * 2) = cvt4<E>(g[0], g[1], g[2], g[3]);
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  LL_BARRIER();
+  // its sparse cells: entries 0 .. k - 1 the list, k the label; an entry whose token an earlier one names is written by that one
+  for (int x = tid; x < nv * (p.k + 1); x += 512) {
+    const int r = x / (p.k + 1), e = x - r * (p.k + 1);
+    const int lab = p.lab[r], row = p.order[r];
+    const int t = e == p.k ? lab : p.top_idx[row * p.ld_top + e];
+    if (t < n0 || t >= n0 + 256 || t >= p.V) continue;
+    float soft = 0.f;
+    bool first = true;
+    for (int o = 0; o < p.k; ++o)
+      if (p.top_idx[row * p.ld_top + o] == t) { soft += p.pk[(int64_t)r * p.k + o]; first = first && o >= e; }
+    if (!first) continue;
+    const float z = p.z[(int64_t)r * p.ldz + t];
+    float v = __builtin_amdgcn_exp2f(z * p.c1 - p.La[r]);
+    if (DUAL) v += __builtin_amdgcn_exp2f(z * p.c2 - p.Lb[r]);
+    v -= p.w2s * soft;
+    if (t == lab) v -= p.w1s;
+    *(E*)(gs_ + r * FG_LD + (t - n0) * 2) = (E)v;
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  LL_BARRIER();
+  auto tr8 = [&](const char* at, int four_rows) __attribute__((always_inline)) {      // 8 k-rows of 16 columns, transposed
+    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at);
+    const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + four_rows));
+    const short8v r = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(v8, r);
+  };
+  const int q = l15 >> 2, pp = l15 & 3;
+  const float gs = (p.loss_scale ? *p.loss_scale : 1.f) / (float)max(nv, 1) * p.unscale;
+  // dW: this wave's 32 tokens as the MFMA's columns (dz transposed), the rows as K
+  constexpr int KS = KR / 32;
+  v8 gt[2][KS];
+  if (p.dw) {
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int r = ks * 32 + 8 * lg + q;
+        if (MT == 1 && lg >= 2) gt[f][ks] = v8{};       // (16 rows: the upper half of K is zero)
+        else gt[f][ks] = v8{};
+        const int rr = MT == 1 ? (8 * (lg & 1) + q) : r;
+        const v8 v = tr8(gs_ + rr * FG_LD + (wave * 32 + f * 16 + 4 * pp) * 2, 4 * FG_LD);
+        if (!(MT == 1 && lg >= 2)) gt[f][ks] = v;
+      }
+  }
+  // dh: output block `id` = (16 rows, 16 of the chunk's 64 columns), K = the 256 tokens
+  for (int c = c_begin; c < c_end; ++c) {
+    if (p.dw) {
+      for (int x = tid; x < KR * 8; x += 512) {
+        const int r = x >> 3, cc = (x & 7) * 8;
+        const int s_ = r < nv ? p.order[r] : -1;
+        const uint4 v = s_ >= 0 && c * 64 + cc < p.d ? *(const uint4*)((const E*)p.h + (int64_t)s_ * p.ldh + c * 64 + cc) : make_uint4(0, 0, 0, 0);
+        *(uint4*)(hs + r * FH_LD + cc * 2) = v;
+      }
+    }
+    if (p.dh) {
+      stage(c + 2);
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");        // the chunk requested two steps ago has landed (this wave's part; the barrier covers the others)
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    LL_BARRIER();
+    if (p.dh) {
+      const char* const ws = smem + (c % 3) * FW_BYTES;
+#pragma unroll
+      for (int id0 = 0; id0 < 4 * MT; id0 += 8) {
+        const int id = id0 + wave;
+        if (id < 4 * MT) {
+          const int mt = id >> 2, ct = id & 3;
+          f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const int r = ks * 32 + 8 * lg + q, f = ((r >> 1) & 1) | (((r >> 3) & 1) << 1);      // (four rows further: the same f)
+            const v8 wt = tr8(ws + r * 128 + ((ct ^ f) << 5) + pp * 8, 512);
+            const v8 g = *(const v8*)(gs_ + (mt * 16 + l15) * FG_LD + (ks * 32 + 8 * lg) * 2);
+            a = T::mma(wt, g, a);
+          }
+          const int cc = c * 64 + ct * 16 + 4 * lg;
+          if (cc < p.d) *(f32x4*)(p.slab + ((int64_t)blockIdx.x * 16 * MT + mt * 16 + l15) * p.d + cc) = a;
+        }
+      }
+    }
+    if (p.dw) {
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        v8 ht[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) ht[ks] = tr8(hs + (ks * 32 + 8 * lg + q) * FH_LD + (ct * 16 + 4 * pp) * 2, 4 * FH_LD);
+        const int cc = c * 64 + ct * 16 + 4 * lg;
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) a = T::mma(ht[ks], gt[f][ks], a);
+          const int v = n0 + wave * 32 + f * 16 + l15;
+          if (v >= p.V || cc >= p.d) continue;
+          a *= gs;
+          if (p.f32) {
+            f32x4* const at = (f32x4*)((float*)p.dw + (int64_t)v * p.lddw + cc);
+            if (p.add) a += *at;
+            *at = a;
+          } else {
+            *(ushort4v*)((E*)p.dw + (int64_t)v * p.lddw + cc) = cvt4<E>(a[0], a[1], a[2], a[3]);
+          }
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    LL_BARRIER();                                              // everyone has read this chunk before its slot and h's are filled again
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
+  int few;                                    // 0, or MT of the few-row path
   int R, dp, dt, tiles_n, piece_tiles, pieces, splits, chunk;
   size_t order, inv, lab, hp, hT, zk, pk, pm, p1, p2, La, Lb, ploss, G, slab, total;
 };
@@ -736,7 +1109,8 @@ struct Plan {
 bool dual_of(const ns_linear_ce_desc* d) { return d->k > 0 && d->alpha > 0.f && d->alpha < 1.f && d->temperature != 1.f; }
 
 Plan plan_of(const ns_linear_ce_desc* d) {
-  Plan p;
+  Plan p = {};
+  p.few = d->rows > LL_FEW_ROWS ? 0 : d->rows <= 16 ? 1 : d->rows <= 32 ? 2 : 4;
   p.R = (d->rows > 0 ? d->rows + BM - 1 : BM) / BM * BM;
   p.dp = (d->d + BK - 1) / BK * BK;
   p.dt = (d->d + BM - 1) / BM * BM;
@@ -756,14 +1130,15 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   if (p.splits < 1) p.splits = 1;
   if (p.splits > p.piece_tiles / 2) p.splits = p.piece_tiles / 2 > 0 ? p.piece_tiles / 2 : 1;
   p.chunk = ((p.piece_tiles * BN + p.splits - 1) / p.splits + BK - 1) / BK * BK;
+  if (p.few) { p.R = LL_FEW_ROWS; p.splits = p.tiles_n; }
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
   p.order = take((size_t)d->rows * 4);
   p.inv = take((size_t)d->rows * 4);
   p.lab = take((size_t)d->rows * 4);
-  p.hp = take((size_t)p.R * p.dp * 2);
-  p.hT = d->dw ? take((size_t)p.dt * p.R * 2) : 0;
-  p.zk = take((size_t)p.R * (d->k + 1) * 4);
+  p.hp = p.few ? 0 : take((size_t)p.R * p.dp * 2);
+  p.hT = d->dw && !p.few ? take((size_t)p.dt * p.R * 2) : 0;
+  p.zk = take(p.few ? (size_t)16 * p.few * p.tiles_n * BN * 4 : (size_t)p.R * (d->k + 1) * 4);       // (few rows: all logits)
   p.pk = take((size_t)p.R * d->k * 4);
   p.pm = take((size_t)p.tiles_n * p.R * 4);
   p.p1 = take((size_t)p.tiles_n * p.R * 4);
@@ -771,14 +1146,38 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   p.La = take((size_t)p.R * 4);
   p.Lb = take((size_t)p.R * 4);
   p.ploss = take((size_t)p.R * 4);
-  p.G = grad ? take((size_t)p.R * p.piece_tiles * BN * 2) : 0;
-  p.slab = d->dh ? take((size_t)p.splits * p.R * d->d * 4) : 0;
+  p.G = grad && !p.few ? take((size_t)p.R * p.piece_tiles * BN * 2) : 0;
+  p.slab = d->dh ? take((size_t)p.splits * (p.few ? 16 * p.few : p.R) * d->d * 4) : 0;
   p.total = at;
   return p;
 }
 
 bool ll_sizes_ok(const ns_linear_ce_desc* d) {
   return d->rows >= 0 && d->rows <= (1 << 21) && d->vocab > 0 && d->vocab <= (1 << 28) && d->d > 0 && d->d % 8 == 0 && d->d <= (1 << 16) && d->k >= 0 && d->k <= LL_MAX_K;
+}
+
+template <class T, int MT>
+int few_launch(const ns_linear_ce_desc* d, const FewArgs& f, const RowArgs& r, bool dual, hipStream_t st) {
+  typedef typename T::e E;
+  static ns_dev_once once;
+  if (!ns_dyn_lds_once(once, {(const void*)ll_few_grad_kernel<T, MT, false>, (const void*)ll_few_grad_kernel<T, MT, true>}, few_lds<MT>(), "ns_linear_cross_entropy"))
+    return NS_ERR_HIP;
+  if (dual) hipLaunchKernelGGL((ll_few_logits_kernel<T, MT, true>), dim3(f.tiles_n), dim3(512), 0, st, f);
+  else hipLaunchKernelGGL((ll_few_logits_kernel<T, MT, false>), dim3(f.tiles_n), dim3(512), 0, st, f);
+  hipLaunchKernelGGL(ll_rows_kernel<1024>, dim3(1), dim3(1024), 0, st, r);
+  if (d->dh || d->dw) {
+    // a workgroup per CU: where the vocabulary is small, its column chunks are dealt to several
+    const int chunks = (d->d + 63) / 64;
+    int gy = 256 / f.tiles_n;
+    if (gy < 1) gy = 1;
+    if (gy > chunks) gy = chunks;
+    gy = (chunks + (chunks + gy - 1) / gy - 1) / ((chunks + gy - 1) / gy);
+    if (dual) hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, true>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
+    else hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, false>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
+    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n, 16 * MT, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, st);
+  }
+  NS_CHECK_LAUNCH("ns_linear_cross_entropy");
+  return NS_OK;
 }
 
 template <class T>
@@ -802,6 +1201,24 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
                               (const void*)ll_logits_kernel<T, true, false, true>, (const void*)ll_logits_kernel<T, true, false, false>,
                               (const void*)ll_logits_kernel<T, true, true, false>, (const void*)ll_dh_kernel<T>, (const void*)ll_dw_kernel<T>}, LL_LDS, "ns_linear_cross_entropy"))
     return NS_ERR_HIP;
+  const float c1 = soft_only ? LOG2E / T_ : LOG2E, c2 = LOG2E / T_;
+  RowArgs r = {};
+  r.pm = (float*)(ws + p.pm); r.p1 = (float*)(ws + p.p1); r.p2 = (float*)(ws + p.p2); r.tiles_n = p.tiles_n; r.R = p.R; r.k = d->k; r.V = d->vocab;
+  r.c1 = c1; r.c2 = c2; r.invT = 1.f / T_; r.w1 = w1; r.w2 = w2; r.kd = alpha * T_ * T_;
+  r.lw1 = (d->k > 0 && !dual) ? (float)s : log2f(w1) + (float)s;
+  r.lw2 = log2f(w2) + (float)s;
+  r.dual = dual; r.soft_only = soft_only; r.nvalid = d->nvalid_dev; r.order = order; r.lab = lab; r.zk = zk; r.top_vals = d->top_vals; r.top_idx = d->top_idx;
+  r.ld_top = d->ld_top; r.La = La; r.Lb = dual ? Lb : nullptr; r.pk = pk; r.row_loss = d->row_loss; r.packed_loss = ploss; r.loss = d->loss_dev;
+  if (p.few) {
+    FewArgs f = {};
+    f.h = d->h; f.ldh = d->ldh; f.w = d->w; f.ldw = d->ldw; f.labels = d->labels; f.rows = d->rows; f.d = d->d; f.V = d->vocab; f.tiles_n = p.tiles_n;
+    f.c1 = c1; f.c2 = c2; f.z = zk; f.ldz = (int64_t)p.tiles_n * BN; f.pm = (float*)(ws + p.pm); f.p1 = (float*)(ws + p.p1); f.p2 = (float*)(ws + p.p2); f.R = p.R;
+    f.order = order; f.inv = inv; f.lab = lab; f.nvalid = d->nvalid_dev; f.row_loss = d->row_loss;
+    f.La = La; f.Lb = dual ? Lb : nullptr; f.pk = pk; f.top_idx = d->top_idx; f.ld_top = d->ld_top; f.k = d->k; f.w1s = w1 * up; f.w2s = w2 * up; f.unscale = 1.f / up;
+    f.loss_scale = d->loss_scale_dev; f.slab = (float*)(ws + p.slab); f.dw = d->dw; f.lddw = d->lddw; f.f32 = d->dw_f32; f.add = d->dw_add; f.dh = d->dh != nullptr;
+    r.z = zk; r.ldz = f.ldz;
+    return p.few == 1 ? few_launch<T, 1>(d, f, r, dual, st) : p.few == 2 ? few_launch<T, 2>(d, f, r, dual, st) : few_launch<T, 4>(d, f, r, dual, st);
+  }
   hipLaunchKernelGGL(ll_compact_kernel, dim3(1), dim3(1024), 0, st, d->labels, d->rows, d->vocab, order, inv, lab, d->row_loss, d->nvalid_dev);
   hipLaunchKernelGGL(ll_pack_kernel<T>, dim3(p.R / 4), dim3(256), 0, st, d->h, d->ldh, d->w, d->ldw, d->d, p.dp, d->vocab, order, lab, d->top_idx, d->ld_top, d->k,
                      d->nvalid_dev, (void*)(ws + p.hp), zk);
@@ -809,21 +1226,13 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
     hipLaunchKernelGGL(ll_transpose_kernel, dim3(p.R / 64, p.dp / 64), dim3(256), 0, st, (const uint16_t*)(ws + p.hp), p.dp, d->nvalid_dev, (uint16_t*)(ws + p.hT), p.R);
   LogitsArgs a = {};
   a.hp = ws + p.hp; a.w = d->w; a.ldw = d->ldw; a.dp = p.dp; a.d = d->d; a.V = d->vocab; a.col0 = 0; a.tiles_n = p.tiles_n; a.R = p.R; a.nvalid = d->nvalid_dev;
-  a.c1 = soft_only ? LOG2E / T_ : LOG2E;
-  a.c2 = LOG2E / T_;
+  a.c1 = c1; a.c2 = c2;
   a.pm = (float*)(ws + p.pm); a.p1 = (float*)(ws + p.p1); a.p2 = (float*)(ws + p.p2);
   a.La = La; a.Lb = Lb; a.G = ws + p.G; a.ldg = p.piece_tiles * BN; a.lab = lab; a.zk = zk; a.wlab = w1 * up;
   const dim3 all(p.R / BM * p.tiles_n);
   if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, false, true, false>), all, dim3(NTH), LL_LDS, st, a);
   else hipLaunchKernelGGL((ll_logits_kernel<T, false, false, false>), all, dim3(NTH), LL_LDS, st, a);
-  RowArgs r = {};
-  r.pm = a.pm; r.p1 = a.p1; r.p2 = a.p2; r.tiles_n = p.tiles_n; r.R = p.R; r.k = d->k; r.V = d->vocab;
-  r.c1 = a.c1; r.c2 = a.c2; r.invT = 1.f / T_; r.w1 = w1; r.w2 = w2; r.kd = alpha * T_ * T_;
-  r.lw1 = (d->k > 0 && !dual) ? (float)s : log2f(w1) + (float)s;
-  r.lw2 = log2f(w2) + (float)s;
-  r.dual = dual; r.soft_only = soft_only; r.nvalid = d->nvalid_dev; r.order = order; r.zk = zk; r.top_vals = d->top_vals; r.top_idx = d->top_idx; r.ld_top = d->ld_top;
-  r.La = La; r.Lb = dual ? Lb : nullptr; r.pk = pk; r.row_loss = d->row_loss; r.packed_loss = ploss;
-  hipLaunchKernelGGL(ll_rows_kernel, dim3(p.R / 16), dim3(256), 0, st, r);
+  hipLaunchKernelGGL(ll_rows_kernel<256>, dim3(p.R / 16), dim3(256), 0, st, r);
   hipLaunchKernelGGL(ll_mean_kernel, dim3(1), dim3(1024), 0, st, ploss, d->nvalid_dev, d->loss_dev);
   if (grad) {
     for (int pc = 0; pc < p.pieces; ++pc) {
@@ -850,8 +1259,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
       }
     }
     if (d->dh)
-      hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)(((int64_t)d->rows * (d->d / 8) + 255) / 256)), dim3(256), 0, st, (const float*)(ws + p.slab), p.splits, p.R,
-                         d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh, d->lddh);
+      launch_dh_out<E>((const float*)(ws + p.slab), p.splits, p.R, d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh, d->lddh, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;

@@ -80,7 +80,8 @@ def check_linear(ops, dev, h, w, labels, lists=(None, None), temp=1.0, alpha=0.0
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("rows,d,v", [(1, 8, 1), (1, 64, 300), (3, 72, 7), (5, 8, 257), (64, 64, 256), (65, 136, 511), (255, 256, 1000), (257, 264, 1001),
+@pytest.mark.parametrize("rows,d,v", [(1, 8, 1), (1, 64, 300), (3, 72, 7), (5, 8, 257), (64, 64, 256), (16, 192, 300), (17, 136, 600), (32, 1288, 300),
+                                      (33, 64, 5000), (64, 328, 2049), (65, 136, 511), (255, 256, 1000), (257, 264, 1001),
                                       (300, 512, 2600), (700, 776, 513)])
 def test_linear_cross_entropy(ops, dev, dtype, rows, d, v):
     h, w, labels, _ = make_linear(dev, rows, d, v, dtype)
@@ -88,7 +89,7 @@ def test_linear_cross_entropy(ops, dev, dtype, rows, d, v):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("rows,d,v,k", [(1, 64, 300, 5), (9, 72, 50, 1), (130, 128, 1000, 64), (300, 256, 777, 256), (40, 64, 40, 40)])
+@pytest.mark.parametrize("rows,d,v,k", [(1, 64, 300, 5), (9, 72, 50, 1), (30, 200, 900, 17), (130, 128, 1000, 64), (300, 256, 777, 256), (40, 64, 40, 40)])
 @pytest.mark.parametrize("temp,alpha", [(1.0, 0.5), (2.0, 0.5), (3.5, 1.0), (1.0, 1.0), (0.5, 0.25), (2.0, 0.0)])
 def test_linear_cross_entropy_with_a_teacher(ops, dev, dtype, rows, d, v, k, temp, alpha):
     h, w, labels, lists = make_linear(dev, rows, d, v, dtype, seed=1, k=k)
@@ -97,14 +98,16 @@ def test_linear_cross_entropy_with_a_teacher(ops, dev, dtype, rows, d, v, k, tem
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("grad,dw_dtype", [("", None), ("h", None), ("w", None), ("w", F32), ("hw", F32)])
-def test_linear_cross_entropy_gradients_on_request(ops, dev, dtype, grad, dw_dtype):
-    h, w, labels, _ = make_linear(dev, 90, 192, 700, dtype, seed=2)
-    check_linear(ops, dev, h, w, labels, grad=grad, dw_dtype=dw_dtype, scale=512.0)
+@pytest.mark.parametrize("rows", [12, 50, 90])
+def test_linear_cross_entropy_gradients_on_request(ops, dev, dtype, grad, dw_dtype, rows):
+    h, w, labels, _ = make_linear(dev, rows, 192, 700, dtype, seed=2)
+    check_linear(ops, dev, h, w, labels, grad=grad, dw_dtype=dw_dtype, scale=32.0)
 
 
-def test_linear_cross_entropy_adds_to_a_float32_weight_gradient(ops, dev):
-    h, w, labels, _ = make_linear(dev, 90, 192, 700, BF16, seed=3)
-    o = outputs(dev, 90)
+@pytest.mark.parametrize("rows", [20, 90])
+def test_linear_cross_entropy_adds_to_a_float32_weight_gradient(ops, dev, rows):
+    h, w, labels, _ = make_linear(dev, rows, 192, 700, BF16, seed=3)
+    o = outputs(dev, rows)
     base = torch.randn(700, 192, device=dev)
     dw = base.clone()
     ops.linear_cross_entropy(h, w, labels, dweight=dw, accumulate=True, **o)
@@ -119,9 +122,10 @@ def test_linear_cross_entropy_in_two_pieces_of_the_vocabulary(ops, dev, dtype):
     check_linear(ops, dev, h, w, labels, lists, 2.0, 0.5)
 
 
-def test_rows_without_a_label_are_not_read(ops, dev):
+@pytest.mark.parametrize("rows", [14, 60, 300])
+def test_rows_without_a_label_are_not_read(ops, dev, rows):
     """infinities and NaN in masked rows reach neither loss nor gradients; their gradient is zero"""
-    h, w, labels, lists = make_linear(dev, 300, 128, 600, BF16, seed=5, k=9)
+    h, w, labels, lists = make_linear(dev, rows, 128, 600, BF16, seed=5, k=9)
     off = ~((labels >= 0) & (labels < 600))
     h[off] = float("nan")
     h[off.nonzero()[::2, 0]] = float("inf")
@@ -141,9 +145,10 @@ def test_no_row_has_a_label(ops, dev, rows):
     assert int(o["nvalid"]) == 0 and float(o["loss"]) == 0 and (o["row_loss"] == 0).all() and (dh == 0).all() and (dw == 0).all()
 
 
-def test_strided_operands_and_what_lies_beside_them(ops, dev):
+@pytest.mark.parametrize("rows", [13, 130])
+def test_strided_operands_and_what_lies_beside_them(ops, dev, rows):
     g = gen(6, dev)
-    rows, d, v = 130, 72, 301
+    d, v = 72, 301
     hb = torch.full((rows, 136), float("nan"), device=dev, dtype=F16)
     wb = torch.full((v + 3, 200), float("inf"), device=dev, dtype=F16)
     h, w = hb[:, 64:136], wb[2:v + 2, 8:80]
@@ -170,14 +175,15 @@ def test_large_logits(ops, dev):
     check_linear(ops, dev, h * 64, w * 4, labels)
 
 
-def test_same_inputs_give_the_same_bits_and_workspaces_are_not_shared(ops, dev):
+@pytest.mark.parametrize("rows", [40, 600])
+def test_same_inputs_give_the_same_bits_and_workspaces_are_not_shared(ops, dev, rows):
     """repeated, interleaved with another call, on another stream and with a caller's workspace: equal bits; nothing past the workspace is written"""
-    h, w, labels, lists = make_linear(dev, 600, 256, 3001, F16, seed=8, k=20)
+    h, w, labels, lists = make_linear(dev, rows, 256, 3001, F16, seed=8, k=20)
     h2, w2, labels2, _ = make_linear(dev, 500, 128, 900, F16, seed=9)
     kw = dict(top_vals=lists[0], top_idx=lists[1], temperature=2.0, alpha=0.5)
 
     def once(**more):
-        o = outputs(dev, 600)
+        o = outputs(dev, rows)
         dh, dw = torch.empty_like(h), torch.empty_like(w)
         ops.linear_cross_entropy(h, w, labels, dh=dh, dweight=dw, **o, **kw, **more)
         return [o["row_loss"], o["loss"], dh, dw]
@@ -189,7 +195,7 @@ def test_same_inputs_give_the_same_bits_and_workspaces_are_not_shared(ops, dev):
     with torch.cuda.stream(side):
         b = once()
     c = once()
-    need = ops.linear_ce_workspace_bytes(h, w, labels, dh=torch.empty_like(h), dweight=torch.empty_like(w), **outputs(dev, 600), **kw)
+    need = ops.linear_ce_workspace_bytes(h, w, labels, dh=torch.empty_like(h), dweight=torch.empty_like(w), **outputs(dev, rows), **kw)
     ws = torch.full((need + 4096,), 0xA5, device=dev, dtype=torch.uint8)
     e = once(workspace=ws[:need])
     torch.cuda.synchronize()
@@ -201,14 +207,15 @@ def test_same_inputs_give_the_same_bits_and_workspaces_are_not_shared(ops, dev):
         once(workspace=ws[:need - 256])
 
 
-def test_captured_graphs_replay_with_new_data(ops, dev):
+@pytest.mark.parametrize("rows", [50, 260])
+def test_captured_graphs_replay_with_new_data(ops, dev, rows):
     """two graphs, replayed several times between eager calls, against eager results"""
-    sets = [make_linear(dev, 260, 128, 1200, BF16, seed=s, k=6) for s in (10, 11, 12)]
+    sets = [make_linear(dev, rows, 128, 1200, BF16, seed=s, k=6) for s in (10, 11, 12)]
     h, w, labels = (t.clone() for t in sets[0][:3])
     tv, ti = (t.clone() for t in sets[0][3])
 
     def bufs():
-        return dict(outputs(dev, 260), dh=torch.empty_like(h), dweight=torch.empty_like(w))
+        return dict(outputs(dev, rows), dh=torch.empty_like(h), dweight=torch.empty_like(w))
 
     def call(b):
         ops.linear_cross_entropy(h, w, labels, top_vals=tv, top_idx=ti, temperature=2.0, alpha=0.5, **b)
@@ -340,14 +347,17 @@ def test_distill_topk_without_labels_and_with_masked_rows(ops, dev):
     assert float(o["loss"]) == 0 and int(o["nvalid"]) == 0
 
 
-def test_distill_topk_with_masked_logits(ops, dev):
-    """student logits of -inf and of the type's lowest value: finite losses where the targets do not name them, zero probability there"""
-    buf, z, labels, lists = make_logits(dev, 6, 900, F16, 23, ignored=0.0, k=5)
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_distill_topk_with_masked_logits(ops, dev, dtype):
+    """student logits of -inf and of the type's lowest value: finite losses where the targets do not name them, zero probability there; a row of the lowest
+    value alone is a uniform distribution"""
+    buf, z, labels, lists = make_logits(dev, 6, 900, dtype, 23, ignored=0.0, k=5)
     named = torch.zeros(6, 900, dtype=torch.bool, device=dev)
     named.scatter_(1, lists[1].clamp(0, 899).long(), True)
     named.scatter_(1, labels.clamp(0, 899).unsqueeze(1), True)
     z[:, ::3] = torch.where(named[:, ::3], z[:, ::3], float("-inf"))
-    z[:, 1::3] = torch.where(named[:, 1::3], z[:, 1::3], torch.finfo(F16).min)
+    z[:, 1::3] = torch.where(named[:, 1::3], z[:, 1::3], torch.finfo(dtype).min)
+    z[2] = torch.finfo(dtype).min
     dz = torch.empty_like(z)
     o = outputs(dev, 6)
     ops.distill_topk(z, labels, *lists, temperature=2.0, alpha=0.5, dlogits=dz, **o)
@@ -355,7 +365,10 @@ def test_distill_topk_with_masked_logits(ops, dev):
     fin = torch.isfinite(ref["row_loss"])
     assert torch.isfinite(o["row_loss"][fin]).all() and fin.any() and torch.isfinite(dz[fin]).all()
     assert ((o["row_loss"].double() - ref["row_loss"]).abs()[fin] <= 1e-4).all()      # (z of -65504 in the tolerance's |z| would say nothing)
-    assert (dz[:, ::3][~named[:, ::3]] == 0).all() and (dz[:, 1::3][~named[:, 1::3]] == 0).all()
+    rest = [0, 1, 3, 4, 5]
+    assert (dz[rest, ::3][~named[rest, ::3]] == 0).all() and (dz[rest, 1::3][~named[rest, 1::3]] == 0).all()
+    flat = dz[2][~named[2]].double() * 6
+    assert ((flat - 1.5 / 900).abs() <= (2 * R.half_step(dtype) + 200 * R.U32) * 1.5 / 900).all()       # w1 + w2 = 0.5 + 0.5 * 2 over 900 tokens
 
 
 # ------------------------------------------------------------------------------------------------ the teacher's lists

@@ -41,6 +41,9 @@ def losses(z, dz_err, labels, temp=1.0, alpha=0.0, top_vals=None, top_idx=None):
     cell = torch.zeros_like(z)
     cell_err = torch.zeros_like(z)
     mag = z.abs().amax(1).clamp(min=1.0)
+    # (every term is unchanged when a row's logits move together: with the maximum taken out, lse - z keeps its digits also where |z| is 1e38)
+    top = z.amax(1, keepdim=True)
+    z = z - torch.where(torch.isfinite(top), top, torch.zeros_like(top))
     dz_err = dz_err.expand(rows) if dz_err.dim() == 0 else dz_err
     if alpha < 1.0:
         w1 = 1.0 - alpha
