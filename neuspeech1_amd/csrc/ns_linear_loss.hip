@@ -31,7 +31,7 @@ constexpr int REGION = 128 * 128;            // 16 KiB
 constexpr int BUF = 4 * REGION;              // 64 KiB
 constexpr int RA0 = 0, RA1 = 1, RB0 = 2, RB1 = 3;
 constexpr int LDH = BN * 2 + 16;             // epilogue: bytes per staged 16-bit row
-constexpr int LL_LDS = BM * LDH > 2 * BUF ? BM * LDH : 2 * BUF;
+constexpr int LL_LDS = BM * LDH > 2 * BUF ? BM * LDH : 2 * BUF;      // (also what every kernel's attribute allows)
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr size_t LL_PIECE_BYTES = 256u << 20;
 constexpr int LL_MAX_K = 256;
@@ -138,7 +138,7 @@ __device__ __forceinline__ void ll_tile(f32x4 (&acc)[2][4][2][2], char* smem, co
     const bool isb = region >= 2;
     const int klen = (isb ? kB : kA) - k0;
     const int soff = isb ? (BT ? k0 * ldb * 2 : k0 * 2) : k0 * 2;
-    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_base + buf * BUF + region * REGION + wave * 2048);
+    const uint32_t dst = lds_base + buf * BUF + region * REGION + wave * 2048;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const bool ok = (isb ? b_k[j] : a_k[j]) < klen;
@@ -327,119 +327,301 @@ struct LogitsArgs {
   float wlab;                            // w1 2^s
 };
 
+// reference exponent of a softmax at scale c: an integer, so that taking it out of z c (inside the fma) and moving sums between references are exact
+__device__ __forceinline__ float ll_ref(float mx, float c) { return ceilf(mx * c); }
+
+// One workgroup per CU walks the tiles of its XCD's run.  The ring never drains: the pieces that a tile's last two K tiles request are the next tile's first
+// ones, so a tile has no prologue, and its epilogue runs while they land (one-tile workgroups spent 26 k cycles a tile outside the main loop, which is
+// 16 k at d = 512).  Statistics meet in LDS behind the ring.  dz is staged 32 rows x 64 columns at a time in 4 KiB that belong to ONE wave (the two regions
+// of ring buffer 1 that hold nothing yet), 16-B chunk c of row r at chunk c ^ (r & 7): no barrier between staging and storing, a wave's own LDS operations
+// are in order; its 16 stores are left in flight under the next tile's first K tile, whose waits count them.
+constexpr int LL_SIDE = 2 * BUF;                              // behind the ring
+constexpr int LL_LOGITS_LDS = LL_SIDE + 3 * 4096;             // statistics: 3 x 4 x 256 floats; dz: two parities of 4 x 256 row constants (8 KiB)
+
 template <class T, bool GRAD, bool DUAL, bool FIX>
 __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef typename T::e E;
-  const int nv = *p.nvalid;
-  const int tiles_m = (nv + BM - 1) / BM;
-  const int pos = ll_pos(tiles_m * p.tiles_n);
-  if (pos < 0) return;
-  // eight row tiles by the columns: the 32 workgroups of an XCD that run together read 8 + 4 operand tiles instead of 1 + 32
-  constexpr int GM = 8;
-  const int grp = pos / (GM * p.tiles_n), rem = pos - grp * GM * p.tiles_n;
-  const int gm = min(GM, tiles_m - grp * GM);
-  const int tm = grp * GM + rem % gm, tn = rem / gm;
-  const int m0 = tm * BM, n0 = p.col0 + tn * BN;
-  f32x4 acc[2][4][2][2];
-  ll_tile<T, false, false>(acc, smem, (const E*)p.hp + (int64_t)m0 * p.dp, p.dp, p.dp, (const E*)p.w + (int64_t)n0 * p.ldw, (int)p.ldw, p.d,
-                           min(BN, p.V - n0), p.d);
+  typedef typename T::v8 v8;
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 2, wn = wave & 3;
-  const bool edge = n0 + BN > p.V;
-  if (!GRAD) {
-    // a lane holds 16 of the wave's 64 columns of 8 rows; the row's other lanes are 16 and 32 apart, its other columns in the waves of equal wm
-    float* const sm = (float*)smem;
+  const int nv = *p.nvalid;
+  const int tiles_m = (nv + BM - 1) / BM, total = tiles_m * p.tiles_n;
+  // XCD x (= block % 8) owns a contiguous run of tiles, its workgroups take every nx-th of it
+  const int xcd = blockIdx.x & 7, nx = (gridDim.x - xcd + 7) >> 3;
+  const int q8 = total >> 3, r8 = total & 7;
+  const int x0 = xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8, xn = q8 + (xcd < r8 ? 1 : 0);
+  int ti = blockIdx.x >> 3;
+  if (ti >= xn) return;
+  // eight row tiles by the columns: the 32 workgroups of an XCD that run together read 8 + 4 operand tiles instead of 1 + 32
+  auto place = [&](int t, int& tm, int& tn) __attribute__((always_inline)) {
+    constexpr int GM = 8;
+    const int pos = x0 + t, grp = pos / (GM * p.tiles_n), rem = pos - grp * GM * p.tiles_n;
+    const int gm = min(GM, tiles_m - grp * GM);
+    tn = rem / gm;
+    tm = grp * GM + rem - tn * gm;
+  };
+  const int ne = ((p.d + BK - 1) / BK + 1) & ~1;              // K tiles, an even number
+  uint32_t a_off[2][2], b_off[2][2];
+  int my_k[2];
 #pragma unroll
-    for (int ah = 0; ah < 2; ++ah)
+  for (int j = 0; j < 2; ++j) {
+    const int rr = 16 * wave + 8 * j + (lane >> 3), ch = (lane & 7) ^ ((rr >> 1) & 7);
+    my_k[j] = ch * 8;
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        float z[16];
-        float mx = -INFINITY;
+    for (int h = 0; h < 2; ++h) {
+      a_off[h][j] = (uint32_t)((((rr >> 6) << 7) + h * 64 + (rr & 63)) * p.dp + ch * 8) * 2u;
+      b_off[h][j] = (uint32_t)((((rr >> 5) << 6) + h * 32 + (rr & 31)) * (int)p.ldw + ch * 8) * 2u;
+    }
+  }
+  // operands of the current and the next tile; W's rows end with the vocabulary (a row past it starts behind the resource's last byte)
+  auto rsrc_a_of = [&](int tm) __attribute__((always_inline)) { return ll_rsrc((const E*)p.hp + (int64_t)tm * BM * p.dp); };
+  auto rsrc_b_of = [&](int tn) __attribute__((always_inline)) {
+    const int n0 = p.col0 + tn * BN;
+    ns_u4v r = ll_rsrc((const E*)p.w + (int64_t)n0 * p.ldw);
+    r[2] = (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)min(BN, p.V - n0) * (uint32_t)p.ldw * 2u));
+    return r;
+  };
+  int tm, tn, tm2 = 0, tn2 = 0;
+  place(ti, tm, tn);
+  bool more = ti + nx < xn;
+  if (more) place(ti + nx, tm2, tn2);
+  ns_u4v ra = rsrc_a_of(tm), rb = rsrc_b_of(tn), ra2 = rsrc_a_of(tm2), rb2 = rsrc_b_of(tn2);
+  const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)smem;
+  auto stage = [&](int tt, int region, int buf) __attribute__((always_inline)) {
+    const bool nxt = tt >= ne;
+    const int k0 = (nxt ? tt - ne : tt) * BK, h = region & 1;
+    const bool isb = region >= 2;
+    const int klen = nxt && !more ? 0 : (isb ? p.d : p.dp) - k0;
+    const ns_u4v rs = isb ? (nxt ? rb2 : rb) : (nxt ? ra2 : ra);
+    const uint32_t dst = lds_base + buf * BUF + region * REGION + wave * 2048;
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+    for (int j = 0; j < 2; ++j) ll_dma16(rs, my_k[j] < klen ? (isb ? b_off[h][j] : a_off[h][j]) : OUT, klen > 0 ? k0 * 2 : 0, dst + j * 1024);
+  };
+  const int fsw = ((lg ^ (l15 >> 1)) & 7) << 4;
+  const int a_rd = (wm * 64 + l15) * 128 + fsw, b_rd = (wn * 32 + l15) * 128 + fsw;
+  f32x4 acc[2][4][2][2];
+  v8 af[4][2], bq[2][2][2];
+  auto read_a = [&](int buf, int ah) __attribute__((always_inline)) {
+    const char* st = smem + buf * BUF + (ah ? RA1 : RA0) * REGION;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float v = acc[ah][mt][b >> 1][b & 1][r];
-            if (edge && n0 + wn * 64 + b * 16 + 4 * lg + r >= p.V) v = -INFINITY;
-            z[b * 4 + r] = v;
-            mx = fmaxf(mx, v);
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) af[mt][ks] = *(const v8*)(st + ((a_rd ^ (ks << 6)) + mt * 2048));
+  };
+  auto read_b = [&](int buf, int bh) __attribute__((always_inline)) {
+    const char* st = smem + buf * BUF + (bh ? RB1 : RB0) * REGION;
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) bq[bh][nt][ks] = *(const v8*)(st + ((b_rd ^ (ks << 6)) + nt * 2048));
+  };
+  auto mma = [&](int ah, int bh) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) acc[ah][mt][bh][nt] = T::mma(bq[bh][nt][ks], af[mt][ks], acc[ah][mt][bh][nt]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  // (FIRST, GRAD only: the 16 stores of the tile before lie between the pieces that the first K tile waits for and those it requests)
+#define LL_RUN(AH, BH, FIRST)                                               \
+  do {                                                                      \
+    if (GRAD && (FIRST)) asm volatile("s_waitcnt vmcnt(24)" ::: "memory");  \
+    else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");                   \
+    LL_BARRIER();                                                           \
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                      \
+    __builtin_amdgcn_sched_barrier(0);                                      \
+    mma(AH, BH);                                                            \
+    __builtin_amdgcn_sched_barrier(0);                                      \
+    LL_BARRIER();                                                           \
+  } while (0)
+#define LL_KTILE(t, b, FIRST)                               \
+  do {                                                      \
+    read_b(b, 0);                                           \
+    __builtin_amdgcn_sched_barrier(0);                      \
+    read_a(b, 0);                                           \
+    stage((t) + 1, RB1, (b) ^ 1);                           \
+    LL_RUN(0, 0, FIRST);                                    \
+    read_b(b, 1);                                           \
+    stage((t) + 1, RA1, (b) ^ 1);                           \
+    LL_RUN(0, 1, FIRST);                                    \
+    read_a(b, 1);                                           \
+    stage((t) + 2, RA0, b);                                 \
+    LL_RUN(1, 1, FIRST);                                    \
+    stage((t) + 2, RB0, b);                                 \
+    LL_RUN(1, 0, FIRST);                                    \
+  } while (0)
+  // row constants of a dz tile, 256 each: La, Lb, the label's column, its cell
+  float* const side = (float*)(smem + LL_SIDE);
+  auto row_consts = [&](int t, int id, float (&c)[4]) __attribute__((always_inline)) {
+    if (GRAD && id < 256) {
+      const int i = t * BM + id;
+      c[0] = p.La[i];
+      c[1] = DUAL ? p.Lb[i] : 0.f;
+      c[2] = c[3] = 0.f;
+      if (FIX) {
+        c[2] = __int_as_float(i < nv ? p.lab[i] : -1);
+        c[3] = i < nv ? __builtin_amdgcn_exp2f(p.zk[i] * p.c1 - c[0]) - p.wlab : 0.f;
+      }
+    }
+  };
+  auto put_consts = [&](int par, int id, const float (&c)[4]) __attribute__((always_inline)) {
+    if (GRAD && id < 256) {
+      side[par * 1024 + id] = c[0];
+      if (DUAL) side[par * 1024 + 256 + id] = c[1];
+      if (FIX) { side[par * 1024 + 512 + id] = c[2]; side[par * 1024 + 768 + id] = c[3]; }
+    }
+  };
+  int par = 0;
+  {
+    float c[4];
+    row_consts(tm, tid, c);
+    put_consts(0, tid, c);
+  }
+  stage(0, RA0, 0); stage(0, RB0, 0); stage(0, RB1, 0); stage(0, RA1, 0);
+  stage(1, RA0, 1); stage(1, RB0, 1);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // (all of it: the first K tile's waits below count a tile's stores, and here are none)
+  while (true) {
+    LL_BARRIER();
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[a][i][b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (wm == 1) LL_BARRIER();        // group 1 runs one barrier interval behind group 0
+    for (int t = 0; t < ne; t += 2) {
+      int first = t;                  // (laundered: hipcc would peel the first K tile, whose copy spills)
+      asm volatile("" : "+s"(first));
+      LL_KTILE(t, 0, first == 0);
+      LL_KTILE(t + 1, 1, false);
+    }
+    if (wm == 0) LL_BARRIER();
+    const int m0 = tm * BM, n0 = p.col0 + tn * BN;
+    // (lane numbers from a laundered copy: hipcc otherwise carries every address of the epilogue through the main loop, and spills)
+    int et = tid;
+    asm volatile("" : "+v"(et));
+    const int el = et & 63, e15 = el & 15, eg = el >> 4;
+    const bool edge = n0 + BN > p.V;
+    if (edge) {                       // columns past the vocabulary: no part of a row
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n0 + wn * 64 + b * 16 + 4 * eg + r >= p.V) {
+#pragma unroll
+            for (int ah = 0; ah < 2; ++ah)
+#pragma unroll
+              for (int mt = 0; mt < 4; ++mt) acc[ah][mt][b >> 1][b & 1][r] = -INFINITY;
           }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float ms = mx == -INFINITY ? 0.f : mx;     // a strip past the vocabulary: sums of zeros
+    }
+    if (!GRAD) {
+      // a el holds 16 of the wave's 64 columns of 8 rows; the row's other lanes are 16 and 32 apart, its other columns in the waves of equal wm
+#pragma unroll
+      for (int ah = 0; ah < 2; ++ah)
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[ah][mt][b >> 1][b & 1][r]);
+          mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+          const float e1 = mx == -INFINITY ? 0.f : ll_ref(mx, p.c1), e2 = DUAL ? (mx == -INFINITY ? 0.f : ll_ref(mx, p.c2)) : 0.f;     // (a strip past the vocabulary)
+          float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float z = acc[ah][mt][b >> 1][b & 1][r];
+              s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(z, p.c1, -e1));
+              if (DUAL) s2 += __builtin_amdgcn_exp2f(__builtin_fmaf(z, p.c2, -e2));
+            }
+          s1 += __shfl_xor(s1, 16, 64);
+          s1 += __shfl_xor(s1, 32, 64);
+          if (DUAL) { s2 += __shfl_xor(s2, 16, 64); s2 += __shfl_xor(s2, 32, 64); }
+          if (eg == 0) {
+            const int row = wm * 128 + ah * 64 + mt * 16 + e15;
+            side[wn * 256 + row] = mx;
+            side[1024 + wn * 256 + row] = s1;
+            if (DUAL) side[2048 + wn * 256 + row] = s2;
+          }
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      LL_BARRIER();
+      if (et < 256) {
+        float mw[4], mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) { mw[w] = side[w * 256 + et]; mx = fmaxf(mx, mw[w]); }
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          s1 += __builtin_amdgcn_exp2f((z[x] - ms) * p.c1);
-          if (DUAL) s2 += __builtin_amdgcn_exp2f((z[x] - ms) * p.c2);
+        for (int w = 0; w < 4; ++w) {
+          s1 += side[1024 + w * 256 + et] * (mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mw[w], p.c1) - ll_ref(mx, p.c1)));
+          if (DUAL) s2 += side[2048 + w * 256 + et] * (mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mw[w], p.c2) - ll_ref(mx, p.c2)));
         }
-        s1 += __shfl_xor(s1, 16, 64);
-        s1 += __shfl_xor(s1, 32, 64);
-        if (DUAL) { s2 += __shfl_xor(s2, 16, 64); s2 += __shfl_xor(s2, 32, 64); }
-        if (lg == 0) {
-          const int row = wm * 128 + ah * 64 + mt * 16 + l15;
-          sm[wn * 256 + row] = mx;
-          sm[1024 + wn * 256 + row] = s1;
-          if (DUAL) sm[2048 + wn * 256 + row] = s2;
+        const int64_t o = (int64_t)tn * p.R + m0 + et;
+        p.pm[o] = mx;
+        p.p1[o] = s1;
+        if (DUAL) p.p2[o] = s2;
+      }
+    } else {
+      float c[4];
+      if (more) row_consts(tm2, et, c);
+      char* const st = smem + BUF + (wave < 4 ? RA1 : RB1) * REGION + (wave & 3) * 4096;       // this wave's 32 rows x 128 B
+      const float* const rc = side + par * 1024;
+      char* const G = (char*)p.G + ((int64_t)(m0 + wm * 128) * p.ldg + tn * BN + wn * 64) * 2;
+#pragma unroll
+      for (int qt = 0; qt < 4; ++qt) {
+        const int ah = qt >> 1;
+#pragma unroll
+        for (int m2 = 0; m2 < 2; ++m2) {
+          const int mt = (qt & 1) * 2 + m2, rl = m2 * 16 + e15, row = wm * 128 + qt * 32 + rl;
+          const float la = rc[row], lb = DUAL ? rc[256 + row] : 0.f;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const f32x4 a = acc[ah][mt][b >> 1][b & 1];
+            float g[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              g[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(a[r], p.c1, -la));
+              if (DUAL) g[r] += __builtin_amdgcn_exp2f(__builtin_fmaf(a[r], p.c2, -lb));
+            }
+            *(ushort4v*)(st + rl * 128 + (((b * 2 + (eg >> 1)) ^ (rl & 7)) << 4) + (eg & 1) * 8) = cvt4<E>(g[0], g[1], g[2], g[3]);
+          }
+        }
+        if (FIX && el < 32) {
+          const int row = wm * 128 + qt * 32 + el, cl = __float_as_int(rc[512 + row]) - (n0 + wn * 64);
+          if (cl >= 0 && cl < 64) *(E*)(st + el * 128 + (((cl >> 3) ^ (el & 7)) << 4) + (cl & 7) * 2) = (E)rc[768 + row];
+        }
+        if (qt == 0 && more) put_consts(par ^ 1, et, c);           // (before the first store: the wait for these loads must not wait for stores)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rl = i * 8 + (el >> 3);
+          const uint4 v = *(const uint4*)(st + rl * 128 + (((el & 7) ^ (rl & 7)) << 4));
+          *(uint4*)(G + (int64_t)(qt * 32 + rl) * p.ldg * 2 + (el & 7) * 16) = v;
         }
       }
-    __syncthreads();
-    if (tid < 256) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, sm[w * 256 + tid]);
-      float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float dm = sm[w * 256 + tid] - mx;
-        s1 += sm[1024 + w * 256 + tid] * __builtin_amdgcn_exp2f(dm * p.c1);
-        if (DUAL) s2 += sm[2048 + w * 256 + tid] * __builtin_amdgcn_exp2f(dm * p.c2);
-      }
-      const int64_t o = (int64_t)tn * p.R + m0 + tid;
-      p.pm[o] = mx;
-      p.p1[o] = s1;
-      if (DUAL) p.p2[o] = s2;
+      par ^= 1;
     }
-    return;
+    if (!more) break;
+    ti += nx;
+    tm = tm2; tn = tn2;
+    ra = ra2; rb = rb2;
+    more = ti + nx < xn;
+    if (more) place(ti + nx, tm2, tn2);
+    ra2 = rsrc_a_of(tm2); rb2 = rsrc_b_of(tn2);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // this wave's staging reads are done: behind the next barrier its 4 KiB are the ring's again
   }
-  // ---- dz of this tile: exponentials in place, one rounding, staged as rows of 256 columns, stored 512 B a row
-#pragma unroll
-  for (int ah = 0; ah < 2; ++ah)
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      const int rl = wm * 128 + ah * 64 + mt * 16 + l15;
-      const float la = p.La[m0 + rl], lb = DUAL ? p.Lb[m0 + rl] : 0.f;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const f32x4 a = acc[ah][mt][b >> 1][b & 1];
-        const int cl = wn * 64 + b * 16 + 4 * lg;
-        float g[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          g[r] = __builtin_amdgcn_exp2f(a[r] * p.c1 - la);
-          if (DUAL) g[r] += __builtin_amdgcn_exp2f(a[r] * p.c2 - lb);
-          if (edge && n0 + cl + r >= p.V) g[r] = 0.f;
-        }
-        *(ushort4v*)(smem + rl * LDH + cl * 2) = cvt4<E>(g[0], g[1], g[2], g[3]);
-      }
-    }
-  __syncthreads();
-  if (FIX) {
-    if (tid < 256) {
-      const int i = m0 + tid;
-      const int c = i < nv ? p.lab[i] - n0 : -1;
-      if (c >= 0 && c < BN) *(E*)(smem + tid * LDH + c * 2) = (E)(__builtin_amdgcn_exp2f(p.zk[i] * p.c1 - p.La[i]) - p.wlab);
-    }
-    __syncthreads();
-  }
-  char* const G = (char*)p.G + ((int64_t)m0 * p.ldg + tn * BN) * 2;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int rl = (tid >> 5) + 16 * i, cg = tid & 31;
-    *(uint4*)(G + (int64_t)rl * p.ldg * 2 + cg * 16) = *(const uint4*)(smem + rl * LDH + cg * 16);
-  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // the last zero chunks land before the workgroup's LDS is given away
+#undef LL_KTILE
+#undef LL_RUN
 }
 
 // ------------------------------------------------------------------------------------------------ rows: log-sum-exp, losses, weights
@@ -471,9 +653,9 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
       const int64_t o = (int64_t)t * p.R + i0 + r;
       const float m = p.pm[o];
       const float nm = fmaxf(mx, m);
-      const float f = __builtin_amdgcn_exp2f((mx - nm) * p.c1), g = __builtin_amdgcn_exp2f((m - nm) * p.c1);
-      s1 = s1 * (mx == -INFINITY ? 0.f : f) + p.p1[o] * g;
-      if (p.dual) s2 = s2 * (mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mx - nm) * p.c2)) + p.p2[o] * __builtin_amdgcn_exp2f((m - nm) * p.c2);
+      s1 = (mx == -INFINITY ? 0.f : s1 * __builtin_amdgcn_exp2f(ll_ref(mx, p.c1) - ll_ref(nm, p.c1))) + p.p1[o] * __builtin_amdgcn_exp2f(ll_ref(m, p.c1) - ll_ref(nm, p.c1));
+      if (p.dual)
+        s2 = (mx == -INFINITY ? 0.f : s2 * __builtin_amdgcn_exp2f(ll_ref(mx, p.c2) - ll_ref(nm, p.c2))) + p.p2[o] * __builtin_amdgcn_exp2f(ll_ref(m, p.c2) - ll_ref(nm, p.c2));
       mx = nm;
     }
     sm[0][r][q] = mx; sm[1][r][q] = s1; sm[2][r][q] = s2;
@@ -484,8 +666,9 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
   const float own = mx;
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-  float s1 = own == -INFINITY ? 0.f : sm[1][r][q] * __builtin_amdgcn_exp2f((own - mx) * p.c1);
-  float s2 = own == -INFINITY ? 0.f : sm[2][r][q] * __builtin_amdgcn_exp2f((own - mx) * p.c2);
+  const float e1 = ll_ref(mx, p.c1), e2 = ll_ref(mx, p.c2);      // the sums are relative to 2^e1, 2^e2
+  float s1 = own == -INFINITY ? 0.f : sm[1][r][q] * __builtin_amdgcn_exp2f(ll_ref(own, p.c1) - e1);
+  float s2 = own == -INFINITY ? 0.f : sm[2][r][q] * __builtin_amdgcn_exp2f(ll_ref(own, p.c2) - e2);
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
   const bool live = i < nv;
@@ -512,14 +695,14 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) ts += __shfl_xor(ts, o, 64);
     const float lt = logf(ts), inv = 1.f / ts;
-    const float ls = logf(p.dual ? s2 : s1);      // lse(z / T) - max / T  (one softmax: it is the one at T)
+    const float ls = log2f(p.dual ? s2 : s1);     // (one softmax: it is the one at T)
     float kl = 0.f;
     for (int e = q; e < p.k; e += 16) {
       float pr = 0.f;
       if (soft && ti[e] >= 0 && ti[e] < p.V) {
         const float lp = tv[e] * p.invT - tm;
         pr = expf(lp) * inv;
-        if (pr > 0.f) kl += pr * ((lp - lt) - ((logit(e, ti[e]) - mx) * p.invT - ls));
+        if (pr > 0.f) kl += pr * ((lp - lt) - (__builtin_fmaf(logit(e, ti[e]), p.c2, -e2) - ls) * LN2);
       }
       p.pk[(int64_t)i * p.k + e] = pr;
     }
@@ -528,11 +711,11 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
     if (soft) loss += p.kd * kl;
   }
   if (q == 0) {
-    if (!p.soft_only) loss += p.w1 * ((mx - logit(p.k, p.lab[i])) + logf(s1));
-    const float l1 = mx * p.c1 + log2f(s1);
+    if (!p.soft_only) loss -= p.w1 * (__builtin_fmaf(logit(p.k, p.lab[i]), p.c1, -e1) - log2f(s1)) * LN2;      // (lse - z in units of ln 2)
+    const float l1 = e1 + log2f(s1);
     if (p.dual) {
       p.La[i] = l1 - p.lw1;
-      p.Lb[i] = soft ? mx * p.c2 + log2f(s2) - p.lw2 : INFINITY;
+      p.Lb[i] = soft ? e2 + log2f(s2) - p.lw2 : INFINITY;
     } else if (p.k > 0) {
       // one softmax carries both weights (T = 1), or the soft weight alone
       const float w = (p.soft_only ? 0.f : p.w1) + (soft ? p.w2 : 0.f);
@@ -670,7 +853,7 @@ __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict_
                                                         const int* __restrict__ nvalid, const float* __restrict__ loss_scale, float unscale, E* __restrict__ dh, int64_t lddh) {
   typedef E e4 __attribute__((ext_vector_type(4)));
   __shared__ f32x4 sm[16][16];
-  const int groups = splits >= 16 ? 16 : splits >= 4 ? 4 : 1;             // slab groups; the rest of the 16 lanes-of-16 take further column blocks
+  const int groups = splits >= 64 ? 16 : splits >= 32 ? 4 : 1;             // slab groups; the rest of the 16 lanes-of-16 take further column blocks
   const int sub = threadIdx.x >> 4, g = sub & (groups - 1), blk = sub / groups;
   const int per = (d + 63) / 64, nblk = 16 / groups;
   const int64_t x = (int64_t)blockIdx.x * nblk + blk;
@@ -698,7 +881,7 @@ __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict_
 }
 template <class E> void launch_dh_out(const float* slab, int splits, int R, int d, int rows, const int* inv, const int* nvalid, const float* loss_scale, float unscale, E* dh,
                                       int64_t lddh, hipStream_t st) {
-  const int nblk = splits >= 16 ? 1 : splits >= 4 ? 4 : 16;
+  const int nblk = splits >= 64 ? 1 : splits >= 32 ? 4 : 16;
   const int64_t items = (int64_t)rows * ((d + 63) / 64);
   hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)((items + nblk - 1) / nblk)), dim3(256), 0, st, slab, splits, R, d, rows, inv, nvalid, loss_scale, unscale, dh, lddh);
 }
@@ -899,14 +1082,14 @@ __global__ __launch_bounds__(512) void ll_few_logits_kernel(const FewArgs p) {
     }
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float ms = mx == -INFINITY ? 0.f : mx;
+    const float e1 = mx == -INFINITY ? 0.f : ll_ref(mx, p.c1), e2 = mx == -INFINITY ? 0.f : ll_ref(mx, p.c2);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int f = 0; f < 2; ++f)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s1 += __builtin_amdgcn_exp2f((acc[f][m][e] - ms) * p.c1);
-        if (DUAL) s2 += __builtin_amdgcn_exp2f((acc[f][m][e] - ms) * p.c2);
+        s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][m][e], p.c1, -e1));
+        if (DUAL) s2 += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][m][e], p.c2, -e2));
       }
     s1 += __shfl_xor(s1, 16, 64);
     s1 += __shfl_xor(s1, 32, 64);
@@ -921,9 +1104,10 @@ __global__ __launch_bounds__(512) void ll_few_logits_kernel(const FewArgs p) {
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      const float dm = sm[0][w][tid] - mx;
-      s1 += sm[1][w][tid] * __builtin_amdgcn_exp2f(dm * p.c1);
-      if (DUAL) s2 += sm[2][w][tid] * __builtin_amdgcn_exp2f(dm * p.c2);
+      const float m = sm[0][w][tid];
+      if (m == -INFINITY) continue;
+      s1 += sm[1][w][tid] * __builtin_amdgcn_exp2f(ll_ref(m, p.c1) - ll_ref(mx, p.c1));
+      if (DUAL) s2 += sm[2][w][tid] * __builtin_amdgcn_exp2f(ll_ref(m, p.c2) - ll_ref(mx, p.c2));
     }
     const int64_t o = (int64_t)blockIdx.x * p.R + tid;
     p.pm[o] = mx;
@@ -963,7 +1147,7 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
     off[j] = n0 + r < p.V ? (uint32_t)(r * (int)p.ldw + col[j]) * 2u : OUT;
   }
   auto stage = [&](int c) __attribute__((always_inline)) {
-    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_base + (c % 3) * FW_BYTES + wave * 4096);
+    const uint32_t dst = lds_base + (c % 3) * FW_BYTES + wave * 4096;
 #pragma unroll
     for (int j = 0; j < 4; ++j) ll_dma16(rsrc, c < c_end && c * 64 + col[j] < p.d ? off[j] : OUT, c < c_end ? c * 128 : 0, dst + j * 1024);
   };
@@ -1229,19 +1413,20 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   a.c1 = c1; a.c2 = c2;
   a.pm = (float*)(ws + p.pm); a.p1 = (float*)(ws + p.p1); a.p2 = (float*)(ws + p.p2);
   a.La = La; a.Lb = Lb; a.G = ws + p.G; a.ldg = p.piece_tiles * BN; a.lab = lab; a.zk = zk; a.wlab = w1 * up;
-  const dim3 all(p.R / BM * p.tiles_n);
-  if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, false, true, false>), all, dim3(NTH), LL_LDS, st, a);
-  else hipLaunchKernelGGL((ll_logits_kernel<T, false, false, false>), all, dim3(NTH), LL_LDS, st, a);
+  auto grid_of = [&](int tiles_n) { const int64_t t = (int64_t)(p.R / BM) * tiles_n; return dim3((unsigned)(t < 256 ? t : 256)); };
+  const dim3 all = grid_of(p.tiles_n);
+  if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, false, true, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
+  else hipLaunchKernelGGL((ll_logits_kernel<T, false, false, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
   hipLaunchKernelGGL(ll_rows_kernel<256>, dim3(p.R / 16), dim3(256), 0, st, r);
   hipLaunchKernelGGL(ll_mean_kernel, dim3(1), dim3(1024), 0, st, ploss, d->nvalid_dev, d->loss_dev);
   if (grad) {
     for (int pc = 0; pc < p.pieces; ++pc) {
       a.col0 = pc * p.piece_tiles * BN;
       a.tiles_n = p.tiles_n - pc * p.piece_tiles < p.piece_tiles ? p.tiles_n - pc * p.piece_tiles : p.piece_tiles;
-      const dim3 grid(p.R / BM * a.tiles_n);
-      if (d->k == 0) hipLaunchKernelGGL((ll_logits_kernel<T, true, false, true>), grid, dim3(NTH), LL_LDS, st, a);
-      else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, true, true, false>), grid, dim3(NTH), LL_LDS, st, a);
-      else hipLaunchKernelGGL((ll_logits_kernel<T, true, false, false>), grid, dim3(NTH), LL_LDS, st, a);
+      const dim3 grid = grid_of(a.tiles_n);
+      if (d->k == 0) hipLaunchKernelGGL((ll_logits_kernel<T, true, false, true>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
+      else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, true, true, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
+      else hipLaunchKernelGGL((ll_logits_kernel<T, true, false, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
       if (d->k > 0)
         hipLaunchKernelGGL(ll_cells_kernel<E>, dim3(p.R / 4), dim3(256), 0, st, d->nvalid_dev, order, lab, d->top_idx, d->ld_top, d->k, zk, pk, La, dual ? Lb : nullptr,
                            a.c1, a.c2, w1 * up, w2 * up, a.col0, a.tiles_n * BN, d->vocab, (E*)a.G, a.ldg);
