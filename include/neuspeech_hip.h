@@ -358,7 +358,8 @@ typedef enum { NS_F16 = 0, NS_BF16 = 1, NS_F32 = 2 } ns_dtype;
  *  - workspace: ns_linear_ce_workspace_bytes(d) bytes (host-only call: sizes, k,
  *    alpha, temperature, ldw and whether dh / dw are set decide), 16-B aligned,
  *    free again when the call's work has run; it holds at most 256 MiB of dz at a
- *    time (one piece of the vocabulary) plus fp32 partial sums of dh.
+ *    time (one piece of the vocabulary) and fp32 partial sums of dh (128 MiB, or 4 d bytes
+ *    a row where that is more).
  *  - the same inputs give the same bits (no atomics).  dh, dw must not overlap h, w. */
 typedef struct {
   const void *h, *w;

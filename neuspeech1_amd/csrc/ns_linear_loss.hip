@@ -71,6 +71,29 @@ __device__ __forceinline__ ns_u4v ll_rsrc(const void* base) {
   return ns_u4v{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)), OUT, 0x00020000u};
 }
 
+// reductions over the four lanes that are 16 apart (equal lane & 15): the swap instructions exchange 16-lane rows / 32-lane halves of two copies
+__device__ __forceinline__ void ll_swap(float v, bool by32, float& a, float& b) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  const u2 r = by32 ? __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false)
+                    : __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  a = __uint_as_float(r[0]);
+  b = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float ll_max4(float v) {
+  float a, b;
+  ll_swap(v, false, a, b);
+  v = fmaxf(a, b);
+  ll_swap(v, true, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float ll_sum4(float v) {
+  float a, b;
+  ll_swap(v, false, a, b);
+  v = a + b;
+  ll_swap(v, true, a, b);
+  return a + b;
+}
+
 #define LL_BARRIER()                            \
   do {                                          \
     asm volatile("" ::: "memory");              \
@@ -241,39 +264,39 @@ __device__ __forceinline__ int ll_pos(int total) {
 // order[i] = i-th row with a label, inv[row] = its place or -1, *nvalid; ignored rows get their zero loss here
 __global__ __launch_bounds__(1024) void ll_compact_kernel(const int64_t* __restrict__ labels, int rows, int V, int* __restrict__ order,
                                                           int* __restrict__ inv, int* __restrict__ lab, float* __restrict__ row_loss, int* __restrict__ nvalid) {
-  __shared__ int sh[17];
+  __shared__ int sh[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int base = 0;
-  for (int r0 = 0; r0 < rows; r0 += 1024) {
-    const int row = r0 + tid;
-    const int64_t l = row < rows ? labels[row] : -1;
-    const bool ok = l >= 0 && l < V;
-    const uint64_t m = __ballot(ok);
-    if (lane == 0) sh[wave] = __popcll(m);
-    __syncthreads();
-    int before = base, all = 0;
-    for (int w = 0; w < 16; ++w) {
-      if (w < wave) before += sh[w];
-      all += sh[w];
-    }
-    const int at = before + __popcll(m & ((1ull << lane) - 1ull));
-    if (row < rows) {
-      inv[row] = ok ? at : -1;
-      if (ok) { order[at] = row; lab[at] = (int)l; }
-      else row_loss[row] = 0.f;
-    }
-    base += all;
-    __syncthreads();
+  const int per = (rows + 1023) / 1024, r0 = tid * per, r1 = min(rows, r0 + per);
+  int n = 0;
+#pragma unroll 4
+  for (int r = r0; r < r1; ++r) n += labels[r] >= 0 && labels[r] < V;
+  int at = n;                                     // inclusive scan over the wave, then over the waves
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_up(at, o, 64);
+    at += lane >= o ? t : 0;
   }
-  if (tid == 0) *nvalid = base;
+  if (lane == 63) sh[wave] = at;
+  __syncthreads();
+  at -= n;
+  for (int w = 0; w < wave; ++w) at += sh[w];
+#pragma unroll 4
+  for (int r = r0; r < r1; ++r) {
+    const int64_t l = labels[r];
+    const bool ok = l >= 0 && l < V;
+    inv[r] = ok ? at : -1;
+    if (ok) { order[at] = r; lab[at] = (int)l; ++at; }
+    else row_loss[r] = 0.f;
+  }
+  if (tid == 1023) *nvalid = at;
 }
 
-// hp[i] = h[order[i]], columns [d, dp) and rows [nvalid, next multiple of 256) zero; zk[i][e] = h_i . W[token e], e = 0 .. k - 1 the teacher's
-// list, e = k the label.  One wave per row; products in fp32, added over the lanes' partial sums.
+// hp[i] = h[order[i]], columns [d, dp) and rows [nvalid, next multiple of 256) zero; without a list also zk[i] = h_i . W[label_i] (fp32 products, added
+// over the lanes' partial sums).  One wave per row.
 template <class T>
-__global__ __launch_bounds__(256) void ll_pack_kernel(const void* __restrict__ h_, int64_t ldh, const void* __restrict__ w_, int64_t ldw, int d, int dp, int V,
-                                                      const int* __restrict__ order, const int* __restrict__ lab, const int32_t* __restrict__ top_idx,
-                                                      int64_t ld_top, int k, const int* __restrict__ nvalid, void* __restrict__ hp_, float* __restrict__ zk) {
+__global__ __launch_bounds__(256) void ll_pack_kernel(const void* __restrict__ h_, int64_t ldh, const void* __restrict__ w_, int64_t ldw, int d, int dp,
+                                                      const int* __restrict__ order, const int* __restrict__ lab, int k, const int* __restrict__ nvalid,
+                                                      void* __restrict__ hp_, float* __restrict__ zk) {
   typedef typename T::v8 v8;
   typedef typename T::e E;
   const int lane = threadIdx.x & 63, i = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -284,22 +307,50 @@ __global__ __launch_bounds__(256) void ll_pack_kernel(const void* __restrict__ h
     for (int c = lane * 8; c < dp; c += 512) *(uint4*)(dst + c) = make_uint4(0, 0, 0, 0);
     return;
   }
+  const E* const src = (const E*)h_ + order[i] * ldh;
+  const E* const wr = (const E*)w_ + lab[i] * ldw;
+  float s = 0.f;
+  for (int c = lane * 8; c < dp; c += 512) {
+    const uint4 v = c < d ? *(const uint4*)(src + c) : make_uint4(0, 0, 0, 0);
+    *(uint4*)(dst + c) = v;
+    if (k == 0 && c < d) {
+      const v8 a = __builtin_bit_cast(v8, v), b = *(const v8*)(wr + c);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) s += (float)a[x] * (float)b[x];
+    }
+  }
+  if (k > 0) return;
+  s = ns_wave_sum(s);
+  if (lane == 0) zk[i] = s;
+}
+
+// zk[i][e] = h_i . W[token e], e = 0 .. k - 1 the teacher's list, e = k the label: a workgroup per row, 16 lanes per entry (256 B of W a step, 16 entries
+// side by side; one entry after the other on a wave, 64 entries took 77 us for 1434 rows at d = 512, this 24)
+template <class T>
+__global__ __launch_bounds__(256) void ll_gather_kernel(const void* __restrict__ hp_, int dp, const void* __restrict__ w_, int64_t ldw, int d, int V,
+                                                        const int* __restrict__ order, const int* __restrict__ lab, const int32_t* __restrict__ top_idx,
+                                                        int64_t ld_top, int k, const int* __restrict__ nvalid, float* __restrict__ zk) {
+  typedef typename T::v8 v8;
+  typedef typename T::e E;
+  const int i = blockIdx.x, l = threadIdx.x & 15;
+  if (i >= *nvalid) return;
+  const E* const src = (const E*)hp_ + (int64_t)i * dp;
   const int row = order[i];
-  const E* const src = (const E*)h_ + row * ldh;
-  for (int c = lane * 8; c < dp; c += 512) *(uint4*)(dst + c) = c < d ? *(const uint4*)(src + c) : make_uint4(0, 0, 0, 0);
-  for (int e = 0; e <= k; ++e) {
+  for (int e = threadIdx.x >> 4; e <= k; e += 16) {
     const int tok = e == k ? lab[i] : top_idx[row * ld_top + e];
     float s = 0.f;
     if (tok >= 0 && tok < V) {
       const E* const wr = (const E*)w_ + tok * ldw;
-      for (int c = lane * 8; c < d; c += 512) {
+#pragma unroll 4
+      for (int c = l * 8; c < d; c += 128) {
         const v8 a = *(const v8*)(src + c), b = *(const v8*)(wr + c);
 #pragma unroll
         for (int x = 0; x < 8; ++x) s += (float)a[x] * (float)b[x];
       }
     }
-    s = ns_wave_sum(s);
-    if (lane == 0) zk[(int64_t)i * (k + 1) + e] = s;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (l == 0) zk[(int64_t)i * (k + 1) + e] = s;
   }
 }
 
@@ -476,7 +527,24 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
       if (FIX) { side[par * 1024 + 512 + id] = c[2]; side[par * 1024 + 768 + id] = c[3]; }
     }
   };
-  int par = 0;
+  // statistics of a finished tile from its four column strips, by the wave group that waits at a tile's start anyway
+  auto join = [&](int jm, int jn) __attribute__((always_inline)) {
+    const int r = tid & 255;
+    float mw[4], mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) { mw[w] = side[w * 256 + r]; mx = fmaxf(mx, mw[w]); }
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      s1 += side[1024 + w * 256 + r] * (mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mw[w], p.c1) - ll_ref(mx, p.c1)));
+      if (DUAL) s2 += side[2048 + w * 256 + r] * (mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mw[w], p.c2) - ll_ref(mx, p.c2)));
+    }
+    const int64_t o = (int64_t)jn * p.R + jm * BM + r;
+    p.pm[o] = mx;
+    p.p1[o] = s1;
+    if (DUAL) p.p2[o] = s2;
+  };
+  int par = 0, jm = -1, jn = 0;
   {
     float c[4];
     row_consts(tm, tid, c);
@@ -495,7 +563,10 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int j = 0; j < 2; ++j) acc[a][i][b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (wm == 1) LL_BARRIER();        // group 1 runs one barrier interval behind group 0
+    if (wm == 1) {                    // group 1 runs one barrier interval behind group 0
+      if (!GRAD && jm >= 0) join(jm, jn);
+      LL_BARRIER();
+    }
     for (int t = 0; t < ne; t += 2) {
       int first = t;                  // (laundered: hipcc would peel the first K tile, whose copy spills)
       asm volatile("" : "+s"(first));
@@ -532,8 +603,7 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
           for (int b = 0; b < 4; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[ah][mt][b >> 1][b & 1][r]);
-          mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+          mx = ll_max4(mx);
           const float e1 = mx == -INFINITY ? 0.f : ll_ref(mx, p.c1), e2 = DUAL ? (mx == -INFINITY ? 0.f : ll_ref(mx, p.c2)) : 0.f;     // (a strip past the vocabulary)
           float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -544,9 +614,8 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
               s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(z, p.c1, -e1));
               if (DUAL) s2 += __builtin_amdgcn_exp2f(__builtin_fmaf(z, p.c2, -e2));
             }
-          s1 += __shfl_xor(s1, 16, 64);
-          s1 += __shfl_xor(s1, 32, 64);
-          if (DUAL) { s2 += __shfl_xor(s2, 16, 64); s2 += __shfl_xor(s2, 32, 64); }
+          s1 = ll_sum4(s1);
+          if (DUAL) s2 = ll_sum4(s2);
           if (eg == 0) {
             const int row = wm * 128 + ah * 64 + mt * 16 + e15;
             side[wn * 256 + row] = mx;
@@ -554,23 +623,6 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
             if (DUAL) side[2048 + wn * 256 + row] = s2;
           }
         }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      LL_BARRIER();
-      if (et < 256) {
-        float mw[4], mx = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) { mw[w] = side[w * 256 + et]; mx = fmaxf(mx, mw[w]); }
-        float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          s1 += side[1024 + w * 256 + et] * (mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mw[w], p.c1) - ll_ref(mx, p.c1)));
-          if (DUAL) s2 += side[2048 + w * 256 + et] * (mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mw[w], p.c2) - ll_ref(mx, p.c2)));
-        }
-        const int64_t o = (int64_t)tn * p.R + m0 + et;
-        p.pm[o] = mx;
-        p.p1[o] = s1;
-        if (DUAL) p.p2[o] = s2;
-      }
     } else {
       float c[4];
       if (more) row_consts(tm2, et, c);
@@ -610,6 +662,7 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
       }
       par ^= 1;
     }
+    jm = tm; jn = tn;
     if (!more) break;
     ti += nx;
     tm = tm2; tn = tn2;
@@ -618,6 +671,11 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
     if (more) place(ti + nx, tm2, tn2);
     ra2 = rsrc_a_of(tm2); rb2 = rsrc_b_of(tn2);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // this wave's staging reads are done: behind the next barrier its 4 KiB are the ring's again
+  }
+  if (!GRAD) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    LL_BARRIER();
+    if (wm == 1) join(jm, jn);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // the last zero chunks land before the workgroup's LDS is given away
 #undef LL_KTILE
@@ -737,18 +795,36 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
   }
 }
 
-__global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__ packed_loss, const int* __restrict__ nvalid, float* __restrict__ loss) {
+// How many ways dh's product over one piece of the vocabulary (kt K tiles of 64) is split for `tiles` output tiles: the number that ends soonest when 256
+// CUs take (tile, split) pairs in rounds, a pair costing its K tiles and about LL_PAIR more (ring start, fp32 tile to and from its slab).  At most LL_PAIRS
+// pairs, eight K tiles each at least.  Depends on sizes and the number of rows with a label alone: the same inputs are added in the same order.
+constexpr int LL_PAIRS = 512, LL_PAIR = 6;
+__host__ __device__ inline int ll_cost(int tiles, int kt, int s) { return (tiles * s + 255) / 256 * ((kt + s - 1) / s + LL_PAIR); }
+__host__ __device__ inline int ll_most_splits(int tiles, int kt) {
+  const int a = tiles > 0 ? LL_PAIRS / tiles : 1, b = kt / 8, m = a < b ? a : b;
+  return m < 1 ? 1 : m > 1024 ? 1024 : m;
+}
+
+// the loss, and *splits for dh
+__global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__ packed_loss, const int* __restrict__ nvalid, float* __restrict__ loss, int tiles_d, int kt,
+                                                       int* __restrict__ splits) {
   __shared__ float sh[16];
+  __shared__ unsigned best[16];
   const int nv = *nvalid;
   float s = 0.f;
   for (int i = threadIdx.x; i < nv; i += 1024) s += packed_loss[i];
   s = ns_wave_sum(s);
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+  const int tiles = (nv + BM - 1) / BM * tiles_d, n = threadIdx.x + 1;
+  unsigned c = n <= ll_most_splits(tiles, kt) ? (unsigned)min(ll_cost(tiles, kt, n), 0x1FFFFF) << 11 | (unsigned)n : ~0u;      // (a tie: the fewest)
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) c = min(c, (unsigned)__shfl_xor((int)c, o, 64));
+  if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = s; best[threadIdx.x >> 6] = c; }
   __syncthreads();
   if (threadIdx.x == 0) {
     s = 0.f;
-    for (int w = 0; w < 16; ++w) s += sh[w];
+    for (int w = 0; w < 16; ++w) { s += sh[w]; c = min(c, best[w]); }
     *loss = s / (float)max(nv, 1);
+    *splits = (int)(c & 2047);
   }
 }
 
@@ -794,9 +870,9 @@ __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ n
 // ------------------------------------------------------------------------------------------------ dh += dz W,  dW = dz^T h
 struct DhArgs {
   const void* G; const void* w; int64_t ldw;
-  int ldg, col0, cols, V, d, R, splits, chunk, add;
-  const int* nvalid;
-  float* slab;                      // (splits, R, d)
+  int ldg, col0, cols, V, d, kt, add;
+  const int *nvalid, *splits;
+  float* slab;                      // (splits, tiles, 256, 256)
 };
 
 template <class T>
@@ -804,20 +880,20 @@ __global__ __launch_bounds__(NTH) void ll_dh_kernel(const DhArgs p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef typename T::e E;
   const int tiles_m = (*p.nvalid + BM - 1) / BM, tiles_d = (p.d + BN - 1) / BN;
-  const int tiles = tiles_m * tiles_d;
-  const int pos = ll_pos(tiles * p.splits);
+  const int tiles = tiles_m * tiles_d, splits = *p.splits;
+  const int pos = ll_pos(tiles * splits);
   if (pos < 0) return;
   const int split = pos / tiles, t = pos - split * tiles;
   const int tm = t / tiles_d, td = t - tm * tiles_d;
   const int m0 = tm * BM, n0 = td * BN;
-  const int k0 = split * p.chunk, kn = min(p.chunk, p.cols - k0);          // (a split past the end leaves its zeros)
+  const int chunk = (p.kt + splits - 1) / splits * BK, k0 = split * chunk, kn = min(chunk, p.cols - k0);          // (a split past the end leaves its zeros)
   f32x4 acc[2][4][2][2];
   ll_tile<T, true, false>(acc, smem, (const E*)p.G + (int64_t)m0 * p.ldg + k0, p.ldg, kn,
                           (const E*)p.w + (int64_t)(p.col0 + k0) * p.ldw + n0, (int)p.ldw, min(kn, p.V - p.col0 - k0), min(BN, p.d - n0), max(kn, 0));
   const int lane = threadIdx.x & 63, l15 = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 2, wn = wave & 3;
-  float* const out = p.slab + ((int64_t)split * p.R + m0) * p.d + n0;
+  float* const out = p.slab + (int64_t)pos * (BM * BN);
   // eight 16-B loads in flight before the first addition (a load, an addition and a store at a time cost a memory latency each)
 #pragma unroll
   for (int ah = 0; ah < 2; ++ah)
@@ -830,7 +906,7 @@ __global__ __launch_bounds__(NTH) void ll_dh_kernel(const DhArgs p) {
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
             const int rl = wm * 128 + ah * 64 + (mp + m) * 16 + l15, cl = wn * 64 + b * 16 + 4 * lg;
-            if (n0 + cl < p.d) old[m][b] = *(const f32x4*)(out + (int64_t)rl * p.d + cl);
+            old[m][b] = *(const f32x4*)(out + rl * BN + cl);
           }
       }
 #pragma unroll
@@ -838,22 +914,22 @@ __global__ __launch_bounds__(NTH) void ll_dh_kernel(const DhArgs p) {
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const int rl = wm * 128 + ah * 64 + (mp + m) * 16 + l15, cl = wn * 64 + b * 16 + 4 * lg;
-          if (n0 + cl >= p.d) continue;
           f32x4 v = acc[ah][mp + m][b >> 1][b & 1];
           if (p.add) v += old[m][b];
-          *(f32x4*)(out + (int64_t)rl * p.d + cl) = v;
+          *(f32x4*)(out + rl * BN + cl) = v;
         }
     }
 }
 
 // dh[row] = g 2^-s sum of the slabs (in their order), zero for a row without a label.  A workgroup takes 64 columns of a row with 16 threads of 4 columns,
 // and 16 groups of slabs side by side: with one token and 203 slabs a single chain of loads took 28 us
+// (R > 0: slabs of (R, d); R = 0: slabs of 256 x 256 tiles, their number read from splits_dev.)
 template <class E>
-__global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict__ slab, int splits, int R, int d, int rows, const int* __restrict__ inv,
+__global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict__ slab, int groups, int splits, const int* __restrict__ splits_dev, int R, int d, int rows, const int* __restrict__ inv,
                                                         const int* __restrict__ nvalid, const float* __restrict__ loss_scale, float unscale, E* __restrict__ dh, int64_t lddh) {
   typedef E e4 __attribute__((ext_vector_type(4)));
   __shared__ f32x4 sm[16][16];
-  const int groups = splits >= 64 ? 16 : splits >= 32 ? 4 : 1;             // slab groups; the rest of the 16 lanes-of-16 take further column blocks
+  // `groups` slab groups; the rest of the 16 lanes-of-16 take further column blocks
   const int sub = threadIdx.x >> 4, g = sub & (groups - 1), blk = sub / groups;
   const int per = (d + 63) / 64, nblk = 16 / groups;
   const int64_t x = (int64_t)blockIdx.x * nblk + blk;
@@ -862,9 +938,13 @@ __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict_
   const int i = in ? inv[row] : -1;
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
   if (i >= 0) {
+    if (splits_dev) splits = *splits_dev;
     const int per_g = (splits + groups - 1) / groups, s1 = min(splits, (g + 1) * per_g);
+    const int tiles_d = (d + BN - 1) / BN, tiles = (*nvalid + BM - 1) / BM * tiles_d;
+    const int64_t at = R > 0 ? (int64_t)i * d + c : ((int64_t)(i / BM * tiles_d + c / BN) * BM + i % BM) * BN + c % BN;
+    const int64_t step = R > 0 ? (int64_t)R * d : (int64_t)tiles * BM * BN;
 #pragma unroll 4
-    for (int s = g * per_g; s < s1; ++s) a += *(const f32x4*)(slab + ((int64_t)s * R + i) * d + c);
+    for (int s = g * per_g; s < s1; ++s) a += *(const f32x4*)(slab + s * step + at);
   }
   if (groups > 1) {
     sm[sub][threadIdx.x & 15] = a;
@@ -879,11 +959,12 @@ __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict_
   for (int e = 0; e < 4; ++e) o[e] = (E)(i < 0 ? 0.f : a[e] * gs);
   *(e4*)(dh + row * lddh + c) = o;
 }
-template <class E> void launch_dh_out(const float* slab, int splits, int R, int d, int rows, const int* inv, const int* nvalid, const float* loss_scale, float unscale, E* dh,
+template <class E> void launch_dh_out(const float* slab, int groups, int splits, const int* splits_dev, int R, int d, int rows, const int* inv, const int* nvalid, const float* loss_scale, float unscale, E* dh,
                                       int64_t lddh, hipStream_t st) {
-  const int nblk = splits >= 64 ? 1 : splits >= 32 ? 4 : 16;
+  const int nblk = 16 / groups;
   const int64_t items = (int64_t)rows * ((d + 63) / 64);
-  hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)((items + nblk - 1) / nblk)), dim3(256), 0, st, slab, splits, R, d, rows, inv, nvalid, loss_scale, unscale, dh, lddh);
+  hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)((items + nblk - 1) / nblk)), dim3(256), 0, st, slab, groups, splits, splits_dev, R, d, rows, inv, nvalid,
+                     loss_scale, unscale, dh, lddh);
 }
 
 struct DwArgs {
@@ -1080,8 +1161,7 @@ __global__ __launch_bounds__(512) void ll_few_logits_kernel(const FewArgs p) {
         mx = fmaxf(mx, acc[f][m][e]);
       }
     }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    mx = ll_max4(mx);
     const float e1 = mx == -INFINITY ? 0.f : ll_ref(mx, p.c1), e2 = mx == -INFINITY ? 0.f : ll_ref(mx, p.c2);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -1091,9 +1171,8 @@ __global__ __launch_bounds__(512) void ll_few_logits_kernel(const FewArgs p) {
         s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][m][e], p.c1, -e1));
         if (DUAL) s2 += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][m][e], p.c2, -e2));
       }
-    s1 += __shfl_xor(s1, 16, 64);
-    s1 += __shfl_xor(s1, 32, 64);
-    if (DUAL) { s2 += __shfl_xor(s2, 16, 64); s2 += __shfl_xor(s2, 32, 64); }
+    s1 = ll_sum4(s1);
+    if (DUAL) s2 = ll_sum4(s2);
     if (lg == 0) { sm[0][wave][r] = mx; sm[1][wave][r] = s1; if (DUAL) sm[2][wave][r] = s2; }
   }
   __syncthreads();
@@ -1286,8 +1365,8 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
   int few;                                    // 0, or MT of the few-row path
-  int R, dp, dt, tiles_n, piece_tiles, pieces, splits, chunk;
-  size_t order, inv, lab, hp, hT, zk, pk, pm, p1, p2, La, Lb, ploss, G, slab, total;
+  int R, dp, dt, tiles_n, piece_tiles, pieces, pairs;
+  size_t splits_at, order, inv, lab, hp, hT, zk, pk, pm, p1, p2, La, Lb, ploss, G, slab, total;
 };
 
 bool dual_of(const ns_linear_ce_desc* d) { return d->k > 0 && d->alpha > 0.f && d->alpha < 1.f && d->temperature != 1.f; }
@@ -1308,15 +1387,14 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   p.pieces = (int)((p.tiles_n + most - 1) / most);
   p.piece_tiles = (p.tiles_n + p.pieces - 1) / p.pieces;
   p.pieces = (p.tiles_n + p.piece_tiles - 1) / p.piece_tiles;
-  // dh: (row tile, column tile, split of the piece's vocabulary): about one workgroup per CU, splits of 512 tokens at least
-  const int tiles = (p.R / BM) * ((d->d + BN - 1) / BN);
-  p.splits = 256 / tiles;
-  if (p.splits < 1) p.splits = 1;
-  if (p.splits > p.piece_tiles / 2) p.splits = p.piece_tiles / 2 > 0 ? p.piece_tiles / 2 : 1;
-  p.chunk = ((p.piece_tiles * BN + p.splits - 1) / p.splits + BK - 1) / BK * BK;
-  if (p.few) { p.R = LL_FEW_ROWS; p.splits = p.tiles_n; }
+  // dh's slabs: one 256 x 256 fp32 tile per (output tile, split of the piece's vocabulary)
+  const int tiles = (p.R / BM) * ((d->d + BN - 1) / BN), kt = p.piece_tiles * (BN / BK);
+  p.pairs = tiles;                                 // (fewer live tiles may be split more ways: at most LL_PAIRS pairs, or kt / 8 a tile)
+  if (p.pairs < LL_PAIRS) p.pairs = (int64_t)tiles * (kt / 8) < LL_PAIRS ? (tiles * (kt / 8) > tiles ? tiles * (kt / 8) : tiles) : LL_PAIRS;
+  if (p.few) p.R = LL_FEW_ROWS;
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
+  p.splits_at = take(4);
   p.order = take((size_t)d->rows * 4);
   p.inv = take((size_t)d->rows * 4);
   p.lab = take((size_t)d->rows * 4);
@@ -1331,7 +1409,7 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   p.Lb = take((size_t)p.R * 4);
   p.ploss = take((size_t)p.R * 4);
   p.G = grad && !p.few ? take((size_t)p.R * p.piece_tiles * BN * 2) : 0;
-  p.slab = d->dh ? take((size_t)p.splits * (p.few ? 16 * p.few : p.R) * d->d * 4) : 0;
+  p.slab = d->dh ? take(p.few ? (size_t)p.tiles_n * 16 * p.few * d->d * 4 : (size_t)p.pairs * BM * BN * 4) : 0;
   p.total = at;
   return p;
 }
@@ -1358,7 +1436,7 @@ int few_launch(const ns_linear_ce_desc* d, const FewArgs& f, const RowArgs& r, b
     gy = (chunks + (chunks + gy - 1) / gy - 1) / ((chunks + gy - 1) / gy);
     if (dual) hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, true>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
     else hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, false>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
-    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n, 16 * MT, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, st);
+    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n >= 64 ? 16 : f.tiles_n >= 16 ? 4 : 1, f.tiles_n, nullptr, 16 * MT, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;
@@ -1369,6 +1447,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   typedef typename T::e E;
   char* const ws = (char*)d->workspace;
   int *order = (int*)(ws + p.order), *inv = (int*)(ws + p.inv), *lab = (int*)(ws + p.lab);
+  int* const splits = (int*)(ws + p.splits_at);
   float *zk = (float*)(ws + p.zk), *pk = (float*)(ws + p.pk), *La = (float*)(ws + p.La), *Lb = (float*)(ws + p.Lb), *ploss = (float*)(ws + p.ploss);
   const bool dual = dual_of(d), soft_only = d->k > 0 && d->alpha == 1.f, grad = d->dh || d->dw;
   const float alpha = d->k > 0 ? d->alpha : 0.f, T_ = d->k > 0 ? d->temperature : 1.f;
@@ -1404,8 +1483,10 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
     return p.few == 1 ? few_launch<T, 1>(d, f, r, dual, st) : p.few == 2 ? few_launch<T, 2>(d, f, r, dual, st) : few_launch<T, 4>(d, f, r, dual, st);
   }
   hipLaunchKernelGGL(ll_compact_kernel, dim3(1), dim3(1024), 0, st, d->labels, d->rows, d->vocab, order, inv, lab, d->row_loss, d->nvalid_dev);
-  hipLaunchKernelGGL(ll_pack_kernel<T>, dim3(p.R / 4), dim3(256), 0, st, d->h, d->ldh, d->w, d->ldw, d->d, p.dp, d->vocab, order, lab, d->top_idx, d->ld_top, d->k,
-                     d->nvalid_dev, (void*)(ws + p.hp), zk);
+  hipLaunchKernelGGL(ll_pack_kernel<T>, dim3(p.R / 4), dim3(256), 0, st, d->h, d->ldh, d->w, d->ldw, d->d, p.dp, order, lab, d->k, d->nvalid_dev, (void*)(ws + p.hp), zk);
+  if (d->k > 0)
+    hipLaunchKernelGGL(ll_gather_kernel<T>, dim3(p.R), dim3(256), 0, st, (const void*)(ws + p.hp), p.dp, d->w, d->ldw, d->d, d->vocab, order, lab, d->top_idx, d->ld_top, d->k,
+                       d->nvalid_dev, zk);
   if (d->dw)
     hipLaunchKernelGGL(ll_transpose_kernel, dim3(p.R / 64, p.dp / 64), dim3(256), 0, st, (const uint16_t*)(ws + p.hp), p.dp, d->nvalid_dev, (uint16_t*)(ws + p.hT), p.R);
   LogitsArgs a = {};
@@ -1418,7 +1499,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, false, true, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
   else hipLaunchKernelGGL((ll_logits_kernel<T, false, false, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
   hipLaunchKernelGGL(ll_rows_kernel<256>, dim3(p.R / 16), dim3(256), 0, st, r);
-  hipLaunchKernelGGL(ll_mean_kernel, dim3(1), dim3(1024), 0, st, ploss, d->nvalid_dev, d->loss_dev);
+  hipLaunchKernelGGL(ll_mean_kernel, dim3(1), dim3(1024), 0, st, ploss, d->nvalid_dev, d->loss_dev, (d->d + BN - 1) / BN, p.piece_tiles * (BN / BK), splits);
   if (grad) {
     for (int pc = 0; pc < p.pieces; ++pc) {
       a.col0 = pc * p.piece_tiles * BN;
@@ -1432,9 +1513,9 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
                            a.c1, a.c2, w1 * up, w2 * up, a.col0, a.tiles_n * BN, d->vocab, (E*)a.G, a.ldg);
       if (d->dh) {
         DhArgs q = {};
-        q.G = a.G; q.w = d->w; q.ldw = d->ldw; q.ldg = a.ldg; q.col0 = a.col0; q.cols = a.tiles_n * BN; q.V = d->vocab; q.d = d->d; q.R = p.R;
-        q.splits = p.splits; q.chunk = p.chunk; q.add = pc > 0; q.nvalid = d->nvalid_dev; q.slab = (float*)(ws + p.slab);
-        hipLaunchKernelGGL(ll_dh_kernel<T>, dim3(p.R / BM * ((d->d + BN - 1) / BN) * p.splits), dim3(NTH), LL_LDS, st, q);
+        q.G = a.G; q.w = d->w; q.ldw = d->ldw; q.ldg = a.ldg; q.col0 = a.col0; q.cols = a.tiles_n * BN; q.V = d->vocab; q.d = d->d;
+        q.kt = p.piece_tiles * (BN / BK); q.splits = splits; q.add = pc > 0; q.nvalid = d->nvalid_dev; q.slab = (float*)(ws + p.slab);
+        hipLaunchKernelGGL(ll_dh_kernel<T>, dim3(p.pairs), dim3(NTH), LL_LDS, st, q);
       }
       if (d->dw) {
         DwArgs q = {};
@@ -1444,7 +1525,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
       }
     }
     if (d->dh)
-      launch_dh_out<E>((const float*)(ws + p.slab), p.splits, p.R, d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh, d->lddh, st);
+      launch_dh_out<E>((const float*)(ws + p.slab), p.R <= 512 ? 16 : 1, 0, splits, 0, d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh, d->lddh, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;
