@@ -264,31 +264,51 @@ __device__ __forceinline__ int ll_pos(int total) {
 // order[i] = i-th row with a label, inv[row] = its place or -1, *nvalid; ignored rows get their zero loss here
 __global__ __launch_bounds__(1024) void ll_compact_kernel(const int64_t* __restrict__ labels, int rows, int V, int* __restrict__ order,
                                                           int* __restrict__ inv, int* __restrict__ lab, float* __restrict__ row_loss, int* __restrict__ nvalid) {
-  __shared__ int sh[16];
+  __shared__ int cnt[128], pre[128], all;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = (rows + 1023) / 1024, r0 = tid * per, r1 = min(rows, r0 + per);
-  int n = 0;
-#pragma unroll 4
-  for (int r = r0; r < r1; ++r) n += labels[r] >= 0 && labels[r] < V;
-  int at = n;                                     // inclusive scan over the wave, then over the waves
+  int base = 0;
+  for (int r0 = 0; r0 < rows; r0 += 8192) {       // eight labels a thread at a time, loaded together
+    int l[8];
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(at, o, 64);
-    at += lane >= o ? t : 0;
+    for (int c = 0; c < 8; ++c) {
+      const int r = r0 + c * 1024 + tid;
+      const int64_t v = r < rows ? labels[r] : -1;
+      l[c] = v >= 0 && v < V ? (int)v : -1;
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const uint64_t m = __ballot(l[c] >= 0);
+      if (lane == 0) cnt[c * 16 + wave] = __popcll(m);
+    }
+    __syncthreads();
+    if (wave == 0) {                              // 128 (chunk, wave) counts: exclusive prefix sums
+      const int a = cnt[2 * lane], b = cnt[2 * lane + 1];
+      int t = a + b;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(t, o, 64);
+        t += lane >= o ? u : 0;
+      }
+      pre[2 * lane] = t - a - b;
+      pre[2 * lane + 1] = t - b;
+      if (lane == 63) all = t;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const int r = r0 + c * 1024 + tid;
+      const uint64_t m = __ballot(l[c] >= 0);
+      if (r < rows) {
+        const int at = base + pre[c * 16 + wave] + __popcll(m & ((1ull << lane) - 1ull));
+        inv[r] = l[c] >= 0 ? at : -1;
+        if (l[c] >= 0) { order[at] = r; lab[at] = l[c]; }
+        else row_loss[r] = 0.f;
+      }
+    }
+    base += all;
+    __syncthreads();
   }
-  if (lane == 63) sh[wave] = at;
-  __syncthreads();
-  at -= n;
-  for (int w = 0; w < wave; ++w) at += sh[w];
-#pragma unroll 4
-  for (int r = r0; r < r1; ++r) {
-    const int64_t l = labels[r];
-    const bool ok = l >= 0 && l < V;
-    inv[r] = ok ? at : -1;
-    if (ok) { order[at] = r; lab[at] = (int)l; ++at; }
-    else row_loss[r] = 0.f;
-  }
-  if (tid == 1023) *nvalid = at;
+  if (tid == 0) *nvalid = base;
 }
 
 // hp[i] = h[order[i]], columns [d, dp) and rows [nvalid, next multiple of 256) zero; without a list also zk[i] = h_i . W[label_i] (fp32 products, added
@@ -374,6 +394,7 @@ struct LogitsArgs {
   float *pm, *p1, *p2;                   // (tiles_n, R): maximum, sum of exp2((z - max) c1), the same with c2
   const float *La, *Lb;                  // (R): base-2 log-sum-exp minus log2 of the weight and of 2^s
   void* G; int ldg;
+  int row0; float *strip, shift, unshift;   // first packed row; LL_KEEP: (4 tiles_n, R) maxima of the 64-column strips, s and 2^-s
   const int* lab; const float* zk;       // FIX: the label's cell of dz is put right in the staged tile
   float wlab;                            // w1 2^s
 };
@@ -389,15 +410,21 @@ __device__ __forceinline__ float ll_ref(float mx, float c) { return ceilf(mx * c
 constexpr int LL_SIDE = 2 * BUF;                              // behind the ring
 constexpr int LL_LOGITS_LDS = LL_SIDE + 3 * 4096;             // statistics: 3 x 4 x 256 floats; dz: two parities of 4 x 256 row constants (8 KiB)
 
-template <class T, bool GRAD, bool DUAL, bool FIX>
+// MODE LL_STATS: the statistics alone.  LL_KEEP: and 2^(z c1 - e) of every logit in the operands' type, e = the reference of its row and 64-column
+// strip (minus s for fp16's range), which ll_scale_kernel turns into dz once the rows' sums are known: no logit is formed twice.  LL_GRAD: dz from
+// the rows' sums.
+enum { LL_STATS, LL_KEEP, LL_GRAD };
+template <class T, int MODE, bool DUAL, bool FIX>
 __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
+  constexpr bool GRAD = MODE == LL_GRAD, STORES = MODE != LL_STATS;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef typename T::e E;
   typedef typename T::v8 v8;
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 2, wn = wave & 3;
-  const int nv = *p.nvalid;
+  const int nv = min(*p.nvalid - p.row0, p.R);
+  if (nv <= 0) return;
   const int tiles_m = (nv + BM - 1) / BM, total = tiles_m * p.tiles_n;
   // XCD x (= block % 8) owns a contiguous run of tiles, its workgroups take every nx-th of it
   const int xcd = blockIdx.x & 7, nx = (gridDim.x - xcd + 7) >> 3;
@@ -427,7 +454,7 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
     }
   }
   // operands of the current and the next tile; W's rows end with the vocabulary (a row past it starts behind the resource's last byte)
-  auto rsrc_a_of = [&](int tm) __attribute__((always_inline)) { return ll_rsrc((const E*)p.hp + (int64_t)tm * BM * p.dp); };
+  auto rsrc_a_of = [&](int tm) __attribute__((always_inline)) { return ll_rsrc((const E*)p.hp + (int64_t)(p.row0 + tm * BM) * p.dp); };
   auto rsrc_b_of = [&](int tn) __attribute__((always_inline)) {
     const int n0 = p.col0 + tn * BN;
     ns_u4v r = ll_rsrc((const E*)p.w + (int64_t)n0 * p.ldw);
@@ -478,10 +505,11 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
         for (int nt = 0; nt < 2; ++nt) acc[ah][mt][bh][nt] = T::mma(bq[bh][nt][ks], af[mt][ks], acc[ah][mt][bh][nt]);
     __builtin_amdgcn_s_setprio(0);
   };
-  // (FIRST, GRAD only: the 16 stores of the tile before lie between the pieces that the first K tile waits for and those it requests)
+  // (FIRST, where tiles are stored: the 16 stores of the tile before, 24 with the strips' maxima, lie between the pieces that the first K tile waits for and those it requests)
 #define LL_RUN(AH, BH, FIRST)                                               \
   do {                                                                      \
     if (GRAD && (FIRST)) asm volatile("s_waitcnt vmcnt(24)" ::: "memory");  \
+    else if (STORES && (FIRST)) asm volatile("s_waitcnt vmcnt(32)" ::: "memory"); \
     else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");                   \
     LL_BARRIER();                                                           \
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                      \
@@ -515,8 +543,8 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
       c[1] = DUAL ? p.Lb[i] : 0.f;
       c[2] = c[3] = 0.f;
       if (FIX) {
-        c[2] = __int_as_float(i < nv ? p.lab[i] : -1);
-        c[3] = i < nv ? __builtin_amdgcn_exp2f(p.zk[i] * p.c1 - c[0]) - p.wlab : 0.f;
+        c[2] = __int_as_float(i < nv ? p.lab[p.row0 + i] : -1);
+        c[3] = i < nv ? __builtin_amdgcn_exp2f(p.zk[p.row0 + i] * p.c1 - c[0]) - p.wlab : 0.f;
       }
     }
   };
@@ -592,7 +620,7 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
               for (int mt = 0; mt < 4; ++mt) acc[ah][mt][b >> 1][b & 1][r] = -INFINITY;
           }
     }
-    if (!GRAD) {
+    if (MODE == LL_STATS) {
       // a el holds 16 of the wave's 64 columns of 8 rows; the row's other lanes are 16 and 32 apart, its other columns in the waves of equal wm
 #pragma unroll
       for (int ah = 0; ah < 2; ++ah)
@@ -623,6 +651,50 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
             if (DUAL) side[2048 + wn * 256 + row] = s2;
           }
         }
+    } else if (MODE == LL_KEEP) {
+      char* const st = smem + BUF + (wave < 4 ? RA1 : RB1) * REGION + (wave & 3) * 4096;       // this wave's 32 rows x 128 B
+      char* const G = (char*)p.G + ((int64_t)(m0 + wm * 128) * p.ldg + tn * BN + wn * 64) * 2;
+      float* const strip = p.strip + (int64_t)(tn * 4 + wn) * p.R + m0 + wm * 128;
+#pragma unroll
+      for (int qt = 0; qt < 4; ++qt) {
+        const int ah = qt >> 1;
+#pragma unroll
+        for (int m2 = 0; m2 < 2; ++m2) {
+          const int mt = (qt & 1) * 2 + m2, rl = m2 * 16 + e15, row = wm * 128 + qt * 32 + rl;
+          float mx = -INFINITY;
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[ah][mt][b >> 1][b & 1][r]);
+          mx = ll_max4(mx);
+          const float e1 = (mx == -INFINITY ? 0.f : ll_ref(mx, p.c1)) - p.shift;
+          float s1 = 0.f;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            float g[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              g[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[ah][mt][b >> 1][b & 1][r], p.c1, -e1));
+              s1 += g[r];
+            }
+            *(ushort4v*)(st + rl * 128 + (((b * 2 + (eg >> 1)) ^ (rl & 7)) << 4) + (eg & 1) * 8) = cvt4<E>(g[0], g[1], g[2], g[3]);
+          }
+          s1 = ll_sum4(s1) * p.unshift;
+          if (eg == 0) {
+            side[wn * 256 + row] = mx;
+            side[1024 + wn * 256 + row] = s1;
+            strip[qt * 32 + rl] = mx;
+          }
+        }
+        asm volatile("" ::: "memory");       // (other lanes' 8-byte writes and these 16-byte reads: the wave's LDS order is all that is needed, hipcc must keep it)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rl = i * 8 + (el >> 3);
+          const uint4 v = *(const uint4*)(st + rl * 128 + (((el & 7) ^ (rl & 7)) << 4));
+          *(uint4*)(G + (int64_t)(qt * 32 + rl) * p.ldg * 2 + (el & 7) * 16) = v;
+        }
+        asm volatile("" ::: "memory");
+      }
     } else {
       float c[4];
       if (more) row_consts(tm2, et, c);
@@ -653,12 +725,14 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
           if (cl >= 0 && cl < 64) *(E*)(st + el * 128 + (((cl >> 3) ^ (el & 7)) << 4) + (cl & 7) * 2) = (E)rc[768 + row];
         }
         if (qt == 0 && more) put_consts(par ^ 1, et, c);           // (before the first store: the wait for these loads must not wait for stores)
+        asm volatile("" ::: "memory");       // (other lanes' 8-byte writes and these 16-byte reads: the wave's LDS order is all that is needed, hipcc must keep it)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int rl = i * 8 + (el >> 3);
           const uint4 v = *(const uint4*)(st + rl * 128 + (((el & 7) ^ (rl & 7)) << 4));
           *(uint4*)(G + (int64_t)(qt * 32 + rl) * p.ldg * 2 + (el & 7) * 16) = v;
         }
+        asm volatile("" ::: "memory");
       }
       par ^= 1;
     }
@@ -682,10 +756,84 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
 #undef LL_RUN
 }
 
+// dz from what LL_KEEP left, in place: the strip's exponentials times 2^(e - La), one rounding more; a row's label cell (no list) is formed from its own
+// logit.  64 rows x 512 columns a workgroup, 16 B per lane; the pass is bound by its bytes (read and written once, mostly in the last-level cache).
+template <class T, bool FIX>
+__global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
+  typedef typename T::e E;
+  typedef typename T::v8 v8;
+  __shared__ float f[8][64];
+  __shared__ int lc[64];
+  __shared__ float lv[64];
+  const int nv = min(*p.nvalid - p.row0, p.R);
+  const int i0 = blockIdx.y * 64, t0 = blockIdx.x * 2;
+  if (nv <= 0 || i0 >= (nv + BM - 1) / BM * BM) return;
+  for (int x = threadIdx.x; x < 512; x += 256) {
+    const int sidx = t0 * 4 + (x >> 6), i = i0 + (x & 63);
+    if (sidx < p.tiles_n * 4) {
+      const float mx = p.strip[(int64_t)sidx * p.R + i];
+      f[x >> 6][x & 63] = __builtin_amdgcn_exp2f((mx == -INFINITY ? 0.f : ll_ref(mx, p.c1)) - p.shift - p.La[i]);
+    }
+  }
+  if (FIX && threadIdx.x < 64) {
+    const int i = i0 + threadIdx.x;
+    lc[threadIdx.x] = i < nv ? p.lab[p.row0 + i] - t0 * BN : -1;
+    lv[threadIdx.x] = i < nv ? __builtin_amdgcn_exp2f(p.zk[p.row0 + i] * p.c1 - p.La[i]) - p.wlab : 0.f;
+  }
+  __syncthreads();
+  const int c = (threadIdx.x & 63) * 8, r0 = threadIdx.x >> 6;
+  if (t0 * BN + c >= p.tiles_n * BN) return;
+  E* const G = (E*)p.G + (int64_t)i0 * p.ldg + t0 * BN + c;
+  // (eight loads ahead of the first store: in place, hipcc orders every load behind the store before it)
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    v8 v[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = *(const v8*)(G + (int64_t)(r0 + 4 * (8 * h + x)) * p.ldg);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int r = r0 + 4 * (8 * h + x);
+      const float a = f[c >> 6][r];
+      const int at = FIX ? lc[r] - c : -1;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float g = (float)v[x][e] * a;
+        if (FIX && at == e) g = lv[r];
+        v[x][e] = (E)g;
+      }
+      *(v8*)(G + (int64_t)r * p.ldg) = v[x];
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ rows: log-sum-exp, losses, weights
+// How many ways dh's product over one piece of the vocabulary (kt K tiles of 64) is split for `tiles` output tiles: the number that ends soonest when 256
+// CUs take (tile, split) pairs in rounds, a pair costing its K tiles and about LL_PAIR more (ring start, fp32 tile to and from its slab).  At most LL_PAIRS
+// pairs, eight K tiles each at least.  Depends on sizes and the number of rows with a label alone: the same inputs are added in the same order.
+constexpr int LL_PAIRS = 512, LL_PAIR = 6;
+__host__ __device__ inline int ll_cost(int tiles, int kt, int s) { return (tiles * s + 255) / 256 * ((kt + s - 1) / s + LL_PAIR); }
+__host__ __device__ inline int ll_most_splits(int tiles, int kt) {
+  const int a = tiles > 0 ? LL_PAIRS / tiles : 1, b = kt / 8, m = a < b ? a : b;
+  return m < 1 ? 1 : m > 1024 ? 1024 : m;
+}
+
+// by one workgroup of 256 threads
+__device__ __forceinline__ void ll_choose_splits(int nv, int tiles_d, int kt, int* splits) {
+  __shared__ unsigned best[4];
+  const int tiles = (nv + BM - 1) / BM * tiles_d, most = ll_most_splits(tiles, kt);
+  unsigned c = ~0u;
+  for (int n = threadIdx.x + 1; n <= most; n += 256) c = min(c, (unsigned)min(ll_cost(tiles, kt, n), 0x1FFFFF) << 11 | (unsigned)n);      // (a tie: the fewest)
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) c = min(c, (unsigned)__shfl_xor((int)c, o, 64));
+  if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = c;
+  __syncthreads();
+  if (threadIdx.x == 0) *splits = (int)(min(min(best[0], best[1]), min(best[2], best[3])) & 2047);
+}
+
 struct RowArgs {
   const float *pm, *p1, *p2;
-  int tiles_n, R, k, V;
+  int tiles_n, R, k, V, row0;
+  int tiles_d, kt; int* splits;
   float c1, c2, invT, w1, w2, lw1, lw2, kd;     // lw*: log2(w* 2^s), -inf for a zero weight; kd: alpha T^2
   int dual, soft_only;                          // one softmax: p1 is at temperature T when only soft targets count
   const int* nvalid; const int *order, *lab;
@@ -701,8 +849,9 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
   constexpr int RB = NT / 16;
   __shared__ float sm[3][RB][17];
   __shared__ float all[RB];
-  const int nv = *p.nvalid, i0 = blockIdx.x * RB;
-  if (NT == 256 && i0 >= (nv + BM - 1) / BM * BM) return;
+  const int nv = min(*p.nvalid - p.row0, p.R), i0 = blockIdx.x * RB;
+  if (NT == 256 && blockIdx.x == 0) ll_choose_splits(max(nv, 0), p.tiles_d, p.kt, p.splits);
+  if (NT == 256 && (nv <= 0 || i0 >= (nv + BM - 1) / BM * BM)) return;
   {
     const int r = threadIdx.x & (RB - 1), q = threadIdx.x / RB;
     float mx = -INFINITY, s1 = 0.f, s2 = 0.f;
@@ -736,8 +885,8 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
     if (NT == 256) return;
   }
   if (live) {
-  const int row = p.order[i];
-  auto logit = [&](int e, int tok) __attribute__((always_inline)) { return p.z ? p.z[(int64_t)i * p.ldz + tok] : p.zk[(int64_t)i * (p.k + 1) + e]; };
+  const int pi = p.row0 + i, row = p.order[pi];
+  auto logit = [&](int e, int tok) __attribute__((always_inline)) { return p.z ? p.z[(int64_t)i * p.ldz + tok] : p.zk[(int64_t)pi * (p.k + 1) + e]; };
   bool soft = false;
   if (p.k > 0) {
     // the teacher's distribution over the entries that name a token; a list without any leaves the hard label alone
@@ -762,14 +911,14 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
         pr = expf(lp) * inv;
         if (pr > 0.f) kl += pr * ((lp - lt) - (__builtin_fmaf(logit(e, ti[e]), p.c2, -e2) - ls) * LN2);
       }
-      p.pk[(int64_t)i * p.k + e] = pr;
+      p.pk[(int64_t)pi * p.k + e] = pr;
     }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) kl += __shfl_xor(kl, o, 64);
     if (soft) loss += p.kd * kl;
   }
   if (q == 0) {
-    if (!p.soft_only) loss -= p.w1 * (__builtin_fmaf(logit(p.k, p.lab[i]), p.c1, -e1) - log2f(s1)) * LN2;      // (lse - z in units of ln 2)
+    if (!p.soft_only) loss -= p.w1 * (__builtin_fmaf(logit(p.k, p.lab[pi]), p.c1, -e1) - log2f(s1)) * LN2;      // (lse - z in units of ln 2)
     const float l1 = e1 + log2f(s1);
     if (p.dual) {
       p.La[i] = l1 - p.lw1;
@@ -782,7 +931,7 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
       p.La[i] = l1 - p.lw1;
     }
     p.row_loss[row] = loss;
-    if (NT == 256) p.packed_loss[i] = loss;
+    if (NT == 256) p.packed_loss[pi] = loss;
   }
   }
   if (NT == 1024) {
@@ -795,56 +944,39 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
   }
 }
 
-// How many ways dh's product over one piece of the vocabulary (kt K tiles of 64) is split for `tiles` output tiles: the number that ends soonest when 256
-// CUs take (tile, split) pairs in rounds, a pair costing its K tiles and about LL_PAIR more (ring start, fp32 tile to and from its slab).  At most LL_PAIRS
-// pairs, eight K tiles each at least.  Depends on sizes and the number of rows with a label alone: the same inputs are added in the same order.
-constexpr int LL_PAIRS = 512, LL_PAIR = 6;
-__host__ __device__ inline int ll_cost(int tiles, int kt, int s) { return (tiles * s + 255) / 256 * ((kt + s - 1) / s + LL_PAIR); }
-__host__ __device__ inline int ll_most_splits(int tiles, int kt) {
-  const int a = tiles > 0 ? LL_PAIRS / tiles : 1, b = kt / 8, m = a < b ? a : b;
-  return m < 1 ? 1 : m > 1024 ? 1024 : m;
-}
-
-// the loss, and *splits for dh
-__global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__ packed_loss, const int* __restrict__ nvalid, float* __restrict__ loss, int tiles_d, int kt,
-                                                       int* __restrict__ splits) {
+// the loss
+__global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__ packed_loss, const int* __restrict__ nvalid, float* __restrict__ loss) {
   __shared__ float sh[16];
-  __shared__ unsigned best[16];
   const int nv = *nvalid;
   float s = 0.f;
   for (int i = threadIdx.x; i < nv; i += 1024) s += packed_loss[i];
   s = ns_wave_sum(s);
-  const int tiles = (nv + BM - 1) / BM * tiles_d, n = threadIdx.x + 1;
-  unsigned c = n <= ll_most_splits(tiles, kt) ? (unsigned)min(ll_cost(tiles, kt, n), 0x1FFFFF) << 11 | (unsigned)n : ~0u;      // (a tie: the fewest)
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) c = min(c, (unsigned)__shfl_xor((int)c, o, 64));
-  if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = s; best[threadIdx.x >> 6] = c; }
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     s = 0.f;
-    for (int w = 0; w < 16; ++w) { s += sh[w]; c = min(c, best[w]); }
+    for (int w = 0; w < 16; ++w) s += sh[w];
     *loss = s / (float)max(nv, 1);
-    *splits = (int)(c & 2047);
   }
 }
 
 // the sparse cells of dz in one piece: one wave per row, each token written once whatever number of entries name it
 template <class E>
-__global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ nvalid, const int* __restrict__ order, const int* __restrict__ lab,
+__global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ nvalid, int row0, int R, const int* __restrict__ order, const int* __restrict__ lab,
                                                        const int32_t* __restrict__ top_idx, int64_t ld_top, int k, const float* __restrict__ zk,
                                                        const float* __restrict__ pk, const float* __restrict__ La, const float* __restrict__ Lb, float c1, float c2,
                                                        float w1s, float w2s, int col0, int cols, int V, E* __restrict__ G, int ldg) {
   __shared__ int sidx[4][LL_MAX_K + 1];
   __shared__ float sp[4][LL_MAX_K];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = blockIdx.x * 4 + wave;
-  const int nv = *nvalid;
+  const int nv = min(*nvalid - row0, R), pi = row0 + i;
   const bool live = i < nv;
   if (live) {
-    const int row = order[i];
+    const int row = order[pi];
     for (int e = lane; e <= k; e += 64) {
-      const int t = e == k ? lab[i] : top_idx[row * ld_top + e];
+      const int t = e == k ? lab[pi] : top_idx[row * ld_top + e];
       sidx[wave][e] = t >= 0 && t < V ? t : -1;
-      if (e < k) sp[wave][e] = pk[(int64_t)i * k + e];
+      if (e < k) sp[wave][e] = pk[(int64_t)pi * k + e];
     }
   }
   __syncthreads();
@@ -858,11 +990,11 @@ __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ n
     for (int o = 0; o < k; ++o)
       if (sidx[wave][o] == t) { soft += sp[wave][o]; first = first && o >= e; }
     if (!first) continue;                                   // an earlier entry of the list names the same token: that one writes
-    const float z = zk[(int64_t)i * (k + 1) + e];
+    const float z = zk[(int64_t)pi * (k + 1) + e];
     float v = __builtin_amdgcn_exp2f(z * c1 - la);
     if (Lb) v += __builtin_amdgcn_exp2f(z * c2 - lb);
     v -= w2s * soft;
-    if (t == lab[i]) v -= w1s;
+    if (t == lab[pi]) v -= w1s;
     G[(int64_t)i * ldg + c] = (E)v;
   }
 }
@@ -870,7 +1002,7 @@ __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ n
 // ------------------------------------------------------------------------------------------------ dh += dz W,  dW = dz^T h
 struct DhArgs {
   const void* G; const void* w; int64_t ldw;
-  int ldg, col0, cols, V, d, kt, add;
+  int ldg, col0, cols, V, d, kt, add, row0, R;
   const int *nvalid, *splits;
   float* slab;                      // (splits, tiles, 256, 256)
 };
@@ -879,7 +1011,9 @@ template <class T>
 __global__ __launch_bounds__(NTH) void ll_dh_kernel(const DhArgs p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef typename T::e E;
-  const int tiles_m = (*p.nvalid + BM - 1) / BM, tiles_d = (p.d + BN - 1) / BN;
+  const int nv = min(*p.nvalid - p.row0, p.R);
+  if (nv <= 0) return;
+  const int tiles_m = (nv + BM - 1) / BM, tiles_d = (p.d + BN - 1) / BN;
   const int tiles = tiles_m * tiles_d, splits = *p.splits;
   const int pos = ll_pos(tiles * splits);
   if (pos < 0) return;
@@ -925,7 +1059,7 @@ __global__ __launch_bounds__(NTH) void ll_dh_kernel(const DhArgs p) {
 // and 16 groups of slabs side by side: with one token and 203 slabs a single chain of loads took 28 us
 // (R > 0: slabs of (R, d); R = 0: slabs of 256 x 256 tiles, their number read from splits_dev.)
 template <class E>
-__global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict__ slab, int groups, int splits, const int* __restrict__ splits_dev, int R, int d, int rows, const int* __restrict__ inv,
+__global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict__ slab, int groups, int splits, const int* __restrict__ splits_dev, int R, int row0, int chunk, int d, int rows, const int* __restrict__ inv,
                                                         const int* __restrict__ nvalid, const float* __restrict__ loss_scale, float unscale, E* __restrict__ dh, int64_t lddh) {
   typedef E e4 __attribute__((ext_vector_type(4)));
   __shared__ f32x4 sm[16][16];
@@ -935,12 +1069,12 @@ __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict_
   const int64_t x = (int64_t)blockIdx.x * nblk + blk;
   const int row = (int)(x / per), c = (int)(x - (int64_t)row * per) * 64 + (threadIdx.x & 15) * 4;
   const bool in = row < rows && c < d;
-  const int i = in ? inv[row] : -1;
+  const int pi = in ? inv[row] : -1, i = pi >= row0 && pi - row0 < chunk ? pi - row0 : -1;      // a chunk writes its own rows, the first one the ignored ones
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
   if (i >= 0) {
     if (splits_dev) splits = *splits_dev;
     const int per_g = (splits + groups - 1) / groups, s1 = min(splits, (g + 1) * per_g);
-    const int tiles_d = (d + BN - 1) / BN, tiles = (*nvalid + BM - 1) / BM * tiles_d;
+    const int tiles_d = (d + BN - 1) / BN, tiles = (min(*nvalid - row0, chunk) + BM - 1) / BM * tiles_d;
     const int64_t at = R > 0 ? (int64_t)i * d + c : ((int64_t)(i / BM * tiles_d + c / BN) * BM + i % BM) * BN + c % BN;
     const int64_t step = R > 0 ? (int64_t)R * d : (int64_t)tiles * BM * BN;
 #pragma unroll 4
@@ -952,24 +1086,24 @@ __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict_
     if (g == 0)
       for (int o = 1; o < groups; ++o) a += sm[sub + o][threadIdx.x & 15];
   }
-  if (!in || g != 0) return;
+  if (!in || g != 0 || (pi >= 0 ? i < 0 : row0 > 0)) return;
   const float gs = (loss_scale ? *loss_scale : 1.f) / (float)max(*nvalid, 1) * unscale;
   e4 o;
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] = (E)(i < 0 ? 0.f : a[e] * gs);
   *(e4*)(dh + row * lddh + c) = o;
 }
-template <class E> void launch_dh_out(const float* slab, int groups, int splits, const int* splits_dev, int R, int d, int rows, const int* inv, const int* nvalid, const float* loss_scale, float unscale, E* dh,
+template <class E> void launch_dh_out(const float* slab, int groups, int splits, const int* splits_dev, int R, int row0, int chunk, int d, int rows, const int* inv, const int* nvalid, const float* loss_scale, float unscale, E* dh,
                                       int64_t lddh, hipStream_t st) {
   const int nblk = 16 / groups;
   const int64_t items = (int64_t)rows * ((d + 63) / 64);
-  hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)((items + nblk - 1) / nblk)), dim3(256), 0, st, slab, groups, splits, splits_dev, R, d, rows, inv, nvalid,
+  hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)((items + nblk - 1) / nblk)), dim3(256), 0, st, slab, groups, splits, splits_dev, R, row0, chunk, d, rows, inv, nvalid,
                      loss_scale, unscale, dh, lddh);
 }
 
 struct DwArgs {
   const void* hT; int ldt;
-  const void* G; int ldg, col0, tiles_v, V, d;
+  const void* G; int ldg, col0, tiles_v, V, d, row0, R;
   const int* nvalid; const float* loss_scale;
   float unscale;
   void* dw; int64_t lddw; int f32, add;
@@ -984,9 +1118,9 @@ __global__ __launch_bounds__(NTH) void ll_dw_kernel(const DwArgs p) {
   if (pos < 0) return;
   const int tv = pos / tiles_d, td = pos - tv * tiles_d;
   const int m0 = td * BM, n0 = tv * BN;                    // columns of h, columns of dz (= rows of W)
-  const int nv = *p.nvalid, K = (nv + BK - 1) / BK * BK;
+  const int nv = *p.nvalid, K = max(min(nv - p.row0, p.R) + BK - 1, 0) / BK * BK;
   f32x4 acc[2][4][2][2];
-  ll_tile<T, true, true>(acc, smem, (const E*)p.hT + (int64_t)m0 * p.ldt, p.ldt, K, (const E*)p.G + n0, p.ldg, K, BN, K);
+  ll_tile<T, true, true>(acc, smem, (const E*)p.hT + (int64_t)m0 * p.ldt + p.row0, p.ldt, K, (const E*)p.G + n0, p.ldg, K, BN, K);
   const float gs = (p.loss_scale ? *p.loss_scale : 1.f) / (float)max(nv, 1) * p.unscale;
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1365,8 +1499,8 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
   int few;                                    // 0, or MT of the few-row path
-  int R, dp, dt, tiles_n, piece_tiles, pieces, pairs;
-  size_t splits_at, order, inv, lab, hp, hT, zk, pk, pm, p1, p2, La, Lb, ploss, G, slab, total;
+  int keep, R, Rc, dp, dt, tiles_n, piece_tiles, pieces, pairs;      // keep: LL_KEEP, in chunks of Rc rows (else Rc = R, in pieces of the vocabulary)
+  size_t splits_at, order, inv, lab, hp, hT, zk, pk, pm, p1, p2, strip, La, Lb, ploss, G, slab, total;
 };
 
 bool dual_of(const ns_linear_ce_desc* d) { return d->k > 0 && d->alpha > 0.f && d->alpha < 1.f && d->temperature != 1.f; }
@@ -1379,19 +1513,33 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   p.dt = (d->d + BM - 1) / BM * BM;
   p.tiles_n = (d->vocab + BN - 1) / BN;
   const bool grad = d->dh || d->dw;
-  // pieces: the 16-bit dz of one piece fits LL_PIECE_BYTES, and a k-range of the head stays addressable with 32-bit byte offsets
-  int64_t most = (int64_t)(LL_PIECE_BYTES / ((size_t)p.R * BN * 2));
-  const int64_t by_ld = ((int64_t)0x7FF00000 / 2 / (d->ldw > d->d ? d->ldw : d->d)) / BN;
-  if (most > by_ld) most = by_ld;
-  if (most < 1) most = 1;
-  p.pieces = (int)((p.tiles_n + most - 1) / most);
-  p.piece_tiles = (p.tiles_n + p.pieces - 1) / p.pieces;
-  p.pieces = (p.tiles_n + p.piece_tiles - 1) / p.piece_tiles;
+  // Either whole rows of 16-bit exponentials in chunks of rows, no logit formed twice: one softmax, and dW not spread over chunks; or dz of one piece of the
+  // vocabulary at a time for all rows.  Both within LL_PIECE_BYTES, and a k-range of the head addressable with 32-bit byte offsets.
+  const int64_t ldw = d->ldw > d->d ? d->ldw : d->d;
+  const int64_t by_ld = ((int64_t)0x7FF00000 / 2 / ldw) / BN;
+  const int64_t rows_fit = (int64_t)(LL_PIECE_BYTES / ((size_t)p.tiles_n * BN * 2)) / BM * BM;
+  p.keep = grad && !dual_of(d) && rows_fit >= BM && p.tiles_n <= by_ld && (p.R <= rows_fit || !d->dw);
+  p.Rc = p.R;
+  if (p.keep) {
+    if (p.R > rows_fit) {
+      const int n = (int)((p.R + rows_fit - 1) / rows_fit);
+      p.Rc = ((p.R / BM + n - 1) / n) * BM;
+    }
+    p.pieces = 1;
+    p.piece_tiles = p.tiles_n;
+  } else {
+    int64_t most = (int64_t)(LL_PIECE_BYTES / ((size_t)p.R * BN * 2));
+    if (most > by_ld) most = by_ld;
+    if (most < 1) most = 1;
+    p.pieces = (int)((p.tiles_n + most - 1) / most);
+    p.piece_tiles = (p.tiles_n + p.pieces - 1) / p.pieces;
+    p.pieces = (p.tiles_n + p.piece_tiles - 1) / p.piece_tiles;
+  }
   // dh's slabs: one 256 x 256 fp32 tile per (output tile, split of the piece's vocabulary)
-  const int tiles = (p.R / BM) * ((d->d + BN - 1) / BN), kt = p.piece_tiles * (BN / BK);
+  const int tiles = (p.Rc / BM) * ((d->d + BN - 1) / BN), kt = p.piece_tiles * (BN / BK);
   p.pairs = tiles;                                 // (fewer live tiles may be split more ways: at most LL_PAIRS pairs, or kt / 8 a tile)
   if (p.pairs < LL_PAIRS) p.pairs = (int64_t)tiles * (kt / 8) < LL_PAIRS ? (tiles * (kt / 8) > tiles ? tiles * (kt / 8) : tiles) : LL_PAIRS;
-  if (p.few) p.R = LL_FEW_ROWS;
+  if (p.few) p.R = p.Rc = LL_FEW_ROWS;
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
   p.splits_at = take(4);
@@ -1402,13 +1550,14 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   p.hT = d->dw && !p.few ? take((size_t)p.dt * p.R * 2) : 0;
   p.zk = take(p.few ? (size_t)16 * p.few * p.tiles_n * BN * 4 : (size_t)p.R * (d->k + 1) * 4);       // (few rows: all logits)
   p.pk = take((size_t)p.R * d->k * 4);
-  p.pm = take((size_t)p.tiles_n * p.R * 4);
-  p.p1 = take((size_t)p.tiles_n * p.R * 4);
-  p.p2 = dual_of(d) ? take((size_t)p.tiles_n * p.R * 4) : 0;
-  p.La = take((size_t)p.R * 4);
-  p.Lb = take((size_t)p.R * 4);
+  p.pm = take((size_t)p.tiles_n * p.Rc * 4);
+  p.p1 = take((size_t)p.tiles_n * p.Rc * 4);
+  p.p2 = dual_of(d) ? take((size_t)p.tiles_n * p.Rc * 4) : 0;
+  p.strip = p.keep && !p.few ? take((size_t)p.tiles_n * 4 * p.Rc * 4) : 0;
+  p.La = take((size_t)p.Rc * 4);
+  p.Lb = take((size_t)p.Rc * 4);
   p.ploss = take((size_t)p.R * 4);
-  p.G = grad && !p.few ? take((size_t)p.R * p.piece_tiles * BN * 2) : 0;
+  p.G = grad && !p.few ? take((size_t)p.Rc * p.piece_tiles * BN * 2) : 0;
   p.slab = d->dh ? take(p.few ? (size_t)p.tiles_n * 16 * p.few * d->d * 4 : (size_t)p.pairs * BM * BN * 4) : 0;
   p.total = at;
   return p;
@@ -1436,7 +1585,7 @@ int few_launch(const ns_linear_ce_desc* d, const FewArgs& f, const RowArgs& r, b
     gy = (chunks + (chunks + gy - 1) / gy - 1) / ((chunks + gy - 1) / gy);
     if (dual) hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, true>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
     else hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, false>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
-    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n >= 64 ? 16 : f.tiles_n >= 16 ? 4 : 1, f.tiles_n, nullptr, 16 * MT, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, st);
+    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n >= 64 ? 16 : f.tiles_n >= 16 ? 4 : 1, f.tiles_n, nullptr, 16 * MT, 0, LL_FEW_ROWS, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;
@@ -1460,9 +1609,10 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   }
   const float up = ldexpf(1.f, s);
   static ns_dev_once once;
-  if (!ns_dyn_lds_once(once, {(const void*)ll_logits_kernel<T, false, false, false>, (const void*)ll_logits_kernel<T, false, true, false>,
-                              (const void*)ll_logits_kernel<T, true, false, true>, (const void*)ll_logits_kernel<T, true, false, false>,
-                              (const void*)ll_logits_kernel<T, true, true, false>, (const void*)ll_dh_kernel<T>, (const void*)ll_dw_kernel<T>}, LL_LDS, "ns_linear_cross_entropy"))
+  if (!ns_dyn_lds_once(once, {(const void*)ll_logits_kernel<T, LL_STATS, false, false>, (const void*)ll_logits_kernel<T, LL_STATS, true, false>,
+                              (const void*)ll_logits_kernel<T, LL_KEEP, false, false>, (const void*)ll_logits_kernel<T, LL_GRAD, false, true>,
+                              (const void*)ll_logits_kernel<T, LL_GRAD, false, false>, (const void*)ll_logits_kernel<T, LL_GRAD, true, false>,
+                              (const void*)ll_dh_kernel<T>, (const void*)ll_dw_kernel<T>}, LL_LOGITS_LDS > LL_LDS ? LL_LOGITS_LDS : LL_LDS, "ns_linear_cross_entropy"))
     return NS_ERR_HIP;
   const float c1 = soft_only ? LOG2E / T_ : LOG2E, c2 = LOG2E / T_;
   RowArgs r = {};
@@ -1490,42 +1640,53 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   if (d->dw)
     hipLaunchKernelGGL(ll_transpose_kernel, dim3(p.R / 64, p.dp / 64), dim3(256), 0, st, (const uint16_t*)(ws + p.hp), p.dp, d->nvalid_dev, (uint16_t*)(ws + p.hT), p.R);
   LogitsArgs a = {};
-  a.hp = ws + p.hp; a.w = d->w; a.ldw = d->ldw; a.dp = p.dp; a.d = d->d; a.V = d->vocab; a.col0 = 0; a.tiles_n = p.tiles_n; a.R = p.R; a.nvalid = d->nvalid_dev;
+  a.hp = ws + p.hp; a.w = d->w; a.ldw = d->ldw; a.dp = p.dp; a.d = d->d; a.V = d->vocab; a.col0 = 0; a.tiles_n = p.tiles_n; a.R = p.Rc; a.nvalid = d->nvalid_dev;
   a.c1 = c1; a.c2 = c2;
   a.pm = (float*)(ws + p.pm); a.p1 = (float*)(ws + p.p1); a.p2 = (float*)(ws + p.p2);
   a.La = La; a.Lb = Lb; a.G = ws + p.G; a.ldg = p.piece_tiles * BN; a.lab = lab; a.zk = zk; a.wlab = w1 * up;
-  auto grid_of = [&](int tiles_n) { const int64_t t = (int64_t)(p.R / BM) * tiles_n; return dim3((unsigned)(t < 256 ? t : 256)); };
-  const dim3 all = grid_of(p.tiles_n);
-  if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, false, true, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
-  else hipLaunchKernelGGL((ll_logits_kernel<T, false, false, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
-  hipLaunchKernelGGL(ll_rows_kernel<256>, dim3(p.R / 16), dim3(256), 0, st, r);
-  hipLaunchKernelGGL(ll_mean_kernel, dim3(1), dim3(1024), 0, st, ploss, d->nvalid_dev, d->loss_dev, (d->d + BN - 1) / BN, p.piece_tiles * (BN / BK), splits);
-  if (grad) {
+  a.strip = (float*)(ws + p.strip); a.shift = (float)s; a.unshift = 1.f / up;
+  r.R = p.Rc; r.tiles_d = (d->d + BN - 1) / BN; r.kt = p.piece_tiles * (BN / BK); r.splits = splits;
+  auto grid_of = [&](int tiles_n) { const int64_t t = (int64_t)(p.Rc / BM) * tiles_n; return dim3((unsigned)(t < 256 ? t : 256)); };
+  for (int row0 = 0; row0 < p.R; row0 += p.Rc) {
+    a.row0 = r.row0 = row0;
+    a.col0 = 0; a.tiles_n = p.tiles_n;
+    const dim3 all = grid_of(p.tiles_n);
+    if (p.keep) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, false, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
+    else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, LL_STATS, true, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
+    else hipLaunchKernelGGL((ll_logits_kernel<T, LL_STATS, false, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
+    hipLaunchKernelGGL(ll_rows_kernel<256>, dim3(p.Rc / 16), dim3(256), 0, st, r);
+    if (row0 + p.Rc >= p.R) hipLaunchKernelGGL(ll_mean_kernel, dim3(1), dim3(1024), 0, st, ploss, d->nvalid_dev, d->loss_dev);
+    if (!grad) continue;
     for (int pc = 0; pc < p.pieces; ++pc) {
       a.col0 = pc * p.piece_tiles * BN;
       a.tiles_n = p.tiles_n - pc * p.piece_tiles < p.piece_tiles ? p.tiles_n - pc * p.piece_tiles : p.piece_tiles;
       const dim3 grid = grid_of(a.tiles_n);
-      if (d->k == 0) hipLaunchKernelGGL((ll_logits_kernel<T, true, false, true>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
-      else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, true, true, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
-      else hipLaunchKernelGGL((ll_logits_kernel<T, true, false, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
+      if (p.keep) {
+        const dim3 sg((a.tiles_n + 1) / 2, p.Rc / 64);
+        if (d->k == 0) hipLaunchKernelGGL((ll_scale_kernel<T, true>), sg, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((ll_scale_kernel<T, false>), sg, dim3(256), 0, st, a);
+      } else if (d->k == 0) hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, false, true>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
+      else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, true, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
+      else hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, false, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
       if (d->k > 0)
-        hipLaunchKernelGGL(ll_cells_kernel<E>, dim3(p.R / 4), dim3(256), 0, st, d->nvalid_dev, order, lab, d->top_idx, d->ld_top, d->k, zk, pk, La, dual ? Lb : nullptr,
-                           a.c1, a.c2, w1 * up, w2 * up, a.col0, a.tiles_n * BN, d->vocab, (E*)a.G, a.ldg);
+        hipLaunchKernelGGL(ll_cells_kernel<E>, dim3(p.Rc / 4), dim3(256), 0, st, d->nvalid_dev, row0, p.Rc, order, lab, d->top_idx, d->ld_top, d->k, zk, pk, La,
+                           dual ? Lb : nullptr, a.c1, a.c2, w1 * up, w2 * up, a.col0, a.tiles_n * BN, d->vocab, (E*)a.G, a.ldg);
       if (d->dh) {
         DhArgs q = {};
-        q.G = a.G; q.w = d->w; q.ldw = d->ldw; q.ldg = a.ldg; q.col0 = a.col0; q.cols = a.tiles_n * BN; q.V = d->vocab; q.d = d->d;
+        q.G = a.G; q.w = d->w; q.ldw = d->ldw; q.ldg = a.ldg; q.col0 = a.col0; q.cols = a.tiles_n * BN; q.V = d->vocab; q.d = d->d; q.row0 = row0; q.R = p.Rc;
         q.kt = p.piece_tiles * (BN / BK); q.splits = splits; q.add = pc > 0; q.nvalid = d->nvalid_dev; q.slab = (float*)(ws + p.slab);
         hipLaunchKernelGGL(ll_dh_kernel<T>, dim3(p.pairs), dim3(NTH), LL_LDS, st, q);
       }
       if (d->dw) {
         DwArgs q = {};
-        q.hT = ws + p.hT; q.ldt = p.R; q.G = a.G; q.ldg = a.ldg; q.col0 = a.col0; q.tiles_v = a.tiles_n; q.V = d->vocab; q.d = d->d; q.nvalid = d->nvalid_dev;
-        q.loss_scale = d->loss_scale_dev; q.unscale = 1.f / up; q.dw = d->dw; q.lddw = d->lddw; q.f32 = d->dw_f32; q.add = d->dw_add;
+        q.hT = ws + p.hT; q.ldt = p.R; q.G = a.G; q.ldg = a.ldg; q.col0 = a.col0; q.tiles_v = a.tiles_n; q.V = d->vocab; q.d = d->d; q.row0 = row0; q.R = p.Rc;
+        q.nvalid = d->nvalid_dev; q.loss_scale = d->loss_scale_dev; q.unscale = 1.f / up; q.dw = d->dw; q.lddw = d->lddw; q.f32 = d->dw_f32; q.add = d->dw_add;
         hipLaunchKernelGGL(ll_dw_kernel<T>, dim3(p.dt / BM * a.tiles_n), dim3(NTH), LL_LDS, st, q);
       }
     }
     if (d->dh)
-      launch_dh_out<E>((const float*)(ws + p.slab), p.R <= 512 ? 16 : 1, 0, splits, 0, d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh, d->lddh, st);
+      launch_dh_out<E>((const float*)(ws + p.slab), p.Rc <= 512 ? 16 : 1, 0, splits, 0, row0, p.Rc, d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh,
+                       d->lddh, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;

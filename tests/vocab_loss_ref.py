@@ -5,7 +5,8 @@ Tolerances are bounds, term by term, on what the kernels round (u = 2^-24 for fp
   exp         argument a = (z - max) c: rounded twice (2 u |a|), the instruction itself within 1 ulp (2 u); a term e^a with |a| large counts
               little (|a| e^a <= 0.37), so a sum of such terms and each p = e^a / sum is within 8 u of that rounding where p matters; n terms in
               16-term runs, lane and tile trees and <= 32 merges: <= 64 u more.  Together: E = 2 max|dz| c + (96 + 2 |a|) u
-  a cell      dz_ij = w1 p + w2 q - w1 [j = label] - w2 sum t: E on the p and q terms, (k + 12) u on t, one rounding to the cell's type
+  a cell      dz_ij = w1 p + w2 q - w1 [j = label] - w2 sum t: E on the p and q terms, (k + 12) u on t, and two roundings to the cell's type (the
+              exponential relative to its strip, then dz)
   a product   of n cells: the cells' errors times |operand|, n u of the sum of absolute values, one rounding at the end"""
 import torch
 
@@ -40,6 +41,7 @@ def losses(z, dz_err, labels, temp=1.0, alpha=0.0, top_vals=None, top_idx=None):
     tol = torch.zeros_like(row)
     cell = torch.zeros_like(z)
     cell_err = torch.zeros_like(z)
+    prob = torch.zeros_like(z)                  # the dense part of a cell: what is rounded before a label's or a list's part comes off
     mag = z.abs().amax(1).clamp(min=1.0)
     # (every term is unchanged when a row's logits move together: with the maximum taken out, lse - z keeps its digits also where |z| is 1e38)
     top = z.amax(1, keepdim=True)
@@ -53,6 +55,7 @@ def losses(z, dz_err, labels, temp=1.0, alpha=0.0, top_vals=None, top_idx=None):
         tol += w1 * (2 * dz_err + (160 + 8 * mag) * U32)
         one = torch.nn.functional.one_hot(lab, v).double()
         cell += w1 * (p - one)
+        prob += w1 * p
         a = (z - z.amax(1, keepdim=True)).abs()
         cell_err += w1 * (p * (2 * dz_err.unsqueeze(1) + (96 + 4 * a + 4 * mag.unsqueeze(1)) * U32) + 4 * U32 * one)
     if k and alpha > 0.0:
@@ -71,15 +74,17 @@ def losses(z, dz_err, labels, temp=1.0, alpha=0.0, top_vals=None, top_idx=None):
         a = (zt - zt.amax(1, keepdim=True)).abs()
         on = some.double().unsqueeze(1)
         cell += w2 * on * (q - dense)
+        prob += w2 * on * q
         cell_err += w2 * on * (q * (2 * dz_err.unsqueeze(1) / temp + (96 + 4 * a + 4 * mag.unsqueeze(1)) * U32) + dense * rel.unsqueeze(1))
     off = ~valid
     row[off] = 0
     tol[off] = 0
     cell[off] = 0
     cell_err[off] = 0
+    prob[off] = 0
     n = max(int(valid.sum()), 1)
     return dict(row_loss=row, row_tol=tol + 4 * U32 * row.abs(), loss=row.sum() / n, loss_tol=(tol.sum() + (rows + 4) * U32 * row.abs().sum()) / n, cell=cell,
-                cell_err=cell_err, n=n, nvalid=int(valid.sum()))
+                cell_err=cell_err, prob=prob, n=n, nvalid=int(valid.sum()))
 
 
 def linear(h, w, labels, scale=1.0, dw_dtype=None, temp=1.0, alpha=0.0, top_vals=None, top_idx=None):
@@ -94,9 +99,9 @@ def linear(h, w, labels, scale=1.0, dw_dtype=None, temp=1.0, alpha=0.0, top_vals
     dz_err = ((d + 4) * U32 * (hd.abs() @ wd.abs().t())).amax(1) if rows else torch.zeros(0, dtype=torch.float64, device=h.device)
     r = losses(z, dz_err, labels, temp, alpha, top_vals, top_idx)
     g = scale / r["n"]
-    tiny = 2.0 ** -40 if h.dtype == torch.float16 else 0.0          # half of the smallest fp16 step at a factor of at least 2^15 / 2^(w1 + w2)
+    tiny = 3 * 2.0 ** -40 if h.dtype == torch.float16 else 0.0      # half of the smallest fp16 step, twice, at a factor of at least 2^15 / 2^(w1 + w2)
     tiny *= max(1.0, 2.0 * ((1 - alpha) + alpha * temp))
-    cell_tol = r["cell_err"] + U * (r["cell"].abs() + r["cell_err"]) + tiny * valid.double().unsqueeze(1)
+    cell_tol = r["cell_err"] + U * (2 + U) * (r["cell"].abs() + r["prob"] + r["cell_err"]) + tiny * valid.double().unsqueeze(1)
     for name, out, err, mass, n, dt in (("dh", r["cell"] @ wd, cell_tol @ wd.abs(), r["cell"].abs() @ wd.abs(), v, h.dtype),
                                         ("dw", r["cell"].t() @ hd, cell_tol.t() @ hd.abs(), r["cell"].abs().t() @ hd.abs(), rows, dw_dtype or w.dtype)):
         out, err = out * g, (err + (n + 8) * U32 * mass) * g
