@@ -855,14 +855,29 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
   {
     const int r = threadIdx.x & (RB - 1), q = threadIdx.x / RB;
     float mx = -INFINITY, s1 = 0.f, s2 = 0.f;
-#pragma unroll 4
-    for (int t = q; t < p.tiles_n; t += 16) {
-      const int64_t o = (int64_t)t * p.R + i0 + r;
-      const float m = p.pm[o];
-      const float nm = fmaxf(mx, m);
-      s1 = (mx == -INFINITY ? 0.f : s1 * __builtin_amdgcn_exp2f(ll_ref(mx, p.c1) - ll_ref(nm, p.c1))) + p.p1[o] * __builtin_amdgcn_exp2f(ll_ref(m, p.c1) - ll_ref(nm, p.c1));
-      if (p.dual)
-        s2 = (mx == -INFINITY ? 0.f : s2 * __builtin_amdgcn_exp2f(ll_ref(mx, p.c2) - ll_ref(nm, p.c2))) + p.p2[o] * __builtin_amdgcn_exp2f(ll_ref(m, p.c2) - ll_ref(nm, p.c2));
+    // sixteen partials a thread in flight, joined with one exponential each
+    for (int t0 = q; t0 < p.tiles_n; t0 += 256) {
+      float m[16], a[16], b[16];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int t = t0 + 16 * x;
+        const int64_t o = (int64_t)min(t, p.tiles_n - 1) * p.R + i0 + r;
+        m[x] = p.pm[o];
+        a[x] = p.p1[o];
+        b[x] = p.dual ? p.p2[o] : 0.f;
+        if (t >= p.tiles_n) m[x] = -INFINITY;
+      }
+      float nm = mx;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) nm = fmaxf(nm, m[x]);
+      const float n1 = ll_ref(nm, p.c1), n2 = ll_ref(nm, p.c2);
+      s1 = mx == -INFINITY ? 0.f : s1 * __builtin_amdgcn_exp2f(ll_ref(mx, p.c1) - n1);
+      s2 = mx == -INFINITY ? 0.f : s2 * __builtin_amdgcn_exp2f(ll_ref(mx, p.c2) - n2);
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        s1 += m[x] == -INFINITY ? 0.f : a[x] * __builtin_amdgcn_exp2f(ll_ref(m[x], p.c1) - n1);
+        if (p.dual) s2 += m[x] == -INFINITY ? 0.f : b[x] * __builtin_amdgcn_exp2f(ll_ref(m[x], p.c2) - n2);
+      }
       mx = nm;
     }
     sm[0][r][q] = mx; sm[1][r][q] = s1; sm[2][r][q] = s2;
@@ -944,20 +959,23 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
   }
 }
 
-// the loss
-__global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__ packed_loss, const int* __restrict__ nvalid, float* __restrict__ loss) {
-  __shared__ float sh[16];
-  const int nv = *nvalid;
+// the loss: a launch of its own where no dh is asked for, else a workgroup of the kernel that writes dh
+template <int NT> __device__ __forceinline__ void ll_mean(const float* __restrict__ packed_loss, int nv, float* __restrict__ loss) {
+  __shared__ float sh[NT / 64];
   float s = 0.f;
-  for (int i = threadIdx.x; i < nv; i += 1024) s += packed_loss[i];
+#pragma unroll 4
+  for (int i = threadIdx.x; i < nv; i += NT) s += packed_loss[i];
   s = ns_wave_sum(s);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     s = 0.f;
-    for (int w = 0; w < 16; ++w) s += sh[w];
+    for (int w = 0; w < NT / 64; ++w) s += sh[w];
     *loss = s / (float)max(nv, 1);
   }
+}
+__global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__ packed_loss, const int* __restrict__ nvalid, float* __restrict__ loss) {
+  ll_mean<1024>(packed_loss, *nvalid, loss);
 }
 
 // the sparse cells of dz in one piece: one wave per row, each token written once whatever number of entries name it
@@ -1060,7 +1078,12 @@ __global__ __launch_bounds__(NTH) void ll_dh_kernel(const DhArgs p) {
 // (R > 0: slabs of (R, d); R = 0: slabs of 256 x 256 tiles, their number read from splits_dev.)
 template <class E>
 __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict__ slab, int groups, int splits, const int* __restrict__ splits_dev, int R, int row0, int chunk, int d, int rows, const int* __restrict__ inv,
-                                                        const int* __restrict__ nvalid, const float* __restrict__ loss_scale, float unscale, E* __restrict__ dh, int64_t lddh) {
+                                                        const int* __restrict__ nvalid, const float* __restrict__ loss_scale, float unscale, E* __restrict__ dh, int64_t lddh,
+                                                        const float* __restrict__ packed_loss, float* __restrict__ loss) {
+  if (loss && blockIdx.x == gridDim.x - 1) {      // one workgroup more: the mean of the row losses
+    ll_mean<256>(packed_loss, *nvalid, loss);
+    return;
+  }
   typedef E e4 __attribute__((ext_vector_type(4)));
   __shared__ f32x4 sm[16][16];
   // `groups` slab groups; the rest of the 16 lanes-of-16 take further column blocks
@@ -1094,11 +1117,11 @@ __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict_
   *(e4*)(dh + row * lddh + c) = o;
 }
 template <class E> void launch_dh_out(const float* slab, int groups, int splits, const int* splits_dev, int R, int row0, int chunk, int d, int rows, const int* inv, const int* nvalid, const float* loss_scale, float unscale, E* dh,
-                                      int64_t lddh, hipStream_t st) {
+                                      int64_t lddh, const float* packed_loss, float* loss, hipStream_t st) {
   const int nblk = 16 / groups;
   const int64_t items = (int64_t)rows * ((d + 63) / 64);
-  hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)((items + nblk - 1) / nblk)), dim3(256), 0, st, slab, groups, splits, splits_dev, R, row0, chunk, d, rows, inv, nvalid,
-                     loss_scale, unscale, dh, lddh);
+  hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)((items + nblk - 1) / nblk) + (loss ? 1 : 0)), dim3(256), 0, st, slab, groups, splits, splits_dev, R, row0, chunk, d, rows, inv, nvalid,
+                     loss_scale, unscale, dh, lddh, packed_loss, loss);
 }
 
 struct DwArgs {
@@ -1170,7 +1193,7 @@ __global__ __launch_bounds__(NTH) void ll_dw_kernel(const DwArgs p) {
 // ------------------------------------------------------------------------------------------------ few rows
 // Up to LL_FEW_ROWS rows: the time is W's bytes, read once for the logits and once more for dh (dW is written once).  No 256-row tiles, no packing, and
 // the logits of so few rows (N V fp32, 13 MB at 64) ARE kept, in the workspace: nothing is formed twice.
-//   ll_few_logits  a workgroup takes 256 rows of W, a wave 32 of them, straight from memory into MFMA operands (16 B per lane and 32 columns, four steps ahead)
+//   ll_few_logits  a workgroup takes 256 rows of W, a wave 32 of them, 64 columns at a time by LDS-DMA, three chunks in flight
 //   ll_rows        as for many rows, one workgroup for all of them, and the mean
 //   ll_few_grad    a workgroup takes 256 tokens: dz of those (rows x 256, in LDS, sparse cells put right there), then 64 columns of W at a time by LDS-DMA,
 //                  three chunks in flight: dh's part of these tokens, and the tokens' rows of dW
@@ -1210,8 +1233,13 @@ struct FewArgs {
   void* dw; int64_t lddw; int f32, add, dh;
 };
 
+constexpr int FW_BYTES = 256 * 128;          // a chunk of W: 256 tokens x 64 columns
+constexpr int FH_BYTES = 64 * 128;           // a chunk of h: 64 rows x 64 columns
+constexpr int FL_LDS = 3 * (FW_BYTES + FH_BYTES);
+
 template <class T, int MT, bool DUAL>
 __global__ __launch_bounds__(512) void ll_few_logits_kernel(const FewArgs p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef typename T::e E;
   typedef typename T::v8 v8;
   __shared__ float sm[3][8][16 * MT];
@@ -1230,57 +1258,61 @@ __global__ __launch_bounds__(512) void ll_few_logits_kernel(const FewArgs p) {
     if (lane == 0) *p.nvalid = nv;
   }
   const int n0 = blockIdx.x * 256, v0 = n0 + wave * 32;
-  const E* wr[2];
-  bool wok[2];
+  // W and h by LDS-DMA, 64 columns at a time, three slots (straight from memory into MFMA operands, 64 B of a row per load, W came at 2.5 - 3.5 TB/s): wave w
+  // fills and reads rows [32 w, 32 w + 32) of W in four pieces of 8 rows x 128 B, and fills rows [8 w, 8 w + 8) of h.  Chunk c of row r at c ^ ((r >> 1) & 7).
+  const ns_u4v rsrc = ll_rsrc((const E*)p.w + (int64_t)n0 * p.ldw), rsrc_h = ll_rsrc(p.h);
+  const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)smem;
+  uint32_t off[4], off_h;
+  int col[4], col_h;
 #pragma unroll
-  for (int f = 0; f < 2; ++f) {
-    const int v = v0 + f * 16 + l15;
-    wok[f] = v < p.V;
-    wr[f] = (const E*)p.w + (int64_t)(wok[f] ? v : p.V - 1) * p.ldw;
+  for (int j = 0; j < 4; ++j) {
+    const int r = 32 * wave + 8 * j + (lane >> 3);
+    col[j] = ((lane & 7) ^ ((r >> 1) & 7)) * 8;
+    off[j] = n0 + r < p.V ? (uint32_t)(r * (int)p.ldw + col[j]) * 2u : OUT;
   }
-  const E* hr[MT];
-  bool hok[MT];
+  {
+    const int r = 8 * wave + (lane >> 3), at = __shfl(src, r, 64);
+    col_h = ((lane & 7) ^ ((r >> 1) & 7)) * 8;
+    off_h = at >= 0 ? (uint32_t)(at * (int)p.ldh + col_h) * 2u : OUT;
+  }
+  const int chunks = (p.d + 63) / 64;
+  auto stage = [&](int c) __attribute__((always_inline)) {
+    const bool in = c < chunks;
+    const uint32_t dst = lds_base + (c % 3) * FW_BYTES + wave * 4096;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int s_ = __shfl(src, m * 16 + l15, 64);
-    hok[m] = s_ >= 0;
-    hr[m] = (const E*)p.h + (int64_t)(s_ >= 0 ? s_ : 0) * p.ldh;
-  }
-  const v8 zero = {};
+    for (int j = 0; j < 4; ++j) ll_dma16(rsrc, in && c * 64 + col[j] < p.d ? off[j] : OUT, in ? c * 128 : 0, dst + j * 1024);
+    ll_dma16(rsrc_h, in && c * 64 + col_h < p.d ? off_h : OUT, in ? c * 128 : 0, lds_base + 3 * FW_BYTES + (c % 3) * FH_BYTES + wave * 1024);
+  };
   f32x4 acc[2][MT];
 #pragma unroll
   for (int f = 0; f < 2; ++f)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[f][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  v8 wf[2][4][2];
-  auto fetch = [&](v8 (&to)[4][2], int k0) __attribute__((always_inline)) {
+  stage(0);
+  stage(1);
+  for (int c = 0; c < chunks; ++c) {
+    stage(c + 2);
+    asm volatile("s_waitcnt vmcnt(10)" ::: "memory");          // chunk c has landed (this wave's pieces; the barrier covers the others)
+    LL_BARRIER();
+    const char* const ws = smem + (c % 3) * FW_BYTES + (wave * 32 + l15) * 128;
+    const char* const hs = smem + 3 * FW_BYTES + (c % 3) * FH_BYTES + l15 * 128;
 #pragma unroll
-    for (int s_ = 0; s_ < 4; ++s_)
+    for (int ks = 0; ks < 2; ++ks) {
+      const int at = ((4 * ks + lg) ^ (l15 >> 1)) << 4;        // (16 rows further: the same permutation)
+      v8 a[2];
 #pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const int k = k0 + s_ * 32 + 8 * lg;
-        to[s_][f] = k < p.d ? *(const v8*)(wr[f] + k) : zero;
-      }
-  };
-  auto mul = [&](v8 (&a)[4][2], int k0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int s_ = 0; s_ < 4; ++s_) {
-      const int k = k0 + s_ * 32 + 8 * lg;
+      for (int f = 0; f < 2; ++f) a[f] = *(const v8*)(ws + f * 2048 + at);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const v8 b = hok[m] && k < p.d ? *(const v8*)(hr[m] + k) : zero;
+        const v8 b = *(const v8*)(hs + m * 2048 + at);
 #pragma unroll
-        for (int f = 0; f < 2; ++f) acc[f][m] = T::mma(a[s_][f], b, acc[f][m]);
+        for (int f = 0; f < 2; ++f) acc[f][m] = T::mma(a[f], b, acc[f][m]);
       }
     }
-  };
-  fetch(wf[0], 0);
-  for (int k0 = 0; k0 < p.d; k0 += 256) {
-    fetch(wf[1], k0 + 128);
-    mul(wf[0], k0);
-    fetch(wf[0], k0 + 256);
-    mul(wf[1], k0 + 128);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    LL_BARRIER();                                              // everyone has read this chunk before its slot is filled again
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   // a lane holds 4 neighbouring tokens of 16 MT rows, twice
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -1288,7 +1320,7 @@ __global__ __launch_bounds__(512) void ll_few_logits_kernel(const FewArgs p) {
     float mx = -INFINITY;
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
-      if (hok[m]) *(f32x4*)(p.z + (int64_t)r * p.ldz + v0 + f * 16 + 4 * lg) = acc[f][m];
+      if (r < nv) *(f32x4*)(p.z + (int64_t)r * p.ldz + v0 + f * 16 + 4 * lg) = acc[f][m];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (v0 + f * 16 + 4 * lg + e >= p.V) acc[f][m][e] = -INFINITY;
@@ -1330,9 +1362,7 @@ __global__ __launch_bounds__(512) void ll_few_logits_kernel(const FewArgs p) {
 }
 
 constexpr int FG_LD = 256 * 2 + 16;          // bytes per staged row of dz
-constexpr int FW_BYTES = 256 * 128;          // a chunk of W: 256 tokens x 64 columns
-constexpr int FH_LD = 64 * 2 + 16;           // bytes per staged row of h (64 columns)
-template <int MT> constexpr int few_lds() { return 3 * FW_BYTES + 16 * MT * FG_LD + (MT < 2 ? 32 : 16 * MT) * FH_LD; }
+template <int MT> constexpr int few_lds() { return 3 * FW_BYTES + 3 * FH_BYTES + 16 * MT * FG_LD; }
 
 // grid (tiles_n, column groups).  K of dW is the rows, padded to 32 with zeros.
 template <class T, int MT, bool DUAL>
@@ -1340,33 +1370,43 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef typename T::e E;
   typedef typename T::v8 v8;
-  constexpr int KR = MT < 2 ? 32 : 16 * MT;            // rows of h in LDS
-  char* const gs_ = smem + 3 * FW_BYTES;
-  char* const hs = gs_ + 16 * MT * FG_LD;
+  char* const hs = smem + 3 * FW_BYTES;
+  char* const gs_ = hs + 3 * FH_BYTES;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, lg = lane >> 4;
   const int n0 = blockIdx.x * 256;
   const int chunks = (p.d + 63) / 64, per = (chunks + gridDim.y - 1) / gridDim.y;
   const int c_begin = blockIdx.y * per, c_end = min(chunks, c_begin + per);
-  // W by LDS-DMA: wave w fills rows [32 w, 32 w + 32) of a chunk in four pieces of 8 rows x 128 B.  The 32-B windows of row r are permuted by
-  // f(r) = bit 1 | bit 3 << 1, so that the eight row segments of half a transposed read lie in different banks (even and odd rows already do).
-  const ns_u4v rsrc = ll_rsrc((const E*)p.w + (int64_t)n0 * p.ldw);
+  int src;
+  const int nv = few_rows(p.labels, p.rows, p.V, lane, src);
+  // Chunks of 64 columns by LDS-DMA, three slots: of W (for dh) wave w fills rows [32 w, 32 w + 32) in four pieces of 8 rows x 128 B, of h (for dW) rows
+  // [8 w, 8 w + 8) in one, packed rows of h by their original place.  The 32-B windows of row r are permuted by f(r) = bit 1 | bit 3 << 1, so that the eight
+  // row segments of half a transposed read lie in different banks (even and odd rows already do).
+  const ns_u4v rsrc = ll_rsrc((const E*)p.w + (int64_t)n0 * p.ldw), rsrc_h = ll_rsrc(p.h);
   const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)smem;
-  uint32_t off[4];
-  int col[4];
+  uint32_t off[4], off_h;
+  int col[4], col_h;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int r = 32 * wave + 8 * j + (lane >> 3), f = ((r >> 1) & 1) | (((r >> 3) & 1) << 1);
     col[j] = ((lane & 7) ^ (f << 1)) * 8;
     off[j] = n0 + r < p.V ? (uint32_t)(r * (int)p.ldw + col[j]) * 2u : OUT;
   }
+  {
+    const int r = 8 * wave + (lane >> 3), f = ((r >> 1) & 1) | (((r >> 3) & 1) << 1), at = __shfl(src, r, 64);
+    col_h = ((lane & 7) ^ (f << 1)) * 8;
+    off_h = at >= 0 ? (uint32_t)(at * (int)p.ldh + col_h) * 2u : OUT;
+  }
   auto stage = [&](int c) __attribute__((always_inline)) {
-    const uint32_t dst = lds_base + (c % 3) * FW_BYTES + wave * 4096;
+    const bool in = c < c_end;
+    if (p.dh) {
+      const uint32_t dst = lds_base + (c % 3) * FW_BYTES + wave * 4096;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ll_dma16(rsrc, c < c_end && c * 64 + col[j] < p.d ? off[j] : OUT, c < c_end ? c * 128 : 0, dst + j * 1024);
+      for (int j = 0; j < 4; ++j) ll_dma16(rsrc, in && c * 64 + col[j] < p.d ? off[j] : OUT, in ? c * 128 : 0, dst + j * 1024);
+    }
+    if (p.dw) ll_dma16(rsrc_h, in && c * 64 + col_h < p.d ? off_h : OUT, in ? c * 128 : 0, lds_base + 3 * FW_BYTES + (c % 3) * FH_BYTES + wave * 1024);
   };
-  int src;
-  const int nv = few_rows(p.labels, p.rows, p.V, lane, src);
-  if (p.dh) { stage(c_begin); stage(c_begin + 1); }
+  stage(c_begin);
+  stage(c_begin + 1);
   // dz of these 256 tokens
   for (int x = tid; x < 16 * MT * 64; x += 512) {
     const int r = x >> 6, c = (x & 63) * 4;
@@ -1413,85 +1453,114 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
   };
   const int q = l15 >> 2, pp = l15 & 3;
   const float gs = (p.loss_scale ? *p.loss_scale : 1.f) / (float)max(nv, 1) * p.unscale;
-  // dW: this wave's 32 tokens as the MFMA's columns (dz transposed), the rows as K
-  constexpr int KS = KR / 32;
+  // dW: this wave's 32 tokens as the MFMA's columns (dz transposed), the rows as K (16 rows: the upper half of a K step is zero)
+  constexpr int KS = MT < 2 ? 1 : MT / 2;
   v8 gt[2][KS];
   if (p.dw) {
 #pragma unroll
     for (int f = 0; f < 2; ++f)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const int r = ks * 32 + 8 * lg + q;
-        if (MT == 1 && lg >= 2) gt[f][ks] = v8{};       // (16 rows: the upper half of K is zero)
-        else gt[f][ks] = v8{};
-        const int rr = MT == 1 ? (8 * (lg & 1) + q) : r;
+        const int rr = MT == 1 ? 8 * (lg & 1) + q : ks * 32 + 8 * lg + q;
         const v8 v = tr8(gs_ + rr * FG_LD + (wave * 32 + f * 16 + 4 * pp) * 2, 4 * FG_LD);
-        if (!(MT == 1 && lg >= 2)) gt[f][ks] = v;
+        gt[f][ks] = MT == 1 && lg >= 2 ? v8{} : v;
       }
   }
-  // dh: output block `id` = (16 rows, 16 of the chunk's 64 columns), K = the 256 tokens
+  // how many stores a wave issues behind a chunk's pieces in a full chunk (fewer in a ragged one: there the waits count none)
+  const bool full_v = n0 + 256 <= p.V;
   for (int c = c_begin; c < c_end; ++c) {
-    if (p.dw) {
-      for (int x = tid; x < KR * 8; x += 512) {
-        const int r = x >> 3, cc = (x & 7) * 8;
-        const int s_ = r < nv ? p.order[r] : -1;
-        const uint4 v = s_ >= 0 && c * 64 + cc < p.d ? *(const uint4*)((const E*)p.h + (int64_t)s_ * p.ldh + c * 64 + cc) : make_uint4(0, 0, 0, 0);
-        *(uint4*)(hs + r * FH_LD + cc * 2) = v;
-      }
-    }
-    if (p.dh) {
-      stage(c + 2);
-      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");        // the chunk requested two steps ago has landed (this wave's part; the barrier covers the others)
+    stage(c + 2);
+    // chunk c has landed when, behind it, only chunk c + 1, the stores of step c - 1 and chunk c + 2 may be in flight (this wave's; the barrier covers the others)
+    const bool counted = full_v && c > c_begin && !p.f32;     // (step c - 1 is a full chunk: only the last may be ragged)
+    constexpr int SH = MT / 2;                                // stores of dh per wave and step (16 rows: half of the waves have one, not counted)
+    if (p.dh && p.dw) {
+      if (counted) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(14 + SH) : "memory");      // 5 + 4 + SH + 5
+      else asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+    } else if (p.dh) {
+      if (c > c_begin) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(8 + SH) : "memory");   // 4 + SH + 4
+      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    } else {
+      if (counted) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");                    // 1 + 4 + 1
+      else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     LL_BARRIER();
+    f32x4 dha[MT < 2 ? 1 : MT / 2];
     if (p.dh) {
+      // output block `id` = (16 rows, 16 of the chunk's 64 columns), K = the 256 tokens
       const char* const ws = smem + (c % 3) * FW_BYTES;
 #pragma unroll
-      for (int id0 = 0; id0 < 4 * MT; id0 += 8) {
-        const int id = id0 + wave;
+      for (int n = 0; n < (MT < 2 ? 1 : MT / 2); ++n) {
+        const int id = n * 8 + wave;
+        dha[n] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (id < 4 * MT) {
           const int mt = id >> 2, ct = id & 3;
-          f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
             const int r = ks * 32 + 8 * lg + q, f = ((r >> 1) & 1) | (((r >> 3) & 1) << 1);      // (four rows further: the same f)
             const v8 wt = tr8(ws + r * 128 + ((ct ^ f) << 5) + pp * 8, 512);
             const v8 g = *(const v8*)(gs_ + (mt * 16 + l15) * FG_LD + (ks * 32 + 8 * lg) * 2);
-            a = T::mma(wt, g, a);
+            dha[n] = T::mma(wt, g, dha[n]);
           }
-          const int cc = c * 64 + ct * 16 + 4 * lg;
-          if (cc < p.d) *(f32x4*)(p.slab + ((int64_t)blockIdx.x * 16 * MT + mt * 16 + l15) * p.d + cc) = a;
         }
       }
     }
+    f32x4 da[4][2];
     if (p.dw) {
+      const char* const hc = hs + (c % 3) * FH_BYTES;
 #pragma unroll
       for (int ct = 0; ct < 4; ++ct) {
         v8 ht[KS];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) ht[ks] = tr8(hs + (ks * 32 + 8 * lg + q) * FH_LD + (ct * 16 + 4 * pp) * 2, 4 * FH_LD);
-        const int cc = c * 64 + ct * 16 + 4 * lg;
+        for (int ks = 0; ks < KS; ++ks) {
+          const int r = ks * 32 + 8 * lg + q, f = ((r >> 1) & 1) | (((r >> 3) & 1) << 1);
+          ht[ks] = tr8(hc + r * 128 + ((ct ^ f) << 5) + pp * 8, 512);
+        }
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
           f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) a = T::mma(ht[ks], gt[f][ks], a);
-          const int v = n0 + wave * 32 + f * 16 + l15;
-          if (v >= p.V || cc >= p.d) continue;
-          a *= gs;
-          if (p.f32) {
-            f32x4* const at = (f32x4*)((float*)p.dw + (int64_t)v * p.lddw + cc);
-            if (p.add) a += *at;
-            *at = a;
-          } else {
-            *(ushort4v*)((E*)p.dw + (int64_t)v * p.lddw + cc) = cvt4<E>(a[0], a[1], a[2], a[3]);
-          }
+          da[ct][f] = a * gs;
         }
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    LL_BARRIER();                                              // everyone has read this chunk before its slot and h's are filled again
+    LL_BARRIER();                                              // everyone has read this chunk before its slot is filled again
+    if (p.dw) {
+      if (p.f32) {
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+          for (int f = 0; f < 2; ++f) {
+            const int v = n0 + wave * 32 + f * 16 + l15, cc = c * 64 + ct * 16 + 4 * lg;
+            if (v >= p.V || cc >= p.d) continue;
+            f32x4* const at = (f32x4*)((float*)p.dw + (int64_t)v * p.lddw + cc);
+            *at = p.add ? *at + da[ct][f] : da[ct][f];
+          }
+      } else {
+        // two column blocks of 16: the lanes of odd 16-lane rows give their 4 columns of the first for the even rows' 4 of the second, so that a lane holds 8
+        // neighbouring columns (16 B) and four lanes 64 B of a row of W
+#pragma unroll
+        for (int cp = 0; cp < 2; ++cp)
+#pragma unroll
+          for (int f = 0; f < 2; ++f) {
+            typedef unsigned u2 __attribute__((ext_vector_type(2)));
+            const f32x4 x = da[2 * cp][f], y = da[2 * cp + 1][f];
+            const u2 xa = __builtin_bit_cast(u2, cvt4<E>(x[0], x[1], x[2], x[3])), ya = __builtin_bit_cast(u2, cvt4<E>(y[0], y[1], y[2], y[3]));
+            const u2 r0 = __builtin_amdgcn_permlane16_swap(xa[0], ya[0], false, false), r1 = __builtin_amdgcn_permlane16_swap(xa[1], ya[1], false, false);
+            const int v = n0 + wave * 32 + f * 16 + l15, cc = c * 64 + (2 * cp + (lg & 1)) * 16 + (lg >> 1) * 8;
+            if (v < p.V && cc < p.d) *(uint4*)((E*)p.dw + (int64_t)v * p.lddw + cc) = make_uint4(r0[0], r1[0], r0[1], r1[1]);
+          }
+      }
+    }
+    if (p.dh) {
+#pragma unroll
+      for (int n = 0; n < (MT < 2 ? 1 : MT / 2); ++n) {
+        const int id = n * 8 + wave, mt = id >> 2, ct = id & 3, cc = c * 64 + ct * 16 + 4 * lg;
+        if (id < 4 * MT && cc < p.d) *(f32x4*)(p.slab + ((int64_t)blockIdx.x * 16 * MT + mt * 16 + l15) * p.d + cc) = dha[n];
+      }
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
@@ -1571,10 +1640,11 @@ template <class T, int MT>
 int few_launch(const ns_linear_ce_desc* d, const FewArgs& f, const RowArgs& r, bool dual, hipStream_t st) {
   typedef typename T::e E;
   static ns_dev_once once;
-  if (!ns_dyn_lds_once(once, {(const void*)ll_few_grad_kernel<T, MT, false>, (const void*)ll_few_grad_kernel<T, MT, true>}, few_lds<MT>(), "ns_linear_cross_entropy"))
+  if (!ns_dyn_lds_once(once, {(const void*)ll_few_grad_kernel<T, MT, false>, (const void*)ll_few_grad_kernel<T, MT, true>, (const void*)ll_few_logits_kernel<T, MT, false>,
+                              (const void*)ll_few_logits_kernel<T, MT, true>}, few_lds<MT>() > FL_LDS ? few_lds<MT>() : FL_LDS, "ns_linear_cross_entropy"))
     return NS_ERR_HIP;
-  if (dual) hipLaunchKernelGGL((ll_few_logits_kernel<T, MT, true>), dim3(f.tiles_n), dim3(512), 0, st, f);
-  else hipLaunchKernelGGL((ll_few_logits_kernel<T, MT, false>), dim3(f.tiles_n), dim3(512), 0, st, f);
+  if (dual) hipLaunchKernelGGL((ll_few_logits_kernel<T, MT, true>), dim3(f.tiles_n), dim3(512), FL_LDS, st, f);
+  else hipLaunchKernelGGL((ll_few_logits_kernel<T, MT, false>), dim3(f.tiles_n), dim3(512), FL_LDS, st, f);
   hipLaunchKernelGGL(ll_rows_kernel<1024>, dim3(1), dim3(1024), 0, st, r);
   if (d->dh || d->dw) {
     // a workgroup per CU: where the vocabulary is small, its column chunks are dealt to several
@@ -1585,7 +1655,7 @@ int few_launch(const ns_linear_ce_desc* d, const FewArgs& f, const RowArgs& r, b
     gy = (chunks + (chunks + gy - 1) / gy - 1) / ((chunks + gy - 1) / gy);
     if (dual) hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, true>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
     else hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, false>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
-    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n >= 64 ? 16 : f.tiles_n >= 16 ? 4 : 1, f.tiles_n, nullptr, 16 * MT, 0, LL_FEW_ROWS, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, st);
+    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n >= 64 ? 16 : f.tiles_n >= 16 ? 4 : 1, f.tiles_n, nullptr, 16 * MT, 0, LL_FEW_ROWS, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, nullptr, nullptr, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;
@@ -1655,7 +1725,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
     else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, LL_STATS, true, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     else hipLaunchKernelGGL((ll_logits_kernel<T, LL_STATS, false, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     hipLaunchKernelGGL(ll_rows_kernel<256>, dim3(p.Rc / 16), dim3(256), 0, st, r);
-    if (row0 + p.Rc >= p.R) hipLaunchKernelGGL(ll_mean_kernel, dim3(1), dim3(1024), 0, st, ploss, d->nvalid_dev, d->loss_dev);
+    if (!d->dh && row0 + p.Rc >= p.R) hipLaunchKernelGGL(ll_mean_kernel, dim3(1), dim3(1024), 0, st, ploss, d->nvalid_dev, d->loss_dev);
     if (!grad) continue;
     for (int pc = 0; pc < p.pieces; ++pc) {
       a.col0 = pc * p.piece_tiles * BN;
@@ -1686,7 +1756,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
     }
     if (d->dh)
       launch_dh_out<E>((const float*)(ws + p.slab), p.Rc <= 512 ? 16 : 1, 0, splits, 0, row0, p.Rc, d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh,
-                       d->lddh, st);
+                       d->lddh, ploss, row0 + p.Rc >= p.R ? d->loss_dev : nullptr, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;
