@@ -355,11 +355,13 @@ typedef enum { NS_F16 = 0, NS_BF16 = 1, NS_F32 = 2 } ns_dtype;
  *  - row_loss fp32 (rows), *loss_dev, *nvalid_dev (rows with a label).
  *  - dh (or NULL) and dw (or NULL): gradients of loss_scale x loss; loss_scale_dev
  *    may be NULL (1).  dw_f32: dw is fp32; dw_add (fp32 only): added to what is there.
+ *    0.05 <= temperature <= 100, 0 <= alpha <= 1, k <= 256.
  *  - workspace: ns_linear_ce_workspace_bytes(d) bytes (host-only call: sizes, k,
  *    alpha, temperature, ldw and whether dh / dw are set decide), 16-B aligned,
- *    free again when the call's work has run; it holds at most 256 MiB of dz at a
- *    time (one piece of the vocabulary) and fp32 partial sums of dh (128 MiB, or 4 d bytes
- *    a row where that is more).
+ *    free again when the call's work has run.  It holds at most 256 MiB of dz at a
+ *    time (or 256 tokens of all rows where that is more), at most 128 MiB of partial
+ *    sums of dh (or 4 d bytes a row), copies of h, and a few numbers per row and 64
+ *    tokens; up to 64 rows, their fp32 logits and 4 d bytes per row and 256 tokens.
  *  - the same inputs give the same bits (no atomics).  dh, dw must not overlap h, w. */
 typedef struct {
   const void *h, *w;
@@ -383,7 +385,7 @@ size_t ns_linear_ce_workspace_bytes(const ns_linear_ce_desc* d);   /* 0: sizes t
  * `dtype` (any ns_dtype): the loss of ns_linear_cross_entropy at z = logits, and
  * dlogits (or NULL; may be the logits themselves).  Rows may start at any element;
  * columns [vocab, ldz) are neither read nor written.  labels NULL (alpha = 1 only):
- * every row counts. */
+ * every row counts.  0.05 <= temperature <= 100, 0 < alpha <= 1, k <= 256. */
 typedef struct {
   const void* logits;
   const int64_t* labels;
@@ -400,7 +402,7 @@ typedef struct {
 int ns_distill_topk(const ns_distill_desc* d, void* stream);
 
 /* The teacher's side: the k largest logits of each row, largest first, equal ones
- * by the lowest token; vals fp32, idx int32 (rows, ldo), lse (or NULL): the row's
+ * by the lowest token; k <= 256; vals fp32, idx int32 (rows, ldo), lse (or NULL): the row's
  * log-sum-exp (fp32).  A NaN ranks above +inf. */
 typedef struct {
   const void* logits;

@@ -488,7 +488,7 @@ extern "C" int ns_distill_topk(const ns_distill_desc* d, void* stream) {
   NS_CHECK_ARG(d->dtype == NS_F16 || d->dtype == NS_BF16 || d->dtype == NS_F32, "ns_distill_topk: dtype %d", d->dtype);
   NS_CHECK_ARG(d->rows <= 1 || (d->ldz >= d->vocab && d->ld_top >= d->k && (!d->dlogits || d->lddz >= d->vocab)), "ns_distill_topk: row strides shorter than the rows");
   NS_CHECK_ARG(elem_aligned(d->logits, d->dtype) && elem_aligned(d->dlogits, d->dtype), "ns_distill_topk: logits not aligned to their elements");
-  NS_CHECK_ARG(d->temperature >= 1e-3f && d->temperature <= 1e3f && d->alpha > 0.f && d->alpha <= 1.f, "ns_distill_topk: temperature %g in [1e-3, 1e3], alpha %g in (0, 1]",
+  NS_CHECK_ARG(d->temperature >= 0.05f && d->temperature <= 100.f && d->alpha > 0.f && d->alpha <= 1.f, "ns_distill_topk: temperature %g in [0.05, 100], alpha %g in (0, 1]",
                (double)d->temperature, (double)d->alpha);
   NS_CHECK_ARG(d->labels || d->alpha == 1.f || d->rows == 0, "ns_distill_topk: alpha %g < 1 needs labels", (double)d->alpha);
   hipStream_t st = (hipStream_t)stream;

@@ -7,18 +7,24 @@
 //   dz_i = g [ w1 softmax(z_i) + w2 softmax(z_i / T) - w1 onehot(label_i) - w2 sum_k p_ik onehot(idx_ik) ],   w1 = 1 - alpha, w2 = alpha T
 //   dh = dz W,  dW = dz^T h,                        g = loss_scale / rows with a label
 //
-// The logits pass twice through the registers of a 256 x 256 tile and are never stored: a first pass keeps the running maximum and sum of
-// every row (fp32, one pair per row and 256 columns, joined by ll_rows_kernel), a second one forms dz of one PIECE of the vocabulary, rounds
-// it to the operands' type and leaves it in a workspace of at most LL_PIECE_BYTES (it stays in the 256-MiB last-level cache), from where the two products
-// dh += dz W and dW = dz^T h take it.  4 products instead of 3 (the logits are formed again) against 4 N V bytes written and read three times.
+// The logits pass through the registers of 256 x 256 MFMA tiles and are never stored as such.  One pass keeps the running maximum and sum of every row (fp32,
+// one pair per row and 256 columns, joined by ll_rows_kernel).  dz in the operands' type then lies in a workspace of at most LL_PIECE_BYTES (it stays in the
+// 256-MiB last-level cache), from where the products dh = dz W and dW = dz^T h take it.  It comes about in one of two ways:
+//   kept     the same pass leaves 2^(z - reference of the row's 64-column strip), ll_scale_kernel makes dz of it in place: no logit is formed twice.  One softmax
+//            (or two at 1 <= T <= 2), and whole rows: all of them within the workspace, or, where dW is not asked for, chunks of rows one after the other.
+//   formed again   a second pass over the logits writes dz of one PIECE of the vocabulary for all rows, piece after piece: 4 products instead of 3, but dW, of V d
+//            elements, is written once (chunks of rows would read and write it per chunk).
 //   * Rows without a label are packed away first: they cost nothing, and an infinity or NaN in a masked row reaches neither loss nor gradient.
 //   * A row's sparse terms (its label, the teacher's list) are no part of the dense epilogue: their logits are gathered as dot products in fp32
-//     and their cells of dz are written afterwards from those.
+//     and their cells of dz are written from those.
 //   * dz in the operands' type: fp16 cells carry a factor 2^s (exact; taken out in fp32 at the end), so that a probability of 1 / V does
 //     not fall among the subnormals; a probability below 2^-29 of full scale is a subnormal, below 2^-40 zero.  bf16 has the range of fp32.
-//     The label's cell is rounded once, after the subtraction.
-//   * Sums over the vocabulary (dh) and over the rows (dW) stay in fp32 MFMA accumulators / fp32 slabs added in a fixed order: no atomics,
+//     The label's cell is rounded once, after the subtraction; a kept cell twice (its exponential, dz).
+//   * Sums over the vocabulary (dh) and over the rows (dW) stay in fp32 MFMA accumulators / fp32 tiles added in a fixed order: no atomics,
 //     the same bits every time.
+//   * What bounds it: the 256 x 256 main loops (8 waves, two 64 KiB ring buffers, one workgroup per CU) run at 2.9 k cycles per K tile of 64 against 2.05 k of MFMA,
+//     LDS-port bound (192 KiB of fragments + 64 KiB of DMA per K tile), and at 1.6 GHz under that load: 1.1 - 1.46 PFLOP/s per launch, what a plain library
+//     product of the same shapes reaches (1.13 - 1.30).  Fewer cycles outside the main loops did not make them shorter, fewer products did.
 // The 256 x 256 main loop is ns_gemm_p8.hip's four-phase LDS-DMA ring (see there: two wave groups one barrier interval apart), here for both
 // 16-bit types and with a second operand that may be K-major (W for dh, dz for dW): such a region holds 64 k-rows of 256 B and its fragments are
 // read transposed by ds_read_b64_tr_b16.
@@ -394,6 +400,7 @@ struct LogitsArgs {
   float *pm, *p1, *p2;                   // (tiles_n, R): maximum, sum of exp2((z - max) c1), the same with c2
   const float *La, *Lb;                  // (R): base-2 log-sum-exp minus log2 of the weight and of 2^s
   void* G; int ldg;
+  float T;
   int row0; float *strip, shift, unshift;   // first packed row; LL_KEEP: (4 tiles_n, R) maxima of the 64-column strips, s and 2^-s
   const int* lab; const float* zk;       // FIX: the label's cell of dz is put right in the staged tile
   float wlab;                            // w1 2^s
@@ -667,22 +674,28 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[ah][mt][b >> 1][b & 1][r]);
           mx = ll_max4(mx);
-          const float e1 = (mx == -INFINITY ? 0.f : ll_ref(mx, p.c1)) - p.shift;
-          float s1 = 0.f;
+          // (two softmaxes: what is kept is the one at T, c2 < c1; the sum of the other is taken here from its own exponentials)
+          const float ck = DUAL ? p.c2 : p.c1, e1 = (mx == -INFINITY ? 0.f : ll_ref(mx, ck)) - p.shift;
+          const float e2 = DUAL && mx > -INFINITY ? ll_ref(mx, p.c1) : 0.f;
+          float s1 = 0.f, s2 = 0.f;
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
             float g[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              g[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[ah][mt][b >> 1][b & 1][r], p.c1, -e1));
+              const float z = acc[ah][mt][b >> 1][b & 1][r];
+              g[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(z, ck, -e1));
               s1 += g[r];
+              if (DUAL) s2 += __builtin_amdgcn_exp2f(__builtin_fmaf(z, p.c1, -e2));
             }
             *(ushort4v*)(st + rl * 128 + (((b * 2 + (eg >> 1)) ^ (rl & 7)) << 4) + (eg & 1) * 8) = cvt4<E>(g[0], g[1], g[2], g[3]);
           }
           s1 = ll_sum4(s1) * p.unshift;
+          if (DUAL) s2 = ll_sum4(s2);
           if (eg == 0) {
             side[wn * 256 + row] = mx;
-            side[1024 + wn * 256 + row] = s1;
+            side[1024 + wn * 256 + row] = DUAL ? s2 : s1;
+            if (DUAL) side[2048 + wn * 256 + row] = s1;
             strip[qt * 32 + rl] = mx;
           }
         }
@@ -758,11 +771,12 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
 
 // dz from what LL_KEEP left, in place: the strip's exponentials times 2^(e - La), one rounding more; a row's label cell (no list) is formed from its own
 // logit.  64 rows x 512 columns a workgroup, 16 B per lane; the pass is bound by its bytes (read and written once, mostly in the last-level cache).
-template <class T, bool FIX>
+// DUAL: what was kept is x = 2^(z c2 - e); softmax(z)'s share is x^T, by its logarithm (a relative rounding of x becomes T of them: T <= 2 only).
+template <class T, bool FIX, bool DUAL>
 __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
   typedef typename T::e E;
   typedef typename T::v8 v8;
-  __shared__ float f[8][64];
+  __shared__ float f[8][64], f1[DUAL ? 8 : 1][64];
   __shared__ int lc[64];
   __shared__ float lv[64];
   const int nv = min(*p.nvalid - p.row0, p.R);
@@ -772,7 +786,9 @@ __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
     const int sidx = t0 * 4 + (x >> 6), i = i0 + (x & 63);
     if (sidx < p.tiles_n * 4) {
       const float mx = p.strip[(int64_t)sidx * p.R + i];
-      f[x >> 6][x & 63] = __builtin_amdgcn_exp2f((mx == -INFINITY ? 0.f : ll_ref(mx, p.c1)) - p.shift - p.La[i]);
+      const float e = (mx == -INFINITY ? 0.f : ll_ref(mx, DUAL ? p.c2 : p.c1)) - p.shift;
+      f[x >> 6][x & 63] = __builtin_amdgcn_exp2f(e - (DUAL ? p.Lb[i] : p.La[i]));
+      if (DUAL) f1[x >> 6][x & 63] = e * p.T - p.La[i];
     }
   }
   if (FIX && threadIdx.x < 64) {
@@ -793,11 +809,12 @@ __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
       const int r = r0 + 4 * (8 * h + x);
-      const float a = f[c >> 6][r];
+      const float a = f[c >> 6][r], a1 = DUAL ? f1[c >> 6][r] : 0.f;
       const int at = FIX ? lc[r] - c : -1;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float g = (float)v[x][e] * a;
+        if (DUAL) g += __builtin_amdgcn_exp2f(__builtin_fmaf(__builtin_amdgcn_logf((float)v[x][e]), p.T, a1));
         if (FIX && at == e) g = lv[r];
         v[x][e] = (E)g;
       }
@@ -1582,12 +1599,12 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   p.dt = (d->d + BM - 1) / BM * BM;
   p.tiles_n = (d->vocab + BN - 1) / BN;
   const bool grad = d->dh || d->dw;
-  // Either whole rows of 16-bit exponentials in chunks of rows, no logit formed twice: one softmax, and dW not spread over chunks; or dz of one piece of the
+  // Either whole rows of 16-bit exponentials in chunks of rows, no logit formed twice: one softmax, or two at 1 <= T <= 2, and dW not spread over chunks; or dz of one piece of the
   // vocabulary at a time for all rows.  Both within LL_PIECE_BYTES, and a k-range of the head addressable with 32-bit byte offsets.
   const int64_t ldw = d->ldw > d->d ? d->ldw : d->d;
   const int64_t by_ld = ((int64_t)0x7FF00000 / 2 / ldw) / BN;
   const int64_t rows_fit = (int64_t)(LL_PIECE_BYTES / ((size_t)p.tiles_n * BN * 2)) / BM * BM;
-  p.keep = grad && !dual_of(d) && rows_fit >= BM && p.tiles_n <= by_ld && (p.R <= rows_fit || !d->dw);
+  p.keep = grad && (!dual_of(d) || d->temperature <= 2.f && d->temperature >= 1.f) && rows_fit >= BM && p.tiles_n <= by_ld && (p.R <= rows_fit || !d->dw);
   p.Rc = p.R;
   if (p.keep) {
     if (p.R > rows_fit) {
@@ -1680,7 +1697,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   const float up = ldexpf(1.f, s);
   static ns_dev_once once;
   if (!ns_dyn_lds_once(once, {(const void*)ll_logits_kernel<T, LL_STATS, false, false>, (const void*)ll_logits_kernel<T, LL_STATS, true, false>,
-                              (const void*)ll_logits_kernel<T, LL_KEEP, false, false>, (const void*)ll_logits_kernel<T, LL_GRAD, false, true>,
+                              (const void*)ll_logits_kernel<T, LL_KEEP, false, false>, (const void*)ll_logits_kernel<T, LL_KEEP, true, false>, (const void*)ll_logits_kernel<T, LL_GRAD, false, true>,
                               (const void*)ll_logits_kernel<T, LL_GRAD, false, false>, (const void*)ll_logits_kernel<T, LL_GRAD, true, false>,
                               (const void*)ll_dh_kernel<T>, (const void*)ll_dw_kernel<T>}, LL_LOGITS_LDS > LL_LDS ? LL_LOGITS_LDS : LL_LDS, "ns_linear_cross_entropy"))
     return NS_ERR_HIP;
@@ -1711,7 +1728,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
     hipLaunchKernelGGL(ll_transpose_kernel, dim3(p.R / 64, p.dp / 64), dim3(256), 0, st, (const uint16_t*)(ws + p.hp), p.dp, d->nvalid_dev, (uint16_t*)(ws + p.hT), p.R);
   LogitsArgs a = {};
   a.hp = ws + p.hp; a.w = d->w; a.ldw = d->ldw; a.dp = p.dp; a.d = d->d; a.V = d->vocab; a.col0 = 0; a.tiles_n = p.tiles_n; a.R = p.Rc; a.nvalid = d->nvalid_dev;
-  a.c1 = c1; a.c2 = c2;
+  a.c1 = c1; a.c2 = c2; a.T = T_;
   a.pm = (float*)(ws + p.pm); a.p1 = (float*)(ws + p.p1); a.p2 = (float*)(ws + p.p2);
   a.La = La; a.Lb = Lb; a.G = ws + p.G; a.ldg = p.piece_tiles * BN; a.lab = lab; a.zk = zk; a.wlab = w1 * up;
   a.strip = (float*)(ws + p.strip); a.shift = (float)s; a.unshift = 1.f / up;
@@ -1721,7 +1738,8 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
     a.row0 = r.row0 = row0;
     a.col0 = 0; a.tiles_n = p.tiles_n;
     const dim3 all = grid_of(p.tiles_n);
-    if (p.keep) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, false, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
+    if (p.keep && dual) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, true, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
+    else if (p.keep) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, false, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, LL_STATS, true, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     else hipLaunchKernelGGL((ll_logits_kernel<T, LL_STATS, false, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     hipLaunchKernelGGL(ll_rows_kernel<256>, dim3(p.Rc / 16), dim3(256), 0, st, r);
@@ -1733,8 +1751,9 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
       const dim3 grid = grid_of(a.tiles_n);
       if (p.keep) {
         const dim3 sg((a.tiles_n + 1) / 2, p.Rc / 64);
-        if (d->k == 0) hipLaunchKernelGGL((ll_scale_kernel<T, true>), sg, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((ll_scale_kernel<T, false>), sg, dim3(256), 0, st, a);
+        if (d->k == 0) hipLaunchKernelGGL((ll_scale_kernel<T, true, false>), sg, dim3(256), 0, st, a);
+        else if (dual) hipLaunchKernelGGL((ll_scale_kernel<T, false, true>), sg, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((ll_scale_kernel<T, false, false>), sg, dim3(256), 0, st, a);
       } else if (d->k == 0) hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, false, true>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
       else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, true, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
       else hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, false, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
@@ -1783,8 +1802,8 @@ extern "C" int ns_linear_cross_entropy(const ns_linear_ce_desc* desc, void* stre
   for (const void* q : {d->h, d->w, (const void*)d->dh, (const void*)d->dw, (const void*)d->workspace})
     NS_CHECK_ARG(((size_t)q & 15) == 0, "ns_linear_cross_entropy: a tensor does not start on 16 bytes");
   NS_CHECK_ARG(d->k == 0 || (d->top_vals && d->top_idx && d->ld_top >= d->k), "ns_linear_cross_entropy: the teacher's list needs values, tokens and a row stride >= k");
-  NS_CHECK_ARG(d->k == 0 || (d->temperature >= 1e-3f && d->temperature <= 1e3f && d->alpha >= 0.f && d->alpha <= 1.f),
-               "ns_linear_cross_entropy: temperature %g in [1e-3, 1e3], alpha %g in [0, 1]", (double)d->temperature, (double)d->alpha);
+  NS_CHECK_ARG(d->k == 0 || (d->temperature >= 0.05f && d->temperature <= 100.f && d->alpha >= 0.f && d->alpha <= 1.f),
+               "ns_linear_cross_entropy: temperature %g in [0.05, 100], alpha %g in [0, 1]", (double)d->temperature, (double)d->alpha);
   NS_CHECK_ARG(!d->dw_add || d->dw_f32, "ns_linear_cross_entropy: only an fp32 weight gradient is added to");
   if (d->alpha == 0.f) d->k = 0;     // the hard labels alone: the teacher's list is not read
   const Plan p = plan_of(d);

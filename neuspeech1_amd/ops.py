@@ -420,8 +420,8 @@ def _targets(d, rows, labels, row_loss, loss, nvalid, loss_scale, top_vals, top_
         raise ValueError(f"top_vals and top_idx: different row strides ({ld}, {li})")
     if not 1 <= k <= 256:
         raise ValueError(f"top_vals: {k} entries a row, 1 to 256 are supported")
-    if not 1e-3 <= temperature <= 1e3:
-        raise ValueError(f"temperature {temperature}: expected 1e-3 to 1e3")
+    if not 0.05 <= temperature <= 100.0:
+        raise ValueError(f"temperature {temperature}: expected 0.05 to 100")
     if not 0.0 <= alpha <= 1.0:
         raise ValueError(f"alpha {alpha}: expected 0 to 1")
     d.k, d.ld_top, d.top_vals, d.top_idx = k, ld, top_vals.data_ptr(), top_idx.data_ptr()
@@ -478,8 +478,7 @@ def linear_ce_workspace_bytes(h, weight, labels, *, row_loss, loss, nvalid, dh=N
 
 def linear_cross_entropy(h, weight, labels, *, row_loss, loss, nvalid, dh=None, dweight=None, loss_scale=None, top_vals=None, top_idx=None,
                          temperature=1.0, alpha=0.0, accumulate=False, workspace=None):
-    """The LM head and its loss without the logits (ns_linear_cross_entropy): z = h weight^T is formed in tiles, once for the losses and, when dh
-    or dweight is given, once more for dz.
+    """The LM head and its loss without the logits (ns_linear_cross_entropy): z = h weight^T only ever exists as tiles.
 
     h (rows, d), weight (vocab, d): float16 or bfloat16; labels (rows) int64, outside [0, vocab) = the row is ignored.  Written: row_loss (rows) and
     loss (1) float32, nvalid (1) int32, dh like h, dweight like weight or float32 (`accumulate`: added to a float32 one): gradients of

@@ -61,7 +61,7 @@ BAD_LINEAR = [
     (dict(**lists(), alpha=1.5), "alpha"),
     (dict(**lists(), alpha=-0.1), "alpha"),
     (dict(**lists(), alpha=float("nan")), "alpha"),
-    (dict(**lists(), alpha=0.5, temperature=0.0), "temperature"),
+    (dict(**lists(), alpha=0.5, temperature=0.04), "temperature"),
     (dict(**lists(), alpha=0.5, temperature=float("inf")), "temperature"),
     ({}, "expected a GPU"),
 ]

@@ -6,7 +6,7 @@ Tolerances are bounds, term by term, on what the kernels round (u = 2^-24 for fp
               little (|a| e^a <= 0.37), so a sum of such terms and each p = e^a / sum is within 8 u of that rounding where p matters; n terms in
               16-term runs, lane and tile trees and <= 32 merges: <= 64 u more.  Together: E = 2 max|dz| c + (96 + 2 |a|) u
   a cell      dz_ij = w1 p + w2 q - w1 [j = label] - w2 sum t: E on the p and q terms, (k + 12) u on t, and two roundings to the cell's type (the
-              exponential relative to its strip, then dz)
+              exponential relative to its strip, then dz; of two softmaxes the first one's exponential may be the T-th power of a rounded one, T <= 2: three)
   a product   of n cells: the cells' errors times |operand|, n u of the sum of absolute values, one rounding at the end"""
 import torch
 
@@ -101,7 +101,7 @@ def linear(h, w, labels, scale=1.0, dw_dtype=None, temp=1.0, alpha=0.0, top_vals
     g = scale / r["n"]
     tiny = 3 * 2.0 ** -40 if h.dtype == torch.float16 else 0.0      # half of the smallest fp16 step, twice, at a factor of at least 2^15 / 2^(w1 + w2)
     tiny *= max(1.0, 2.0 * ((1 - alpha) + alpha * temp))
-    cell_tol = r["cell_err"] + U * (2 + U) * (r["cell"].abs() + r["prob"] + r["cell_err"]) + tiny * valid.double().unsqueeze(1)
+    cell_tol = r["cell_err"] + U * (3 + 3 * U) * (r["cell"].abs() + r["prob"] + r["cell_err"]) + tiny * valid.double().unsqueeze(1)
     for name, out, err, mass, n, dt in (("dh", r["cell"] @ wd, cell_tol @ wd.abs(), r["cell"].abs() @ wd.abs(), v, h.dtype),
                                         ("dw", r["cell"].t() @ hd, cell_tol.t() @ hd.abs(), r["cell"].abs().t() @ hd.abs(), rows, dw_dtype or w.dtype)):
         out, err = out * g, (err + (n + 8) * U32 * mass) * g
