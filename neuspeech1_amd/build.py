@@ -17,10 +17,7 @@ BUILD = os.path.join(HERE, "csrc", "build")
 LIB = os.path.join(HERE, "libneuspeech_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wno-unused-value",
-         "-fno-gpu-rdc", "-ffp-contract=fast",
-         # no v_pk_{add,mul,fma}_f32: some of their forms have given wrong results on this hardware now and then.  (Device feature only: hipcc's
-         # host pass warns that it does not know it, which _compile drops.)
-         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+         "-fno-gpu-rdc", "-ffp-contract=fast"]
 FLAGS += os.environ.get("NS_EXTRA_HIPCC_FLAGS", "").split()   # diagnostic builds only (e.g. -DNS_P8_STAMPS)
 
 
@@ -44,9 +41,8 @@ def _compile(src: str, force: bool) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed for {src}:\n{r.stdout}\n{r.stderr}")
-    err = "".join(ln for ln in r.stderr.splitlines(True) if "packed-fp32-ops" not in ln)
-    if err.strip():
-        sys.stderr.write(err)
+    if r.stderr.strip():
+        sys.stderr.write(r.stderr)
     return obj
 
 

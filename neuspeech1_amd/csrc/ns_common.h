@@ -91,8 +91,8 @@ __device__ __forceinline__ void ns_gelu_both(float x, float& g, float& dg) {
   g = x * cdf;
   dg = cdf + x * pdf;
 }
-// Two elements at a time: same formula, same constants, same rounding per element as ns_gelu_both.  (The build turns packed fp32
-// instructions off -- build.py -- so a pair is two scalar streams.)
+// Two elements at a time with packed fp32 arithmetic (v_pk_mul / v_pk_fma_f32: two lanes' worth of FMA per issue slot on
+// gfx950); exp and rcp stay scalar.  Same formula, same constants, same rounding per element as ns_gelu_both.
 typedef float ns_f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void ns_gelu_both2(ns_f2 x, ns_f2& g, ns_f2& dg) {
   const ns_f2 ax = {fabsf(x.x), fabsf(x.y)};
