@@ -15,7 +15,7 @@ pytestmark = pytest.mark.skipif(not os.path.exists(build.HIPCC), reason="needs h
 @pytest.fixture(scope="module")
 def kernels(tmp_path_factory):
     out = str(tmp_path_factory.mktemp("isa") / "ll.s")
-    flags = [f for f in build.FLAGS if f != "-fPIC"]
+    flags = [f for f in build.flags_of("ns_linear_loss.hip") if f != "-fPIC"]
     subprocess.run([build.HIPCC, *flags, "-S", "--cuda-device-only", os.path.join(build.CSRC, "ns_linear_loss.hip"), "-o", out], check=True, capture_output=True)
     text = open(out).read()
     return {m.group(1): m.group(2) for m in re.finditer(r"^(_Z\w+):[^\n]*\n(.*?)\.Lfunc_end", text, re.S | re.M)}
