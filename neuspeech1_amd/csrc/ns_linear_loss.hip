@@ -19,7 +19,7 @@
 //     and their cells of dz are written from those.
 //   * dz in the operands' type: fp16 cells carry a factor 2^s (exact; taken out in fp32 at the end), so that a probability of 1 / V does
 //     not fall among the subnormals; a probability below 2^-29 of full scale is a subnormal, below 2^-40 zero.  bf16 has the range of fp32.
-//     The label's cell is rounded once, after the subtraction; a kept cell twice (its exponential, dz).
+//     The label's cell is rounded once, after the subtraction; a kept cell twice (its exponential, dz); with few labels a cell is two numbers (ll_few_grad).
 //   * Sums over the vocabulary (dh) and over the rows (dW) stay in fp32 MFMA accumulators / fp32 tiles added in a fixed order: no atomics,
 //     the same bits every time.
 //   * What bounds it: the 256 x 256 main loops (8 waves, two 64 KiB ring buffers, one workgroup per CU) run at 2.9 k cycles per K tile of 64 against 2.05 k of MFMA,
@@ -1092,7 +1092,7 @@ __global__ __launch_bounds__(NTH) void ll_dh_kernel(const DhArgs p) {
 
 // dh[row] = g 2^-s sum of the slabs (in their order), zero for a row without a label.  A workgroup takes 64 columns of a row with 16 threads of 4 columns,
 // and 16 groups of slabs side by side: with one token and 203 slabs a single chain of loads took 28 us
-// (R > 0: slabs of (R, d); R = 0: slabs of 256 x 256 tiles, their number read from splits_dev.)
+// (R > 0: slabs of (R, d) from the few-row path; R = 0: slabs of 256 x 256 tiles, their number read from splits_dev.)
 template <class E>
 __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict__ slab, int groups, int splits, const int* __restrict__ splits_dev, int R, int row0, int chunk, int d, int rows, const int* __restrict__ inv,
                                                         const int* __restrict__ nvalid, const float* __restrict__ loss_scale, float unscale, E* __restrict__ dh, int64_t lddh,
@@ -1117,8 +1117,13 @@ __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict_
     const int tiles_d = (d + BN - 1) / BN, tiles = (min(*nvalid - row0, chunk) + BM - 1) / BM * tiles_d;
     const int64_t at = R > 0 ? (int64_t)i * d + c : ((int64_t)(i / BM * tiles_d + c / BN) * BM + i % BM) * BN + c % BN;
     const int64_t step = R > 0 ? (int64_t)R * d : (int64_t)tiles * BM * BN;
+    if (R > 0 && 2 * *nvalid <= R) {             // (rows that are in two parts: R / 2 further is what the first part's rounding lost)
 #pragma unroll 4
-    for (int s = g * per_g; s < s1; ++s) a += *(const f32x4*)(slab + s * step + at);
+      for (int s = g * per_g; s < s1; ++s) a += *(const f32x4*)(slab + s * step + at) + *(const f32x4*)(slab + s * step + at + (int64_t)(R / 2) * d);
+    } else {
+#pragma unroll 4
+      for (int s = g * per_g; s < s1; ++s) a += *(const f32x4*)(slab + s * step + at);
+    }
   }
   if (groups > 1) {
     sm[sub][threadIdx.x & 15] = a;
@@ -1395,6 +1400,11 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
   const int c_begin = blockIdx.y * per, c_end = min(chunks, c_begin + per);
   int src;
   const int nv = few_rows(p.labels, p.rows, p.V, lane, src);
+  // Few enough rows with a label leave half of dz's rows free: row r + HALF then holds what row r's rounding lost, dh's two rows are added at the end and h's row
+  // stands there twice for dW.  The label's cell is most of such a row's dz, and its one rounding would be a factor on the whole gradient: with many
+  // rows these factors average out, with one fp16 row dh was off by 3.1e-4 where its own rounding is 2.1e-4.
+  constexpr int HALF = 8 * MT;
+  const bool twice = nv <= HALF;
   // Chunks of 64 columns by LDS-DMA, three slots: of W (for dh) wave w fills rows [32 w, 32 w + 32) in four pieces of 8 rows x 128 B, of h (for dW) rows
   // [8 w, 8 w + 8) in one, packed rows of h by their original place.  The 32-B windows of row r are permuted by f(r) = bit 1 | bit 3 << 1, so that the eight
   // row segments of half a transposed read lie in different banks (even and odd rows already do).
@@ -1409,7 +1419,7 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
     off[j] = n0 + r < p.V ? (uint32_t)(r * (int)p.ldw + col[j]) * 2u : OUT;
   }
   {
-    const int r = 8 * wave + (lane >> 3), f = ((r >> 1) & 1) | (((r >> 3) & 1) << 1), at = __shfl(src, r, 64);
+    const int r = 8 * wave + (lane >> 3), f = ((r >> 1) & 1) | (((r >> 3) & 1) << 1), at = __shfl(src, twice && r >= HALF ? r - HALF : r, 64);
     col_h = ((lane & 7) ^ (f << 1)) * 8;
     off_h = at >= 0 ? (uint32_t)(at * (int)p.ldh + col_h) * 2u : OUT;
   }
@@ -1427,6 +1437,7 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
   // dz of these 256 tokens
   for (int x = tid; x < 16 * MT * 64; x += 512) {
     const int r = x >> 6, c = (x & 63) * 4;
+    if (twice && r >= HALF) break;
     float g[4] = {0.f, 0.f, 0.f, 0.f};
     if (r < nv) {
       const f32x4 z = *(const f32x4*)(p.z + (int64_t)r * p.ldz + n0 + c);
@@ -1439,6 +1450,8 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
       }
     }
     *(ushort4v*)(gs_ + r * FG_LD + c * 2) = cvt4<E>(g[0], g[1], g[2], g[3]);
+    if (twice)
+      *(ushort4v*)(gs_ + (r + HALF) * FG_LD + c * 2) = cvt4<E>(g[0] - (float)(E)g[0], g[1] - (float)(E)g[1], g[2] - (float)(E)g[2], g[3] - (float)(E)g[3]);
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   LL_BARRIER();
@@ -1459,6 +1472,7 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
     v -= p.w2s * soft;
     if (t == lab) v -= p.w1s;
     *(E*)(gs_ + r * FG_LD + (t - n0) * 2) = (E)v;
+    if (twice) *(E*)(gs_ + (r + HALF) * FG_LD + (t - n0) * 2) = (E)(v - (float)(E)v);
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   LL_BARRIER();

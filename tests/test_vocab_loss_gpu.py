@@ -59,7 +59,7 @@ def close(got, want, tol, what):
     assert not bad.any(), (what, int(bad.sum()), bad.numel(), float((got - want).abs()[bad].max()), float(tol[bad].min()), bad.nonzero()[:4].tolist())
 
 
-def check_linear(ops, dev, h, w, labels, lists=(None, None), temp=1.0, alpha=0.0, scale=None, grad="hw", dw_dtype=None, **kw):
+def check_linear(ops, dev, h, w, labels, lists=(None, None), temp=1.0, alpha=0.0, scale=None, grad="hw", dw_dtype=None, parts=1, **kw):
     rows, d = h.shape
     o = outputs(dev, rows)
     dh = torch.full_like(h, 3.0) if "h" in grad else None
@@ -68,7 +68,7 @@ def check_linear(ops, dev, h, w, labels, lists=(None, None), temp=1.0, alpha=0.0
     more = dict(top_vals=lists[0], top_idx=lists[1], temperature=temp, alpha=alpha) if lists[0] is not None else {}
     ops.linear_cross_entropy(h, w, labels, dh=dh, dweight=dw, loss_scale=sc, **o, **more, **kw)
     torch.cuda.synchronize()
-    ref = R.linear(h, w, labels, 1.0 if scale is None else scale, dw_dtype, temp, alpha, *lists)
+    ref = R.linear(h, w, labels, 1.0 if scale is None else scale, dw_dtype, temp, alpha, *lists, parts=parts)
     assert int(o["nvalid"]) == ref["nvalid"]
     close(o["row_loss"], ref["row_loss"], ref["row_tol"], "row_loss")
     close(o["loss"], ref["loss"].reshape(1), ref["loss_tol"].reshape(1), "loss")
@@ -94,6 +94,18 @@ def test_linear_cross_entropy(ops, dev, dtype, rows, d, v):
 def test_linear_cross_entropy_with_a_teacher(ops, dev, dtype, rows, d, v, k, temp, alpha):
     h, w, labels, lists = make_linear(dev, rows, d, v, dtype, seed=1, k=k)
     check_linear(ops, dev, h, w, labels, lists, temp, alpha)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,live,d,v", [(1, 1, 64, 300), (2, 2, 512, 5000), (8, 8, 136, 257), (16, 5, 64, 1000), (32, 16, 72, 300), (64, 1, 64, 513), (64, 32, 200, 700)])
+@pytest.mark.parametrize("k,temp,alpha", [(0, 1.0, 0.0), (7, 2.0, 0.5), (3, 1.0, 0.5)])
+def test_few_labels_keep_their_digits(ops, dev, dtype, rows, live, d, v, k, temp, alpha):
+    """the gradient of a few tokens is as exact as its own rounding: the one rounding of a label's cell would be a factor on all of it"""
+    h, w, labels, lists = make_linear(dev, rows, d, v, dtype, seed=11, ignored=0.0, k=k)
+    labels = torch.arange(rows, device=dev) * 7 % v
+    h = (h.float() * 0.5 + w[labels].float()).to(dtype)
+    labels[torch.randperm(rows, generator=gen(rows, dev), device=dev)[live:]] = -100
+    check_linear(ops, dev, h, w, labels, lists, temp, alpha, parts=2, dw_dtype=F32 if rows == 16 else None)
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])

@@ -87,8 +87,9 @@ def losses(z, dz_err, labels, temp=1.0, alpha=0.0, top_vals=None, top_idx=None):
                 cell_err=cell_err, prob=prob, n=n, nvalid=int(valid.sum()))
 
 
-def linear(h, w, labels, scale=1.0, dw_dtype=None, temp=1.0, alpha=0.0, top_vals=None, top_idx=None):
-    """linear_cross_entropy in 64 bits: losses' dict + dh, dw and their tolerances.  Rows without a label are taken out first."""
+def linear(h, w, labels, scale=1.0, dw_dtype=None, temp=1.0, alpha=0.0, top_vals=None, top_idx=None, parts=1):
+    """linear_cross_entropy in 64 bits: losses' dict + dh, dw and their tolerances.  Rows without a label are taken out first.  parts = 2: the cells are
+    sums of two numbers of their type (the first off by U of the cell, the second by U of that; formed from fp32, so 2 u of the terms as well)"""
     rows, d = h.shape
     v = w.shape[0]
     U = half_step(h.dtype)
@@ -101,7 +102,8 @@ def linear(h, w, labels, scale=1.0, dw_dtype=None, temp=1.0, alpha=0.0, top_vals
     g = scale / r["n"]
     tiny = 3 * 2.0 ** -40 if h.dtype == torch.float16 else 0.0      # half of the smallest fp16 step, twice, at a factor of at least 2^15 / 2^(w1 + w2)
     tiny *= max(1.0, 2.0 * ((1 - alpha) + alpha * temp))
-    cell_tol = r["cell_err"] + U * (3 + 3 * U) * (r["cell"].abs() + r["prob"] + r["cell_err"]) + tiny * valid.double().unsqueeze(1)
+    each = U * (3 + 3 * U) if parts == 1 else U * U + 2 * U32
+    cell_tol = r["cell_err"] + each * (r["cell"].abs() + r["prob"] + r["cell_err"]) + tiny * valid.double().unsqueeze(1)
     for name, out, err, mass, n, dt in (("dh", r["cell"] @ wd, cell_tol @ wd.abs(), r["cell"].abs() @ wd.abs(), v, h.dtype),
                                         ("dw", r["cell"].t() @ hd, cell_tol.t() @ hd.abs(), r["cell"].abs().t() @ hd.abs(), rows, dw_dtype or w.dtype)):
         out, err = out * g, (err + (n + 8) * U32 * mass) * g
