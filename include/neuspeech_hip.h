@@ -358,8 +358,9 @@ typedef enum { NS_F16 = 0, NS_BF16 = 1, NS_F32 = 2 } ns_dtype;
  *    0.05 <= temperature <= 100, 0 <= alpha <= 1, k <= 256.
  *  - workspace: ns_linear_ce_workspace_bytes(d) bytes (host-only call: sizes, k,
  *    alpha, temperature, ldw and whether dh / dw are set decide), 16-B aligned,
- *    free again when the call's work has run.  It holds at most 256 MiB of dz at a
- *    time (or 256 tokens of all rows where that is more), at most 128 MiB of partial
+ *    free again when the call's work has run.  It holds dz of all rows where that
+ *    is at most 1 GiB and dw is asked for, else at most 256 MiB of dz at a time (or
+ *    256 tokens of all rows where that is more); at most 128 MiB of partial
  *    sums of dh (or 4 d bytes a row), copies of h, and a few numbers per row and 64
  *    tokens; up to 64 rows, their fp32 logits and 4 d bytes per row and 256 tokens.
  *  - the same inputs give the same bits (no atomics).  dh, dw must not overlap h, w. */

@@ -121,17 +121,21 @@ def test_the_c_entry_points_refuse_too():
 
 
 def test_workspace_rule():
-    """one piece of dz stays within 256 MiB however many rows and tokens there are, dh's partial sums within 128; the loss alone needs none of it; the list costs what it holds"""
-    def need(rows, d, v, grad, k=0):
+    """one piece of dz stays within 256 MiB (all of it within 1 GiB where the head learns) however many rows and tokens there are, dh's partial sums within 128; the loss alone needs none of it; the list costs what it holds"""
+    def need(rows, d, v, grad, k=0, head=False):
         a = linear_args(rows, d, v)
         if grad:
             a.update(dh=torch.empty_like(a["h"]))
+        if head:
+            a.update(dweight=torch.empty_like(a["weight"]))
         if k:
             a.update(lists(rows, k), alpha=0.5, temperature=2.0)
         return ops.linear_ce_workspace_bytes(a.pop("h"), a.pop("weight"), a.pop("labels"), **a)
     full = 2048 * 51968 * 2
     assert full < need(2048, 64, 51865, True) - need(2048, 64, 51865, False) <= full + 136 * (1 << 20)
     assert need(9000, 64, 51865, True) - need(9000, 64, 51865, False) <= 400 * (1 << 20) < 9000 * 51865 * 2
+    assert 9000 * 51865 * 2 < need(9000, 64, 51865, True, head=True) < 9216 * 51968 * 2 + 256 * (1 << 20)
+    assert need(11000, 64, 51865, True, head=True) < 400 * (1 << 20)
     assert need(100, 64, 1000, False, 64) > need(100, 64, 1000, False)
     assert need(1, 8, 1, True) > 0 and need(0, 8, 1, True) > 0
     assert lib.load().ns_linear_ce_workspace_bytes(C.byref(lib.LinearCeDesc())) == 0

@@ -129,12 +129,21 @@ def test_linear_cross_entropy_adds_to_a_float32_weight_gradient(ops, dev, rows):
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("grad,k,temp,alpha,ignored", [("hw", 3, 2.0, 0.5, 0.0), ("hw", 0, 1.0, 0.0, 0.1), ("hw", 3, 1.0, 0.5, 0.6), ("h", 0, 1.0, 0.0, 0.0), ("h", 3, 1.0, 0.5, 0.1),
-                                                       ("h", 0, 1.0, 0.0, 0.5), ("h", 4, 3.0, 1.0, 0.0), ("", 0, 1.0, 0.0, 0.0)])
+                                                       ("h", 0, 1.0, 0.0, 0.5), ("h", 4, 3.0, 1.0, 0.0), ("", 0, 1.0, 0.0, 0.0),
+                                                       ("hw", 3, 4.0, 0.5, 0.1), ("h", 3, 0.5, 0.5, 0.0)])
 def test_linear_cross_entropy_beyond_one_workspace(ops, dev, dtype, grad, k, temp, alpha, ignored):
-    """more rows x tokens than 256 MiB of dz: pieces of the vocabulary where the head learns or two softmaxes are mixed, chunks of rows (the last one full,
+    """more rows x tokens than 256 MiB of dz: all of it where the head learns, pieces of the vocabulary where two softmaxes are mixed, chunks of rows (the last one full,
     partly filled or without a row) elsewhere"""
     h, w, labels, lists = make_linear(dev, 2049, 64, 60001, dtype, seed=4, ignored=ignored, k=k)
     check_linear(ops, dev, h, w, labels, lists, temp, alpha, grad=grad)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("k", [0, 3])
+def test_linear_cross_entropy_beyond_all_rows_of_dz(ops, dev, dtype, k):
+    """more than 1 GiB of dz and the head learns: pieces of the vocabulary"""
+    h, w, labels, lists = make_linear(dev, 2049, 64, 240001, dtype, seed=12, ignored=0.1, k=k)
+    check_linear(ops, dev, h, w, labels, lists, 1.0, 0.5 if k else 0.0)
 
 
 @pytest.mark.parametrize("rows", [14, 60, 300])
