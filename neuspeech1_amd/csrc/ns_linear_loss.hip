@@ -353,7 +353,7 @@ __global__ __launch_bounds__(256) void ll_pack_kernel(const void* __restrict__ h
 }
 
 // zk[i][e] = h_i . W[token e], e = 0 .. k - 1 the teacher's list, e = k the label: a workgroup per row, 16 lanes per entry (256 B of W a step, 16 entries
-// side by side; one entry after the other on a wave, 64 entries took 77 us for 1434 rows at d = 512, this 24)
+// side by side; one entry after the other on a wave, 64 entries took 77 us for 1434 rows at d = 512, this 19)
 template <class T>
 __global__ __launch_bounds__(256) void ll_gather_kernel(const void* __restrict__ hp_, int dp, const void* __restrict__ w_, int64_t ldw, int d, int V,
                                                         const int* __restrict__ order, const int* __restrict__ lab, const int32_t* __restrict__ top_idx,
