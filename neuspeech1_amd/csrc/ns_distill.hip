@@ -129,10 +129,11 @@ struct DistillArgs {
   int* nvalid; const float* loss_scale;
 };
 
-// DUAL: two softmaxes (0 < alpha < 1 at T != 1), else one, at T when only soft targets count.
+// DUAL: two softmaxes (0 < alpha < 1 at T != 1), else one, at T when only soft targets count.  2 and 4: the temperature is that, and e^z is a power of
+// e^(z / T) by multiplication (its relative error T times the other's, which is what the argument's rounding in e^z itself amounts to).
 // Per logit: a conversion and a maximum, then an fma, an exponential (a quarter-rate instruction) and an addition per softmax, and the same again for the
-// gradient: with DUAL ~30 issue slots, 26 k cycles of a CU a row of 51 865 against the 20 k that the row's 208 KB take at the copy rate.
-template <class E, int NC, int NT, bool DUAL>
+// gradient: with DUAL = 1 ~30 issue slots, 26 k cycles of a CU a row of 51 865 against the 20 k that the row's 208 KB take at the copy rate.
+template <class E, int NC, int NT, int DUAL>
 __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_kernel(const DistillArgs p) {
   constexpr int NW = NT / 64;
   __shared__ float sh[3][NW];
@@ -196,8 +197,13 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
   {
     const float m = finite_or_zero(mx);      // (subtracted first: a maximum near the type's lowest value times c would overflow)
     auto add = [&](float x) __attribute__((always_inline)) {
-      s1 += __builtin_amdgcn_exp2f((x - m) * c1);
-      if (DUAL) s2 += __builtin_amdgcn_exp2f((x - m) * c2);
+      if (DUAL < 2) s1 += __builtin_amdgcn_exp2f((x - m) * c1);
+      if (DUAL) {
+        const float y = __builtin_amdgcn_exp2f((x - m) * c2), y2 = y * y;
+        s2 += y;
+        if (DUAL == 2) s1 += y2;
+        if (DUAL == 4) s1 = __builtin_fmaf(y2, y2, s1);
+      }
     };
     r.each([&](int, typename RV::V v) __attribute__((always_inline)) {
 #pragma unroll
@@ -251,8 +257,13 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
   const float f1 = fabsf(gs) * (DUAL ? p.w1 : (p.soft_only ? 0.f : p.w1) + w2), f2 = fabsf(gs) * w2;
   const float a1 = log2f(s1) - log2f(f1), a2 = DUAL ? log2f(s2) - log2f(f2) : 0.f;
   const float sign = gs < 0.f ? -1.f : 1.f;
+  const float k1 = gs * p.w1 / s1, k2 = gs * w2 / s2;      // (DUAL 2, 4)
   auto grad = [&](float z) __attribute__((always_inline)) {
     const float x = z - ms;
+    if (DUAL >= 2) {
+      const float y = __builtin_amdgcn_exp2f(x * c2);
+      return y * __builtin_fmaf(DUAL == 2 ? y : y * y * y, k1, k2);
+    }
     float g = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c1, -a1));
     if (DUAL) g += __builtin_amdgcn_exp2f(__builtin_fmaf(x, c2, -a2));
     return g * sign;
@@ -466,8 +477,10 @@ template <class E, int NC, int NT> struct distill_go {
   static void go(DistillArgs a, bool dual, hipStream_t st) {
     a.count_here = a.rows <= DT_COUNT_HERE * NT;
     if (!a.count_here) hipLaunchKernelGGL(dt_count_kernel, dim3(1), dim3(1024), 0, st, a.labels, a.rows, a.V, a.nvalid);
-    if (dual) hipLaunchKernelGGL((distill_kernel<E, NC, NT, true>), dim3(a.rows), dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((distill_kernel<E, NC, NT, false>), dim3(a.rows), dim3(NT), 0, st, a);
+    if (!dual) hipLaunchKernelGGL((distill_kernel<E, NC, NT, 0>), dim3(a.rows), dim3(NT), 0, st, a);
+    else if (a.T == 2.f) hipLaunchKernelGGL((distill_kernel<E, NC, NT, 2>), dim3(a.rows), dim3(NT), 0, st, a);
+    else if (a.T == 4.f) hipLaunchKernelGGL((distill_kernel<E, NC, NT, 4>), dim3(a.rows), dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((distill_kernel<E, NC, NT, 1>), dim3(a.rows), dim3(NT), 0, st, a);
   }
 };
 template <class E, int NC, int NT> struct topk_go {

@@ -330,7 +330,7 @@ def check_distill(ops, dev, z, labels, lists, temp, alpha, dz=None, scale=None):
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("rows,v,pad,first,k", [(1, 1, 0, 0, 1), (7, 9, 0, 0, 3), (9, 1000, 24, 0, 8), (8, 1001, 2, 3, 33), (3, 2050, 1, 1, 256), (5, 9001, 0, 0, 64),
                                                 (2, 33003, 5, 2, 12), (3, 51865, 103, 0, 64), (2, 70001, 0, 0, 20)])
-@pytest.mark.parametrize("temp,alpha", [(2.0, 0.5), (1.0, 0.5), (4.0, 1.0)])
+@pytest.mark.parametrize("temp,alpha", [(2.0, 0.5), (1.0, 0.5), (4.0, 1.0), (4.0, 0.5), (1.5, 0.3)])
 def test_distill_topk(ops, dev, dtype, rows, v, pad, first, k, temp, alpha):
     buf, z, labels, lists = make_logits(dev, rows, v, dtype, rows + v, pad, first, k=k)
     ob = torch.full_like(buf, 5.0)
