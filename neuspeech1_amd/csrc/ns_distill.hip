@@ -138,8 +138,9 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
   constexpr int NW = NT / 64;
   __shared__ float sh[3][NW];
   __shared__ int shc[NW];
-  __shared__ int sidx[DT_MAX_K + 1];
-  __shared__ float sp[DT_MAX_K], sz[DT_MAX_K + 1];
+  __shared__ __attribute__((aligned(16))) int sidx[DT_MAX_K + 4];
+  __shared__ __attribute__((aligned(16))) float sp[DT_MAX_K + 4];
+  __shared__ float sz[DT_MAX_K + 1];
   typedef row_view<E, NC, NT> RV;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t lab64 = p.labels ? p.labels[row] : -1;
@@ -184,6 +185,10 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
     sidx[e] = ok ? t : -1;
     sz[e] = ok ? (float)r.p[t] : 0.f;
     if (e < p.k) sp[e] = ok ? p.tv[row * p.ldt + e] / p.T : -INFINITY;
+  }
+  if (tid < 4) {                           // no entries behind the last (the sparse cells read four at a time)
+    sp[p.k + tid] = 0.f;
+    if (tid > 0) sidx[p.k + tid] = -1;
   }
   const float c1 = p.soft_only ? LOG2E / p.T : LOG2E, c2 = LOG2E / p.T;
   // every wave's maximum and sums relative to it, joined over the workgroup
@@ -290,8 +295,13 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
     if (t < 0) continue;
     float q = 0.f;
     bool first = true;
-    for (int o = 0; o < p.k; ++o)
-      if (sidx[o] == t) { q += sp[o]; first = first && o >= e; }
+#pragma unroll 4
+    for (int o = 0; o < p.k; o += 4) {     // (sp[k] is zero, and entry k comes no earlier than any)
+      const int4 s = *(const int4*)&sidx[o];
+      const float4 r4 = *(const float4*)&sp[o];
+      q += (s.x == t ? r4.x : 0.f) + (s.y == t ? r4.y : 0.f) + (s.z == t ? r4.z : 0.f) + (s.w == t ? r4.w : 0.f);
+      first = first && !((s.x == t && o < e) || (s.y == t && o + 1 < e) || (s.z == t && o + 2 < e) || (s.w == t && o + 3 < e));
+    }
     if (!first) continue;
     float g = grad(sz[e]) - gs * w2 * q;
     if (has && t == (int)lab64) g -= gs * p.w1;

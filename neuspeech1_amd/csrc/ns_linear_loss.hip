@@ -935,23 +935,38 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
     const float* const tv = p.top_vals + row * p.ld_top;
     const int32_t* const ti = p.top_idx + row * p.ld_top;
     float tm = -INFINITY;
-    for (int e = q; e < p.k; e += 16) if (ti[e] >= 0 && ti[e] < p.V) tm = fmaxf(tm, tv[e] * p.invT);
+    // (value and token loaded side by side, four entries in flight: a value behind its token's test took a memory latency more per entry)
+#pragma unroll 4
+    for (int e = q; e < p.k; e += 16) {
+      const int t = ti[e];
+      const float v = tv[e] * p.invT;
+      tm = t >= 0 && t < p.V ? fmaxf(tm, v) : tm;
+    }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor(tm, o, 64));
     soft = tm > -INFINITY;
     float ts = 0.f;
-    for (int e = q; e < p.k; e += 16) if (soft && ti[e] >= 0 && ti[e] < p.V) ts += expf(tv[e] * p.invT - tm);
+#pragma unroll 4
+    for (int e = q; e < p.k; e += 16) {
+      const int t = ti[e];
+      const float v = tv[e] * p.invT;
+      ts += soft && t >= 0 && t < p.V ? expf(v - tm) : 0.f;
+    }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) ts += __shfl_xor(ts, o, 64);
     const float lt = logf(ts), inv = 1.f / ts;
     const float ls = log2f(p.dual ? s2 : s1);     // (one softmax: it is the one at T)
     float kl = 0.f;
+#pragma unroll 4
     for (int e = q; e < p.k; e += 16) {
       float pr = 0.f;
-      if (soft && ti[e] >= 0 && ti[e] < p.V) {
-        const float lp = tv[e] * p.invT - tm;
+      const int t = ti[e];
+      const float lp = tv[e] * p.invT - tm;
+      const bool ok = soft && t >= 0 && t < p.V;
+      const float z = logit(e, ok ? t : 0);
+      if (ok) {
         pr = expf(lp) * inv;
-        if (pr > 0.f) kl += pr * ((lp - lt) - (__builtin_fmaf(logit(e, ti[e]), p.c2, -e2) - ls) * LN2);
+        if (pr > 0.f) kl += pr * ((lp - lt) - (__builtin_fmaf(z, p.c2, -e2) - ls) * LN2);
       }
       p.pk[(int64_t)pi * p.k + e] = pr;
     }
@@ -1011,17 +1026,17 @@ __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ n
                                                        const int32_t* __restrict__ top_idx, int64_t ld_top, int k, const float* __restrict__ zk,
                                                        const float* __restrict__ pk, const float* __restrict__ La, const float* __restrict__ Lb, float c1, float c2,
                                                        float w1s, float w2s, int col0, int cols, int V, E* __restrict__ G, int ldg) {
-  __shared__ int sidx[4][LL_MAX_K + 1];
-  __shared__ float sp[4][LL_MAX_K];
+  __shared__ __attribute__((aligned(16))) int sidx[4][LL_MAX_K + 4];
+  __shared__ __attribute__((aligned(16))) float sp[4][LL_MAX_K + 4];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = blockIdx.x * 4 + wave;
   const int nv = min(*nvalid - row0, R), pi = row0 + i;
   const bool live = i < nv;
   if (live) {
     const int row = order[pi];
-    for (int e = lane; e <= k; e += 64) {
-      const int t = e == k ? lab[pi] : top_idx[row * ld_top + e];
+    for (int e = lane; e < k + 4; e += 64) {       // (k + 1 entries and none behind them)
+      const int t = e == k ? lab[pi] : e < k ? top_idx[row * ld_top + e] : -1;
       sidx[wave][e] = t >= 0 && t < V ? t : -1;
-      if (e < k) sp[wave][e] = pk[(int64_t)pi * k + e];
+      sp[wave][e] = e < k ? pk[(int64_t)pi * k + e] : 0.f;
     }
   }
   __syncthreads();
@@ -1032,8 +1047,13 @@ __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ n
     if (t < 0 || c < 0 || c >= cols) continue;
     float soft = 0.f;
     bool first = true;
-    for (int o = 0; o < k; ++o)
-      if (sidx[wave][o] == t) { soft += sp[wave][o]; first = first && o >= e; }
+#pragma unroll 4
+    for (int o = 0; o < k; o += 4) {                        // (sp[k] is zero, and entry k comes no earlier than any)
+      const int4 s = *(const int4*)&sidx[wave][o];
+      const f32x4 q = *(const f32x4*)&sp[wave][o];
+      soft += (s.x == t ? q[0] : 0.f) + (s.y == t ? q[1] : 0.f) + (s.z == t ? q[2] : 0.f) + (s.w == t ? q[3] : 0.f);
+      first = first && !((s.x == t && o < e) || (s.y == t && o + 1 < e) || (s.z == t && o + 2 < e) || (s.w == t && o + 3 < e));
+    }
     if (!first) continue;                                   // an earlier entry of the list names the same token: that one writes
     const float z = zk[(int64_t)pi * (k + 1) + e];
     float v = __builtin_amdgcn_exp2f(z * c1 - la);
@@ -1473,6 +1493,7 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
     if (t < n0 || t >= n0 + 256 || t >= p.V) continue;
     float soft = 0.f;
     bool first = true;
+#pragma unroll 8
     for (int o = 0; o < p.k; ++o)
       if (p.top_idx[row * p.ld_top + o] == t) { soft += p.pk[(int64_t)r * p.k + o]; first = first && o >= e; }
     if (!first) continue;
