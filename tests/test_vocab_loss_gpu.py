@@ -199,6 +199,36 @@ def test_large_logits(ops, dev):
     check_linear(ops, dev, h * 64, w * 4, labels)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,v,grad,k,alpha,temp", [(300, 2600, "hw", 0, 0.0, 1.0), (300, 2600, "hw", 5, 0.5, 1.0), (130, 900, "h", 3, 1.0, 2.0), (100, 70, "w", 0, 0.0, 1.0), (2049, 60001, "h", 0, 0.0, 1.0)])
+def test_labels_far_below_the_largest_logit(ops, dev, dtype, rows, v, grad, k, alpha, temp):
+    """rows from nearly flat to logits of hundreds, the label anywhere among them: a reference taken from the label's logit holds for some rows, by a little
+    for others and not for the rest; one row of a tile, all of them or none; label and maximum in one strip and far apart"""
+    h, w, labels, lists = make_linear(dev, rows, 64, v, dtype, seed=13, ignored=0.1, k=k, sharp=0.0)
+    grow = torch.linspace(0.05, 12.0, rows, device=dev).unsqueeze(1)
+    for i, part in enumerate((grow, torch.where(torch.arange(rows, device=dev).unsqueeze(1) % 97 == 0, 12.0, 0.3), torch.full_like(grow, 6.0))):
+        check_linear(ops, dev, (h * part).to(dtype), w, labels, lists, temp, alpha, grad=grad, scale=8.0)
+        if rows > 2000:
+            break
+
+
+def test_labels_whose_logit_is_a_small_difference_of_large_products(ops, dev):
+    """the gathered logit and the tile's may then differ by more than a reference allows for; rows that lose all digits are held to no value, the others to theirs"""
+    h, w, labels, _ = make_linear(dev, 300, 64, 700, BF16, seed=14, ignored=0.0)
+    w[:, 32:] = -w[:, :32]
+    big = torch.arange(300, device=dev) % 3 == 0
+    h[:, 32:] = torch.where(big.unsqueeze(1), h[:, :32], h[:, 32:])
+    h[big] *= 2.0 ** 40                        # products of 2^40 that cancel in pairs: logits of zero but for what the order of the sum leaves
+    o = outputs(dev, 300)
+    dh = torch.full_like(h, 3.0)
+    ops.linear_cross_entropy(h, w, labels, dh=dh, **o)
+    ref = R.linear(h, w, labels)
+    small = (labels >= 0) & (labels < 700) & ~big
+    close(o["row_loss"][small], ref["row_loss"][small], ref["row_tol"][small], "row_loss")
+    assert torch.isfinite(o["row_loss"]).all() and torch.isfinite(dh).all()
+    close(dh[small], ref["dh"][small], ref["dh_tol"][small], "dh")
+
+
 @pytest.mark.parametrize("rows", [40, 600])
 def test_same_inputs_give_the_same_bits_and_workspaces_are_not_shared(ops, dev, rows):
     """repeated, interleaved with another call, on another stream and with a caller's workspace: equal bits; nothing past the workspace is written"""
