@@ -52,11 +52,13 @@ typedef unsigned short ushort4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v lds_s4;
 
 struct tf16 {
+  static constexpr float HEAD = 15.f, BELOW = 6.f;       // (see ll_label_ref)
   typedef half_t e;
   typedef half8 v8;
   static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 struct tbf16 {
+  static constexpr float HEAD = 60.f, BELOW = 0.f;
   typedef __bf16 e;
   typedef bf8 v8;
   static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -105,18 +107,21 @@ __device__ __forceinline__ float ll_sum4(float v) {
 // reference exponent of a softmax at scale c: an integer, so that taking it out of z c (inside the fma) and moving sums between references are exact
 __device__ __forceinline__ float ll_ref(float mx, float c) { return ceilf(mx * c); }
 
-// LL_KEEP with one reference for a whole row (REF: bfloat16, one softmax).  The label's logit is known before the pass: its exponent is the row's reference
-// as long as no logit exceeds it by more than 2^LL_HEAD -- bf16 has the exponents for that, and what lies 2^-126 below the label counts for nothing.  A 64-column strip
-// that does exceed it takes its own maximum, and its row is brought to one reference afterwards.  So dz = x F with ONE factor per row, which dh's last
-// step and h's transposed copy take in, and the pass over dz falls away (8192 rows, d = 1280: 2.93 -> 2.67 ms; 1844 rows, d = 512:
-// 425 -> 371 us).
+// LL_KEEP with one reference for a whole row (REF: one softmax).  The label's logit is known before the pass: its exponent (less BELOW, which moves fp16's range)
+// is the row's reference as long as no logit exceeds it by more than 2^HEAD.  A 64-column strip that does exceed it takes its own maximum, and its row is brought to
+// one reference afterwards.  So dz = x F with ONE factor per row, which dh's last step and h's transposed copy take in, and the pass over dz falls away
+// (bf16, 8192 rows, d = 1280: 2.93 -> 2.67 ms; 1844 rows, d = 512: 425 -> 371 us; fp16, 1229 rows, dh alone: NNN us).
+//   bfloat16   has the exponents for x and for the label's cell x - sum x, up to 2^77 of it; what lies 2^-126 below the label counts for nothing.
+//   float16    has room for x alone, 2^-30 of the label's to 2^9 times it: where the label's cell can stay out of dz (dh alone, no list: the label's x is cleared and
+//              dh = g (F x W + (p - 1) W[label]); subtracting W[label] from a product that holds p W[label] would leave p's rounding of 1 - p).
 // The gathered logit and the tile's differ by the order of their sums, each within (d + 4) u sum |h w| of the exact one: where that could exceed 4 the row gets no
 // reference (NaN: every comparison fails).
-constexpr float LL_HEAD = 60.f;
-__device__ __forceinline__ float ll_label_ref(float z, float mass, int d, float c) {
-  return (float)(d + 4) * 5.9604645e-8f * mass * c <= 4.f ? ll_ref(z, c) : NAN;
+template <class T> __device__ __forceinline__ float ll_label_ref(float z, float mass, int d, float c) {
+  return (float)(d + 4) * 5.9604645e-8f * mass * c <= 4.f ? ll_ref(z, c) - T::BELOW : NAN;
 }
-__device__ __forceinline__ float ll_strip_ref(float mx, float eref, float c) { return mx * c <= eref + LL_HEAD ? eref : mx == -INFINITY ? 0.f : ll_ref(mx, c); }
+template <class T> __device__ __forceinline__ float ll_strip_ref(float mx, float eref, float c, float shift) {
+  return mx * c <= eref + T::HEAD ? eref : mx == -INFINITY ? 0.f : ll_ref(mx, c) - shift;
+}
 
 #define LL_BARRIER()                            \
   do {                                          \
@@ -372,7 +377,7 @@ __global__ __launch_bounds__(256) void ll_pack_kernel(const void* __restrict__ h
   if (lane == 0) zk[i] = s;
   if (!eref) return;
   mass = ns_wave_sum(mass);
-  if (lane == 0) eref[i] = ll_label_ref(s, mass, d, c);
+  if (lane == 0) eref[i] = ll_label_ref<T>(s, mass, d, c);
 }
 
 // zk[i][e] = h_i . W[token e], e = 0 .. k - 1 the teacher's list, e = k the label: a workgroup per row, 16 lanes per entry (256 B of W a step, 16 entries
@@ -405,7 +410,7 @@ __global__ __launch_bounds__(256) void ll_gather_kernel(const void* __restrict__
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); mass += __shfl_xor(mass, o, 64); }
     if (l == 0) zk[(int64_t)i * (k + 1) + e] = s;
-    if (l == 0 && e == k && eref) eref[i] = ll_label_ref(s, mass, d, c1);
+    if (l == 0 && e == k && eref) eref[i] = ll_label_ref<T>(s, mass, d, c1);
   }
 }
 
@@ -439,6 +444,7 @@ struct LogitsArgs {
   const int* lab; const float* zk;       // FIX: the label's cell of dz is put right in the staged tile
   float wlab;                            // w1 2^s
   const float *eref, *efin;              // REF: (R) the rows' references before and behind the pass
+  int apart;                             // REF, FIX: the label's cell is cleared
 };
 
 // One workgroup per CU walks the tiles of its XCD's run.  The ring never drains: the pieces that a tile's last two K tiles request are the next tile's first
@@ -718,7 +724,7 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
           mx = ll_max4(mx);
           // (two softmaxes: what is kept is the one at T, c2 < c1; the sum of the other is taken here from its own exponentials)
           const float ck = DUAL ? p.c2 : p.c1, own = mx == -INFINITY ? 0.f : ll_ref(mx, ck);
-          const float e1 = REF ? ll_strip_ref(mx, side[2048 + par * 256 + row], p.c1) : own - p.shift;
+          const float e1 = REF ? ll_strip_ref<T>(mx, side[2048 + par * 256 + row], p.c1, p.shift) : own - p.shift;
           const float e2 = DUAL && mx > -INFINITY ? ll_ref(mx, p.c1) : 0.f;
           float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -819,8 +825,7 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
 // dz from what LL_KEEP left, in place: the strip's exponentials times 2^(e - La), one rounding more; a row's label cell (no list) is formed from its own
 // logit.  64 rows x 512 columns a workgroup, 16 B per lane; the pass is bound by its bytes (read and written once, mostly in the last-level cache).
 // DUAL: what was kept is x = 2^(z c2 - e); softmax(z)'s share is x^T, by its logarithm (a relative rounding of x becomes T of them: T <= 2 only).
-// REF: only rows whose reference changed are touched (and the label's cells written): mostly none.
-template <class T, bool FIX, bool DUAL, bool REF>
+template <class T, bool FIX, bool DUAL>
 __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
   typedef typename T::e E;
   typedef typename T::v8 v8;
@@ -830,24 +835,10 @@ __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
   const int nv = min(*p.nvalid - p.row0, p.R);
   const int i0 = blockIdx.y * 64, t0 = blockIdx.x * 2;
   if (nv <= 0 || i0 >= (nv + BM - 1) / BM * BM) return;
-  if (REF) {
-    const int i = i0 + (threadIdx.x & 63), l = i < nv ? p.lab[p.row0 + i] - t0 * BN : -1;
-    const float e = p.efin[i];
-    if (!__syncthreads_or(p.eref[p.row0 + i] != e)) {
-      if (FIX && threadIdx.x < 64 && l >= 0 && l < 2 * BN)
-        ((E*)p.G)[(int64_t)i * p.ldg + t0 * BN + l] = (E)(__builtin_amdgcn_exp2f(__builtin_fmaf(p.zk[p.row0 + i], p.c1, -e)) - p.wlab * __builtin_amdgcn_exp2f(p.La[i] - e));
-      return;
-    }
-  }
   for (int x = threadIdx.x; x < 512; x += 256) {
     const int sidx = t0 * 4 + (x >> 6), i = i0 + (x & 63);
     if (sidx < p.tiles_n * 4) {
       const float mx = p.strip[(int64_t)sidx * p.R + i];
-      if (REF) {
-        const float a = p.eref[p.row0 + i], b = p.efin[i];
-        f[x >> 6][x & 63] = a == b ? 1.f : __builtin_amdgcn_exp2f(ll_strip_ref(mx, a, p.c1) - b);
-        continue;
-      }
       const float e = (mx == -INFINITY ? 0.f : ll_ref(mx, DUAL ? p.c2 : p.c1)) - p.shift;
       f[x >> 6][x & 63] = __builtin_amdgcn_exp2f(e - (DUAL ? p.Lb[i] : p.La[i]));
       if (DUAL) f1[x >> 6][x & 63] = e * p.T - p.La[i];
@@ -856,8 +847,7 @@ __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
   if (FIX && threadIdx.x < 64) {
     const int i = i0 + threadIdx.x;
     lc[threadIdx.x] = i < nv ? p.lab[p.row0 + i] - t0 * BN : -1;
-    if (REF) lv[threadIdx.x] = i < nv ? __builtin_amdgcn_exp2f(__builtin_fmaf(p.zk[p.row0 + i], p.c1, -p.efin[i])) - p.wlab * __builtin_amdgcn_exp2f(p.La[i] - p.efin[i]) : 0.f;
-    else lv[threadIdx.x] = i < nv ? __builtin_amdgcn_exp2f(p.zk[p.row0 + i] * p.c1 - p.La[i]) - p.wlab : 0.f;
+    lv[threadIdx.x] = i < nv ? __builtin_amdgcn_exp2f(p.zk[p.row0 + i] * p.c1 - p.La[i]) - p.wlab : 0.f;
   }
   __syncthreads();
   const int c = (threadIdx.x & 63) * 8, r0 = threadIdx.x >> 6;
@@ -882,6 +872,57 @@ __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
         v[x][e] = (E)g;
       }
       *(v8*)(G + (int64_t)r * p.ldg) = v[x];
+    }
+  }
+}
+
+// REF: the rows whose reference changed are brought to it, in place, and with FIX the labels' cells are written (cleared where `apart`).  64 rows x 512 columns a
+// workgroup, a wave per changed row, four rows' loads ahead of the first store.  With few changed rows the launch is all it takes (all of them: 44 us at 1229 rows).
+template <class T, bool FIX>
+__global__ __launch_bounds__(256) void ll_rebase_kernel(const LogitsArgs p) {
+  typedef typename T::e E;
+  typedef typename T::v8 v8;
+  const int nv = min(*p.nvalid - p.row0, p.R);
+  const int i0 = blockIdx.y * 64, t0 = blockIdx.x * 2;
+  if (nv <= 0 || i0 >= (nv + BM - 1) / BM * BM) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = i0 + lane;
+  const float from = p.eref[p.row0 + i], to = p.efin[i];
+  uint64_t m = __ballot(from != to);                        // (no reference, NaN: changed)
+  int lc = -1;
+  float lv = 0.f;
+  if (FIX && i < nv) {
+    lc = p.lab[p.row0 + i] - t0 * BN;
+    if (lc >= 0 && lc < 2 * BN && !p.apart) lv = __builtin_amdgcn_exp2f(__builtin_fmaf(p.zk[p.row0 + i], p.c1, -to)) - p.wlab * __builtin_amdgcn_exp2f(p.La[i] - to);
+    if (wave == 0 && lc >= 0 && lc < 2 * BN && !(m >> lane & 1)) ((E*)p.G)[(int64_t)i * p.ldg + t0 * BN + lc] = (E)lv;
+  }
+  const int c = lane * 8, tn = t0 + (c >> 8);
+  for (int x = 0; x < wave; ++x) m &= m - 1;                // this wave: every fourth changed row
+  const bool in = tn < p.tiles_n;                           // (the other lanes stay: rows' numbers come from all 64)
+  E* const G = (E*)p.G + (int64_t)i0 * p.ldg + t0 * BN + c;
+  const float* const strip = p.strip + (int64_t)(t0 * 4 + (c >> 6)) * p.R + i0;
+  while (m) {
+    int r[4];
+    v8 v[4];
+    float mx[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      r[x] = m ? __builtin_ctzll(m) : -1;
+      if (r[x] >= 0 && in) {
+        v[x] = *(const v8*)(G + (int64_t)r[x] * p.ldg);
+        mx[x] = strip[r[x]];
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) m &= m - 1;
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (r[x] < 0) continue;
+      const float a = __builtin_amdgcn_exp2f(ll_strip_ref<T>(mx[x], __shfl(from, r[x], 64), p.c1, p.shift) - __shfl(to, r[x], 64));
+      const int at = FIX ? __shfl(lc, r[x], 64) - c : -1;
+      const float cell = FIX ? __shfl(lv, r[x], 64) : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[x][e] = (E)(FIX && at == e ? cell : (float)v[x][e] * a);
+      if (in) *(v8*)(G + (int64_t)r[x] * p.ldg) = v[x];
     }
   }
 }
@@ -921,7 +962,8 @@ struct RowArgs {
   float* loss;
   const float* zk; const float* top_vals; const int32_t* top_idx; int64_t ld_top;
   float *La, *Lb, *pk, *row_loss, *packed_loss;
-  const float* eref; float *efin, *F;           // REF: the rows' references before and behind the logits' pass, their factors
+  const float* eref; float *efin, *F, head, shift;     // REF: the rows' references before and behind the logits' pass, their factors
+  float* cl;                                    // p - 1 of the label, where dh's last step takes it
 };
 
 // 16 threads per row; one workgroup of 1024 threads (the few-row path) also takes the mean
@@ -1046,9 +1088,10 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
       p.La[i] = l1 - p.lw1;
     }
     if (p.eref) {
-      const float a = p.eref[pi], e = mx * p.c1 <= a + LL_HEAD ? a : ll_ref(mx, p.c1);
+      const float a = p.eref[pi], e = mx * p.c1 <= a + p.head ? a : ll_ref(mx, p.c1) - p.shift;
       p.efin[i] = e;
-      p.F[i] = __builtin_amdgcn_exp2f(e - p.La[i]);
+      p.F[i] = __builtin_amdgcn_exp2f(e - p.La[i] - p.shift);      // (La is for cells times 2^shift)
+      if (p.cl) p.cl[i] = __builtin_amdgcn_exp2f(p.zk[pi] * p.c1 - l1) - 1.f;
     }
     p.row_loss[row] = loss;
     if (NT == 256) p.packed_loss[pi] = loss;
@@ -1191,7 +1234,8 @@ __global__ __launch_bounds__(NTH) void ll_dh_kernel(const DhArgs p) {
 template <class E>
 __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict__ slab, int groups, int splits, const int* __restrict__ splits_dev, int R, int row0, int chunk, int d, int rows, const int* __restrict__ inv,
                                                         const int* __restrict__ nvalid, const float* __restrict__ loss_scale, float unscale, E* __restrict__ dh, int64_t lddh,
-                                                        const float* __restrict__ packed_loss, float* __restrict__ loss, const float* __restrict__ F) {
+                                                        const float* __restrict__ packed_loss, float* __restrict__ loss, const float* __restrict__ F, const E* __restrict__ w,
+                                                        int64_t ldw, const int* __restrict__ lab, const float* __restrict__ cl) {
   if (loss && blockIdx.x == gridDim.x - 1) {      // one workgroup more: the mean of the row losses
     ll_mean<256>(packed_loss, *nvalid, loss);
     return;
@@ -1227,18 +1271,26 @@ __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict_
       for (int o = 1; o < groups; ++o) a += sm[sub + o][threadIdx.x & 15];
   }
   if (!in || g != 0 || (pi >= 0 ? i < 0 : row0 > 0)) return;
-  const float gs = (loss_scale ? *loss_scale : 1.f) / (float)max(*nvalid, 1) * (F ? (i < 0 ? 0.f : F[i]) : unscale);
+  const float gs = (loss_scale ? *loss_scale : 1.f) / (float)max(*nvalid, 1);
+  if (i >= 0) {
+    a *= F ? F[i] : unscale;
+    if (w) {                                      // the label's part, which is not in dz then
+      const e4 l = *(const e4*)(w + lab[pi] * ldw + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[e] = __builtin_fmaf(cl[i], (float)l[e], a[e]);
+    }
+  }
   e4 o;
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] = (E)(i < 0 ? 0.f : a[e] * gs);
   *(e4*)(dh + row * lddh + c) = o;
 }
 template <class E> void launch_dh_out(const float* slab, int groups, int splits, const int* splits_dev, int R, int row0, int chunk, int d, int rows, const int* inv, const int* nvalid, const float* loss_scale, float unscale, E* dh,
-                                      int64_t lddh, const float* packed_loss, float* loss, const float* F, hipStream_t st) {
+                                      int64_t lddh, const float* packed_loss, float* loss, const float* F, const E* w, int64_t ldw, const int* lab, const float* cl, hipStream_t st) {
   const int nblk = 16 / groups;
   const int64_t items = (int64_t)rows * ((d + 63) / 64);
   hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)((items + nblk - 1) / nblk) + (loss ? 1 : 0)), dim3(256), 0, st, slab, groups, splits, splits_dev, R, row0, chunk, d, rows, inv, nvalid,
-                     loss_scale, unscale, dh, lddh, packed_loss, loss, F);
+                     loss_scale, unscale, dh, lddh, packed_loss, loss, F, w, ldw, lab, cl);
 }
 
 struct DwArgs {
@@ -1715,7 +1767,7 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   const int64_t by_ld = ((int64_t)0x7FF00000 / 2 / ldw) / BN;
   const int64_t rows_fit = (int64_t)((d->dw ? LL_WHOLE_BYTES : LL_PIECE_BYTES) / ((size_t)p.tiles_n * BN * 2)) / BM * BM;
   p.keep = grad && (!dual_of(d) || d->temperature <= 2.f && d->temperature >= 1.f) && rows_fit >= BM && p.tiles_n <= by_ld && (p.R <= rows_fit || !d->dw);
-  p.ref = p.keep && !p.few && d->dtype == NS_BF16 && !dual_of(d);
+  p.ref = p.keep && !p.few && !dual_of(d) && (d->dtype == NS_BF16 || (d->k == 0 && !d->dw));
   p.Rc = p.R;
   if (p.keep) {
     if (p.R > rows_fit) {
@@ -1786,7 +1838,7 @@ int few_launch(const ns_linear_ce_desc* d, const FewArgs& f, const RowArgs& r, b
     gy = (chunks + (chunks + gy - 1) / gy - 1) / ((chunks + gy - 1) / gy);
     if (dual) hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, true>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
     else hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, false>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
-    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n >= 64 ? 16 : f.tiles_n >= 16 ? 4 : 1, f.tiles_n, nullptr, 16 * MT, 0, LL_FEW_ROWS, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, nullptr, nullptr, nullptr, st);
+    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n >= 64 ? 16 : f.tiles_n >= 16 ? 4 : 1, f.tiles_n, nullptr, 16 * MT, 0, LL_FEW_ROWS, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, nullptr, nullptr, nullptr, nullptr, 0, nullptr, nullptr, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;
@@ -1801,6 +1853,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   float *zk = (float*)(ws + p.zk), *pk = (float*)(ws + p.pk), *La = (float*)(ws + p.La), *Lb = (float*)(ws + p.Lb), *ploss = (float*)(ws + p.ploss);
   float *const eref = p.ref ? (float*)(ws + p.eref) : nullptr, *const efin = p.ref ? (float*)(ws + p.efin) : nullptr, *const F = p.ref ? (float*)(ws + p.F) : nullptr;
   constexpr bool BF = __is_same(T, tbf16);      // (one softmax of exponentials kept: always with one reference a row)
+  const bool apart = p.ref && d->k == 0 && !d->dw;                 // dz without the labels' cells: dh's last step adds their rows of W
   const bool dual = dual_of(d), soft_only = d->k > 0 && d->alpha == 1.f, grad = d->dh || d->dw;
   const float alpha = d->k > 0 ? d->alpha : 0.f, T_ = d->k > 0 ? d->temperature : 1.f;
   const float w1 = 1.f - alpha, w2 = alpha * T_;
@@ -1814,7 +1867,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   static ns_dev_once once;
   if (!ns_dyn_lds_once(once, {(const void*)ll_logits_kernel<T, LL_STATS, false, false>, (const void*)ll_logits_kernel<T, LL_STATS, true, false>,
                               (const void*)ll_logits_kernel<T, LL_KEEP, true, false>, (const void*)ll_logits_kernel<T, LL_GRAD, false, true>,
-                              (const void*)ll_logits_kernel<T, LL_KEEP, false, false, false, BF>, (const void*)ll_logits_kernel<T, LL_STATS, true, false, true>, (const void*)ll_logits_kernel<T, LL_KEEP, true, false, true>,
+                              (const void*)ll_logits_kernel<T, LL_KEEP, false, false, false, true>, (const void*)ll_logits_kernel<T, LL_KEEP, false, false, false, BF>, (const void*)ll_logits_kernel<T, LL_STATS, true, false, true>, (const void*)ll_logits_kernel<T, LL_KEEP, true, false, true>,
                               (const void*)ll_logits_kernel<T, LL_GRAD, false, false>, (const void*)ll_logits_kernel<T, LL_GRAD, true, false>,
                               (const void*)ll_dh_kernel<T>, (const void*)ll_dw_kernel<T>}, LL_LOGITS_LDS > LL_LDS ? LL_LOGITS_LDS : LL_LDS, "ns_linear_cross_entropy"))
     return NS_ERR_HIP;
@@ -1825,7 +1878,8 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   r.lw1 = (d->k > 0 && !dual) ? (float)s : log2f(w1) + (float)s;
   r.lw2 = log2f(w2) + (float)s;
   r.dual = dual; r.soft_only = soft_only; r.nvalid = d->nvalid_dev; r.order = order; r.lab = lab; r.zk = zk; r.top_vals = d->top_vals; r.top_idx = d->top_idx;
-  r.eref = eref; r.efin = efin; r.F = F;
+  r.eref = eref; r.efin = efin; r.F = F; r.head = T::HEAD; r.shift = (float)s; r.cl = apart ? Lb : nullptr;      // (one softmax: Lb is free)
+ 
   r.ld_top = d->ld_top; r.La = La; r.Lb = dual ? Lb : nullptr; r.pk = pk; r.row_loss = d->row_loss; r.packed_loss = ploss; r.loss = d->loss_dev;
   if (p.few) {
     FewArgs f = {};
@@ -1851,7 +1905,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   a.c1 = c1; a.c2 = c2; a.T = T_;
   a.pm = (float*)(ws + p.pm); a.p1 = (float*)(ws + p.p1); a.p2 = (float*)(ws + p.p2);
   a.La = La; a.Lb = Lb; a.G = ws + p.G; a.ldg = p.piece_tiles * BN; a.lab = lab; a.zk = zk; a.wlab = w1 * up;
-  a.eref = eref; a.efin = efin;
+  a.eref = eref; a.efin = efin; a.apart = apart;
   a.strip = (float*)(ws + p.strip); a.shift = (float)s; a.unshift = 1.f / up;
   r.R = p.Rc; r.tiles_d = (d->d + BN - 1) / BN; r.kt = p.piece_tiles * (BN / BK); r.splits = splits;
   auto grid_of = [&](int tiles_n) { const int64_t t = (int64_t)(p.Rc / BM) * tiles_n; return dim3((unsigned)(t < 256 ? t : 256)); };
@@ -1859,7 +1913,8 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
     a.row0 = r.row0 = row0;
     a.col0 = 0; a.tiles_n = p.tiles_n;
     const dim3 all = grid_of(p.tiles_n);
-    if (p.keep && dual && T_ == 2.f) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, true, false, true>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
+    if (p.ref) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, false, false, false, true>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
+    else if (p.keep && dual && T_ == 2.f) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, true, false, true>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     else if (dual && T_ == 2.f) hipLaunchKernelGGL((ll_logits_kernel<T, LL_STATS, true, false, true>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     else if (p.keep && dual) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, true, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     else if (p.keep) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, false, false, false, BF>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
@@ -1875,9 +1930,11 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
       const dim3 grid = grid_of(a.tiles_n);
       if (p.keep) {
         const dim3 sg((a.tiles_n + 1) / 2, p.Rc / 64);
-        if (d->k == 0) hipLaunchKernelGGL((ll_scale_kernel<T, true, false, BF>), sg, dim3(256), 0, st, a);
-        else if (dual) hipLaunchKernelGGL((ll_scale_kernel<T, false, true, false>), sg, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((ll_scale_kernel<T, false, false, BF>), sg, dim3(256), 0, st, a);
+        if (p.ref && d->k == 0) hipLaunchKernelGGL((ll_rebase_kernel<T, true>), sg, dim3(256), 0, st, a);
+        else if (p.ref) hipLaunchKernelGGL((ll_rebase_kernel<tbf16, false>), sg, dim3(256), 0, st, a);
+        else if (dual) hipLaunchKernelGGL((ll_scale_kernel<T, false, true>), sg, dim3(256), 0, st, a);
+        else if (d->k == 0) hipLaunchKernelGGL((ll_scale_kernel<tf16, true, false>), sg, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((ll_scale_kernel<tf16, false, false>), sg, dim3(256), 0, st, a);
       } else if (d->k == 0) hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, false, true>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
       else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, true, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
       else hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, false, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
@@ -1899,7 +1956,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
     }
     if (d->dh)
       launch_dh_out<E>((const float*)(ws + p.slab), p.Rc <= 512 ? 16 : 1, 0, splits, 0, row0, p.Rc, d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh,
-                       d->lddh, ploss, row0 + p.Rc >= p.R ? d->loss_dev : nullptr, F, st);
+                       d->lddh, ploss, row0 + p.Rc >= p.R ? d->loss_dev : nullptr, F, apart ? (const E*)d->w : nullptr, d->ldw, lab, Lb, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;

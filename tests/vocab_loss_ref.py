@@ -87,9 +87,11 @@ def losses(z, dz_err, labels, temp=1.0, alpha=0.0, top_vals=None, top_idx=None):
                 cell_err=cell_err, prob=prob, n=n, nvalid=int(valid.sum()))
 
 
-def linear(h, w, labels, scale=1.0, dw_dtype=None, temp=1.0, alpha=0.0, top_vals=None, top_idx=None, parts=1):
+def linear(h, w, labels, scale=1.0, dw_dtype=None, temp=1.0, alpha=0.0, top_vals=None, top_idx=None, parts=1, floor=3 * 2.0 ** -40):
     """linear_cross_entropy in 64 bits: losses' dict + dh, dw and their tolerances.  Rows without a label are taken out first.  parts = 2: the cells are
-    sums of two numbers of their type (the first off by U of the cell, the second by U of that; formed from fp32, so 2 u of the terms as well)"""
+    sums of two numbers of their type (the first off by U of the cell, the second by U of that; formed from fp32, so 2 u of the terms as well).  floor: what fp16's
+    smallest step leaves of a cell: half of it, twice, at a factor of at least 2^15 / 2^(w1 + w2).  2^-29 where exponentials are kept relative to the label's: half a
+    step (2^-25) times the row's factor, at most p 2 / 2^6, and 2^-39 of a second rounding in a row whose reference changes."""
     rows, d = h.shape
     v = w.shape[0]
     U = half_step(h.dtype)
@@ -100,10 +102,16 @@ def linear(h, w, labels, scale=1.0, dw_dtype=None, temp=1.0, alpha=0.0, top_vals
     dz_err = ((d + 4) * U32 * (hd.abs() @ wd.abs().t())).amax(1) if rows else torch.zeros(0, dtype=torch.float64, device=h.device)
     r = losses(z, dz_err, labels, temp, alpha, top_vals, top_idx)
     g = scale / r["n"]
-    tiny = 3 * 2.0 ** -40 if h.dtype == torch.float16 else 0.0      # half of the smallest fp16 step, twice, at a factor of at least 2^15 / 2^(w1 + w2)
+    # (the cells of labels and lists are formed in fp32 from their own logits: their dense part is not rounded by itself)
+    prob = r["prob"].clone()
+    prob.scatter_(1, torch.where(valid, labels, 0).unsqueeze(1), 0.0)
+    if top_idx is not None:
+        prob.scatter_(1, torch.where((top_idx >= 0) & (top_idx < v), top_idx, 0).long(), 0.0)
+        prob[:, 0] = r["prob"][:, 0]
+    tiny = floor if h.dtype == torch.float16 else 0.0
     tiny *= max(1.0, 2.0 * ((1 - alpha) + alpha * temp))
     each = U * (3 + 3 * U) if parts == 1 else U * U + 2 * U32
-    cell_tol = r["cell_err"] + each * (r["cell"].abs() + r["prob"] + r["cell_err"]) + tiny * valid.double().unsqueeze(1)
+    cell_tol = r["cell_err"] + each * (r["cell"].abs() + prob + r["cell_err"]) + tiny * valid.double().unsqueeze(1)
     for name, out, err, mass, n, dt in (("dh", r["cell"] @ wd, cell_tol @ wd.abs(), r["cell"].abs() @ wd.abs(), v, h.dtype),
                                         ("dw", r["cell"].t() @ hd, cell_tol.t() @ hd.abs(), r["cell"].abs().t() @ hd.abs(), rows, dw_dtype or w.dtype)):
         out, err = out * g, (err + (n + 8) * U32 * mass) * g
