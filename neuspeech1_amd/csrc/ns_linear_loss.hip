@@ -10,12 +10,13 @@
 // The logits pass through the registers of 256 x 256 MFMA tiles and are never stored as such.  One pass keeps the running maximum and sum of every row (fp32,
 // one pair per row and 256 columns, joined by ll_rows_kernel).  dz in the operands' type then lies in a workspace, from where the products dh = dz W and
 // dW = dz^T h take it.  It comes about in one of two ways:
-//   kept     the same pass leaves 2^(z - reference of the row's 64-column strip), ll_scale_kernel makes dz of it in place: no logit is formed twice.  One softmax
-//            (or two at 1 <= T <= 2), and whole rows.  Where dW is not asked for, chunks of rows one after the other, each within LL_PIECE_BYTES (it stays in the
+//   kept     the same pass leaves 2^(z - reference): no logit is formed twice.  With one reference for the row, taken from its label's logit, this is dz but for the
+//            row's factor (one softmax; bf16, or dh alone from labels: see ll_label_ref); else the reference is that of the row's 64-column strip and ll_scale_kernel
+//            makes dz of it in place.  One softmax (or two at 1 <= T <= 2), and whole rows.  Where dW is not asked for, chunks of rows one after the other, each within LL_PIECE_BYTES (it stays in the
 //            256-MiB last-level cache); dW needs all rows, at most LL_WHOLE_BYTES of them.
 //   formed again   a second pass over the logits writes dz of one PIECE of the vocabulary (LL_PIECE_BYTES) for all rows, piece after piece: 4 products instead of 3,
 //            but no more memory, and dW, of V d elements, is written once (chunks of rows would read and write it per chunk).
-//            8192 rows, d = 1280, V = 51865, bf16, dh and dW: 3.59 ms formed again in 256 MiB, 2.95 ms kept in 852 MB (316 us of it the scaling, 5.4 TB/s).
+//            8192 rows, d = 1280, V = 51865, bf16, dh and dW: 3.59 ms formed again in 256 MiB, 2.72 ms kept in 852 MB.
 //   * Rows without a label are packed away first: they cost nothing, and an infinity or NaN in a masked row reaches neither loss nor gradient.
 //   * A row's sparse terms (its label, the teacher's list) are no part of the dense epilogue: their logits are gathered as dot products in fp32
 //     and their cells of dz are written from those.
@@ -58,7 +59,7 @@ struct tf16 {
   static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 struct tbf16 {
-  static constexpr float HEAD = 60.f, BELOW = 0.f;
+  static constexpr float HEAD = 30.f, BELOW = 0.f;
   typedef __bf16 e;
   typedef bf8 v8;
   static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -110,10 +111,12 @@ __device__ __forceinline__ float ll_ref(float mx, float c) { return ceilf(mx * c
 // LL_KEEP with one reference for a whole row (REF: one softmax).  The label's logit is known before the pass: its exponent (less BELOW, which moves fp16's range)
 // is the row's reference as long as no logit exceeds it by more than 2^HEAD.  A 64-column strip that does exceed it takes its own maximum, and its row is brought to
 // one reference afterwards.  So dz = x F with ONE factor per row, which dh's last step and h's transposed copy take in, and the pass over dz falls away
-// (bf16, 8192 rows, d = 1280: 2.93 -> 2.67 ms; 1844 rows, d = 512: 425 -> 371 us; fp16, 1229 rows, dh alone: NNN us).
-//   bfloat16   has the exponents for x and for the label's cell x - sum x, up to 2^77 of it; what lies 2^-126 below the label counts for nothing.
-//   float16    has room for x alone, 2^-30 of the label's to 2^9 times it: where the label's cell can stay out of dz (dh alone, no list: the label's x is cleared and
-//              dh = g (F x W + (p - 1) W[label]); subtracting W[label] from a product that holds p W[label] would leave p's rounding of 1 - p).
+// (bf16, 8192 rows, d = 1280: 2.93 -> 2.72 ms; 1844 rows, d = 512: 425 -> 382 us; fp16, 1229 rows, dh alone: 218 -> 187 us, and 227 where
+// every row's reference changes).
+//   bfloat16   has the exponents for x and for the cells of a list, up to 2^47; what lies 2^-126 below the label counts for nothing.
+//   float16    has room for x alone, from 2^-30 of the label's to 2^9 times it, and none for h's copy with the factors: dh alone, and no list.
+// Without a list the label's x is cleared, and dh's and dW's last steps add (p - 1) W[label] and (p - 1) h in fp32: a rounded factor or cell would be an error of all of
+// a row's gradient, and subtracting W[label] from a product that holds p W[label] would leave p's rounding of 1 - p.
 // The gathered logit and the tile's differ by the order of their sums, each within (d + 4) u sum |h w| of the exact one: where that could exceed 4 the row gets no
 // reference (NaN: every comparison fails).
 template <class T> __device__ __forceinline__ float ll_label_ref(float z, float mass, int d, float c) {
@@ -444,7 +447,6 @@ struct LogitsArgs {
   const int* lab; const float* zk;       // FIX: the label's cell of dz is put right in the staged tile
   float wlab;                            // w1 2^s
   const float *eref, *efin;              // REF: (R) the rows' references before and behind the pass
-  int apart;                             // REF, FIX: the label's cell is cleared
 };
 
 // One workgroup per CU walks the tiles of its XCD's run.  The ring never drains: the pieces that a tile's last two K tiles request are the next tile's first
@@ -455,8 +457,8 @@ struct LogitsArgs {
 constexpr int LL_SIDE = 2 * BUF;                              // behind the ring
 constexpr int LL_LOGITS_LDS = LL_SIDE + 3 * 4096;             // statistics: 3 x 4 x 256 floats; dz: two parities of 4 x 256 row constants (8 KiB)
 
-// MODE LL_STATS: the statistics alone.  LL_KEEP: and 2^(z c1 - e) of every logit in the operands' type, e = the reference of its row and 64-column
-// strip (minus s for fp16's range), which ll_scale_kernel turns into dz once the rows' sums are known: no logit is formed twice.  LL_GRAD: dz from
+// MODE LL_STATS: the statistics alone.  LL_KEEP: and 2^(z c1 - e) of every logit in the operands' type, e = the reference of its row (REF) or of its row and
+// 64-column strip (minus s for fp16's range), which ll_scale_kernel turns into dz once the rows' sums are known: no logit is formed twice.  LL_GRAD: dz from
 // the rows' sums.
 enum { LL_STATS, LL_KEEP, LL_GRAD };
 // SQ (DUAL at T = 2): e^z is the square of e^(z / T), the references' difference an exact power of two: one exponential a logit (1434 rows, d = 512: 123 -> 110 us).
@@ -876,8 +878,8 @@ __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
   }
 }
 
-// REF: the rows whose reference changed are brought to it, in place, and with FIX the labels' cells are written (cleared where `apart`).  64 rows x 512 columns a
-// workgroup, a wave per changed row, four rows' loads ahead of the first store.  With few changed rows the launch is all it takes (all of them: 44 us at 1229 rows).
+// REF: the rows whose reference changed are brought to it, in place, and with FIX the labels' cells are cleared.  64 rows x 512 columns a
+// workgroup, a wave per changed row, four rows' loads ahead of the first store.  With few changed rows the launch is all it takes.
 template <class T, bool FIX>
 __global__ __launch_bounds__(256) void ll_rebase_kernel(const LogitsArgs p) {
   typedef typename T::e E;
@@ -889,11 +891,9 @@ __global__ __launch_bounds__(256) void ll_rebase_kernel(const LogitsArgs p) {
   const float from = p.eref[p.row0 + i], to = p.efin[i];
   uint64_t m = __ballot(from != to);                        // (no reference, NaN: changed)
   int lc = -1;
-  float lv = 0.f;
   if (FIX && i < nv) {
     lc = p.lab[p.row0 + i] - t0 * BN;
-    if (lc >= 0 && lc < 2 * BN && !p.apart) lv = __builtin_amdgcn_exp2f(__builtin_fmaf(p.zk[p.row0 + i], p.c1, -to)) - p.wlab * __builtin_amdgcn_exp2f(p.La[i] - to);
-    if (wave == 0 && lc >= 0 && lc < 2 * BN && !(m >> lane & 1)) ((E*)p.G)[(int64_t)i * p.ldg + t0 * BN + lc] = (E)lv;
+    if (wave == 0 && lc >= 0 && lc < 2 * BN && !(m >> lane & 1)) ((E*)p.G)[(int64_t)i * p.ldg + t0 * BN + lc] = (E)0.f;
   }
   const int c = lane * 8, tn = t0 + (c >> 8);
   for (int x = 0; x < wave; ++x) m &= m - 1;                // this wave: every fourth changed row
@@ -919,9 +919,8 @@ __global__ __launch_bounds__(256) void ll_rebase_kernel(const LogitsArgs p) {
       if (r[x] < 0) continue;
       const float a = __builtin_amdgcn_exp2f(ll_strip_ref<T>(mx[x], __shfl(from, r[x], 64), p.c1, p.shift) - __shfl(to, r[x], 64));
       const int at = FIX ? __shfl(lc, r[x], 64) - c : -1;
-      const float cell = FIX ? __shfl(lv, r[x], 64) : 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[x][e] = (E)(FIX && at == e ? cell : (float)v[x][e] * a);
+      for (int e = 0; e < 8; ++e) v[x][e] = (E)(FIX && at == e ? 0.f : (float)v[x][e] * a);
       if (in) *(v8*)(G + (int64_t)r[x] * p.ldg) = v[x];
     }
   }
@@ -1299,7 +1298,97 @@ struct DwArgs {
   const int* nvalid; const float* loss_scale;
   float unscale;
   void* dw; int64_t lddw; int f32, add;
+  const void* hp; int dp; const int* lab; const float* cl;      // cl: the labels' cells, which are not in dz then
 };
+
+// The labels' part of dW's tile in fp32, where dz does not hold it (h's copy there is rounded with the rows' factors, and a token's row of dW is mostly its label's
+// h): rows whose label is one of the tile's 256 tokens are listed in order, 4096 labels at a time, and each adds (p - 1) h to its token's accumulators (dW 2.8e-3 -> 1.7e-3 off, its own
+// rounding, for 12 us of 382 at 1844 rows, d = 512).
+constexpr int LL_LIST = 4096;
+template <class T>
+__device__ __forceinline__ void ll_add_labels(f32x4 (&acc)[2][4][2][2], char* smem, const DwArgs& p, int nv, int v0, int m0) {
+  typedef typename T::e E;
+  typedef E e4 __attribute__((ext_vector_type(4)));
+  int2* const list = (int2*)smem;
+  int* const cnt = (int*)(smem + LL_LIST * 8);            // 64 counts, 64 prefixes, the sum
+  char* const rows = (char*)(cnt + 132);
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));                             // (no address of this part is carried through the main loop, where there is no register for it)
+  const int lane = tid & 63, l15 = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
+  for (int base = 0; base < nv; base += LL_LIST) {
+    int t[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int i = base + x * NTH + tid;
+      t[x] = i < nv ? p.lab[i] - v0 : -1;
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const uint64_t m = __ballot(t[x] >= 0 && t[x] < BN);
+      if (lane == 0) cnt[x * 8 + wave] = __popcll(m);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      const int own = cnt[lane];
+      int sum = own;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(sum, o, 64);
+        sum += lane >= o ? u : 0;
+      }
+      cnt[64 + lane] = sum - own;
+      if (lane == 63) cnt[128] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const bool hit = t[x] >= 0 && t[x] < BN;
+      const uint64_t m = __ballot(hit);
+      if (hit) list[cnt[64 + x * 8 + wave] + __popcll(m & ((1ull << lane) - 1ull))] = make_int2(base + x * NTH + tid, t[x]);
+    }
+    __syncthreads();
+    // 64 rows of h at a time through LDS (their loads in flight together, no registers), then a wave takes the rows whose token is one of its 64
+    const int n = cnt[128];
+    for (int e0 = 0; e0 < n; e0 += 64) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int e = (tid >> 5) + 16 * x, col = (tid & 31) * 8;
+        if (e0 + e < n && m0 + col < p.dp) *(uint4*)(rows + e * LDH + col * 2) = *(const uint4*)((const E*)p.hp + (int64_t)list[e0 + e].x * p.dp + m0 + col);
+      }
+      const int2 it = e0 + lane < n ? list[e0 + lane] : make_int2(0, -1);
+      const float cl = it.y >= 0 ? p.cl[it.x] : 0.f;
+      uint64_t m = __ballot(it.y >= 0 && it.y >> 6 == wn);
+      __syncthreads();
+      while (m) {
+        const int e = __builtin_ctzll(m), tok = __builtin_amdgcn_readlane(it.y, e);
+        const float c = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(cl), e));
+        m &= m - 1;
+#pragma unroll
+        for (int ah = 0; ah < 2; ++ah) {
+          f32x4 a[4];
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            const int col = wm * 128 + ah * 64 + mt * 16 + 4 * lg;
+            a[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (l15 == (tok & 15) && m0 + col < p.dp) {
+              const e4 v = *(const e4*)(rows + e * LDH + col * 2);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) a[mt][r] = c * (float)v[r];
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if ((tok >> 4 & 3) == b) {
+#pragma unroll
+              for (int mt = 0; mt < 4; ++mt) acc[ah][mt][b >> 1][b & 1] += a[mt];
+            }
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
 
 template <class T>
 __global__ __launch_bounds__(NTH) void ll_dw_kernel(const DwArgs p) {
@@ -1319,6 +1408,7 @@ __global__ __launch_bounds__(NTH) void ll_dw_kernel(const DwArgs p) {
   const int wm = wave >> 2, wn = wave & 3;
   // a lane owns 4 consecutive columns of h (m) of one row of W (n)
   const int v0 = p.col0 + n0;
+  if (__is_same(T, tbf16) && p.cl) ll_add_labels<T>(acc, smem, p, nv, v0, m0);
   if (p.f32) {
     float* const out = (float*)p.dw + (int64_t)v0 * p.lddw + m0;
 #pragma unroll
@@ -1767,7 +1857,7 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   const int64_t by_ld = ((int64_t)0x7FF00000 / 2 / ldw) / BN;
   const int64_t rows_fit = (int64_t)((d->dw ? LL_WHOLE_BYTES : LL_PIECE_BYTES) / ((size_t)p.tiles_n * BN * 2)) / BM * BM;
   p.keep = grad && (!dual_of(d) || d->temperature <= 2.f && d->temperature >= 1.f) && rows_fit >= BM && p.tiles_n <= by_ld && (p.R <= rows_fit || !d->dw);
-  p.ref = p.keep && !p.few && !dual_of(d) && (d->dtype == NS_BF16 || (d->k == 0 && !d->dw));
+  p.ref = p.keep && !p.few && !dual_of(d) && (d->k == 0 ? d->dtype == NS_BF16 || !d->dw : d->dtype == NS_BF16 && !d->dw);
   p.Rc = p.R;
   if (p.keep) {
     if (p.R > rows_fit) {
@@ -1852,8 +1942,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   int* const splits = (int*)(ws + p.splits_at);
   float *zk = (float*)(ws + p.zk), *pk = (float*)(ws + p.pk), *La = (float*)(ws + p.La), *Lb = (float*)(ws + p.Lb), *ploss = (float*)(ws + p.ploss);
   float *const eref = p.ref ? (float*)(ws + p.eref) : nullptr, *const efin = p.ref ? (float*)(ws + p.efin) : nullptr, *const F = p.ref ? (float*)(ws + p.F) : nullptr;
-  constexpr bool BF = __is_same(T, tbf16);      // (one softmax of exponentials kept: always with one reference a row)
-  const bool apart = p.ref && d->k == 0 && !d->dw;                 // dz without the labels' cells: dh's last step adds their rows of W
+  const bool apart = p.ref && d->k == 0;                           // dz without the labels' cells: dh's last step adds their rows of W, dW's their rows of h
   const bool dual = dual_of(d), soft_only = d->k > 0 && d->alpha == 1.f, grad = d->dh || d->dw;
   const float alpha = d->k > 0 ? d->alpha : 0.f, T_ = d->k > 0 ? d->temperature : 1.f;
   const float w1 = 1.f - alpha, w2 = alpha * T_;
@@ -1867,7 +1956,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   static ns_dev_once once;
   if (!ns_dyn_lds_once(once, {(const void*)ll_logits_kernel<T, LL_STATS, false, false>, (const void*)ll_logits_kernel<T, LL_STATS, true, false>,
                               (const void*)ll_logits_kernel<T, LL_KEEP, true, false>, (const void*)ll_logits_kernel<T, LL_GRAD, false, true>,
-                              (const void*)ll_logits_kernel<T, LL_KEEP, false, false, false, true>, (const void*)ll_logits_kernel<T, LL_KEEP, false, false, false, BF>, (const void*)ll_logits_kernel<T, LL_STATS, true, false, true>, (const void*)ll_logits_kernel<T, LL_KEEP, true, false, true>,
+                              (const void*)ll_logits_kernel<T, LL_KEEP, false, false, false, true>, (const void*)ll_logits_kernel<T, LL_KEEP, false, false>, (const void*)ll_logits_kernel<T, LL_STATS, true, false, true>, (const void*)ll_logits_kernel<T, LL_KEEP, true, false, true>,
                               (const void*)ll_logits_kernel<T, LL_GRAD, false, false>, (const void*)ll_logits_kernel<T, LL_GRAD, true, false>,
                               (const void*)ll_dh_kernel<T>, (const void*)ll_dw_kernel<T>}, LL_LOGITS_LDS > LL_LDS ? LL_LOGITS_LDS : LL_LDS, "ns_linear_cross_entropy"))
     return NS_ERR_HIP;
@@ -1905,7 +1994,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   a.c1 = c1; a.c2 = c2; a.T = T_;
   a.pm = (float*)(ws + p.pm); a.p1 = (float*)(ws + p.p1); a.p2 = (float*)(ws + p.p2);
   a.La = La; a.Lb = Lb; a.G = ws + p.G; a.ldg = p.piece_tiles * BN; a.lab = lab; a.zk = zk; a.wlab = w1 * up;
-  a.eref = eref; a.efin = efin; a.apart = apart;
+  a.eref = eref; a.efin = efin;
   a.strip = (float*)(ws + p.strip); a.shift = (float)s; a.unshift = 1.f / up;
   r.R = p.Rc; r.tiles_d = (d->d + BN - 1) / BN; r.kt = p.piece_tiles * (BN / BK); r.splits = splits;
   auto grid_of = [&](int tiles_n) { const int64_t t = (int64_t)(p.Rc / BM) * tiles_n; return dim3((unsigned)(t < 256 ? t : 256)); };
@@ -1917,7 +2006,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
     else if (p.keep && dual && T_ == 2.f) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, true, false, true>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     else if (dual && T_ == 2.f) hipLaunchKernelGGL((ll_logits_kernel<T, LL_STATS, true, false, true>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     else if (p.keep && dual) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, true, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
-    else if (p.keep) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, false, false, false, BF>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
+    else if (p.keep) hipLaunchKernelGGL((ll_logits_kernel<T, LL_KEEP, false, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, LL_STATS, true, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     else hipLaunchKernelGGL((ll_logits_kernel<T, LL_STATS, false, false>), all, dim3(NTH), LL_LOGITS_LDS, st, a);
     hipLaunchKernelGGL(ll_rows_kernel<256>, dim3(p.Rc / 16), dim3(256), 0, st, r);
@@ -1934,7 +2023,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
         else if (p.ref) hipLaunchKernelGGL((ll_rebase_kernel<tbf16, false>), sg, dim3(256), 0, st, a);
         else if (dual) hipLaunchKernelGGL((ll_scale_kernel<T, false, true>), sg, dim3(256), 0, st, a);
         else if (d->k == 0) hipLaunchKernelGGL((ll_scale_kernel<tf16, true, false>), sg, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((ll_scale_kernel<tf16, false, false>), sg, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((ll_scale_kernel<T, false, false>), sg, dim3(256), 0, st, a);
       } else if (d->k == 0) hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, false, true>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
       else if (dual) hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, true, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
       else hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, false, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
@@ -1951,6 +2040,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
         DwArgs q = {};
         q.hT = ws + p.hT; q.ldt = p.R; q.G = a.G; q.ldg = a.ldg; q.col0 = a.col0; q.tiles_v = a.tiles_n; q.V = d->vocab; q.d = d->d; q.row0 = row0; q.R = p.Rc;
         q.nvalid = d->nvalid_dev; q.loss_scale = d->loss_scale_dev; q.unscale = 1.f / up; q.dw = d->dw; q.lddw = d->lddw; q.f32 = d->dw_f32; q.add = d->dw_add;
+        q.hp = ws + p.hp; q.dp = p.dp; q.lab = lab; q.cl = apart ? Lb : nullptr;
         hipLaunchKernelGGL(ll_dw_kernel<T>, dim3(p.dt / BM * a.tiles_n), dim3(NTH), LL_LDS, st, q);
       }
     }

@@ -200,6 +200,27 @@ def test_large_logits(ops, dev):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dw_dtype", [None, F32])
+@pytest.mark.parametrize("rows,d,v,tokens", [(9000, 72, 300, 1), (4100, 264, 700, 3), (700, 200, 513, 2)])
+def test_many_rows_share_a_label(ops, dev, dtype, dw_dtype, rows, d, v, tokens):
+    h, w, labels, _ = make_linear(dev, rows, d, v, dtype, seed=16, ignored=0.05)
+    labels = torch.where((labels >= 0) & (labels < v), labels % tokens * (v // tokens) + v // tokens - 1, labels)
+    check_linear(ops, dev, h, w, labels, scale=16.0, dw_dtype=dw_dtype)
+
+
+def test_the_heads_gradient_keeps_the_labels_digits(ops, dev):
+    """a token's row of dW is mostly (p - 1) h of the rows that it labels: as exact as its own rounding, in every norm"""
+    h, w, labels, _ = make_linear(dev, 600, 256, 3000, BF16, seed=17, ignored=0.0)
+    o = outputs(dev, 600)
+    dh, dw = torch.empty_like(h), torch.empty_like(w)
+    ops.linear_cross_entropy(h, w, labels, dh=dh, dweight=dw, **o)
+    ref = R.linear(h, w, labels)
+    for got, want in ((dh, ref["dh"]), (dw, ref["dw"])):
+        own = (want.to(BF16).double() - want).norm()             # what the result's own rounding costs
+        assert (got.double() - want).norm() <= 1.3 * own
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("sharp", [4.0, 12.0])
 def test_labels_that_are_almost_certain(ops, dev, dtype, sharp):
     """1 - p from 0.5 down to nothing: the gradient keeps its own digits, none is lost to p's"""
