@@ -158,6 +158,28 @@ def test_rows_without_a_label_are_not_read(ops, dev, rows):
     assert (dh[off] == 0).all() and (o["row_loss"][off] == 0).all() and torch.isfinite(dw).all()
 
 
+@pytest.mark.parametrize("rows", [9, 300])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("k,alpha,temp", [(0, 0.0, 1.0), (4, 0.5, 1.0), (4, 0.5, 2.0), (4, 0.5, 4.0)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_an_overflow_in_a_labelled_row_shows(ops, dev, rows, dtype, k, alpha, temp, bad):
+    """a NaN or infinity in a row that counts: loss, its row of dh and dW are not finite (what a loss scaler looks for), the other rows' dh keep their values"""
+    h, w, labels, lists = make_linear(dev, rows, 72, 700, dtype, seed=19, ignored=0.0, k=k)
+    kw = dict(top_vals=lists[0], top_idx=lists[1], temperature=temp, alpha=alpha) if k else {}
+    good = dict(outputs(dev, rows), dh=torch.empty_like(h), dweight=torch.empty_like(w))
+    ops.linear_cross_entropy(h, w, labels, **good, **kw)
+    h[7, 5] = bad
+    for grad in (("dh",), ("dh", "dweight")):
+        got = dict(outputs(dev, rows), **{n: torch.empty_like(good[n]) for n in grad})
+        ops.linear_cross_entropy(h, w, labels, **got, **kw)
+        assert not torch.isfinite(got["loss"]).any() and not torch.isfinite(got["row_loss"][7]) and not torch.isfinite(got["dh"][7]).all()
+        if "dweight" in grad:
+            assert not torch.isfinite(got["dweight"]).all()
+        rest = torch.arange(rows, device=dev) != 7
+        near = (got["dh"][rest].double() - good["dh"][rest].double()).abs() <= 8 * R.half_step(dtype) * good["dh"][rest].double().abs().amax(1, keepdim=True)
+        assert near.all()
+
+
 @pytest.mark.parametrize("rows", [0, 1, 70])
 def test_no_row_has_a_label(ops, dev, rows):
     h = torch.full((rows, 64), float("nan"), device=dev, dtype=F16)
@@ -290,6 +312,49 @@ def test_same_inputs_give_the_same_bits_and_workspaces_are_not_shared(ops, dev, 
             assert torch.equal(x, y)
     with pytest.raises(ValueError, match="workspace"):
         once(workspace=ws[:need - 256])
+
+
+@pytest.mark.parametrize("rows", [9, 70, 600])
+@pytest.mark.parametrize("dtype,grad,k,alpha,temp", [(F16, "h", 0, 0.0, 1.0), (BF16, "h", 0, 0.0, 1.0), (BF16, "hw", 0, 0.0, 1.0), (BF16, "w", 0, 0.0, 1.0), (BF16, "h", 5, 0.5, 1.0),
+                                                     (BF16, "hw", 5, 0.5, 1.0), (F16, "hw", 0, 0.0, 1.0), (F16, "h", 5, 1.0, 2.0), (F16, "hw", 5, 0.5, 2.0), (BF16, "hw", 5, 0.5, 4.0)])
+def test_what_a_workspace_holds_does_not_matter(ops, dev, rows, dtype, grad, k, alpha, temp):
+    """every form of the call over workspaces full of NaN, of other numbers and of the call before, with NaN in the masked rows: the same bits, on another stream too, twice over at a time"""
+    h, w, labels, lists = make_linear(dev, rows, 136, 1300, dtype, seed=18, ignored=0.4, k=k)
+    off = ~((labels >= 0) & (labels < 1300))
+    h[off] = float("nan")
+    kw = dict(top_vals=lists[0], top_idx=lists[1], temperature=temp, alpha=alpha) if k else {}
+
+    def bufs():
+        b = outputs(dev, rows)
+        if "h" in grad:
+            b["dh"] = torch.full_like(h, 3.0)
+        if "w" in grad:
+            b["dweight"] = torch.full_like(w, 3.0)
+        return b
+    first = bufs()
+    ops.linear_cross_entropy(h, w, labels, **first, **kw)
+    need = ops.linear_ce_workspace_bytes(h, w, labels, **first, **kw)
+    side = torch.cuda.Stream()
+    got = []
+    for fill in (0xFF, 0x3C, 0x00):
+        ws = torch.full((2, (need + 255) // 256 * 256), fill, device=dev, dtype=torch.uint8)
+        side.wait_stream(torch.cuda.current_stream())
+        for i in range(2):
+            b = bufs()
+            ops.linear_cross_entropy(h, w, labels, workspace=ws[0], **b, **kw)
+            got.append(b)
+        with torch.cuda.stream(side):
+            b = bufs()
+            ops.linear_cross_entropy(h, w, labels, workspace=ws[1], **b, **kw)
+            got.append(b)
+        torch.cuda.synchronize()
+    for b in got:
+        for n in first:
+            assert torch.equal(b[n], first[n]), n
+    if "h" in grad:
+        assert (first["dh"][off] == 0).all() and torch.isfinite(first["dh"]).all()
+    if "w" in grad:
+        assert torch.isfinite(first["dweight"]).all()
 
 
 @pytest.mark.parametrize("rows", [50, 260])
