@@ -22,7 +22,8 @@
 //     and their cells of dz are written from those.
 //   * dz in the operands' type: fp16 cells carry a factor 2^s (exact; taken out in fp32 at the end), so that a probability of 1 / V does
 //     not fall among the subnormals; a probability below 2^-29 of full scale is a subnormal, below 2^-40 zero.  bf16 has the range of fp32.
-//     The label's cell is rounded once, after the subtraction; a kept cell twice (its exponential, dz); with few labels a cell is two numbers (ll_few_grad).
+//     A sparse cell is rounded once, after the subtraction, a kept one twice (its exponential, dz).  A row's largest cells count by themselves: with up to 32 labels
+//     a cell is two numbers (ll_few_grad), beyond 64 rows dh's and dW's last steps add in fp32 what their rounding lost (ll_cells_kernel) or all of them (ll_label_ref).
 //   * Sums over the vocabulary (dh) and over the rows (dW) stay in fp32 MFMA accumulators / fp32 tiles added in a fixed order: no atomics,
 //     the same bits every time.
 //   * What bounds it: the 256 x 256 main loops (8 waves, two 64 KiB ring buffers, one workgroup per CU) run at 2.9 k cycles per K tile of 64 against 2.05 k of MFMA,
@@ -593,7 +594,7 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
       c[2] = c[3] = 0.f;
       if (FIX) {
         c[2] = __int_as_float(i < nv ? p.lab[p.row0 + i] : -1);
-        c[3] = i < nv ? __builtin_amdgcn_exp2f(p.zk[p.row0 + i] * p.c1 - c[0]) - p.wlab : 0.f;
+        c[3] = i < nv ? __builtin_amdgcn_exp2f(__builtin_fmaf(p.zk[p.row0 + i], p.c1, -c[0])) - p.wlab : 0.f;
       }
     }
   };
@@ -849,7 +850,7 @@ __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
   if (FIX && threadIdx.x < 64) {
     const int i = i0 + threadIdx.x;
     lc[threadIdx.x] = i < nv ? p.lab[p.row0 + i] - t0 * BN : -1;
-    lv[threadIdx.x] = i < nv ? __builtin_amdgcn_exp2f(p.zk[p.row0 + i] * p.c1 - p.La[i]) - p.wlab : 0.f;
+    lv[threadIdx.x] = i < nv ? __builtin_amdgcn_exp2f(__builtin_fmaf(p.zk[p.row0 + i], p.c1, -p.La[i])) - p.wlab : 0.f;
   }
   __syncthreads();
   const int c = (threadIdx.x & 63) * 8, r0 = threadIdx.x >> 6;
@@ -962,7 +963,8 @@ struct RowArgs {
   const float* zk; const float* top_vals; const int32_t* top_idx; int64_t ld_top;
   float *La, *Lb, *pk, *row_loss, *packed_loss;
   const float* eref; float *efin, *F, head, shift;     // REF: the rows' references before and behind the logits' pass, their factors
-  float* cl;                                    // p - 1 of the label, where dh's last step takes it
+  float* cl;                                    // p - 1 of the label, where dh's and dW's last steps take it
+  int* big_tok; float* big_res; float wlab; int f16;      // (no list, the label's cell in dz) what the cell's rounding loses: see ll_cells_kernel
 };
 
 // 16 threads per row; one workgroup of 1024 threads (the few-row path) also takes the mean
@@ -1092,6 +1094,13 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
       p.F[i] = __builtin_amdgcn_exp2f(e - p.La[i] - p.shift);      // (La is for cells times 2^shift)
       if (p.cl) p.cl[i] = __builtin_amdgcn_exp2f(p.zk[pi] * p.c1 - l1) - 1.f;
     }
+    if (p.big_tok) {
+      const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(p.zk[pi], p.c1, -p.La[i])) - p.wlab;
+      p.big_tok[2 * pi] = p.lab[pi];
+      p.big_tok[2 * pi + 1] = -1;
+      p.big_res[2 * pi] = v - (p.f16 ? (float)(half_t)v : (float)(__bf16)v);
+      p.big_res[2 * pi + 1] = 0.f;
+    }
     p.row_loss[row] = loss;
     if (NT == 256) p.packed_loss[pi] = loss;
   }
@@ -1125,12 +1134,16 @@ __global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__
   ll_mean<1024>(packed_loss, *nvalid, loss);
 }
 
-// the sparse cells of dz in one piece: one wave per row, each token written once whatever number of entries name it
+// the sparse cells of dz in one piece: one wave per row, each token written once whatever number of entries name it.
+// A row's gradient is mostly its one or two largest cells, whose rounding would be an error of all of it (1.5 times the result's own where few rows average it out):
+// what the two largest lose goes to big_tok / big_res, and dh's and dW's last steps add it in fp32 (fp16, 1434 rows with lists, dh and dW: 2.6e-4 -> 2.1e-4 off, the
+// result's own rounding, for 15 us of 398).
 template <class E>
 __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ nvalid, int row0, int R, const int* __restrict__ order, const int* __restrict__ lab,
                                                        const int32_t* __restrict__ top_idx, int64_t ld_top, int k, const float* __restrict__ zk,
                                                        const float* __restrict__ pk, const float* __restrict__ La, const float* __restrict__ Lb, float c1, float c2,
-                                                       float w1s, float w2s, int col0, int cols, int V, E* __restrict__ G, int ldg, const float* __restrict__ efin) {
+                                                       float w1s, float w2s, int col0, int cols, int V, E* __restrict__ G, int ldg, const float* __restrict__ efin,
+                                                       int* __restrict__ big_tok, float* __restrict__ big_res) {
   __shared__ __attribute__((aligned(16))) int sidx[4][LL_MAX_K + 4];
   __shared__ __attribute__((aligned(16))) float sp[4][LL_MAX_K + 4];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = blockIdx.x * 4 + wave;
@@ -1149,9 +1162,12 @@ __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ n
   const float la = La[i], lb = Lb ? Lb[i] : INFINITY;
   // (efin: cells relative to the row's factor; one of zero leaves none)
   const float from = efin ? efin[i] : la, up = efin ? (la < INFINITY ? __builtin_amdgcn_exp2f(la - efin[i]) : 0.f) : 1.f;
+  float m1 = 0.f, m2 = 0.f, r1 = 0.f, r2 = 0.f;             // this lane's two largest
+  int t1 = -1, t2 = -1;
   for (int e = lane; e <= k; e += 64) {
     const int t = sidx[wave][e], c = t - col0;
-    if (t < 0 || c < 0 || c >= cols) continue;
+    const bool in = c >= 0 && c < cols;
+    if (t < 0 || (!in && col0 > 0)) continue;               // (the first piece's launch looks at all of a row's cells)
     float soft = 0.f;
     bool first = true;
 #pragma unroll 4
@@ -1167,7 +1183,23 @@ __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ n
     if (Lb) v += __builtin_amdgcn_exp2f(z * c2 - lb);
     v -= w2s * up * soft;
     if (t == lab[pi]) v -= w1s * up;
-    G[(int64_t)i * ldg + c] = (E)v;
+    if (in) G[(int64_t)i * ldg + c] = (E)v;
+    const float m = fabsf(v), res = v - (float)(E)v;
+    if (m > m1) { m2 = m1; t2 = t1; r2 = r1; m1 = m; t1 = t; r1 = res; }
+    else if (m > m2) { m2 = m; t2 = t; r2 = res; }
+  }
+  if (col0 > 0) return;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float m = ns_wave_max(m1);
+    const uint64_t who = __ballot(m1 == m && m1 > 0.f);
+    if (who == 0) {
+      if (lane == 0) { big_tok[2 * pi + j] = -1; big_res[2 * pi + j] = 0.f; }
+    } else if (lane == __builtin_ctzll(who)) {
+      big_tok[2 * pi + j] = t1;
+      big_res[2 * pi + j] = r1;
+      m1 = m2; t1 = t2; r1 = r2;
+    }
   }
 }
 
@@ -1234,7 +1266,7 @@ template <class E>
 __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict__ slab, int groups, int splits, const int* __restrict__ splits_dev, int R, int row0, int chunk, int d, int rows, const int* __restrict__ inv,
                                                         const int* __restrict__ nvalid, const float* __restrict__ loss_scale, float unscale, E* __restrict__ dh, int64_t lddh,
                                                         const float* __restrict__ packed_loss, float* __restrict__ loss, const float* __restrict__ F, const E* __restrict__ w,
-                                                        int64_t ldw, const int* __restrict__ lab, const float* __restrict__ cl) {
+                                                        int64_t ldw, const int* __restrict__ lab, const float* __restrict__ cl, const int* __restrict__ big_tok, const float* __restrict__ big_res) {
   if (loss && blockIdx.x == gridDim.x - 1) {      // one workgroup more: the mean of the row losses
     ll_mean<256>(packed_loss, *nvalid, loss);
     return;
@@ -1272,8 +1304,19 @@ __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict_
   if (!in || g != 0 || (pi >= 0 ? i < 0 : row0 > 0)) return;
   const float gs = (loss_scale ? *loss_scale : 1.f) / (float)max(*nvalid, 1);
   if (i >= 0) {
+    if (big_tok) {                                // what the two largest cells' rounding lost
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int t = big_tok[2 * pi + j];
+        if (t < 0) continue;
+        const float r = big_res[2 * pi + j];
+        const e4 l = *(const e4*)(w + t * ldw + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = __builtin_fmaf(r, (float)l[e], a[e]);
+      }
+    }
     a *= F ? F[i] : unscale;
-    if (w) {                                      // the label's part, which is not in dz then
+    if (cl) {                                     // the label's part, which is not in dz then
       const e4 l = *(const e4*)(w + lab[pi] * ldw + c);
 #pragma unroll
       for (int e = 0; e < 4; ++e) a[e] = __builtin_fmaf(cl[i], (float)l[e], a[e]);
@@ -1285,11 +1328,11 @@ __global__ __launch_bounds__(256) void ll_dh_out_kernel(const float* __restrict_
   *(e4*)(dh + row * lddh + c) = o;
 }
 template <class E> void launch_dh_out(const float* slab, int groups, int splits, const int* splits_dev, int R, int row0, int chunk, int d, int rows, const int* inv, const int* nvalid, const float* loss_scale, float unscale, E* dh,
-                                      int64_t lddh, const float* packed_loss, float* loss, const float* F, const E* w, int64_t ldw, const int* lab, const float* cl, hipStream_t st) {
+                                      int64_t lddh, const float* packed_loss, float* loss, const float* F, const E* w, int64_t ldw, const int* lab, const float* cl, const int* big_tok, const float* big_res, hipStream_t st) {
   const int nblk = 16 / groups;
   const int64_t items = (int64_t)rows * ((d + 63) / 64);
   hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)((items + nblk - 1) / nblk) + (loss ? 1 : 0)), dim3(256), 0, st, slab, groups, splits, splits_dev, R, row0, chunk, d, rows, inv, nvalid,
-                     loss_scale, unscale, dh, lddh, packed_loss, loss, F, w, ldw, lab, cl);
+                     loss_scale, unscale, dh, lddh, packed_loss, loss, F, w, ldw, lab, cl, big_tok, big_res);
 }
 
 struct DwArgs {
@@ -1298,15 +1341,16 @@ struct DwArgs {
   const int* nvalid; const float* loss_scale;
   float unscale;
   void* dw; int64_t lddw; int f32, add;
-  const void* hp; int dp; const int* lab; const float* cl;      // cl: the labels' cells, which are not in dz then
+  const void* hp; int dp;
+  const int* tok; const float* coef; int per;                   // (2^per a packed row) tokens and coefficients of h that dz does not hold: the labels' cells, or what the largest cells' rounding lost
 };
 
-// The labels' part of dW's tile in fp32, where dz does not hold it (h's copy there is rounded with the rows' factors, and a token's row of dW is mostly its label's
-// h): rows whose label is one of the tile's 256 tokens are listed in order, 4096 labels at a time, and each adds (p - 1) h to its token's accumulators (dW 2.8e-3 -> 1.7e-3 off, its own
-// rounding, for 12 us of 382 at 1844 rows, d = 512).
+// What dz does not hold of dW's tile, in fp32: the labels' part where h's copy is rounded with the rows' factors (a token's row of dW is mostly its labels' h), else what the
+// largest cells' rounding lost.  Entries whose token is one of the tile's 256 are listed in order, 4096 at a time, and each adds coefficient x h to its token's
+// accumulators (bf16, no list: dW 2.8e-3 -> 1.7e-3 off, its own rounding, for 12 us of 382 at 1844 rows, d = 512).
 constexpr int LL_LIST = 4096;
 template <class T>
-__device__ __forceinline__ void ll_add_labels(f32x4 (&acc)[2][4][2][2], char* smem, const DwArgs& p, int nv, int v0, int m0) {
+__device__ __forceinline__ void ll_add_entries(f32x4 (&acc)[2][4][2][2], char* smem, const DwArgs& p, int entries, int v0, int m0) {
   typedef typename T::e E;
   typedef E e4 __attribute__((ext_vector_type(4)));
   int2* const list = (int2*)smem;
@@ -1316,12 +1360,13 @@ __device__ __forceinline__ void ll_add_labels(f32x4 (&acc)[2][4][2][2], char* sm
   asm volatile("" : "+v"(tid));                             // (no address of this part is carried through the main loop, where there is no register for it)
   const int lane = tid & 63, l15 = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
-  for (int base = 0; base < nv; base += LL_LIST) {
+  for (int base = 0; base < entries; base += LL_LIST) {
     int t[8];
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
       const int i = base + x * NTH + tid;
-      t[x] = i < nv ? p.lab[i] - v0 : -1;
+      t[x] = i < entries ? p.tok[i] : -1;
+      t[x] = t[x] < 0 ? -1 : t[x] - v0;
     }
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
@@ -1354,10 +1399,10 @@ __device__ __forceinline__ void ll_add_labels(f32x4 (&acc)[2][4][2][2], char* sm
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int e = (tid >> 5) + 16 * x, col = (tid & 31) * 8;
-        if (e0 + e < n && m0 + col < p.dp) *(uint4*)(rows + e * LDH + col * 2) = *(const uint4*)((const E*)p.hp + (int64_t)list[e0 + e].x * p.dp + m0 + col);
+        if (e0 + e < n && m0 + col < p.dp) *(uint4*)(rows + e * LDH + col * 2) = *(const uint4*)((const E*)p.hp + (int64_t)(list[e0 + e].x >> p.per) * p.dp + m0 + col);
       }
       const int2 it = e0 + lane < n ? list[e0 + lane] : make_int2(0, -1);
-      const float cl = it.y >= 0 ? p.cl[it.x] : 0.f;
+      const float cl = it.y >= 0 ? p.coef[it.x] : 0.f;
       uint64_t m = __ballot(it.y >= 0 && it.y >> 6 == wn);
       __syncthreads();
       while (m) {
@@ -1408,7 +1453,7 @@ __global__ __launch_bounds__(NTH) void ll_dw_kernel(const DwArgs p) {
   const int wm = wave >> 2, wn = wave & 3;
   // a lane owns 4 consecutive columns of h (m) of one row of W (n)
   const int v0 = p.col0 + n0;
-  if (__is_same(T, tbf16) && p.cl) ll_add_labels<T>(acc, smem, p, nv, v0, m0);
+  ll_add_entries<T>(acc, smem, p, nv << p.per, v0, m0);
   if (p.f32) {
     float* const out = (float*)p.dw + (int64_t)v0 * p.lddw + m0;
 #pragma unroll
@@ -1838,14 +1883,15 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
 struct Plan {
   int few;                                    // 0, or MT of the few-row path
   int keep, ref, R, Rc, dp, dt, tiles_n, piece_tiles, pieces, pairs;      // keep: LL_KEEP, in chunks of Rc rows (else Rc = R, in pieces of the vocabulary)
-  size_t splits_at, order, inv, lab, hp, hT, zk, pk, pm, p1, p2, strip, La, Lb, eref, efin, F, ploss, G, slab, total;
+  size_t splits_at, order, inv, lab, hp, hT, zk, pk, pm, p1, p2, strip, La, Lb, eref, efin, F, big, ploss, G, slab, total;
 };
 
 bool dual_of(const ns_linear_ce_desc* d) { return d->k > 0 && d->alpha > 0.f && d->alpha < 1.f && d->temperature != 1.f; }
 
 Plan plan_of(const ns_linear_ce_desc* d) {
   Plan p = {};
-  p.few = d->rows > LL_FEW_ROWS ? 0 : d->rows <= 16 ? 1 : d->rows <= 32 ? 2 : 4;
+  const int parts = d->dh || d->dw ? 2 : 1;       // (a cell in two parts takes two rows of dz: ll_few_grad)
+  p.few = d->rows > LL_FEW_ROWS ? 0 : d->rows * parts <= 16 ? 1 : d->rows * parts <= 32 ? 2 : 4;
   p.R = (d->rows > 0 ? d->rows + BM - 1 : BM) / BM * BM;
   p.dp = (d->d + BK - 1) / BK * BK;
   p.dt = (d->d + BM - 1) / BM * BM;
@@ -1898,6 +1944,7 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   p.eref = p.ref ? take((size_t)p.R * 4) : 0;
   p.efin = p.ref ? take((size_t)p.Rc * 4) : 0;
   p.F = p.ref ? take((size_t)p.Rc * 4) : 0;
+  p.big = grad && !p.few && !(p.ref && d->k == 0) ? take((size_t)p.R * 16) : 0;
   p.ploss = take((size_t)p.R * 4);
   p.G = grad && !p.few ? take((size_t)p.Rc * p.piece_tiles * BN * 2) : 0;
   p.slab = d->dh ? take(p.few ? (size_t)p.tiles_n * 16 * p.few * d->d * 4 : (size_t)p.pairs * BM * BN * 4) : 0;
@@ -1928,7 +1975,7 @@ int few_launch(const ns_linear_ce_desc* d, const FewArgs& f, const RowArgs& r, b
     gy = (chunks + (chunks + gy - 1) / gy - 1) / ((chunks + gy - 1) / gy);
     if (dual) hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, true>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
     else hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, false>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
-    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n >= 64 ? 16 : f.tiles_n >= 16 ? 4 : 1, f.tiles_n, nullptr, 16 * MT, 0, LL_FEW_ROWS, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, nullptr, nullptr, nullptr, nullptr, 0, nullptr, nullptr, st);
+    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n >= 64 ? 16 : f.tiles_n >= 16 ? 4 : 1, f.tiles_n, nullptr, 16 * MT, 0, LL_FEW_ROWS, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, nullptr, nullptr, nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;
@@ -1943,6 +1990,8 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   float *zk = (float*)(ws + p.zk), *pk = (float*)(ws + p.pk), *La = (float*)(ws + p.La), *Lb = (float*)(ws + p.Lb), *ploss = (float*)(ws + p.ploss);
   float *const eref = p.ref ? (float*)(ws + p.eref) : nullptr, *const efin = p.ref ? (float*)(ws + p.efin) : nullptr, *const F = p.ref ? (float*)(ws + p.F) : nullptr;
   const bool apart = p.ref && d->k == 0;                           // dz without the labels' cells: dh's last step adds their rows of W, dW's their rows of h
+  int* const big_tok = p.big ? (int*)(ws + p.big) : nullptr;
+  float* const big_res = p.big ? (float*)(ws + p.big) + 2 * (size_t)p.R : nullptr;
   const bool dual = dual_of(d), soft_only = d->k > 0 && d->alpha == 1.f, grad = d->dh || d->dw;
   const float alpha = d->k > 0 ? d->alpha : 0.f, T_ = d->k > 0 ? d->temperature : 1.f;
   const float w1 = 1.f - alpha, w2 = alpha * T_;
@@ -1967,7 +2016,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   r.lw1 = (d->k > 0 && !dual) ? (float)s : log2f(w1) + (float)s;
   r.lw2 = log2f(w2) + (float)s;
   r.dual = dual; r.soft_only = soft_only; r.nvalid = d->nvalid_dev; r.order = order; r.lab = lab; r.zk = zk; r.top_vals = d->top_vals; r.top_idx = d->top_idx;
-  r.eref = eref; r.efin = efin; r.F = F; r.head = T::HEAD; r.shift = (float)s; r.cl = apart ? Lb : nullptr;      // (one softmax: Lb is free)
+  r.eref = eref; r.efin = efin; r.F = F; r.head = T::HEAD; r.shift = (float)s; r.cl = apart ? Lb : nullptr; r.wlab = w1 * up; r.f16 = d->dtype == NS_F16; r.big_tok = d->k == 0 ? big_tok : nullptr; r.big_res = big_res;      // (one softmax: Lb is free)
  
   r.ld_top = d->ld_top; r.La = La; r.Lb = dual ? Lb : nullptr; r.pk = pk; r.row_loss = d->row_loss; r.packed_loss = ploss; r.loss = d->loss_dev;
   if (p.few) {
@@ -2029,7 +2078,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
       else hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, false, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
       if (d->k > 0)
         hipLaunchKernelGGL(ll_cells_kernel<E>, dim3(p.Rc / 4), dim3(256), 0, st, d->nvalid_dev, row0, p.Rc, order, lab, d->top_idx, d->ld_top, d->k, zk, pk, La,
-                           dual ? Lb : nullptr, a.c1, a.c2, w1 * up, w2 * up, a.col0, a.tiles_n * BN, d->vocab, (E*)a.G, a.ldg, efin);
+                           dual ? Lb : nullptr, a.c1, a.c2, w1 * up, w2 * up, a.col0, a.tiles_n * BN, d->vocab, (E*)a.G, a.ldg, efin, big_tok, big_res);
       if (d->dh) {
         DhArgs q = {};
         q.G = a.G; q.w = d->w; q.ldw = d->ldw; q.ldg = a.ldg; q.col0 = a.col0; q.cols = a.tiles_n * BN; q.V = d->vocab; q.d = d->d; q.row0 = row0; q.R = p.Rc;
@@ -2040,13 +2089,13 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
         DwArgs q = {};
         q.hT = ws + p.hT; q.ldt = p.R; q.G = a.G; q.ldg = a.ldg; q.col0 = a.col0; q.tiles_v = a.tiles_n; q.V = d->vocab; q.d = d->d; q.row0 = row0; q.R = p.Rc;
         q.nvalid = d->nvalid_dev; q.loss_scale = d->loss_scale_dev; q.unscale = 1.f / up; q.dw = d->dw; q.lddw = d->lddw; q.f32 = d->dw_f32; q.add = d->dw_add;
-        q.hp = ws + p.hp; q.dp = p.dp; q.lab = lab; q.cl = apart ? Lb : nullptr;
+        q.hp = ws + p.hp; q.dp = p.dp; q.tok = apart ? lab : big_tok; q.coef = apart ? Lb : big_res; q.per = apart ? 0 : 1;
         hipLaunchKernelGGL(ll_dw_kernel<T>, dim3(p.dt / BM * a.tiles_n), dim3(NTH), LL_LDS, st, q);
       }
     }
     if (d->dh)
       launch_dh_out<E>((const float*)(ws + p.slab), p.Rc <= 512 ? 16 : 1, 0, splits, 0, row0, p.Rc, d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh,
-                       d->lddh, ploss, row0 + p.Rc >= p.R ? d->loss_dev : nullptr, F, apart ? (const E*)d->w : nullptr, d->ldw, lab, Lb, st);
+                       d->lddh, ploss, row0 + p.Rc >= p.R ? d->loss_dev : nullptr, F, (const E*)d->w, d->ldw, lab, apart ? Lb : nullptr, big_tok, big_res, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;

@@ -230,16 +230,29 @@ def test_many_rows_share_a_label(ops, dev, dtype, dw_dtype, rows, d, v, tokens):
     check_linear(ops, dev, h, w, labels, scale=16.0, dw_dtype=dw_dtype)
 
 
-def test_the_heads_gradient_keeps_the_labels_digits(ops, dev):
-    """a token's row of dW is mostly (p - 1) h of the rows that it labels: as exact as its own rounding, in every norm"""
-    h, w, labels, _ = make_linear(dev, 600, 256, 3000, BF16, seed=17, ignored=0.0)
-    o = outputs(dev, 600)
-    dh, dw = torch.empty_like(h), torch.empty_like(w)
-    ops.linear_cross_entropy(h, w, labels, dh=dh, dweight=dw, **o)
-    ref = R.linear(h, w, labels)
-    for got, want in ((dh, ref["dh"]), (dw, ref["dw"])):
-        own = (want.to(BF16).double() - want).norm()             # what the result's own rounding costs
-        assert (got.double() - want).norm() <= 1.3 * own
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [24, 93, 600])
+@pytest.mark.parametrize("grad,k,temp,alpha", [("hw", 0, 1.0, 0.0), ("h", 0, 1.0, 0.0), ("hw", 5, 2.0, 0.3), ("h", 5, 1.0, 1.0), ("hw", 7, 1.0, 0.5), ("hw", 3, 4.0, 0.5)])
+def test_the_largest_cells_keep_their_digits(ops, dev, dtype, rows, grad, k, temp, alpha):
+    """a row's gradient, and a token's row of dW, is mostly one or two cells times a vector: as a whole no more than 1.3 times as far off as its own rounding (one
+    rounding of every cell by itself would make that the square root of 2, and more where few rows average it out)"""
+    h, w, labels, _ = make_linear(dev, rows, 256, 3000, dtype, seed=17, ignored=0.0)
+    labels %= 3000
+    lists = (None, None)
+    if k:
+        g = gen(rows, dev)
+        lists = (6.0 - 2.5 * torch.log1p(torch.arange(k, device=dev).float()) + 0.3 * torch.randn(rows, k, generator=g, device=dev),
+                 ((labels.unsqueeze(1) + 611 * torch.arange(k, device=dev)) % 3000).int())
+    o = outputs(dev, rows)
+    got = dict(dh=torch.empty_like(h), **({"dweight": torch.empty_like(w)} if "w" in grad else {}))
+    more = dict(top_vals=lists[0], top_idx=lists[1], temperature=temp, alpha=alpha) if k else {}
+    sc = torch.tensor([2048.0], device=dev)
+    ops.linear_cross_entropy(h, w, labels, loss_scale=sc, **o, **got, **more)
+    ref = R.linear(h, w, labels, 2048.0, None, temp, alpha, *lists)
+    for n, x in got.items():
+        want = ref["dh" if n == "dh" else "dw"]
+        own = (want.to(dtype).double() - want).norm()             # what the result's own rounding costs
+        assert (x.double() - want).norm() <= 1.3 * own, n
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
