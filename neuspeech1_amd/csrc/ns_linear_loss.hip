@@ -1433,6 +1433,7 @@ __device__ __forceinline__ void ll_add_entries(f32x4 (&acc)[2][4][2][2], char* s
       __syncthreads();
     }
   }
+  __syncthreads();                                          // (a batch of no entries ends with every wave's read of its count: the caller stages over it)
 }
 
 template <class T>
