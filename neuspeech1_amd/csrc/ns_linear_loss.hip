@@ -842,9 +842,10 @@ __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
     const int sidx = t0 * 4 + (x >> 6), i = i0 + (x & 63);
     if (sidx < p.tiles_n * 4) {
       const float mx = p.strip[(int64_t)sidx * p.R + i];
-      const float e = (mx == -INFINITY ? 0.f : ll_ref(mx, DUAL ? p.c2 : p.c1)) - p.shift;
-      f[x >> 6][x & 63] = __builtin_amdgcn_exp2f(e - (DUAL ? p.Lb[i] : p.La[i]));
-      if (DUAL) f1[x >> 6][x & 63] = e * p.T - p.La[i];
+      const bool none = mx == -INFINITY;      // (past the vocabulary: zeros, whatever the row's logits are.  A factor from no maximum is infinite where they lie low)
+      const float e = ll_ref(none ? 0.f : mx, DUAL ? p.c2 : p.c1) - p.shift;
+      f[x >> 6][x & 63] = none ? 0.f : __builtin_amdgcn_exp2f(e - (DUAL ? p.Lb[i] : p.La[i]));
+      if (DUAL) f1[x >> 6][x & 63] = none ? -INFINITY : e * p.T - p.La[i];
     }
   }
   if (FIX && threadIdx.x < 64) {
@@ -918,7 +919,8 @@ __global__ __launch_bounds__(256) void ll_rebase_kernel(const LogitsArgs p) {
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       if (r[x] < 0) continue;
-      const float a = __builtin_amdgcn_exp2f(ll_strip_ref<T>(mx[x], __shfl(from, r[x], 64), p.c1, p.shift) - __shfl(to, r[x], 64));
+      const float ref = ll_strip_ref<T>(mx[x], __shfl(from, r[x], 64), p.c1, p.shift), aim = __shfl(to, r[x], 64);
+      const float a = mx[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - aim);      // (a strip past the vocabulary: zeros)
       const int at = FIX ? __shfl(lc, r[x], 64) - c : -1;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[x][e] = (E)(FIX && at == e ? 0.f : (float)v[x][e] * a);
