@@ -19,7 +19,8 @@
 //            8192 rows, d = 1280, V = 51865, bf16, dh and dW: 3.59 ms formed again in 256 MiB, 2.72 ms kept in 852 MB.
 //   * Rows without a label are packed away first: they cost nothing, and an infinity or NaN in a masked row reaches neither loss nor gradient.
 //   * A row's sparse terms (its label, the teacher's list) are no part of the dense epilogue: their logits are gathered as dot products in fp32
-//     and their cells of dz are written from those.
+//     and their cells of dz are written from those.  One of them a row, its own token, is no part of the statistics either: 1 - p of a row that is almost certain is
+//     then a sum of its own, not what is left of p (ll_rows_kernel).
 //   * dz in the operands' type: fp16 cells carry a factor 2^s (exact; taken out in fp32 at the end), so that a probability of 1 / V does
 //     not fall among the subnormals; a probability below 2^-29 of full scale is a subnormal, below 2^-40 zero.  bf16 has the range of fp32.
 //     A sparse cell is rounded once, after the subtraction, a kept one twice (its exponential, dz).  A row's largest cells count by themselves: with up to 32 labels
@@ -116,7 +117,7 @@ __device__ __forceinline__ float ll_ref(float mx, float c) { return ceilf(mx * c
 // every row's reference changes).
 //   bfloat16   has the exponents for x and for the cells of a list, up to 2^47; what lies 2^-126 below the label counts for nothing.
 //   float16    has room for x alone, from 2^-30 of the label's to 2^9 times it, and none for h's copy with the factors: dh alone, and no list.
-// Without a list the label's x is cleared, and dh's and dW's last steps add (p - 1) W[label] and (p - 1) h in fp32: a rounded factor or cell would be an error of all of
+// Without a list the label's x is zero (it is the row's own token), and dh's and dW's last steps add (p - 1) W[label] and (p - 1) h in fp32: a rounded factor or cell would be an error of all of
 // a row's gradient, and subtracting W[label] from a product that holds p W[label] would leave p's rounding of 1 - p.
 // The gathered logit and the tile's differ by the order of their sums, each within (d + 4) u sum |h w| of the exact one: where that could exceed 4 the row gets no
 // reference (NaN: every comparison fails).
@@ -349,7 +350,7 @@ __global__ __launch_bounds__(1024) void ll_compact_kernel(const int64_t* __restr
 template <class T>
 __global__ __launch_bounds__(256) void ll_pack_kernel(const void* __restrict__ h_, int64_t ldh, const void* __restrict__ w_, int64_t ldw, int d, int dp,
                                                       const int* __restrict__ order, const int* __restrict__ lab, int k, const int* __restrict__ nvalid,
-                                                      void* __restrict__ hp_, float* __restrict__ zk, float c, float* __restrict__ eref) {
+                                                      void* __restrict__ hp_, float* __restrict__ zk, float c, float* __restrict__ eref, int* __restrict__ xtok) {
   typedef typename T::v8 v8;
   typedef typename T::e E;
   const int lane = threadIdx.x & 63, i = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -357,6 +358,7 @@ __global__ __launch_bounds__(256) void ll_pack_kernel(const void* __restrict__ h
   if (i >= (nv + BM - 1) / BM * BM) return;
   E* const dst = (E*)hp_ + (int64_t)i * dp;
   if (i >= nv) {
+    if (lane == 0) xtok[i] = -1;
     if (eref && lane == 0) eref[i] = 0.f;
     for (int c = lane * 8; c < dp; c += 512) *(uint4*)(dst + c) = make_uint4(0, 0, 0, 0);
     return;
@@ -378,20 +380,25 @@ __global__ __launch_bounds__(256) void ll_pack_kernel(const void* __restrict__ h
   }
   if (k > 0) return;
   s = ns_wave_sum(s);
-  if (lane == 0) zk[i] = s;
+  if (lane == 0) { zk[i] = s; xtok[i] = lab[i]; }
   if (!eref) return;
   mass = ns_wave_sum(mass);
   if (lane == 0) eref[i] = ll_label_ref<T>(s, mass, d, c);
 }
 
-// zk[i][e] = h_i . W[token e], e = 0 .. k - 1 the teacher's list, e = k the label: a workgroup per row, 16 lanes per entry (256 B of W a step, 16 entries
+// zk[i][e] = h_i . W[token e], e = 0 .. k - 1 the teacher's list, e = k the label, and the row's own token (see ll_rows_kernel), the largest of these: a workgroup per row, 16 lanes per entry (256 B of W a step, 16 entries
 // side by side; one entry after the other on a wave, 64 entries took 77 us for 1434 rows at d = 512, this 19)
 template <class T>
 __global__ __launch_bounds__(256) void ll_gather_kernel(const void* __restrict__ hp_, int dp, const void* __restrict__ w_, int64_t ldw, int d, int V,
                                                         const int* __restrict__ order, const int* __restrict__ lab, const int32_t* __restrict__ top_idx,
-                                                        int64_t ld_top, int k, const int* __restrict__ nvalid, float* __restrict__ zk, float c1, float* __restrict__ eref) {
+                                                        int64_t ld_top, int k, const int* __restrict__ nvalid, float* __restrict__ zk, float c1, float* __restrict__ eref,
+                                                        int* __restrict__ xtok, float* __restrict__ xz) {
   typedef typename T::v8 v8;
   typedef typename T::e E;
+  __shared__ float bz[16], bm[16], lz[2];
+  __shared__ int bt[16];
+  float top = -INFINITY, top_mass = 0.f;               // this group's largest
+  int top_tok = -1;
   const int i = blockIdx.x, l = threadIdx.x & 15;
   if (i >= *nvalid) return;
   const E* const src = (const E*)hp_ + (int64_t)i * dp;
@@ -414,7 +421,19 @@ __global__ __launch_bounds__(256) void ll_gather_kernel(const void* __restrict__
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); mass += __shfl_xor(mass, o, 64); }
     if (l == 0) zk[(int64_t)i * (k + 1) + e] = s;
-    if (l == 0 && e == k && eref) eref[i] = ll_label_ref<T>(s, mass, d, c1);
+    if (l == 0 && e == k) { lz[0] = s; lz[1] = mass; }
+    if (tok >= 0 && tok < V && s > top) { top = s; top_mass = mass; top_tok = tok; }
+  }
+  if (l == 0) { const int g = threadIdx.x >> 4; bz[g] = top; bm[g] = top_mass; bt[g] = top_tok; }
+  __syncthreads();
+  if (threadIdx.x == 0) {                              // the row's own token: the largest of its list and its label
+    float z = lz[0], mass = lz[1];
+    int tok = lab[i];
+    for (int g = 0; g < 16; ++g)
+      if (bz[g] > z) { z = bz[g]; mass = bm[g]; tok = bt[g]; }
+    xtok[i] = tok;
+    xz[i] = z;
+    if (eref) eref[i] = ll_label_ref<T>(z, mass, d, c1);
   }
 }
 
@@ -445,9 +464,9 @@ struct LogitsArgs {
   void* G; int ldg;
   float T;
   int row0; float *strip, shift, unshift;   // first packed row; LL_KEEP: (4 tiles_n, R) maxima of the 64-column strips, s and 2^-s
-  const int* lab; const float* zk;       // FIX: the label's cell of dz is put right in the staged tile
-  float wlab;                            // w1 2^s
+  const int* lab; const float* rk;       // FIX: the label's cell of dz is put right in the staged tile
   const float *eref, *efin;              // REF: (R) the rows' references before and behind the pass
+  const int* xtok;                       // the rows' own tokens: no part of the statistics, zero among the kept exponentials
 };
 
 // One workgroup per CU walks the tiles of its XCD's run.  The ring never drains: the pieces that a tile's last two K tiles request are the next tile's first
@@ -456,12 +475,17 @@ struct LogitsArgs {
 // of ring buffer 1 that hold nothing yet), 16-B chunk c of row r at chunk c ^ (r & 7): no barrier between staging and storing, a wave's own LDS operations
 // are in order; its 16 stores are left in flight under the next tile's first K tile, whose waits count them.
 constexpr int LL_SIDE = 2 * BUF;                              // behind the ring
-constexpr int LL_LOGITS_LDS = LL_SIDE + 3 * 4096;             // statistics: 3 x 4 x 256 floats; dz: two parities of 4 x 256 row constants (8 KiB)
+constexpr int LL_LOGITS_LDS = LL_SIDE + 3 * 4096 + 2 * 1024;  // statistics: 3 x 4 x 256 floats, two parities of the rows' own tokens; dz: two parities of 4 x 256 row constants (8 KiB)
 
 // MODE LL_STATS: the statistics alone.  LL_KEEP: and 2^(z c1 - e) of every logit in the operands' type, e = the reference of its row (REF) or of its row and
 // 64-column strip (minus s for fp16's range), which ll_scale_kernel turns into dz once the rows' sums are known: no logit is formed twice.  LL_GRAD: dz from
 // the rows' sums.
 enum { LL_STATS, LL_KEEP, LL_GRAD };
+
+// What ll_rows_kernel leaves of a row for its sparse cells, LL_RK floats.  p = 2^(z c1 - E1) I1 with its weight and 2^s, the same with E2, I2 for the second softmax;
+// of the row's own token X what the OTHER tokens hold, 1 - p and 1 - q (REST2: zero without a list); X; the label's cell where there is no list.
+constexpr int LL_RK = 8;
+enum { RK_E1, RK_I1, RK_E2, RK_I2, RK_REST1, RK_REST2, RK_TOKEN, RK_LABEL };
 // SQ (DUAL at T = 2): e^z is the square of e^(z / T), the references' difference an exact power of two: one exponential a logit (1434 rows, d = 512: 123 -> 110 us).
 template <class T, int MODE, bool DUAL, bool FIX, bool SQ = false, bool REF = false>
 __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
@@ -583,10 +607,11 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
     stage((t) + 2, RB0, b);                                 \
     LL_RUN(1, 0, FIRST);                                    \
   } while (0)
-  // row constants of a dz tile, 256 each: La, Lb, the label's column, its cell
+  // row constants of a tile, 256 each: the rows' references and own tokens; of a dz tile La, Lb, the label's column, its cell
   float* const side = (float*)(smem + LL_SIDE);
   auto row_consts = [&](int t, int id, float (&c)[4]) __attribute__((always_inline)) {
     if (REF && id < 256) c[0] = p.eref[p.row0 + t * BM + id];
+    if (!GRAD && id < 256) c[1] = __int_as_float(p.xtok[p.row0 + t * BM + id]);
     if (GRAD && id < 256) {
       const int i = t * BM + id;
       c[0] = p.La[i];
@@ -594,12 +619,13 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
       c[2] = c[3] = 0.f;
       if (FIX) {
         c[2] = __int_as_float(i < nv ? p.lab[p.row0 + i] : -1);
-        c[3] = i < nv ? __builtin_amdgcn_exp2f(__builtin_fmaf(p.zk[p.row0 + i], p.c1, -c[0])) - p.wlab : 0.f;
+        c[3] = i < nv ? p.rk[i * LL_RK + RK_LABEL] : 0.f;
       }
     }
   };
   auto put_consts = [&](int par, int id, const float (&c)[4]) __attribute__((always_inline)) {
     if (REF && id < 256) side[2048 + par * 256 + id] = c[0];      // (one softmax: the third statistic's place is free)
+    if (!GRAD && id < 256) side[3072 + par * 256 + id] = c[1];
     if (GRAD && id < 256) {
       side[par * 1024 + id] = c[0];
       if (DUAL) side[par * 1024 + 256 + id] = c[1];
@@ -671,6 +697,25 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
               for (int mt = 0; mt < 4; ++mt) acc[ah][mt][b >> 1][b & 1][r] = -INFINITY;
           }
     }
+    float nc[4];                      // the next tile's row constants
+    if (!GRAD && more) row_consts(tm2, et, nc);
+    if (!GRAD) {                      // the rows' own tokens: few strips hold one
+      const int* const own = (const int*)(side + 3072 + par * 256) + wm * 128;
+      const int first = n0 + wn * 64;
+      if (__ballot((unsigned)(own[el] - first) < 64u || (unsigned)(own[64 + el] - first) < 64u)) {
+#pragma unroll
+        for (int ah = 0; ah < 2; ++ah)
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            const int cl = own[ah * 64 + mt * 16 + e15] - first - 4 * eg;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (cl == b * 16 + r) acc[ah][mt][b >> 1][b & 1][r] = -INFINITY;
+          }
+      }
+    }
     if (MODE == LL_STATS) {
       // a el holds 16 of the wave's 64 columns of 8 rows; the row's other lanes are 16 and 32 apart, its other columns in the waves of equal wm
 #pragma unroll
@@ -707,12 +752,12 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
             if (DUAL) side[2048 + wn * 256 + row] = s2;
           }
         }
+      if (more) put_consts(par ^ 1, et, nc);
+      par ^= 1;
     } else if (MODE == LL_KEEP) {
       char* const st = smem + BUF + (wave < 4 ? RA1 : RB1) * REGION + (wave & 3) * 4096;       // this wave's 32 rows x 128 B
       char* const G = (char*)p.G + ((int64_t)(m0 + wm * 128) * p.ldg + tn * BN + wn * 64) * 2;
       float* const strip = p.strip + (int64_t)(tn * 4 + wn) * p.R + m0 + wm * 128;
-      float c[4];
-      if (REF && more) row_consts(tm2, et, c);
 #pragma unroll
       for (int qt = 0; qt < 4; ++qt) {
         const int ah = qt >> 1;
@@ -753,7 +798,7 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
             strip[qt * 32 + rl] = mx;
           }
         }
-        if (REF && qt == 0 && more) put_consts(par ^ 1, et, c);    // (before the first 16-B store: the wait for these loads must not wait for stores)
+        if (qt == 0 && more) put_consts(par ^ 1, et, nc);          // (before the first 16-B store: the wait for these loads must not wait for stores)
         asm volatile("" ::: "memory");       // (other lanes' 8-byte writes and these 16-byte reads: the wave's LDS order is all that is needed, hipcc must keep it)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -851,7 +896,7 @@ __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
   if (FIX && threadIdx.x < 64) {
     const int i = i0 + threadIdx.x;
     lc[threadIdx.x] = i < nv ? p.lab[p.row0 + i] - t0 * BN : -1;
-    lv[threadIdx.x] = i < nv ? __builtin_amdgcn_exp2f(__builtin_fmaf(p.zk[p.row0 + i], p.c1, -p.La[i])) - p.wlab : 0.f;
+    lv[threadIdx.x] = i < nv ? p.rk[i * LL_RK + RK_LABEL] : 0.f;
   }
   __syncthreads();
   const int c = (threadIdx.x & 63) * 8, r0 = threadIdx.x >> 6;
@@ -880,9 +925,9 @@ __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
   }
 }
 
-// REF: the rows whose reference changed are brought to it, in place, and with FIX the labels' cells are cleared.  64 rows x 512 columns a
+// REF: the rows whose reference changed are brought to it, in place.  64 rows x 512 columns a
 // workgroup, a wave per changed row, four rows' loads ahead of the first store.  With few changed rows the launch is all it takes.
-template <class T, bool FIX>
+template <class T>
 __global__ __launch_bounds__(256) void ll_rebase_kernel(const LogitsArgs p) {
   typedef typename T::e E;
   typedef typename T::v8 v8;
@@ -892,11 +937,6 @@ __global__ __launch_bounds__(256) void ll_rebase_kernel(const LogitsArgs p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = i0 + lane;
   const float from = p.eref[p.row0 + i], to = p.efin[i];
   uint64_t m = __ballot(from != to);                        // (no reference, NaN: changed)
-  int lc = -1;
-  if (FIX && i < nv) {
-    lc = p.lab[p.row0 + i] - t0 * BN;
-    if (wave == 0 && lc >= 0 && lc < 2 * BN && !(m >> lane & 1)) ((E*)p.G)[(int64_t)i * p.ldg + t0 * BN + lc] = (E)0.f;
-  }
   const int c = lane * 8, tn = t0 + (c >> 8);
   for (int x = 0; x < wave; ++x) m &= m - 1;                // this wave: every fourth changed row
   const bool in = tn < p.tiles_n;                           // (the other lanes stay: rows' numbers come from all 64)
@@ -921,9 +961,8 @@ __global__ __launch_bounds__(256) void ll_rebase_kernel(const LogitsArgs p) {
       if (r[x] < 0) continue;
       const float ref = ll_strip_ref<T>(mx[x], __shfl(from, r[x], 64), p.c1, p.shift), aim = __shfl(to, r[x], 64);
       const float a = mx[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - aim);      // (a strip past the vocabulary: zeros)
-      const int at = FIX ? __shfl(lc, r[x], 64) - c : -1;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[x][e] = (E)(FIX && at == e ? 0.f : (float)v[x][e] * a);
+      for (int e = 0; e < 8; ++e) v[x][e] = (E)((float)v[x][e] * a);
       if (in) *(v8*)(G + (int64_t)r[x] * p.ldg) = v[x];
     }
   }
@@ -964,22 +1003,58 @@ struct RowArgs {
   float* loss;
   const float* zk; const float* top_vals; const int32_t* top_idx; int64_t ld_top;
   float *La, *Lb, *pk, *row_loss, *packed_loss;
+  const int* xtok; const float* xz; float* rk; float up;      // own tokens (many rows) and their logits; LL_RK floats a row; 2^s
   const float* eref; float *efin, *F, head, shift;     // REF: the rows' references before and behind the logits' pass, their factors
   float* cl;                                    // p - 1 of the label, where dh's and dW's last steps take it
-  int* big_tok; float* big_res; float wlab; int f16;      // (no list, the label's cell in dz) what the cell's rounding loses: see ll_cells_kernel
+  int* big_tok; float* big_res; int f16;        // (no list, the label's cell in dz) what the cell's rounding loses: see ll_cells_kernel
 };
 
-// 16 threads per row; one workgroup of 1024 threads (the few-row path) also takes the mean
+// 16 threads per row; one workgroup of 1024 threads (the few-row path) also takes the mean.
+// A row may be almost certain of a token: p - 1 there is what is left of its gradient, and 1 - p what the OTHER tokens hold.  exp(z - lse) - 1 would have neither the digits
+// of 1 - p (lse is rounded at the logits' size: 1 % off at 1 - p = 1e-4) nor, with z gathered and lse from tiles, the same logit on both sides.  So one token a row, its OWN
+// (the label, or the largest logit among it and the list), is no part of the statistics: its exponential is added here, from the gathered logit, and 1 - p is the others' share.
 template <int NT>
 __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
   constexpr int RB = NT / 16;
+  constexpr bool FEW = NT == 1024;
   __shared__ float sm[3][RB][17];
   __shared__ float all[RB];
+  __shared__ int xt[FEW ? RB : 1];
   const int nv = min(*p.nvalid - p.row0, p.R), i0 = blockIdx.x * RB;
   if (NT == 256 && blockIdx.x == 0) ll_choose_splits(max(nv, 0), p.tiles_d, p.kt, p.splits);
   if (NT == 256 && (nv <= 0 || i0 >= (nv + BM - 1) / BM * BM)) return;
+  const int r_ = threadIdx.x >> 4, q_ = threadIdx.x & 15;
+  float xz = -INFINITY;             // the own token's logit
+  if (FEW) {
+    // few rows: all logits are there, the own token is found here and its tile's others are added up again, without it, in place of the tile's partial sums
+    int tok = -1;
+    if (r_ < nv) {
+      const int lab = p.lab[r_], row = p.order[r_];
+      const float* const z = p.z + (int64_t)r_ * p.ldz;
+      xz = z[lab];
+      tok = lab;
+#pragma unroll 4
+      for (int e = q_; e < p.k; e += 16) {
+        const int t = p.top_idx[row * p.ld_top + e];
+        const bool ok = t >= 0 && t < p.V;
+        const float v = z[ok ? t : lab];
+        if (ok && v > xz) { xz = v; tok = t; }
+      }
+      if (p.k > 0) {                // (labels alone: nothing waits for the logit here)
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+          const float v = __shfl_xor(xz, o, 64);
+          const int t = __shfl_xor(tok, o, 64);
+          if (v > xz || (v == xz && t > tok)) { xz = v; tok = t; }
+        }
+      }
+    }
+    if (q_ == 0) xt[r_] = tok;
+    __syncthreads();
+  }
   {
     const int r = threadIdx.x & (RB - 1), q = threadIdx.x / RB;
+    const int skip = FEW && xt[r] >= 0 ? xt[r] / BN : -1;
     float mx = -INFINITY, s1 = 0.f, s2 = 0.f;
     // sixteen partials a thread in flight, joined with one exponential each
     for (int t0 = q; t0 < p.tiles_n; t0 += 256) {
@@ -991,34 +1066,62 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
         m[x] = p.pm[o];
         a[x] = p.p1[o];
         b[x] = p.dual ? p.p2[o] : 0.f;
-        if (t >= p.tiles_n) m[x] = -INFINITY;
+        if (t >= p.tiles_n || t == skip) { m[x] = -INFINITY; a[x] = b[x] = 0.f; }
       }
       float nm = mx;
 #pragma unroll
       for (int x = 0; x < 16; ++x) nm = fmaxf(nm, m[x]);
       const float n1 = ll_ref(nm, p.c1), n2 = ll_ref(nm, p.c2);
-      s1 = mx == -INFINITY ? 0.f : s1 * __builtin_amdgcn_exp2f(ll_ref(mx, p.c1) - n1);
-      s2 = mx == -INFINITY ? 0.f : s2 * __builtin_amdgcn_exp2f(ll_ref(mx, p.c2) - n2);
+      s1 *= mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mx, p.c1) - n1);      // (a NaN stays one)
+      s2 *= mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mx, p.c2) - n2);
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
-        s1 += m[x] == -INFINITY ? 0.f : a[x] * __builtin_amdgcn_exp2f(ll_ref(m[x], p.c1) - n1);
-        if (p.dual) s2 += m[x] == -INFINITY ? 0.f : b[x] * __builtin_amdgcn_exp2f(ll_ref(m[x], p.c2) - n2);
+        s1 += a[x] * (m[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(m[x], p.c1) - n1));
+        if (p.dual) s2 += b[x] * (m[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(m[x], p.c2) - n2));
       }
       mx = nm;
     }
     sm[0][r][q] = mx; sm[1][r][q] = s1; sm[2][r][q] = s2;
   }
   __syncthreads();
-  const int r = threadIdx.x >> 4, q = threadIdx.x & 15, i = i0 + r;
-  float mx = sm[0][r][q];
-  const float own = mx;
+  const int r = r_, q = q_, i = i0 + r;
+  float mo = sm[0][r][q], s1 = sm[1][r][q], s2 = sm[2][r][q];      // of the others, relative to 2^ref(mo)
+  if (FEW && i < nv) {
+    const int tok = xt[r], c0 = tok / BN * BN + q * 16;
+    const float* const z = p.z + (int64_t)i * p.ldz + c0;
+    float v[16], m = mo;
+#pragma unroll
+    for (int x = 0; x < 16; x += 4) *(f32x4*)&v[x] = *(const f32x4*)(z + x);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      if (c0 + x >= p.V || c0 + x == tok) v[x] = -INFINITY;
+      m = fmaxf(m, v[x]);
+    }
+    const float n1 = m == -INFINITY ? 0.f : ll_ref(m, p.c1), n2 = m == -INFINITY ? 0.f : ll_ref(m, p.c2);
+    s1 *= mo == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mo, p.c1) - n1);
+    s2 *= mo == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mo, p.c2) - n2);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(v[x], p.c1, -n1));
+      if (p.dual) s2 += __builtin_amdgcn_exp2f(__builtin_fmaf(v[x], p.c2, -n2));
+    }
+    mo = m;
+  }
+  if (!FEW && i < nv) xz = p.xz[p.row0 + i];
+  float mx = mo;
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+  const float others = mx;          // the largest logit but the own token's
+  mx = fmaxf(mx, xz);
   const float e1 = ll_ref(mx, p.c1), e2 = ll_ref(mx, p.c2);      // the sums are relative to 2^e1, 2^e2
-  float s1 = own == -INFINITY ? 0.f : sm[1][r][q] * __builtin_amdgcn_exp2f(ll_ref(own, p.c1) - e1);
-  float s2 = own == -INFINITY ? 0.f : sm[2][r][q] * __builtin_amdgcn_exp2f(ll_ref(own, p.c2) - e2);
+  s1 *= mo == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mo, p.c1) - e1);
+  s2 *= mo == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(mo, p.c2) - e2);
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o, 64); s2 += __shfl_xor(s2, o, 64); }
+  const float o1 = s1, o2 = s2;
+  s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(xz, p.c1, -e1));
+  s2 += __builtin_amdgcn_exp2f(__builtin_fmaf(xz, p.c2, -e2));
+  const float rest1 = o1 / s1, rest2 = p.dual ? o2 / s2 : rest1;      // (one softmax: it is the one at T)
   const bool live = i < nv;
   float loss = 0.f;
   if (!live) {                      // padding rows of the last tile: no probability
@@ -1091,13 +1194,20 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
       p.La[i] = l1 - p.lw1;
     }
     if (p.eref) {
-      const float a = p.eref[pi], e = mx * p.c1 <= a + p.head ? a : ll_ref(mx, p.c1) - p.shift;
+      const float a = p.eref[pi], e = others * p.c1 <= a + p.head ? a : ll_ref(others == -INFINITY ? mx : others, p.c1) - p.shift;
       p.efin[i] = e;
       p.F[i] = __builtin_amdgcn_exp2f(e - p.La[i] - p.shift);      // (La is for cells times 2^shift)
-      if (p.cl) p.cl[i] = __builtin_amdgcn_exp2f(p.zk[pi] * p.c1 - l1) - 1.f;
+      if (p.cl) p.cl[i] = -rest1;
+    }
+    {
+      const float i1 = (p.dual || p.k == 0 ? p.w1 : (p.soft_only ? 0.f : p.w1) + (soft ? p.w2 : 0.f)) * p.up / s1;
+      f32x4* const rk = (f32x4*)(p.rk + (int64_t)i * LL_RK);
+      rk[0] = f32x4{e1, i1, e2, p.dual && soft ? p.w2 * p.up / s2 : 0.f};
+      const int own = rest1 < 0.5f || rest2 < 0.5f ? (FEW ? xt[r] : p.xtok[pi]) : -1;      // (a row that is certain of nothing: p itself has the digits)
+      rk[1] = f32x4{rest1, soft ? rest2 : 0.f, __int_as_float(own), -p.w1 * p.up * rest1};
     }
     if (p.big_tok) {
-      const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(p.zk[pi], p.c1, -p.La[i])) - p.wlab;
+      const float v = -p.w1 * p.up * rest1;
       p.big_tok[2 * pi] = p.lab[pi];
       p.big_tok[2 * pi + 1] = -1;
       p.big_res[2 * pi] = v - (p.f16 ? (float)(half_t)v : (float)(__bf16)v);
@@ -1136,6 +1246,14 @@ __global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__
   ll_mean<1024>(packed_loss, *nvalid, loss);
 }
 
+// a cell of dz at a token that the label or the list names (soft: the list's probability of it, or of the row's own token that of all others)
+__device__ __forceinline__ float ll_sparse_cell(const float* rk, float z, float c1, float c2, float w1s, float w2s, float soft, bool own, bool label) {
+  if (own) return w2s * (soft - rk[RK_REST2]) + (label ? -w1s * rk[RK_REST1] : w1s * (1.f - rk[RK_REST1]));
+  float v = __builtin_amdgcn_exp2f(__builtin_fmaf(z, c1, -rk[RK_E1])) * rk[RK_I1];
+  if (rk[RK_I2] > 0.f) v = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(z, c2, -rk[RK_E2])), rk[RK_I2], v);
+  return v - w2s * soft - (label ? w1s : 0.f);
+}
+
 // the sparse cells of dz in one piece: one wave per row, each token written once whatever number of entries name it.
 // A row's gradient is mostly its one or two largest cells, whose rounding would be an error of all of it (1.5 times the result's own where few rows average it out):
 // what the two largest lose goes to big_tok / big_res, and dh's and dW's last steps add it in fp32 (fp16, 1434 rows with lists, dh and dW: 2.6e-4 -> 2.1e-4 off, the
@@ -1143,7 +1261,7 @@ __global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__
 template <class E>
 __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ nvalid, int row0, int R, const int* __restrict__ order, const int* __restrict__ lab,
                                                        const int32_t* __restrict__ top_idx, int64_t ld_top, int k, const float* __restrict__ zk,
-                                                       const float* __restrict__ pk, const float* __restrict__ La, const float* __restrict__ Lb, float c1, float c2,
+                                                       const float* __restrict__ pk, const float* __restrict__ La, const float* __restrict__ rk, float c1, float c2,
                                                        float w1s, float w2s, int col0, int cols, int V, E* __restrict__ G, int ldg, const float* __restrict__ efin,
                                                        int* __restrict__ big_tok, float* __restrict__ big_res) {
   __shared__ __attribute__((aligned(16))) int sidx[4][LL_MAX_K + 4];
@@ -1161,30 +1279,29 @@ __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ n
   }
   __syncthreads();
   if (!live) return;
-  const float la = La[i], lb = Lb ? Lb[i] : INFINITY;
   // (efin: cells relative to the row's factor; one of zero leaves none)
-  const float from = efin ? efin[i] : la, up = efin ? (la < INFINITY ? __builtin_amdgcn_exp2f(la - efin[i]) : 0.f) : 1.f;
+  const float la = La[i], up = efin ? (la < INFINITY ? __builtin_amdgcn_exp2f(la - efin[i]) : 0.f) : 1.f;
+  rk += (int64_t)i * LL_RK;
+  const int own = __float_as_int(rk[RK_TOKEN]);
   float m1 = 0.f, m2 = 0.f, r1 = 0.f, r2 = 0.f;             // this lane's two largest
   int t1 = -1, t2 = -1;
   for (int e = lane; e <= k; e += 64) {
     const int t = sidx[wave][e], c = t - col0;
     const bool in = c >= 0 && c < cols;
     if (t < 0 || (!in && col0 > 0)) continue;               // (the first piece's launch looks at all of a row's cells)
+    // the list's probability of this token, or of the own one that of all others: w2 (q - t) = w2 ((1 - t) - (1 - q)) keeps its digits where both are close to 1
     float soft = 0.f;
     bool first = true;
+    const bool self = t == own;
 #pragma unroll 4
     for (int o = 0; o < k; o += 4) {                        // (sp[k] is zero, and entry k comes no earlier than any)
       const int4 s = *(const int4*)&sidx[wave][o];
       const f32x4 q = *(const f32x4*)&sp[wave][o];
-      soft += (s.x == t ? q[0] : 0.f) + (s.y == t ? q[1] : 0.f) + (s.z == t ? q[2] : 0.f) + (s.w == t ? q[3] : 0.f);
+      soft += ((s.x == t) != self ? q[0] : 0.f) + ((s.y == t) != self ? q[1] : 0.f) + ((s.z == t) != self ? q[2] : 0.f) + ((s.w == t) != self ? q[3] : 0.f);
       first = first && !((s.x == t && o < e) || (s.y == t && o + 1 < e) || (s.z == t && o + 2 < e) || (s.w == t && o + 3 < e));
     }
     if (!first) continue;                                   // an earlier entry of the list names the same token: that one writes
-    const float z = zk[(int64_t)pi * (k + 1) + e];
-    float v = __builtin_amdgcn_exp2f(z * c1 - from);
-    if (Lb) v += __builtin_amdgcn_exp2f(z * c2 - lb);
-    v -= w2s * up * soft;
-    if (t == lab[pi]) v -= w1s * up;
+    const float v = up * ll_sparse_cell(rk, zk[(int64_t)pi * (k + 1) + e], c1, c2, w1s, w2s, soft, self, t == lab[pi]);
     if (in) G[(int64_t)i * ldg + c] = (E)v;
     const float m = fabsf(v), res = v - (float)(E)v;
     if (m > m1) { m2 = m1; t2 = t1; r2 = r1; m1 = m; t1 = t; r1 = res; }
@@ -1533,7 +1650,7 @@ struct FewArgs {
   float *pm, *p1, *p2; int R;       // (tiles_n, R)
   int *order, *inv, *lab, *nvalid; float* row_loss;
   // gradient
-  const float *La, *Lb, *pk; const int32_t* top_idx; int64_t ld_top; int k;
+  const float *La, *Lb, *pk, *rk; const int32_t* top_idx; int64_t ld_top; int k;
   float w1s, w2s, unscale;
   const float* loss_scale;
   float* slab;                      // (tiles_n, 16 MT, d)
@@ -1657,9 +1774,8 @@ __global__ __launch_bounds__(512) void ll_few_logits_kernel(const FewArgs p) {
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
       const float m = sm[0][w][tid];
-      if (m == -INFINITY) continue;
-      s1 += sm[1][w][tid] * __builtin_amdgcn_exp2f(ll_ref(m, p.c1) - ll_ref(mx, p.c1));
-      if (DUAL) s2 += sm[2][w][tid] * __builtin_amdgcn_exp2f(ll_ref(m, p.c2) - ll_ref(mx, p.c2));
+      s1 += sm[1][w][tid] * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(m, p.c1) - ll_ref(mx, p.c1)));      // (a NaN stays one)
+      if (DUAL) s2 += sm[2][w][tid] * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ll_ref(m, p.c2) - ll_ref(mx, p.c2)));
     }
     const int64_t o = (int64_t)blockIdx.x * p.R + tid;
     p.pm[o] = mx;
@@ -1748,15 +1864,16 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
     if (t < n0 || t >= n0 + 256 || t >= p.V) continue;
     float soft = 0.f;
     bool first = true;
+    const float* const rk = p.rk + r * LL_RK;
+    const bool self = t == __float_as_int(rk[RK_TOKEN]);
 #pragma unroll 8
-    for (int o = 0; o < p.k; ++o)
-      if (p.top_idx[row * p.ld_top + o] == t) { soft += p.pk[(int64_t)r * p.k + o]; first = first && o >= e; }
+    for (int o = 0; o < p.k; ++o) {
+      const bool same = p.top_idx[row * p.ld_top + o] == t;
+      if (same != self) soft += p.pk[(int64_t)r * p.k + o];
+      first = first && !(same && o < e);
+    }
     if (!first) continue;
-    const float z = p.z[(int64_t)r * p.ldz + t];
-    float v = __builtin_amdgcn_exp2f(z * p.c1 - p.La[r]);
-    if (DUAL) v += __builtin_amdgcn_exp2f(z * p.c2 - p.Lb[r]);
-    v -= p.w2s * soft;
-    if (t == lab) v -= p.w1s;
+    const float v = ll_sparse_cell(rk, p.z[(int64_t)r * p.ldz + t], p.c1, p.c2, p.w1s, p.w2s, soft, self, t == lab);
     *(E*)(gs_ + r * FG_LD + (t - n0) * 2) = (E)v;
     if (twice) *(E*)(gs_ + (r + HALF) * FG_LD + (t - n0) * 2) = (E)(v - (float)(E)v);
   }
@@ -1886,7 +2003,7 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
 struct Plan {
   int few;                                    // 0, or MT of the few-row path
   int keep, ref, R, Rc, dp, dt, tiles_n, piece_tiles, pieces, pairs;      // keep: LL_KEEP, in chunks of Rc rows (else Rc = R, in pieces of the vocabulary)
-  size_t splits_at, order, inv, lab, hp, hT, zk, pk, pm, p1, p2, strip, La, Lb, eref, efin, F, big, ploss, G, slab, total;
+  size_t splits_at, order, inv, lab, xtok, xz, hp, hT, zk, pk, pm, p1, p2, strip, La, Lb, rk, eref, efin, F, big, ploss, G, slab, total;
 };
 
 bool dual_of(const ns_linear_ce_desc* d) { return d->k > 0 && d->alpha > 0.f && d->alpha < 1.f && d->temperature != 1.f; }
@@ -1934,9 +2051,11 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   p.order = take((size_t)d->rows * 4);
   p.inv = take((size_t)d->rows * 4);
   p.lab = take((size_t)d->rows * 4);
+  p.xtok = p.few ? 0 : take((size_t)p.R * 4);
   p.hp = p.few ? 0 : take((size_t)p.R * p.dp * 2);
   p.hT = d->dw && !p.few ? take((size_t)p.dt * p.R * 2) : 0;
   p.zk = take(p.few ? (size_t)16 * p.few * p.tiles_n * BN * 4 : (size_t)p.R * (d->k + 1) * 4);       // (few rows: all logits)
+  p.xz = p.few ? 0 : d->k == 0 ? p.zk : take((size_t)p.R * 4);
   p.pk = take((size_t)p.R * d->k * 4);
   p.pm = take((size_t)p.tiles_n * p.Rc * 4);
   p.p1 = take((size_t)p.tiles_n * p.Rc * 4);
@@ -1944,6 +2063,7 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   p.strip = p.keep && !p.few ? take((size_t)p.tiles_n * 4 * p.Rc * 4) : 0;
   p.La = take((size_t)p.Rc * 4);
   p.Lb = take((size_t)p.Rc * 4);
+  p.rk = take((size_t)p.Rc * LL_RK * 4);
   p.eref = p.ref ? take((size_t)p.R * 4) : 0;
   p.efin = p.ref ? take((size_t)p.Rc * 4) : 0;
   p.F = p.ref ? take((size_t)p.Rc * 4) : 0;
@@ -1990,7 +2110,8 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   char* const ws = (char*)d->workspace;
   int *order = (int*)(ws + p.order), *inv = (int*)(ws + p.inv), *lab = (int*)(ws + p.lab);
   int* const splits = (int*)(ws + p.splits_at);
-  float *zk = (float*)(ws + p.zk), *pk = (float*)(ws + p.pk), *La = (float*)(ws + p.La), *Lb = (float*)(ws + p.Lb), *ploss = (float*)(ws + p.ploss);
+  float *zk = (float*)(ws + p.zk), *pk = (float*)(ws + p.pk), *La = (float*)(ws + p.La), *Lb = (float*)(ws + p.Lb), *ploss = (float*)(ws + p.ploss), *rk = (float*)(ws + p.rk), *xz = (float*)(ws + p.xz);
+  int* const xtok = (int*)(ws + p.xtok);
   float *const eref = p.ref ? (float*)(ws + p.eref) : nullptr, *const efin = p.ref ? (float*)(ws + p.efin) : nullptr, *const F = p.ref ? (float*)(ws + p.F) : nullptr;
   const bool apart = p.ref && d->k == 0;                           // dz without the labels' cells: dh's last step adds their rows of W, dW's their rows of h
   int* const big_tok = p.big ? (int*)(ws + p.big) : nullptr;
@@ -2019,24 +2140,24 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   r.lw1 = (d->k > 0 && !dual) ? (float)s : log2f(w1) + (float)s;
   r.lw2 = log2f(w2) + (float)s;
   r.dual = dual; r.soft_only = soft_only; r.nvalid = d->nvalid_dev; r.order = order; r.lab = lab; r.zk = zk; r.top_vals = d->top_vals; r.top_idx = d->top_idx;
-  r.eref = eref; r.efin = efin; r.F = F; r.head = T::HEAD; r.shift = (float)s; r.cl = apart ? Lb : nullptr; r.wlab = w1 * up; r.f16 = d->dtype == NS_F16; r.big_tok = d->k == 0 ? big_tok : nullptr; r.big_res = big_res;      // (one softmax: Lb is free)
- 
+  r.eref = eref; r.efin = efin; r.F = F; r.head = T::HEAD; r.shift = (float)s; r.cl = apart ? Lb : nullptr; r.f16 = d->dtype == NS_F16; r.big_tok = d->k == 0 ? big_tok : nullptr; r.big_res = big_res;      // (one softmax: Lb is free)
+  r.xtok = xtok; r.xz = xz; r.rk = rk; r.up = up;
   r.ld_top = d->ld_top; r.La = La; r.Lb = dual ? Lb : nullptr; r.pk = pk; r.row_loss = d->row_loss; r.packed_loss = ploss; r.loss = d->loss_dev;
   if (p.few) {
     FewArgs f = {};
     f.h = d->h; f.ldh = d->ldh; f.w = d->w; f.ldw = d->ldw; f.labels = d->labels; f.rows = d->rows; f.d = d->d; f.V = d->vocab; f.tiles_n = p.tiles_n;
     f.c1 = c1; f.c2 = c2; f.z = zk; f.ldz = (int64_t)p.tiles_n * BN; f.pm = (float*)(ws + p.pm); f.p1 = (float*)(ws + p.p1); f.p2 = (float*)(ws + p.p2); f.R = p.R;
     f.order = order; f.inv = inv; f.lab = lab; f.nvalid = d->nvalid_dev; f.row_loss = d->row_loss;
-    f.La = La; f.Lb = dual ? Lb : nullptr; f.pk = pk; f.top_idx = d->top_idx; f.ld_top = d->ld_top; f.k = d->k; f.w1s = w1 * up; f.w2s = w2 * up; f.unscale = 1.f / up;
+    f.La = La; f.Lb = dual ? Lb : nullptr; f.pk = pk; f.rk = rk; f.top_idx = d->top_idx; f.ld_top = d->ld_top; f.k = d->k; f.w1s = w1 * up; f.w2s = w2 * up; f.unscale = 1.f / up;
     f.loss_scale = d->loss_scale_dev; f.slab = (float*)(ws + p.slab); f.dw = d->dw; f.lddw = d->lddw; f.f32 = d->dw_f32; f.add = d->dw_add; f.dh = d->dh != nullptr;
     r.z = zk; r.ldz = f.ldz;
     return p.few == 1 ? few_launch<T, 1>(d, f, r, dual, st) : p.few == 2 ? few_launch<T, 2>(d, f, r, dual, st) : few_launch<T, 4>(d, f, r, dual, st);
   }
   hipLaunchKernelGGL(ll_compact_kernel, dim3(1), dim3(1024), 0, st, d->labels, d->rows, d->vocab, order, inv, lab, d->row_loss, d->nvalid_dev);
-  hipLaunchKernelGGL(ll_pack_kernel<T>, dim3(p.R / 4), dim3(256), 0, st, d->h, d->ldh, d->w, d->ldw, d->d, p.dp, order, lab, d->k, d->nvalid_dev, (void*)(ws + p.hp), zk, c1, eref);
+  hipLaunchKernelGGL(ll_pack_kernel<T>, dim3(p.R / 4), dim3(256), 0, st, d->h, d->ldh, d->w, d->ldw, d->d, p.dp, order, lab, d->k, d->nvalid_dev, (void*)(ws + p.hp), zk, c1, eref, xtok);
   if (d->k > 0)
     hipLaunchKernelGGL(ll_gather_kernel<T>, dim3(p.R), dim3(256), 0, st, (const void*)(ws + p.hp), p.dp, d->w, d->ldw, d->d, d->vocab, order, lab, d->top_idx, d->ld_top, d->k,
-                       d->nvalid_dev, zk, c1, eref);
+                       d->nvalid_dev, zk, c1, eref, xtok, xz);
   auto transpose = [&] {
     hipLaunchKernelGGL(ll_transpose_kernel, dim3(p.R / 64, p.dp / 64), dim3(256), 0, st, (const uint16_t*)(ws + p.hp), p.dp, d->nvalid_dev, (uint16_t*)(ws + p.hT), p.R, F);
   };
@@ -2045,8 +2166,8 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   a.hp = ws + p.hp; a.w = d->w; a.ldw = d->ldw; a.dp = p.dp; a.d = d->d; a.V = d->vocab; a.col0 = 0; a.tiles_n = p.tiles_n; a.R = p.Rc; a.nvalid = d->nvalid_dev;
   a.c1 = c1; a.c2 = c2; a.T = T_;
   a.pm = (float*)(ws + p.pm); a.p1 = (float*)(ws + p.p1); a.p2 = (float*)(ws + p.p2);
-  a.La = La; a.Lb = Lb; a.G = ws + p.G; a.ldg = p.piece_tiles * BN; a.lab = lab; a.zk = zk; a.wlab = w1 * up;
-  a.eref = eref; a.efin = efin;
+  a.La = La; a.Lb = Lb; a.G = ws + p.G; a.ldg = p.piece_tiles * BN; a.lab = lab; a.rk = rk;
+  a.eref = eref; a.efin = efin; a.xtok = xtok;
   a.strip = (float*)(ws + p.strip); a.shift = (float)s; a.unshift = 1.f / up;
   r.R = p.Rc; r.tiles_d = (d->d + BN - 1) / BN; r.kt = p.piece_tiles * (BN / BK); r.splits = splits;
   auto grid_of = [&](int tiles_n) { const int64_t t = (int64_t)(p.Rc / BM) * tiles_n; return dim3((unsigned)(t < 256 ? t : 256)); };
@@ -2071,8 +2192,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
       const dim3 grid = grid_of(a.tiles_n);
       if (p.keep) {
         const dim3 sg((a.tiles_n + 1) / 2, p.Rc / 64);
-        if (p.ref && d->k == 0) hipLaunchKernelGGL((ll_rebase_kernel<T, true>), sg, dim3(256), 0, st, a);
-        else if (p.ref) hipLaunchKernelGGL((ll_rebase_kernel<tbf16, false>), sg, dim3(256), 0, st, a);
+        if (p.ref) hipLaunchKernelGGL(ll_rebase_kernel<T>, sg, dim3(256), 0, st, a);
         else if (dual) hipLaunchKernelGGL((ll_scale_kernel<T, false, true>), sg, dim3(256), 0, st, a);
         else if (d->k == 0) hipLaunchKernelGGL((ll_scale_kernel<tf16, true, false>), sg, dim3(256), 0, st, a);
         else hipLaunchKernelGGL((ll_scale_kernel<T, false, false>), sg, dim3(256), 0, st, a);
@@ -2081,7 +2201,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
       else hipLaunchKernelGGL((ll_logits_kernel<T, LL_GRAD, false, false>), grid, dim3(NTH), LL_LOGITS_LDS, st, a);
       if (d->k > 0)
         hipLaunchKernelGGL(ll_cells_kernel<E>, dim3(p.Rc / 4), dim3(256), 0, st, d->nvalid_dev, row0, p.Rc, order, lab, d->top_idx, d->ld_top, d->k, zk, pk, La,
-                           dual ? Lb : nullptr, a.c1, a.c2, w1 * up, w2 * up, a.col0, a.tiles_n * BN, d->vocab, (E*)a.G, a.ldg, efin, big_tok, big_res);
+                           rk, a.c1, a.c2, w1 * up, w2 * up, a.col0, a.tiles_n * BN, d->vocab, (E*)a.G, a.ldg, efin, big_tok, big_res);
       if (d->dh) {
         DhArgs q = {};
         q.G = a.G; q.w = d->w; q.ldw = d->ldw; q.ldg = a.ldg; q.col0 = a.col0; q.cols = a.tiles_n * BN; q.V = d->vocab; q.d = d->d; q.row0 = row0; q.R = p.Rc;
