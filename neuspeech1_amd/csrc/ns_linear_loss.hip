@@ -55,13 +55,13 @@ typedef unsigned short ushort4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v lds_s4;
 
 struct tf16 {
-  static constexpr float HEAD = 15.f, BELOW = 6.f;       // (see ll_label_ref)
+  static constexpr float HEAD = 15.f, BELOW = 6.f, LOW = -14.f;       // (see ll_label_ref)
   typedef half_t e;
   typedef half8 v8;
   static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 struct tbf16 {
-  static constexpr float HEAD = 30.f, BELOW = 0.f;
+  static constexpr float HEAD = 30.f, BELOW = 0.f, LOW = -INFINITY;
   typedef __bf16 e;
   typedef bf8 v8;
   static __device__ __forceinline__ f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -111,12 +111,15 @@ __device__ __forceinline__ float ll_sum4(float v) {
 __device__ __forceinline__ float ll_ref(float mx, float c) { return ceilf(mx * c); }
 
 // LL_KEEP with one reference for a whole row (REF: one softmax).  The label's logit is known before the pass: its exponent (less BELOW, which moves fp16's range)
-// is the row's reference as long as no logit exceeds it by more than 2^HEAD.  A 64-column strip that does exceed it takes its own maximum, and its row is brought to
+// is the row's reference as long as no logit but the label's exceeds it by more than 2^HEAD.  A 64-column strip that does exceed it takes its own maximum, and its row is brought to
 // one reference afterwards.  So dz = x F with ONE factor per row, which dh's last step and h's transposed copy take in, and the pass over dz falls away
-// (bf16, 8192 rows, d = 1280: 2.93 -> 2.72 ms; 1844 rows, d = 512: 425 -> 382 us; fp16, 1229 rows, dh alone: 218 -> 187 us, and 227 where
-// every row's reference changes).
+// (bf16, 8192 rows, d = 1280: 2.93 -> 2.72 ms; 1844 rows, d = 512: 425 -> 382 us; fp16, 1229 rows, dh alone: 218 -> 173 us, and 204 where
+// every row's reference changes, as with labels that are almost certain).
 //   bfloat16   has the exponents for x and for the cells of a list, up to 2^47; what lies 2^-126 below the label counts for nothing.
-//   float16    has room for x alone, from 2^-30 of the label's to 2^9 times it, and none for h's copy with the factors: dh alone, and no list.
+//   float16    has room for x alone, up to 2^9 times the label's, and none for h's copy with the factors: dh alone, and no list.  Below 2^LOW its numbers lose digits, by at
+//              most 2^-25 each: where the label is almost certain, all that is left of the row's gradient lies there.  So a strip is kept relative to the label only if its
+//              largest x is at least 64 2^LOW, else to its own maximum (either way the strip as a whole is within 2^-11 of itself), and a row of which the V others do not hold
+//              V 2^LOW together goes to the reference of their largest, as one whose largest exceeds 2^HEAD does (2^-39 V of what they hold, at most, is lost there).
 // Without a list the label's x is zero (it is the row's own token), and dh's and dW's last steps add (p - 1) W[label] and (p - 1) h in fp32: a rounded factor or cell would be an error of all of
 // a row's gradient, and subtracting W[label] from a product that holds p W[label] would leave p's rounding of 1 - p.
 // The gathered logit and the tile's differ by the order of their sums, each within (d + 4) u sum |h w| of the exact one: where that could exceed 4 the row gets no
@@ -125,7 +128,7 @@ template <class T> __device__ __forceinline__ float ll_label_ref(float z, float 
   return (float)(d + 4) * 5.9604645e-8f * mass * c <= 4.f ? ll_ref(z, c) - T::BELOW : NAN;
 }
 template <class T> __device__ __forceinline__ float ll_strip_ref(float mx, float eref, float c, float shift) {
-  return mx * c <= eref + T::HEAD ? eref : mx == -INFINITY ? 0.f : ll_ref(mx, c) - shift;
+  return mx * c <= eref + T::HEAD && mx * c >= eref + T::LOW + 6.f ? eref : mx == -INFINITY ? 0.f : ll_ref(mx, c) - shift;
 }
 
 #define LL_BARRIER()                            \
@@ -925,45 +928,54 @@ __global__ __launch_bounds__(256) void ll_scale_kernel(const LogitsArgs p) {
   }
 }
 
-// REF: the rows whose reference changed are brought to it, in place.  64 rows x 512 columns a
-// workgroup, a wave per changed row, four rows' loads ahead of the first store.  With few changed rows the launch is all it takes.
+// REF: the strips that are not kept relative to their row's reference are brought to it, in place.  64 rows x 512 columns a workgroup, a wave per row with such a strip, four
+// rows' loads ahead of the first store.  With few of them the launch is all it takes.
 template <class T>
 __global__ __launch_bounds__(256) void ll_rebase_kernel(const LogitsArgs p) {
   typedef typename T::e E;
   typedef typename T::v8 v8;
+  __shared__ float f[8][64];
+  __shared__ uint64_t hit[4];
   const int nv = min(*p.nvalid - p.row0, p.R);
   const int i0 = blockIdx.y * 64, t0 = blockIdx.x * 2;
   if (nv <= 0 || i0 >= (nv + BM - 1) / BM * BM) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = i0 + lane;
   const float from = p.eref[p.row0 + i], to = p.efin[i];
-  uint64_t m = __ballot(from != to);                        // (no reference, NaN: changed)
-  const int c = lane * 8, tn = t0 + (c >> 8);
-  for (int x = 0; x < wave; ++x) m &= m - 1;                // this wave: every fourth changed row
-  const bool in = tn < p.tiles_n;                           // (the other lanes stay: rows' numbers come from all 64)
+  bool any = false;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int st = wave * 2 + x;
+    const float mx = t0 * 4 + st < p.tiles_n * 4 ? p.strip[(int64_t)(t0 * 4 + st) * p.R + i] : -INFINITY;
+    const float ref = ll_strip_ref<T>(mx, from, p.c1, p.shift);
+    const bool moved = mx > -INFINITY && ref != to;          // (a strip past the vocabulary: zeros)
+    f[st][lane] = moved ? __builtin_amdgcn_exp2f(ref - to) : 1.f;
+    any |= moved;
+  }
+  const uint64_t mine = __ballot(any);
+  if (lane == 0) hit[wave] = mine;
+  __syncthreads();
+  uint64_t m = hit[0] | hit[1] | hit[2] | hit[3];
+  const int c = lane * 8;
+  for (int x = 0; x < wave; ++x) m &= m - 1;                // this wave: every fourth of these rows
   E* const G = (E*)p.G + (int64_t)i0 * p.ldg + t0 * BN + c;
-  const float* const strip = p.strip + (int64_t)(t0 * 4 + (c >> 6)) * p.R + i0;
   while (m) {
     int r[4];
     v8 v[4];
-    float mx[4];
+    float a[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       r[x] = m ? __builtin_ctzll(m) : -1;
-      if (r[x] >= 0 && in) {
-        v[x] = *(const v8*)(G + (int64_t)r[x] * p.ldg);
-        mx[x] = strip[r[x]];
-      }
+      a[x] = r[x] >= 0 ? f[lane >> 3][r[x]] : 1.f;
+      if (a[x] != 1.f) v[x] = *(const v8*)(G + (int64_t)r[x] * p.ldg);
 #pragma unroll
       for (int b = 0; b < 4; ++b) m &= m - 1;
     }
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      if (r[x] < 0) continue;
-      const float ref = ll_strip_ref<T>(mx[x], __shfl(from, r[x], 64), p.c1, p.shift), aim = __shfl(to, r[x], 64);
-      const float a = mx[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - aim);      // (a strip past the vocabulary: zeros)
+      if (a[x] == 1.f) continue;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[x][e] = (E)((float)v[x][e] * a);
-      if (in) *(v8*)(G + (int64_t)r[x] * p.ldg) = v[x];
+      for (int e = 0; e < 8; ++e) v[x][e] = (E)((float)v[x][e] * a[x]);
+      *(v8*)(G + (int64_t)r[x] * p.ldg) = v[x];
     }
   }
 }
@@ -1004,7 +1016,7 @@ struct RowArgs {
   const float* zk; const float* top_vals; const int32_t* top_idx; int64_t ld_top;
   float *La, *Lb, *pk, *row_loss, *packed_loss;
   const int* xtok; const float* xz; float* rk; float up;      // own tokens (many rows) and their logits; LL_RK floats a row; 2^s
-  const float* eref; float *efin, *F, head, shift;     // REF: the rows' references before and behind the logits' pass, their factors
+  const float* eref; float *efin, *F, head, low, shift;     // REF: the rows' references before and behind the logits' pass, their factors
   float* cl;                                    // p - 1 of the label, where dh's and dW's last steps take it
   int* big_tok; float* big_res; int f16;        // (no list, the label's cell in dz) what the cell's rounding loses: see ll_cells_kernel
 };
@@ -1194,7 +1206,9 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
       p.La[i] = l1 - p.lw1;
     }
     if (p.eref) {
-      const float a = p.eref[pi], e = others * p.c1 <= a + p.head ? a : ll_ref(others == -INFINITY ? mx : others, p.c1) - p.shift;
+      const float a = p.eref[pi];
+      const bool keeps = others * p.c1 <= a + p.head && log2f(o1) + e1 >= a + p.low;
+      const float e = keeps ? a : ll_ref(others == -INFINITY ? mx : others, p.c1) - p.shift;
       p.efin[i] = e;
       p.F[i] = __builtin_amdgcn_exp2f(e - p.La[i] - p.shift);      // (La is for cells times 2^shift)
       if (p.cl) p.cl[i] = -rest1;
@@ -2140,7 +2154,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   r.lw1 = (d->k > 0 && !dual) ? (float)s : log2f(w1) + (float)s;
   r.lw2 = log2f(w2) + (float)s;
   r.dual = dual; r.soft_only = soft_only; r.nvalid = d->nvalid_dev; r.order = order; r.lab = lab; r.zk = zk; r.top_vals = d->top_vals; r.top_idx = d->top_idx;
-  r.eref = eref; r.efin = efin; r.F = F; r.head = T::HEAD; r.shift = (float)s; r.cl = apart ? Lb : nullptr; r.f16 = d->dtype == NS_F16; r.big_tok = d->k == 0 ? big_tok : nullptr; r.big_res = big_res;      // (one softmax: Lb is free)
+  r.eref = eref; r.efin = efin; r.F = F; r.head = T::HEAD; r.low = log2f((float)d->vocab) + T::LOW; r.shift = (float)s; r.cl = apart ? Lb : nullptr; r.f16 = d->dtype == NS_F16; r.big_tok = d->k == 0 ? big_tok : nullptr; r.big_res = big_res;      // (one softmax: Lb is free)
   r.xtok = xtok; r.xz = xz; r.rk = rk; r.up = up;
   r.ld_top = d->ld_top; r.La = La; r.Lb = dual ? Lb : nullptr; r.pk = pk; r.row_loss = d->row_loss; r.packed_loss = ploss; r.loss = d->loss_dev;
   if (p.few) {

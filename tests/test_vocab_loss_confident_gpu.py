@@ -16,9 +16,9 @@ def ops():
     return o
 
 
-def make_confident(dev, rows, d, v, dtype, seed, common=0.3, low=0.0):
+def make_confident(dev, rows, d, v, dtype, seed, common=0.3, low=0.0, rival=0.0):
     """hidden states along their label's row of the head, so that 1 - p runs from about a half down to 1e-7 over the rows; the head has a common component, so that the tail of
-    a row's distribution does not average out"""
+    a row's distribution does not average out.  rival: another token's row of the head joins in by this much, and 1 - p without it runs over that range"""
     g = gen(seed, dev)
     w = torch.randn(v, d, generator=g, device=dev) + common * torch.randn(1, d, generator=g, device=dev)
     w = (w * 2.0 * d ** -0.5).to(dtype)
@@ -27,7 +27,7 @@ def make_confident(dev, rows, d, v, dtype, seed, common=0.3, low=0.0):
     if low:
         h[:, 0], w[:, 0] = 8.0, low / 8.0
     wd, hd = w.double(), h.double()
-    along = wd[labels].clone()
+    along = wd[labels] + rival * wd[(labels + v // 2) % v]
     if low:
         along[:, 0] = 0.0
     want = torch.logspace(-0.3, -7.0, rows, dtype=torch.float64, device=dev)
@@ -36,7 +36,10 @@ def make_confident(dev, rows, d, v, dtype, seed, common=0.3, low=0.0):
     for _ in range(40):
         mid = (lo + hi) / 2
         z = base + mid * step
-        e = torch.exp(z - z.gather(1, labels.unsqueeze(1))).scatter(1, labels.unsqueeze(1), 0.0).sum(1)
+        e = torch.exp(z - z.gather(1, labels.unsqueeze(1))).scatter(1, labels.unsqueeze(1), 0.0)
+        if rival:
+            e = e.scatter(1, ((labels + v // 2) % v).unsqueeze(1), 0.0)
+        e = e.sum(1)
         more = (e / (1 + e) > want).unsqueeze(1)
         lo, hi = torch.where(more, mid, lo), torch.where(more, hi, mid)
     return (hd + hi * along).to(dtype), w, labels
@@ -52,7 +55,7 @@ def confident_lists(dev, rows, v, k, labels, seed, other):
     return tv.contiguous(), ti.int().contiguous()
 
 
-def check_confident(ops, dev, h, w, labels, grad, lists=(None, None), temp=1.0, alpha=0.0, dw_dtype=None, scale=2.0 ** 19, parts=1, first=0):
+def check_confident(ops, dev, h, w, labels, grad, lists=(None, None), temp=1.0, alpha=0.0, dw_dtype=None, scale=2.0 ** 19, parts=1, first=0, certain=True):
     rows = h.shape[0]
     o = outputs(dev, rows)
     got = {}
@@ -64,7 +67,7 @@ def check_confident(ops, dev, h, w, labels, grad, lists=(None, None), temp=1.0, 
     ops.linear_cross_entropy(h, w, labels, loss_scale=torch.tensor([scale], device=dev), **o, **got, **kw)
     dh, dh_tol, dw, dw_tol, left, floor = C.linear(h, w, labels, scale, temp, alpha, *lists, to_label=h.dtype == F16 and grad == "h" and lists[0] is None and rows > 64, dw_dtype=dw_dtype,
                                             parts=parts)
-    if alpha == 0.0:
+    if alpha == 0.0 and certain:
         assert float(left.min()) < 1e-6 and float(left.max()) > 0.05      # (the rows are what they are meant to be)
     if "h" in grad:
         close(got["dh"], dh, dh_tol, "dh")
@@ -79,7 +82,7 @@ def check_confident(ops, dev, h, w, labels, grad, lists=(None, None), temp=1.0, 
         close(got["dweight"], dw, dw_tol, "dw")
 
 
-@pytest.mark.parametrize("dtype,grad", [(F16, "hw"), (BF16, "h"), (BF16, "hw")])
+@pytest.mark.parametrize("dtype,grad", [(F16, "h"), (F16, "hw"), (BF16, "h"), (BF16, "hw")])
 @pytest.mark.parametrize("rows,d,v", [(64, 128, 5000), (40, 512, 5000), (200, 512, 5000), (96, 512, 51865), (300, 128, 1500)])
 @pytest.mark.parametrize("low", [0.0, -100.0])
 def test_confident_labels(ops, dev, dtype, rows, d, v, grad, low):
@@ -127,3 +130,11 @@ def test_confident_beyond_all_rows_of_dz(ops, dev, dtype):
     keep = slice(1, 64)                        # (column 0 is the pad's own)
     close(dh[:, keep], want[:, keep], tol[:, keep], "dh")
     close(dw[:9000, keep], dwant[:, keep], dtol[:, keep], "dw")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,d,v,rival", [(200, 256, 5000, 0.98), (96, 512, 51865, 0.9), (130, 512, 51865, 0.8), (40, 128, 3000, 0.95)])
+def test_two_candidates_and_a_tail_far_below(ops, dev, dtype, rows, d, v, rival):
+    """a rival that holds 2^-1 to 2^-20 of the label, all others far below both"""
+    h, w, labels = make_confident(dev, rows, d, v, dtype, rows + d, rival=rival)
+    check_confident(ops, dev, h, w, labels, "h", scale=2.0 ** 18, certain=False)
