@@ -486,9 +486,9 @@ constexpr int LL_LOGITS_LDS = LL_SIDE + 3 * 4096 + 2 * 1024;  // statistics: 3 x
 enum { LL_STATS, LL_KEEP, LL_GRAD };
 
 // What ll_rows_kernel leaves of a row for its sparse cells, LL_RK floats.  p = 2^(z c1 - E1) I1 with its weight and 2^s, the same with E2, I2 for the second softmax;
-// of the row's own token X what the OTHER tokens hold, 1 - p and 1 - q (REST2: zero without a list); X; the label's cell where there is no list.
+// of the row's own token X what the OTHER tokens hold, 1 - p and 1 - q; X; without a list the label's cell, with one (1 - t) - (1 - q) of X.
 constexpr int LL_RK = 8;
-enum { RK_E1, RK_I1, RK_E2, RK_I2, RK_REST1, RK_REST2, RK_TOKEN, RK_LABEL };
+enum { RK_E1, RK_I1, RK_E2, RK_I2, RK_REST1, RK_REST2, RK_TOKEN, RK_LABEL, RK_SOFT = RK_LABEL };
 // SQ (DUAL at T = 2): e^z is the square of e^(z / T), the references' difference an exact power of two: one exponential a logit (1434 rows, d = 512: 123 -> 110 us).
 template <class T, int MODE, bool DUAL, bool FIX, bool SQ = false, bool REF = false>
 __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
@@ -702,14 +702,16 @@ __global__ __launch_bounds__(NTH) void ll_logits_kernel(const LogitsArgs p) {
     }
     float nc[4];                      // the next tile's row constants
     if (!GRAD && more) row_consts(tm2, et, nc);
-    if (!GRAD) {                      // the rows' own tokens: few strips hold one
+    if (!GRAD) {                      // the rows' own tokens: few strips hold one, but most tiles do, and all waves wait for the one whose strip it is
       const int* const own = (const int*)(side + 3072 + par * 256) + wm * 128;
       const int first = n0 + wn * 64;
-      if (__ballot((unsigned)(own[el] - first) < 64u || (unsigned)(own[64 + el] - first) < 64u)) {
+      const uint64_t hit[2] = {__ballot((unsigned)(own[el] - first) < 64u), __ballot((unsigned)(own[64 + el] - first) < 64u)};
+      if (hit[0] | hit[1]) {
 #pragma unroll
         for (int ah = 0; ah < 2; ++ah)
 #pragma unroll
           for (int mt = 0; mt < 4; ++mt) {
+            if (!(hit[ah] >> mt * 16 & 0xFFFF)) continue;
             const int cl = own[ah * 64 + mt * 16 + e15] - first - 4 * eg;
 #pragma unroll
             for (int b = 0; b < 4; ++b)
@@ -1037,6 +1039,7 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
   if (NT == 256 && (nv <= 0 || i0 >= (nv + BM - 1) / BM * BM)) return;
   const int r_ = threadIdx.x >> 4, q_ = threadIdx.x & 15;
   float xz = -INFINITY;             // the own token's logit
+  if (!FEW && i0 + r_ < nv) xz = p.xz[p.row0 + i0 + r_];
   if (FEW) {
     // few rows: all logits are there, the own token is found here and its tile's others are added up again, without it, in place of the tile's partial sums
     int tok = -1;
@@ -1119,7 +1122,6 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
     }
     mo = m;
   }
-  if (!FEW && i < nv) xz = p.xz[p.row0 + i];
   float mx = mo;
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
@@ -1148,6 +1150,7 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
   const int pi = p.row0 + i, row = p.order[pi];
   auto logit = [&](int e, int tok) __attribute__((always_inline)) { return p.z ? p.z[(int64_t)i * p.ldz + tok] : p.zk[(int64_t)pi * (p.k + 1) + e]; };
   bool soft = false;
+  float soft_rest = 0.f;
   if (p.k > 0) {
     // the teacher's distribution over the entries that name a token; a list without any leaves the hard label alone
     const float* const tv = p.top_vals + row * p.ld_top;
@@ -1174,7 +1177,8 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
     for (int o = 8; o > 0; o >>= 1) ts += __shfl_xor(ts, o, 64);
     const float lt = logf(ts), inv = 1.f / ts;
     const float ls = log2f(p.dual ? s2 : s1);     // (one softmax: it is the one at T)
-    float kl = 0.f;
+    float kl = 0.f, lr = 0.f;
+    const int x = FEW ? xt[r] : p.xtok[pi];
 #pragma unroll 4
     for (int e = q; e < p.k; e += 16) {
       float pr = 0.f;
@@ -1187,10 +1191,11 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
         if (pr > 0.f) kl += pr * ((lp - lt) - (__builtin_fmaf(z, p.c2, -e2) - ls) * LN2);
       }
       p.pk[(int64_t)pi * p.k + e] = pr;
+      lr += t == x ? 0.f : pr;
     }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) kl += __shfl_xor(kl, o, 64);
-    if (soft) loss += p.kd * kl;
+    for (int o = 8; o > 0; o >>= 1) { kl += __shfl_xor(kl, o, 64); lr += __shfl_xor(lr, o, 64); }
+    if (soft) { loss += p.kd * kl; soft_rest = lr - rest2; }
   }
   if (q == 0) {
     if (!p.soft_only) loss -= p.w1 * (__builtin_fmaf(logit(p.k, p.lab[pi]), p.c1, -e1) - log2f(s1)) * LN2;      // (lse - z in units of ln 2)
@@ -1213,12 +1218,12 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
       p.F[i] = __builtin_amdgcn_exp2f(e - p.La[i] - p.shift);      // (La is for cells times 2^shift)
       if (p.cl) p.cl[i] = -rest1;
     }
-    {
+    if (p.rk) {
       const float i1 = (p.dual || p.k == 0 ? p.w1 : (p.soft_only ? 0.f : p.w1) + (soft ? p.w2 : 0.f)) * p.up / s1;
       f32x4* const rk = (f32x4*)(p.rk + (int64_t)i * LL_RK);
       rk[0] = f32x4{e1, i1, e2, p.dual && soft ? p.w2 * p.up / s2 : 0.f};
       const int own = rest1 < 0.5f || rest2 < 0.5f ? (FEW ? xt[r] : p.xtok[pi]) : -1;      // (a row that is certain of nothing: p itself has the digits)
-      rk[1] = f32x4{rest1, soft ? rest2 : 0.f, __int_as_float(own), -p.w1 * p.up * rest1};
+      rk[1] = f32x4{rest1, rest2, __int_as_float(own), p.k == 0 ? -p.w1 * p.up * rest1 : soft_rest};
     }
     if (p.big_tok) {
       const float v = -p.w1 * p.up * rest1;
@@ -1260,9 +1265,9 @@ __global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__
   ll_mean<1024>(packed_loss, *nvalid, loss);
 }
 
-// a cell of dz at a token that the label or the list names (soft: the list's probability of it, or of the row's own token that of all others)
+// a cell of dz at a token that the label or the list names (soft: the list's probability of it; own: the row is certain of it, and p - 1 = -(1 - p), q - t = (1 - t) - (1 - q))
 __device__ __forceinline__ float ll_sparse_cell(const float* rk, float z, float c1, float c2, float w1s, float w2s, float soft, bool own, bool label) {
-  if (own) return w2s * (soft - rk[RK_REST2]) + (label ? -w1s * rk[RK_REST1] : w1s * (1.f - rk[RK_REST1]));
+  if (own) return (label ? -w1s * rk[RK_REST1] : w1s * (1.f - rk[RK_REST1])) + (w2s > 0.f ? w2s * rk[RK_SOFT] : 0.f);
   float v = __builtin_amdgcn_exp2f(__builtin_fmaf(z, c1, -rk[RK_E1])) * rk[RK_I1];
   if (rk[RK_I2] > 0.f) v = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(z, c2, -rk[RK_E2])), rk[RK_I2], v);
   return v - w2s * soft - (label ? w1s : 0.f);
@@ -1303,19 +1308,17 @@ __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ n
     const int t = sidx[wave][e], c = t - col0;
     const bool in = c >= 0 && c < cols;
     if (t < 0 || (!in && col0 > 0)) continue;               // (the first piece's launch looks at all of a row's cells)
-    // the list's probability of this token, or of the own one that of all others: w2 (q - t) = w2 ((1 - t) - (1 - q)) keeps its digits where both are close to 1
     float soft = 0.f;
     bool first = true;
-    const bool self = t == own;
 #pragma unroll 4
     for (int o = 0; o < k; o += 4) {                        // (sp[k] is zero, and entry k comes no earlier than any)
       const int4 s = *(const int4*)&sidx[wave][o];
       const f32x4 q = *(const f32x4*)&sp[wave][o];
-      soft += ((s.x == t) != self ? q[0] : 0.f) + ((s.y == t) != self ? q[1] : 0.f) + ((s.z == t) != self ? q[2] : 0.f) + ((s.w == t) != self ? q[3] : 0.f);
+      soft += (s.x == t ? q[0] : 0.f) + (s.y == t ? q[1] : 0.f) + (s.z == t ? q[2] : 0.f) + (s.w == t ? q[3] : 0.f);
       first = first && !((s.x == t && o < e) || (s.y == t && o + 1 < e) || (s.z == t && o + 2 < e) || (s.w == t && o + 3 < e));
     }
     if (!first) continue;                                   // an earlier entry of the list names the same token: that one writes
-    const float v = up * ll_sparse_cell(rk, zk[(int64_t)pi * (k + 1) + e], c1, c2, w1s, w2s, soft, self, t == lab[pi]);
+    const float v = up * ll_sparse_cell(rk, zk[(int64_t)pi * (k + 1) + e], c1, c2, w1s, w2s, soft, t == own, t == lab[pi]);
     if (in) G[(int64_t)i * ldg + c] = (E)v;
     const float m = fabsf(v), res = v - (float)(E)v;
     if (m > m1) { m2 = m1; t2 = t1; r2 = r1; m1 = m; t1 = t; r1 = res; }
@@ -1879,15 +1882,11 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
     float soft = 0.f;
     bool first = true;
     const float* const rk = p.rk + r * LL_RK;
-    const bool self = t == __float_as_int(rk[RK_TOKEN]);
 #pragma unroll 8
-    for (int o = 0; o < p.k; ++o) {
-      const bool same = p.top_idx[row * p.ld_top + o] == t;
-      if (same != self) soft += p.pk[(int64_t)r * p.k + o];
-      first = first && !(same && o < e);
-    }
+    for (int o = 0; o < p.k; ++o)
+      if (p.top_idx[row * p.ld_top + o] == t) { soft += p.pk[(int64_t)r * p.k + o]; first = first && o >= e; }
     if (!first) continue;
-    const float v = ll_sparse_cell(rk, p.z[(int64_t)r * p.ldz + t], p.c1, p.c2, p.w1s, p.w2s, soft, self, t == lab);
+    const float v = ll_sparse_cell(rk, p.z[(int64_t)r * p.ldz + t], p.c1, p.c2, p.w1s, p.w2s, soft, t == __float_as_int(rk[RK_TOKEN]), t == lab);
     *(E*)(gs_ + r * FG_LD + (t - n0) * 2) = (E)v;
     if (twice) *(E*)(gs_ + (r + HALF) * FG_LD + (t - n0) * 2) = (E)(v - (float)(E)v);
   }
@@ -2155,7 +2154,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
   r.lw2 = log2f(w2) + (float)s;
   r.dual = dual; r.soft_only = soft_only; r.nvalid = d->nvalid_dev; r.order = order; r.lab = lab; r.zk = zk; r.top_vals = d->top_vals; r.top_idx = d->top_idx;
   r.eref = eref; r.efin = efin; r.F = F; r.head = T::HEAD; r.low = log2f((float)d->vocab) + T::LOW; r.shift = (float)s; r.cl = apart ? Lb : nullptr; r.f16 = d->dtype == NS_F16; r.big_tok = d->k == 0 ? big_tok : nullptr; r.big_res = big_res;      // (one softmax: Lb is free)
-  r.xtok = xtok; r.xz = xz; r.rk = rk; r.up = up;
+  r.xtok = xtok; r.xz = xz; r.rk = grad ? rk : nullptr; r.up = up;
   r.ld_top = d->ld_top; r.La = La; r.Lb = dual ? Lb : nullptr; r.pk = pk; r.row_loss = d->row_loss; r.packed_loss = ploss; r.loss = d->loss_dev;
   if (p.few) {
     FewArgs f = {};
