@@ -16,6 +16,10 @@ constexpr int DT_MAX_K = 256;
 
 template <class E> struct vec { static constexpr int N = 16 / (int)sizeof(E); typedef E t __attribute__((ext_vector_type(16 / sizeof(E)))); };
 
+template <class E> struct half_of { typedef E t; };
+template <> struct half_of<float> { typedef half_t t; };
+template <class E> using half_or = typename half_of<E>::t;      // (fp32 does not use it)
+
 // A row as 16-B chunks from its first 16-B boundary, plus at most one element per thread from its ragged ends: threads 0 .. take the elements before
 // the boundary, threads 64 .. those behind the last whole chunk (extra_j: this thread's, or -1).
 template <class E, int NC, int NT>
@@ -45,6 +49,28 @@ struct row_view {
         if ((int)threadIdx.x + i * NT < chunks) reg[i] = STREAM ? __builtin_nontemporal_load(body + threadIdx.x + i * NT) : body[threadIdx.x + i * NT];
     }
     if (extra_j >= 0) extra = (float)p[extra_j];
+  }
+  // element e of a chunk goes: an exponential of zero
+  static __device__ __forceinline__ void without(V& v, int e) {
+#pragma unroll
+    for (int x = 0; x < N; ++x)
+      if (x == e) v[x] = (E)-INFINITY;
+  }
+  // element j (e of chunk c, or -1: one of the ragged ends) goes from the registers: one wave has it
+  __device__ __forceinline__ void drop(int j, int c, int e) {
+    if (j >= 0 && extra_j == j) extra = -INFINITY;
+    if (NC > 0 && c >= 0 && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == c % NT >> 6) {
+      const bool me = (int)threadIdx.x == c % NT;
+      const uint32_t keep = N == 4 ? 0u : e & 1 ? 0xFFFFu : 0xFFFF0000u;
+      const uint32_t put = N == 4 ? 0xFF800000u : (uint32_t)__builtin_bit_cast(uint16_t, (half_or<E>)-INFINITY) << (e & 1) * 16;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (i == c / NT) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            if (w == e * 4 / N) reg[i][w] = me ? (reg[i][w] & keep) | put : reg[i][w];
+        }
+    }
   }
   // f(chunk index, chunk).  The empty asm keeps hipcc from carrying the CONVERTED elements of one sweep over to the next (64 more registers per 8 chunks:
   // it spilled them).
@@ -133,6 +159,8 @@ struct DistillArgs {
 // e^(z / T) by multiplication (its relative error T times the other's, which is what the argument's rounding in e^z itself amounts to).
 // Per logit: a conversion and a maximum, then an fma, an exponential (a quarter-rate instruction) and an addition per softmax, and the same again for the
 // gradient: with DUAL = 1 ~30 issue slots, 26 k cycles of a CU a row of 51 865 against the 20 k that the row's 208 KB take at the copy rate.
+// A row that is almost certain of a token has 1 - p for a gradient there, which p itself does not hold: one token of the row, the label or the list's first entry, whichever has
+// the larger logit, is left out of the sums, and 1 - p is what the others hold.
 template <class E, int NC, int NT, int DUAL>
 __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_kernel(const DistillArgs p) {
   constexpr int NW = NT / 64;
@@ -141,9 +169,11 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
   __shared__ __attribute__((aligned(16))) int sidx[DT_MAX_K + 4];
   __shared__ __attribute__((aligned(16))) float sp[DT_MAX_K + 4];
   __shared__ float sz[DT_MAX_K + 1];
+  __shared__ float listed_rest;            // what the list gives to tokens other than the row's own
   typedef row_view<E, NC, NT> RV;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t lab64 = p.labels ? p.labels[row] : -1;
+  const int listed = p.ti[row * p.ldt];      // (here, before any store, a scalar load: behind the row's loads it would wait for them, before them they for it)
   const bool has = lab64 >= 0 && lab64 < p.V;
   E* const out = p.dz ? (E*)p.dz + row * p.lddz : nullptr;
   RV r;
@@ -177,7 +207,21 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
     }
     return;
   }
+  // the row's own token and its logit; it leaves the registers (its cell of the gradient is a sparse one).  (Both logits are asked for ahead of the row: behind it they cost a latency)
+  const bool ok = listed >= 0 && listed < p.V;
+  int own = has ? (int)lab64 : -1;
+  const E z_label = r.p[has ? own : 0], z_listed = r.p[ok ? listed : 0];
+  __builtin_amdgcn_sched_barrier(0);
   r.template load<true>();
+  float zown = (float)z_label;
+  {
+    const float z = (float)z_listed;
+    if (ok && !(has && zown >= z)) { own = listed; zown = z; }
+    own = __builtin_amdgcn_readfirstlane(own);
+    zown = __uint_as_float(__builtin_amdgcn_readfirstlane((int)__float_as_uint(zown)));
+  }
+  const int own_c = own >= r.head && own - r.head < r.chunks * RV::N ? (own - r.head) / RV::N : -1, own_e = (own - r.head) & (RV::N - 1);
+  r.drop(own, own_c, own_e);
   // the lists: token, teacher logit / T, the student's logit there (read before any gradient overwrites it: dz may be z itself)
   for (int e = tid; e <= p.k; e += NT) {
     const int t = e == p.k ? (has ? (int)lab64 : -1) : p.ti[row * p.ldt + e];
@@ -193,7 +237,8 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
   const float c1 = p.soft_only ? LOG2E / p.T : LOG2E, c2 = LOG2E / p.T;
   // every wave's maximum and sums relative to it, joined over the workgroup
   float mx = -INFINITY;
-  r.each([&](int, typename RV::V v) __attribute__((always_inline)) {
+  r.each([&](int c, typename RV::V v) __attribute__((always_inline)) {
+    if (NC == 0 && c == own_c) RV::without(v, own_e);
 #pragma unroll
     for (int e = 0; e < RV::N; ++e) mx = fmaxf(mx, (float)v[e]);
   });
@@ -210,7 +255,8 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
         if (DUAL == 4) s1 = __builtin_fmaf(y2, y2, s1);
       }
     };
-    r.each([&](int, typename RV::V v) __attribute__((always_inline)) {
+    r.each([&](int c, typename RV::V v) __attribute__((always_inline)) {
+      if (NC == 0 && c == own_c) RV::without(v, own_e);
 #pragma unroll
       for (int e = 0; e < RV::N; ++e) add((float)v[e]);
     });
@@ -224,9 +270,24 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
   const int ent = lane & (NW - 1);
   const float wm = sh[0][ent];
   mx = max_over_waves<NW>(wm);
+  if (own >= 0) mx = fmaxf(mx, zown);
   const float ms = finite_or_zero(mx), dm = wm == -INFINITY ? -INFINITY : finite_or_zero(wm) - ms;      // (a wave without elements, or of -inf: no part)
   s1 = over_waves<NW>(sh[1][ent] * __builtin_amdgcn_exp2f(dm * c1));
   if (DUAL) s2 = over_waves<NW>(sh[2][ent] * __builtin_amdgcn_exp2f(dm * c2));
+  // x1, x2: a logit's part of the two sums
+  auto parts = [&](float z, float& x1, float& x2) __attribute__((always_inline)) {
+    x2 = DUAL ? __builtin_amdgcn_exp2f((z - ms) * c2) : 0.f;
+    x1 = DUAL == 2 ? x2 * x2 : DUAL == 4 ? (x2 * x2) * (x2 * x2) : __builtin_amdgcn_exp2f((z - ms) * c1);
+  };
+  float rest1 = 1.f, rest2 = 1.f;          // 1 - p, 1 - q of the row's own token
+  if (own >= 0) {
+    float x1, x2;
+    parts(zown, x1, x2);
+    rest1 = __builtin_fmaf(0.f, x1, s1 / (s1 + x1));      // (an infinity shows)
+    s1 += x1;
+    rest2 = DUAL ? __builtin_fmaf(0.f, x2, s2 / (s2 + x2)) : rest1;
+    s2 += x2;
+  }
   live = over_waves<NW>(shc[ent]);
   if (p.count_here) { if (row == 0 && tid == 0) *p.nvalid = live; }
   else live = *p.nvalid;
@@ -241,15 +302,18 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
     for (int e = lane; e < p.k; e += 64) ts += soft ? expf(sp[e] - tm) : 0.f;
     ts = ns_wave_sum(ts);
     const float lt = logf(ts), its = 1.f / ts, ls = logf(DUAL ? s2 : s1);
-    float kl = 0.f;
+    float kl = 0.f, lr = 0.f;
     for (int e = lane; e < p.k; e += 64) {
       const float lp = sp[e] - tm;
       const float pr = soft ? expf(lp) * its : 0.f;
       if (pr > 0.f) kl += pr * ((lp - lt) - ((sz[e] - ms) / p.T - ls));
       sp[e] = pr;
+      lr += sidx[e] == own ? 0.f : pr;
     }
     kl = ns_wave_sum(kl);
+    lr = ns_wave_sum(lr);
     if (lane == 0) {
+      listed_rest = lr;
       float loss = soft ? p.kd * kl : 0.f;
       if (!p.soft_only) loss += p.w1 * ((ms - sz[p.k]) + logf(s1));
       p.row_loss[row] = loss;
@@ -303,9 +367,13 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
       first = first && !((s.x == t && o < e) || (s.y == t && o + 1 < e) || (s.z == t && o + 2 < e) || (s.w == t && o + 3 < e));
     }
     if (!first) continue;
-    float g = grad(sz[e]) - gs * w2 * q;
-    if (has && t == (int)lab64) g -= gs * p.w1;
-    out[t] = (E)g;
+    const bool label = has && t == (int)lab64;
+    float x1, x2;
+    parts(sz[e], x1, x2);
+    // where the row is certain of this token: p - 1 = -(1 - p), q - t = (1 - t) - (1 - q)
+    const float d1 = t == own && rest1 < 0.5f ? (label ? -rest1 : 1.f - rest1) : x1 / s1 - (label ? 1.f : 0.f);
+    const float d2 = t == own && rest2 < 0.5f ? listed_rest - rest2 : (DUAL ? x2 / s2 : x1 / s1) - q;
+    out[t] = (E)(gs * ((p.soft_only ? 0.f : p.w1 * d1) + (soft ? w2 * d2 : 0.f)));
   }
 }
 

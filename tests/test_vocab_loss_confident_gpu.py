@@ -138,3 +138,32 @@ def test_two_candidates_and_a_tail_far_below(ops, dev, dtype, rows, d, v, rival)
     """a rival that holds 2^-1 to 2^-20 of the label, all others far below both"""
     h, w, labels = make_confident(dev, rows, d, v, dtype, rows + d, rival=rival)
     check_confident(ops, dev, h, w, labels, "h", scale=2.0 ** 18, certain=False)
+
+
+# ------------------------------------------------------------------------------------------------ over logits
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,v,first", [(40, 9, 0), (40, 1001, 3), (64, 5000, 0), (33, 51865, 1), (20, 70001, 0)])
+@pytest.mark.parametrize("temp,alpha", [(1.0, 0.5), (2.0, 0.5), (4.0, 0.5), (1.5, 0.3), (2.0, 1.0)])
+@pytest.mark.parametrize("who", ["label", "teacher"])
+def test_distill_topk_on_almost_certain_rows(ops, dev, dtype, rows, v, first, temp, alpha, who):
+    """student and teacher both certain of one token, the label or another: cells as exact as what the other tokens hold"""
+    g = gen(rows + v, dev)
+    buf = torch.randn(rows, v + first, generator=g, device=dev) * 2
+    labels = torch.randint(0, v, (rows,), generator=g, device=dev)
+    labels[0], labels[1] = 0, v - 1
+    sure = labels if who == "label" else (labels + v // 2) % v
+    buf[:, first:].scatter_(1, sure.unsqueeze(1), torch.linspace(8.0, 26.0, rows, device=dev).unsqueeze(1) + (4.0 if v > 10000 else 0.0))
+    buf = buf.to(dtype)
+    z = buf[:, first:]
+    ti = ((sure.unsqueeze(1) + torch.arange(4, device=dev)) % v).int().contiguous()
+    tv = torch.cat([torch.linspace(20.0, 4.0, rows, device=dev).unsqueeze(1), torch.randn(rows, 3, generator=g, device=dev)], 1).contiguous()
+    dz = torch.full_like(buf, 5.0)[:, first:]
+    o = outputs(dev, rows)
+    scale = 2.0 ** 14
+    ops.distill_topk(z, labels, tv, ti, temperature=temp, alpha=alpha, dlogits=dz, loss_scale=torch.tensor([scale], device=dev), **o)
+    cell, err, _, _ = C.cells(z.double(), torch.zeros(rows, dtype=torch.float64, device=dev), labels, temp, alpha, tv, ti)
+    gs = scale / rows
+    U = R.half_step(dtype)
+    want = cell * gs
+    small = {F16: 2.0 ** -25, BF16: 2.0 ** -126, F32: 2.0 ** -126}[dtype]
+    close(dz, want, (err * gs + 4 * R.U32 * want.abs()) * (1 + U) + U * want.abs() + small, "dlogits")
