@@ -104,6 +104,7 @@ template <int NW> __device__ __forceinline__ float max_over_waves(float v) {
   for (int o = NW / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
   return v;
 }
+__device__ __forceinline__ float max_or_nan(float a, float b) { return b > a || b != b ? b : a; }
 template <int NT> __device__ __forceinline__ float block_sum(float v, float* sh) {
   v = ns_wave_sum(v);
   __syncthreads();
@@ -293,9 +294,10 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
   else live = *p.nvalid;
   // the teacher's distribution: every wave forms its maximum, the first one the row's loss and the probabilities
   float tm = -INFINITY;
-  for (int e = lane; e < p.k; e += 64) tm = fmaxf(tm, sp[e]);
-  tm = ns_wave_max(tm);
-  const bool soft = tm > -INFINITY;        // a list that names no token leaves the hard label alone
+  for (int e = lane; e < p.k; e += 64) tm = max_or_nan(tm, sp[e]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) tm = max_or_nan(tm, __shfl_xor(tm, o, 64));
+  const bool soft = tm != -INFINITY;       // a list that names no token leaves the hard label alone; a NaN or +inf that an entry holds shows in the row's loss
   __syncthreads();                         // every wave has read sp[] before the first one turns it into probabilities
   if (wave == 0) {
     float ts = 0.f;
@@ -306,7 +308,7 @@ __global__ __launch_bounds__(NT, NT == 1024 && NC <= 7 ? 8 : 4) void distill_ker
     for (int e = lane; e < p.k; e += 64) {
       const float lp = sp[e] - tm;
       const float pr = soft ? expf(lp) * its : 0.f;
-      if (pr > 0.f) kl += pr * ((lp - lt) - ((sz[e] - ms) / p.T - ls));
+      if (pr != 0.f) kl += pr * ((lp - lt) - ((sz[e] - ms) / p.T - ls));
       sp[e] = pr;
       lr += sidx[e] == own ? 0.f : pr;
     }

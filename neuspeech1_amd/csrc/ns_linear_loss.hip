@@ -1006,6 +1006,8 @@ __device__ __forceinline__ void ll_choose_splits(int nv, int tiles_d, int kt, in
   if (threadIdx.x == 0) *splits = (int)(min(min(best[0], best[1]), min(best[2], best[3])) & 2047);
 }
 
+__device__ __forceinline__ float ll_max_or_nan(float a, float b) { return b > a || b != b ? b : a; }
+
 struct RowArgs {
   const float *pm, *p1, *p2;
   int tiles_n, R, k, V, row0;
@@ -1161,11 +1163,11 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
     for (int e = q; e < p.k; e += 16) {
       const int t = ti[e];
       const float v = tv[e] * p.invT;
-      tm = t >= 0 && t < p.V ? fmaxf(tm, v) : tm;
+      tm = t >= 0 && t < p.V ? ll_max_or_nan(tm, v) : tm;
     }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor(tm, o, 64));
-    soft = tm > -INFINITY;
+    for (int o = 8; o > 0; o >>= 1) tm = ll_max_or_nan(tm, __shfl_xor(tm, o, 64));
+    soft = tm != -INFINITY;               // (a NaN or +inf that an entry holds shows in the row's loss)
     float ts = 0.f;
 #pragma unroll 4
     for (int e = q; e < p.k; e += 16) {
@@ -1188,7 +1190,7 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
       const float z = logit(e, ok ? t : 0);
       if (ok) {
         pr = expf(lp) * inv;
-        if (pr > 0.f) kl += pr * ((lp - lt) - (__builtin_fmaf(z, p.c2, -e2) - ls) * LN2);
+        if (pr != 0.f) kl += pr * ((lp - lt) - (__builtin_fmaf(z, p.c2, -e2) - ls) * LN2);
       }
       p.pk[(int64_t)pi * p.k + e] = pr;
       lr += t == x ? 0.f : pr;
