@@ -1469,6 +1469,7 @@ template <class E> void launch_dh_out(const float* slab, int groups, int splits,
                                       int64_t lddh, const float* packed_loss, float* loss, const float* F, const E* w, int64_t ldw, const int* lab, const float* cl, const int* big_tok, const float* big_res, hipStream_t st) {
   const int nblk = 16 / groups;
   const int64_t items = (int64_t)rows * ((d + 63) / 64);
+  if (items == 0 && !loss) return;               // (no rows: nothing to write)
   hipLaunchKernelGGL(ll_dh_out_kernel<E>, dim3((unsigned)((items + nblk - 1) / nblk) + (loss ? 1 : 0)), dim3(256), 0, st, slab, groups, splits, splits_dev, R, row0, chunk, d, rows, inv, nvalid,
                      loss_scale, unscale, dh, lddh, packed_loss, loss, F, w, ldw, lab, cl, big_tok, big_res);
 }

@@ -1,0 +1,31 @@
+"""GPU: the C entry points of the vocabulary losses where the Python calls never lead."""
+import ctypes as C
+
+import pytest
+import torch
+
+from neuspeech1_amd import lib
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype,code", [(torch.float16, lib.NS_F16), (torch.bfloat16, lib.NS_BF16)])
+@pytest.mark.parametrize("with_dw", [False, True])
+def test_no_rows_with_gradients_asked_for(dev, dtype, code, with_dw):
+    """rows = 0 with dh set: a loss of zero over no rows, dW zero, nothing else written"""
+    so = lib.load()
+    w = torch.randn(300, 64, device=dev).to(dtype)
+    dh, dw = torch.full((4, 64), 3.0, device=dev, dtype=dtype), torch.full_like(w, 3.0)
+    loss, nvalid = torch.full((1,), 7.0, device=dev), torch.full((1,), 7, device=dev, dtype=torch.int32)
+    d = lib.LinearCeDesc()
+    d.w, d.ldw, d.ldh, d.dh, d.lddh = w.data_ptr(), 64, 64, dh.data_ptr(), 64
+    if with_dw:
+        d.dw, d.lddw = dw.data_ptr(), 64
+    d.loss_dev, d.nvalid_dev = loss.data_ptr(), nvalid.data_ptr()
+    d.rows, d.vocab, d.d, d.dtype, d.temperature = 0, 300, 64, code, 1.0
+    need = so.ns_linear_ce_workspace_bytes(C.byref(d))
+    ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    assert so.ns_linear_cross_entropy(C.byref(d), torch.cuda.current_stream().cuda_stream) == 0, so.ns_last_error()
+    torch.cuda.synchronize()
+    assert float(loss) == 0 and int(nvalid) == 0 and (dh == 3.0).all() and (dw == (0.0 if with_dw else 3.0)).all()
