@@ -569,6 +569,9 @@ template <class E, int NC, int NT> struct topk_go {
   }
 };
 
+// a launch holds less than 2^32 threads: by_length's workgroups, one a row
+bool rows_fit(int rows, int V, int dtype) { return (int64_t)rows * ((V / (dtype == NS_F32 ? 4 : 8) <= 512) ? 256 : 1024) < (1ll << 32); }
+
 bool elem_aligned(const void* q, int dtype) { return ((size_t)q & (dtype == NS_F32 ? 3 : 1)) == 0; }
 
 }  // namespace
@@ -579,6 +582,7 @@ extern "C" int ns_distill_topk(const ns_distill_desc* d, void* stream) {
   NS_CHECK_ARG(d->rows >= 0 && d->vocab > 0 && d->vocab <= (1 << 30) && d->k > 0 && d->k <= DT_MAX_K, "ns_distill_topk: bad sizes rows=%d vocab=%d k=%d (k <= %d)", d->rows,
                d->vocab, d->k, DT_MAX_K);
   NS_CHECK_ARG(d->dtype == NS_F16 || d->dtype == NS_BF16 || d->dtype == NS_F32, "ns_distill_topk: dtype %d", d->dtype);
+  NS_CHECK_ARG(rows_fit(d->rows, d->vocab, d->dtype), "ns_distill_topk: rows=%d are too many for one launch", d->rows);
   NS_CHECK_ARG(d->rows <= 1 || (d->ldz >= d->vocab && d->ld_top >= d->k && (!d->dlogits || d->lddz >= d->vocab)), "ns_distill_topk: row strides shorter than the rows");
   NS_CHECK_ARG(elem_aligned(d->logits, d->dtype) && elem_aligned(d->dlogits, d->dtype), "ns_distill_topk: logits not aligned to their elements");
   NS_CHECK_ARG(d->temperature >= 0.05f && d->temperature <= 100.f && d->alpha > 0.f && d->alpha <= 1.f, "ns_distill_topk: temperature %g in [0.05, 100], alpha %g in (0, 1]",
@@ -609,6 +613,7 @@ extern "C" int ns_topk_logits(const ns_topk_desc* d, void* stream) {
   NS_CHECK_ARG(d->rows >= 0 && d->vocab > 0 && d->vocab <= (1 << 30) && d->k > 0 && d->k <= DT_MAX_K && d->k <= d->vocab,
                "ns_topk_logits: bad sizes rows=%d vocab=%d k=%d (k <= vocab, k <= %d)", d->rows, d->vocab, d->k, DT_MAX_K);
   NS_CHECK_ARG(d->dtype == NS_F16 || d->dtype == NS_BF16 || d->dtype == NS_F32, "ns_topk_logits: dtype %d", d->dtype);
+  NS_CHECK_ARG(rows_fit(d->rows, d->vocab, d->dtype), "ns_topk_logits: rows=%d are too many for one launch", d->rows);
   NS_CHECK_ARG(d->rows <= 1 || (d->ldz >= d->vocab && d->ldo >= d->k), "ns_topk_logits: row strides shorter than the rows");
   NS_CHECK_ARG(elem_aligned(d->logits, d->dtype), "ns_topk_logits: logits not aligned to their elements");
   if (d->rows == 0) return NS_OK;

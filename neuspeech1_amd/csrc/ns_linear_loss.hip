@@ -2091,12 +2091,15 @@ Plan plan_of(const ns_linear_ce_desc* d) {
   return p;
 }
 
+// groups of slabs that ll_dh_out_kernel adds side by side
+int dh_groups(const Plan& p) { return p.few ? (p.tiles_n >= 64 ? 16 : p.tiles_n >= 16 ? 4 : 1) : p.Rc <= 512 ? 16 : 1; }
+
 bool ll_sizes_ok(const ns_linear_ce_desc* d) {
   return d->rows >= 0 && d->rows <= (1 << 21) && d->vocab > 0 && d->vocab <= (1 << 28) && d->d > 0 && d->d % 8 == 0 && d->d <= (1 << 16) && d->k >= 0 && d->k <= LL_MAX_K;
 }
 
 template <class T, int MT>
-int few_launch(const ns_linear_ce_desc* d, const FewArgs& f, const RowArgs& r, bool dual, hipStream_t st) {
+int few_launch(const ns_linear_ce_desc* d, const Plan& p, const FewArgs& f, const RowArgs& r, bool dual, hipStream_t st) {
   typedef typename T::e E;
   static ns_dev_once once;
   if (!ns_dyn_lds_once(once, {(const void*)ll_few_grad_kernel<T, MT, false>, (const void*)ll_few_grad_kernel<T, MT, true>, (const void*)ll_few_logits_kernel<T, MT, false>,
@@ -2114,7 +2117,7 @@ int few_launch(const ns_linear_ce_desc* d, const FewArgs& f, const RowArgs& r, b
     gy = (chunks + (chunks + gy - 1) / gy - 1) / ((chunks + gy - 1) / gy);
     if (dual) hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, true>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
     else hipLaunchKernelGGL((ll_few_grad_kernel<T, MT, false>), dim3(f.tiles_n, gy), dim3(512), few_lds<MT>(), st, f);
-    if (d->dh) launch_dh_out<E>(f.slab, f.tiles_n >= 64 ? 16 : f.tiles_n >= 16 ? 4 : 1, f.tiles_n, nullptr, 16 * MT, 0, LL_FEW_ROWS, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, nullptr, nullptr, nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr, st);
+    if (d->dh) launch_dh_out<E>(f.slab, dh_groups(p), f.tiles_n, nullptr, 16 * MT, 0, LL_FEW_ROWS, d->d, d->rows, f.inv, d->nvalid_dev, d->loss_scale_dev, f.unscale, (E*)d->dh, d->lddh, nullptr, nullptr, nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
   return NS_OK;
@@ -2167,7 +2170,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
     f.La = La; f.Lb = dual ? Lb : nullptr; f.pk = pk; f.rk = rk; f.top_idx = d->top_idx; f.ld_top = d->ld_top; f.k = d->k; f.w1s = w1 * up; f.w2s = w2 * up; f.unscale = 1.f / up;
     f.loss_scale = d->loss_scale_dev; f.slab = (float*)(ws + p.slab); f.dw = d->dw; f.lddw = d->lddw; f.f32 = d->dw_f32; f.add = d->dw_add; f.dh = d->dh != nullptr;
     r.z = zk; r.ldz = f.ldz;
-    return p.few == 1 ? few_launch<T, 1>(d, f, r, dual, st) : p.few == 2 ? few_launch<T, 2>(d, f, r, dual, st) : few_launch<T, 4>(d, f, r, dual, st);
+    return p.few == 1 ? few_launch<T, 1>(d, p, f, r, dual, st) : p.few == 2 ? few_launch<T, 2>(d, p, f, r, dual, st) : few_launch<T, 4>(d, p, f, r, dual, st);
   }
   hipLaunchKernelGGL(ll_compact_kernel, dim3(1), dim3(1024), 0, st, d->labels, d->rows, d->vocab, order, inv, lab, d->row_loss, d->nvalid_dev);
   hipLaunchKernelGGL(ll_pack_kernel<T>, dim3(p.R / 4), dim3(256), 0, st, d->h, d->ldh, d->w, d->ldw, d->d, p.dp, order, lab, d->k, d->nvalid_dev, (void*)(ws + p.hp), zk, c1, eref, xtok);
@@ -2233,7 +2236,7 @@ int ll_launch(const ns_linear_ce_desc* d, const Plan& p, hipStream_t st) {
       }
     }
     if (d->dh)
-      launch_dh_out<E>((const float*)(ws + p.slab), p.Rc <= 512 ? 16 : 1, 0, splits, 0, row0, p.Rc, d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh,
+      launch_dh_out<E>((const float*)(ws + p.slab), dh_groups(p), 0, splits, 0, row0, p.Rc, d->d, d->rows, inv, d->nvalid_dev, d->loss_scale_dev, 1.f / up, (E*)d->dh,
                        d->lddh, ploss, row0 + p.Rc >= p.R ? d->loss_dev : nullptr, F, (const E*)d->w, d->ldw, lab, apart ? Lb : nullptr, big_tok, big_res, st);
   }
   NS_CHECK_LAUNCH("ns_linear_cross_entropy");
@@ -2267,6 +2270,9 @@ extern "C" int ns_linear_cross_entropy(const ns_linear_ce_desc* desc, void* stre
   if (d->alpha == 0.f) d->k = 0;     // the hard labels alone: the teacher's list is not read
   const Plan p = plan_of(d);
   NS_CHECK_ARG(d->workspace && d->workspace_bytes >= p.total, "ns_linear_cross_entropy: workspace of %zu bytes, %zu needed", d->workspace_bytes, p.total);
-  NS_CHECK_ARG((int64_t)(p.R / BM) * p.tiles_n < (1ll << 31) && (int64_t)d->rows * (d->d / 8) < (1ll << 38), "ns_linear_cross_entropy: too many tiles");
+  NS_CHECK_ARG((int64_t)(p.R / BM) * p.tiles_n < (1ll << 31), "ns_linear_cross_entropy: too many tiles");
+  // (a launch holds less than 2^32 threads: dh is written by 16 threads per row and 64 columns, or 256)
+  NS_CHECK_ARG(!d->dh || (int64_t)d->rows * ((d->d + 63) / 64) * (256 / (16 / dh_groups(p))) < (1ll << 32) - 1024, "ns_linear_cross_entropy: rows=%d of d=%d are too many for one dh", d->rows,
+               d->d);
   return d->dtype == NS_F16 ? ll_launch<tf16>(d, p, (hipStream_t)stream) : ll_launch<tbf16>(d, p, (hipStream_t)stream);
 }
