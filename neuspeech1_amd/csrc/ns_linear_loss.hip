@@ -1268,10 +1268,13 @@ __global__ __launch_bounds__(1024) void ll_mean_kernel(const float* __restrict__
 }
 
 // a cell of dz at a token that the label or the list names (soft: the list's probability of it; own: the row is certain of it, and p - 1 = -(1 - p), q - t = (1 - t) - (1 - q))
-__device__ __forceinline__ float ll_sparse_cell(const float* rk, float z, float c1, float c2, float w1s, float w2s, float soft, bool own, bool label) {
-  if (own) return (label ? -w1s * rk[RK_REST1] : w1s * (1.f - rk[RK_REST1])) + (w2s > 0.f ? w2s * rk[RK_SOFT] : 0.f);
-  float v = __builtin_amdgcn_exp2f(__builtin_fmaf(z, c1, -rk[RK_E1])) * rk[RK_I1];
-  if (rk[RK_I2] > 0.f) v = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(z, c2, -rk[RK_E2])), rk[RK_I2], v);
+struct RowK { f32x4 lo, hi; };
+__device__ __forceinline__ RowK ll_row_k(const float* rk) { return {*(const f32x4*)rk, *(const f32x4*)(rk + 4)}; }
+__device__ __forceinline__ float ll_sparse_cell(const RowK& k, float z, float c1, float c2, float w1s, float w2s, float soft, bool own, bool label) {
+  static_assert(RK_E1 == 0 && RK_I1 == 1 && RK_E2 == 2 && RK_I2 == 3 && RK_REST1 == 4 && RK_SOFT == 7, "ll_rows_kernel writes them in this order");
+  if (own) return (label ? -w1s * k.hi[0] : w1s * (1.f - k.hi[0])) + (w2s > 0.f ? w2s * k.hi[3] : 0.f);
+  float v = __builtin_amdgcn_exp2f(__builtin_fmaf(z, c1, -k.lo[0])) * k.lo[1];
+  if (k.lo[3] > 0.f) v = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(z, c2, -k.lo[2])), k.lo[3], v);
   return v - w2s * soft - (label ? w1s : 0.f);
 }
 
@@ -1302,8 +1305,8 @@ __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ n
   if (!live) return;
   // (efin: cells relative to the row's factor; one of zero leaves none)
   const float la = La[i], up = efin ? (la < INFINITY ? __builtin_amdgcn_exp2f(la - efin[i]) : 0.f) : 1.f;
-  rk += (int64_t)i * LL_RK;
-  const int own = __float_as_int(rk[RK_TOKEN]);
+  const RowK kk = ll_row_k(rk + (int64_t)i * LL_RK);
+  const int own = __float_as_int(kk.hi[RK_TOKEN - 4]);
   float m1 = 0.f, m2 = 0.f, r1 = 0.f, r2 = 0.f;             // this lane's two largest
   int t1 = -1, t2 = -1;
   for (int e = lane; e <= k; e += 64) {
@@ -1320,7 +1323,7 @@ __global__ __launch_bounds__(256) void ll_cells_kernel(const int* __restrict__ n
       first = first && !((s.x == t && o < e) || (s.y == t && o + 1 < e) || (s.z == t && o + 2 < e) || (s.w == t && o + 3 < e));
     }
     if (!first) continue;                                   // an earlier entry of the list names the same token: that one writes
-    const float v = up * ll_sparse_cell(rk, zk[(int64_t)pi * (k + 1) + e], c1, c2, w1s, w2s, soft, t == own, t == lab[pi]);
+    const float v = up * ll_sparse_cell(kk, zk[(int64_t)pi * (k + 1) + e], c1, c2, w1s, w2s, soft, t == own, t == lab[pi]);
     if (in) G[(int64_t)i * ldg + c] = (E)v;
     const float m = fabsf(v), res = v - (float)(E)v;
     if (m > m1) { m2 = m1; t2 = t1; r2 = r1; m1 = m; t1 = t; r1 = res; }
@@ -1813,6 +1816,7 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef typename T::e E;
   typedef typename T::v8 v8;
+  typedef E e4 __attribute__((ext_vector_type(4)));
   char* const hs = smem + 3 * FW_BYTES;
   char* const gs_ = hs + 3 * FH_BYTES;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, lg = lane >> 4;
@@ -1824,8 +1828,13 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
   // Few enough rows with a label leave half of dz's rows free: row r + HALF then holds what row r's rounding lost, dh's two rows are added at the end and h's row
   // stands there twice for dW.  The label's cell is most of such a row's dz, and its one rounding would be a factor on the whole gradient: with many
   // rows these factors average out, with one fp16 row dh was off by 3.1e-4 where its own rounding is 2.1e-4.
+  // Where the rows fill them (33 to 64 labels), the largest of a row's cells among these tokens counts by itself: what its rounding lost goes into the row's dh and the
+  // token's dW in fp32, from W's and h's rows in LDS (48 rows, d = 512: 1.2 - 1.5 -> 1.0 times the result's own rounding).  Per row: |cell| above, its residue's upper 24
+  // bits and the token below.
   constexpr int HALF = 8 * MT;
   const bool twice = nv <= HALF;
+  __shared__ unsigned long long big[64];
+  if (tid < 64) big[tid] = 0;
   // Chunks of 64 columns by LDS-DMA, three slots: of W (for dh) wave w fills rows [32 w, 32 w + 32) in four pieces of 8 rows x 128 B, of h (for dW) rows
   // [8 w, 8 w + 8) in one, packed rows of h by their original place.  The 32-B windows of row r are permuted by f(r) = bit 1 | bit 3 << 1, so that the eight
   // row segments of half a transposed read lie in different banks (even and odd rows already do).
@@ -1884,14 +1893,18 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
     if (t < n0 || t >= n0 + 256 || t >= p.V) continue;
     float soft = 0.f;
     bool first = true;
-    const float* const rk = p.rk + r * LL_RK;
+    const RowK kk = ll_row_k(p.rk + r * LL_RK);
+    const float z = p.z[(int64_t)r * p.ldz + t];
 #pragma unroll 8
     for (int o = 0; o < p.k; ++o)
       if (p.top_idx[row * p.ld_top + o] == t) { soft += p.pk[(int64_t)r * p.k + o]; first = first && o >= e; }
     if (!first) continue;
-    const float v = ll_sparse_cell(rk, p.z[(int64_t)r * p.ldz + t], p.c1, p.c2, p.w1s, p.w2s, soft, t == __float_as_int(rk[RK_TOKEN]), t == lab);
+    const float v = ll_sparse_cell(kk, z, p.c1, p.c2, p.w1s, p.w2s, soft, t == __float_as_int(kk.hi[RK_TOKEN - 4]), t == lab);
     *(E*)(gs_ + r * FG_LD + (t - n0) * 2) = (E)v;
-    if (twice) *(E*)(gs_ + (r + HALF) * FG_LD + (t - n0) * 2) = (E)(v - (float)(E)v);
+    const float lost = v - (float)(E)v;
+    if (twice) *(E*)(gs_ + (r + HALF) * FG_LD + (t - n0) * 2) = (E)lost;
+    else if (p.k == 0 || fabsf(v) * 16.f >= p.w1s * kk.hi[RK_REST1 - 4] + p.w2s * kk.hi[RK_REST2 - 4])      // (of a list the small ones stay: 64 rows, 64 entries: 125 -> 117 us)
+      atomicMax(&big[r], (unsigned long long)(__float_as_uint(v) & 0x7FFFFFFFu) << 32 | (__float_as_uint(lost) & 0xFFFFFF00u) | (unsigned)(t - n0));
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   LL_BARRIER();
@@ -1915,6 +1928,22 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
         const v8 v = tr8(gs_ + rr * FG_LD + (wave * 32 + f * 16 + 4 * pp) * 2, 4 * FG_LD);
         gt[f][ks] = MT == 1 && lg >= 2 ? v8{} : v;
       }
+  }
+  // this lane's row of dh's blocks, and which rows' cells lie in this wave's 32 tokens
+  constexpr int NB = MT < 2 ? 1 : MT / 2;
+  int row_tok[NB];
+  float row_lost[NB];
+  uint64_t mine = 0;
+  unsigned long long at_lane = 0;
+  if (!twice) {
+    at_lane = big[lane];
+    mine = __ballot(at_lane != 0 && (int)((unsigned)at_lane & 255) >> 5 == wave);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const unsigned long long b = big[((n * 8 + wave) >> 2) * 16 + l15 & 63];
+      row_tok[n] = b ? (int)((unsigned)b & 255) : -1;
+      row_lost[n] = __uint_as_float((unsigned)b & 0xFFFFFF00u);
+    }
   }
   // how many stores a wave issues behind a chunk's pieces in a full chunk (fewer in a ragged one: there the waits count none)
   const bool full_v = n0 + 256 <= p.V;
@@ -1952,6 +1981,12 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
             const v8 g = *(const v8*)(gs_ + (mt * 16 + l15) * FG_LD + (ks * 32 + 8 * lg) * 2);
             dha[n] = T::mma(wt, g, dha[n]);
           }
+          if (!twice && row_tok[n] >= 0) {
+            const int r = row_tok[n], f = ((r >> 1) & 1) | (((r >> 3) & 1) << 1);
+            const e4 l = *(const e4*)(ws + r * 128 + ((ct ^ f) << 5) + lg * 8);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dha[n][e] = __builtin_fmaf(row_lost[n], (float)l[e], dha[n][e]);
+          }
         }
       }
     }
@@ -1972,6 +2007,21 @@ __global__ __launch_bounds__(512) void ll_few_grad_kernel(const FewArgs p) {
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) a = T::mma(ht[ks], gt[f][ks], a);
           da[ct][f] = a * gs;
+        }
+      }
+      for (uint64_t m = mine; m; m &= m - 1) {
+        const int r = __builtin_ctzll(m), low = __builtin_amdgcn_readlane((int)(unsigned)at_lane, r), rf = ((r >> 1) & 1) | (((r >> 3) & 1) << 1);
+        const float lost = __uint_as_float((unsigned)low & 0xFFFFFF00u) * gs;
+        if (l15 != (low & 15)) continue;
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) {
+          const e4 x = *(const e4*)(hc + r * 128 + ((ct ^ rf) << 5) + lg * 8);
+#pragma unroll
+          for (int f = 0; f < 2; ++f)
+            if ((low >> 4 & 1) == f) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) da[ct][f][e] = __builtin_fmaf(lost, (float)x[e], da[ct][f][e]);
+            }
         }
       }
     }

@@ -167,3 +167,30 @@ def test_distill_topk_on_almost_certain_rows(ops, dev, dtype, rows, v, first, te
     want = cell * gs
     small = {F16: 2.0 ** -25, BF16: 2.0 ** -126, F32: 2.0 ** -126}[dtype]
     close(dz, want, (err * gs + 4 * R.U32 * want.abs()) * (1 + U) + U * want.abs() + small, "dlogits")
+
+
+# ------------------------------------------------------------------------------------------------ 33 to 64 labels
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,d,v", [(33, 256, 3000), (48, 512, 5001), (64, 264, 700), (50, 72, 51865)])
+@pytest.mark.parametrize("grad,k,temp,alpha", [("hw", 0, 1.0, 0.0), ("h", 0, 1.0, 0.0), ("w", 0, 1.0, 0.0), ("hw", 5, 2.0, 0.3), ("h", 5, 1.0, 1.0), ("hw", 64, 1.0, 0.5)])
+@pytest.mark.parametrize("shared", [False, True])
+def test_33_to_64_labels_keep_their_digits(ops, dev, dtype, rows, d, v, grad, k, temp, alpha, shared):
+    """dh and dW as a whole: no more than 1.15 times as far off as their own rounding.  Cells are 16-bit numbers, but a row's largest one in 256 tokens counts in fp32; what stays is
+    the rounding of the others, whose squares add to less than a third of the result's own (1.15^2 - 1).  shared: several rows have the same label"""
+    g = gen(rows + d, dev)
+    w = (torch.randn(v, d, generator=g, device=dev) * 2.0 * d ** -0.5).to(dtype)
+    labels = torch.randint(0, 3 if shared else v, (rows,), generator=g, device=dev) * (v // 3 if shared else 1)
+    h = (torch.randn(rows, d, generator=g, device=dev) + w[labels].float()).to(dtype)
+    lists = (None, None)
+    if k:
+        lists = ((6.0 - 2.5 * torch.log1p(torch.arange(k, device=dev).float()) + 0.3 * torch.randn(rows, k, generator=g, device=dev)).contiguous(),
+                 ((labels.unsqueeze(1) + 611 * torch.arange(k, device=dev)) % v).int().contiguous())
+    got = {n: torch.full_like(x, 3.0) for n, x in (("dh", h), ("dweight", w)) if n[1] in grad}
+    more = dict(top_vals=lists[0], top_idx=lists[1], temperature=temp, alpha=alpha) if k else {}
+    ops.linear_cross_entropy(h, w, labels, loss_scale=torch.tensor([2048.0], device=dev), **outputs(dev, rows), **got, **more)
+    ref = R.linear(h, w, labels, 2048.0, None, temp, alpha, *lists)
+    for n, x in got.items():
+        want = ref["dh" if n == "dh" else "dw"]
+        close(x, want, ref["dh_tol" if n == "dh" else "dw_tol"], n)
+        own = (want.to(dtype).double() - want).norm()
+        assert (x.double() - want).norm() <= 1.15 * own, (n, float((x.double() - want).norm() / own))
