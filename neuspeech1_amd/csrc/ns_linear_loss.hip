@@ -1042,6 +1042,19 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
   const int r_ = threadIdx.x >> 4, q_ = threadIdx.x & 15;
   float xz = -INFINITY;             // the own token's logit
   if (!FEW && i0 + r_ < nv) xz = p.xz[p.row0 + i0 + r_];
+  // sixteen partial sums a thread in flight (the first ones under the search for the own token), joined with one exponential each
+  const int rs = threadIdx.x & (RB - 1), qs = threadIdx.x / RB;
+  float m[16], a[16], b[16];
+  auto partials = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const int64_t o = (int64_t)min(t0 + 16 * x, p.tiles_n - 1) * p.R + i0 + rs;
+      m[x] = p.pm[o];
+      a[x] = p.p1[o];
+      b[x] = p.dual ? p.p2[o] : 0.f;
+    }
+  };
+  partials(qs);
   if (FEW) {
     // few rows: all logits are there, the own token is found here and its tile's others are added up again, without it, in place of the tile's partial sums
     int tok = -1;
@@ -1070,19 +1083,14 @@ __global__ __launch_bounds__(NT) void ll_rows_kernel(const RowArgs p) {
     __syncthreads();
   }
   {
-    const int r = threadIdx.x & (RB - 1), q = threadIdx.x / RB;
+    const int r = rs, q = qs;
     const int skip = FEW && xt[r] >= 0 ? xt[r] / BN : -1;
     float mx = -INFINITY, s1 = 0.f, s2 = 0.f;
-    // sixteen partials a thread in flight, joined with one exponential each
     for (int t0 = q; t0 < p.tiles_n; t0 += 256) {
-      float m[16], a[16], b[16];
+      if (t0 != q) partials(t0);
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         const int t = t0 + 16 * x;
-        const int64_t o = (int64_t)min(t, p.tiles_n - 1) * p.R + i0 + r;
-        m[x] = p.pm[o];
-        a[x] = p.p1[o];
-        b[x] = p.dual ? p.p2[o] : 0.f;
         if (t >= p.tiles_n || t == skip) { m[x] = -INFINITY; a[x] = b[x] = 0.f; }
       }
       float nm = mx;
