@@ -351,7 +351,7 @@ typedef enum { NS_F16 = 0, NS_BF16 = 1, NS_F32 = 2 } ns_dtype;
  *    top_vals (rows, ld_top) fp32 logits and top_idx int32 tokens; a token outside
  *    [0, vocab) is no entry, entries that name a token twice add up, the softmax is
  *    over the entries there are, and a row without one (or with -inf alone) keeps
- *    the hard term only.
+ *    the hard term only.  A NaN or +inf that an entry holds makes the row's loss NaN.
  *  - row_loss fp32 (rows), *loss_dev, *nvalid_dev (rows with a label).
  *  - dh (or NULL) and dw (or NULL): gradients of loss_scale x loss; loss_scale_dev
  *    may be NULL (1).  dw_f32: dw is fp32; dw_add (fp32 only): added to what is there.
@@ -363,7 +363,7 @@ typedef enum { NS_F16 = 0, NS_BF16 = 1, NS_F32 = 2 } ns_dtype;
  *    256 tokens of all rows where that is more); at most 128 MiB of partial
  *    sums of dh (or 4 d bytes a row), copies of h, and a few numbers per row and 64
  *    tokens; up to 64 rows, their fp32 logits and 4 d bytes per row and 256 tokens.
- *  - the same inputs give the same bits (no atomics).  dh, dw must not overlap h, w. */
+ *  - the same inputs give the same bits (sums in a fixed order).  dh, dw must not overlap h, w. */
 typedef struct {
   const void *h, *w;
   const int64_t* labels;

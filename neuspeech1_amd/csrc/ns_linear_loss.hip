@@ -16,20 +16,23 @@
 //            256-MiB last-level cache); dW needs all rows, at most LL_WHOLE_BYTES of them.
 //   formed again   a second pass over the logits writes dz of one PIECE of the vocabulary (LL_PIECE_BYTES) for all rows, piece after piece: 4 products instead of 3,
 //            but no more memory, and dW, of V d elements, is written once (chunks of rows would read and write it per chunk).
-//            8192 rows, d = 1280, V = 51865, bf16, dh and dW: 3.59 ms formed again in 256 MiB, 2.72 ms kept in 852 MB.
+//            8192 rows, d = 1280, V = 51865, bf16, dh and dW: 3.59 ms formed again in 256 MiB, 2.72 ms kept in 852 MB; 1434 rows, d = 512, fp16, a list: 432 us at T = 4, 397 at T = 1.5.
 //   * Rows without a label are packed away first: they cost nothing, and an infinity or NaN in a masked row reaches neither loss nor gradient.
 //   * A row's sparse terms (its label, the teacher's list) are no part of the dense epilogue: their logits are gathered as dot products in fp32
 //     and their cells of dz are written from those.  One of them a row, its own token, is no part of the statistics either: 1 - p of a row that is almost certain is
 //     then a sum of its own, not what is left of p (ll_rows_kernel).
 //   * dz in the operands' type: fp16 cells carry a factor 2^s (exact; taken out in fp32 at the end), so that a probability of 1 / V does
-//     not fall among the subnormals; a probability below 2^-29 of full scale is a subnormal, below 2^-40 zero.  bf16 has the range of fp32.
+//     not fall among the subnormals; a probability below 2^-29 of full scale is a subnormal, below 2^-40 zero (dh alone from labels: of what the other tokens hold, see
+//     ll_label_ref).  bf16 has the range of fp32.
 //     A sparse cell is rounded once, after the subtraction, a kept one twice (its exponential, dz).  A row's largest cells count by themselves: with up to 32 labels
-//     a cell is two numbers (ll_few_grad), beyond 64 rows dh's and dW's last steps add in fp32 what their rounding lost (ll_cells_kernel) or all of them (ll_label_ref).
-//   * Sums over the vocabulary (dh) and over the rows (dW) stay in fp32 MFMA accumulators / fp32 tiles added in a fixed order: no atomics,
-//     the same bits every time.
-//   * What bounds it: the 256 x 256 main loops (8 waves, two 64 KiB ring buffers, one workgroup per CU) run at 2.9 k cycles per K tile of 64 against 2.05 k of MFMA,
-//     LDS-port bound (192 KiB of fragments + 64 KiB of DMA per K tile), and at 1.6 GHz under that load: 1.1 - 1.46 PFLOP/s per launch, what a plain library
-//     product of the same shapes reaches (1.13 - 1.30).  Fewer cycles outside the main loops did not make them shorter, fewer products did.
+//     a cell is two numbers, up to 64 what the largest cell in each 256 tokens lost is added in fp32 (ll_few_grad), beyond 64 rows dh's and dW's last steps add what the two
+//     largest lost (ll_cells_kernel) or all of them (ll_label_ref).
+//   * Sums over the vocabulary (dh) and over the rows (dW) stay in fp32 MFMA accumulators / fp32 tiles added in a fixed order: no atomics
+//     (but a maximum in LDS), the same bits every time.
+//   * What bounds it: the 256 x 256 main loops (8 waves, two 64 KiB ring buffers, one workgroup per CU) take 2.9 k cycles per K tile of 64 against 2.05 k of MFMA: a K tile's
+//     fragments and DMA are 256 KiB, another 2 k cycles of the LDS port, and the two overlap in part.  At d = 1280 a launch reaches 1.1 (logits, with the exponentials) to
+//     1.3 PFLOP/s (dh, dW), the matrix pipes 0.54 - 0.68 busy at a clock that falls to 1.8 - 2.0 GHz (a plain library product of the shape: 1.1 - 1.3); at d = 512, with eight
+//     K tiles to an epilogue, 0.7 - 0.9, the pipes 0.36 - 0.52 busy at 2.25 GHz.
 // The 256 x 256 main loop is ns_gemm_p8.hip's four-phase LDS-DMA ring (see there: two wave groups one barrier interval apart), here for both
 // 16-bit types and with a second operand that may be K-major (W for dh, dz for dW): such a region holds 64 k-rows of 256 B and its fragments are
 // read transposed by ds_read_b64_tr_b16.
