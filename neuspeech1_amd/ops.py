@@ -363,15 +363,19 @@ def _vector(name, t, n, dtype):
     return t.data_ptr()
 
 
-def _apart(name, a, na, *others):
-    """[a, a + na) bytes against (what, first byte, bytes) of the others"""
-    for what, b, nb in others:
+def _area(at, rows, cols, ld, size):
+    """(first byte, bytes of a row, bytes from row to row, bytes from the first to the last) of a matrix"""
+    return at, cols * size, ld * size, ((rows - 1) * ld + cols) * size if rows > 0 and cols > 0 else 0
+
+
+def _apart(name, area, *others):
+    """the matrix `area` shares no byte with the others, given as (what, area).  Columns beside each other in one buffer are apart."""
+    a, wa, la, na = area
+    for what, (b, wb, lb, nb) in others:
         if na > 0 and nb > 0 and a < b + nb and b < a + na:
+            if la == lb and wa + wb <= la and wa <= (b - a) % la <= la - wb:
+                continue
             raise ValueError(f"{name} overlaps {what}")
-
-
-def _extent(n, m, ld, size):
-    return ((n - 1) * ld + m) * size if n > 0 and m > 0 else 0
 
 
 def _one_gpu(*tensors) -> int:
@@ -451,17 +455,17 @@ def _linear_ce_desc(h, weight, labels, row_loss, loss, nvalid, dh, dweight, loss
     d.vocab, d.d, d.dtype = vocab, width, _DTYPES[dtype]
     _targets(d, rows, labels, row_loss, loss, nvalid, loss_scale, top_vals, top_idx, temperature, alpha)
     if dh is not None or dweight is not None:
-        taken = (("h", d.h, _extent(rows, width, d.ldh, 2)), ("weight", d.w, _extent(vocab, width, d.ldw, 2)))
+        taken = (("h", _area(d.h or 0, rows, width, d.ldh, 2)), ("weight", _area(d.w, vocab, width, d.ldw, 2)))
         if dh is not None:
             _, _, d.lddh, at = _head_operand("dh", dh, rows, width, (dtype,))
-            size = _extent(rows, width, d.lddh, 2)
-            _apart("dh", at, size, *taken)
-            taken += (("dh", at, size),)
+            area = _area(at, rows, width, d.lddh, 2)
+            _apart("dh", area, *taken)
+            taken += (("dh", area),)
             d.dh = at if rows else 0              # (no rows: nothing to write)
         if dweight is not None:
             _, _, d.lddw, d.dw = _head_operand("dweight", dweight, vocab, width, (dtype, torch.float32))
             d.dw_f32 = int(dweight.dtype == torch.float32)
-            _apart("dweight", d.dw, _extent(vocab, width, d.lddw, 4 if d.dw_f32 else 2), *taken)
+            _apart("dweight", _area(d.dw, vocab, width, d.lddw, 4 if d.dw_f32 else 2), *taken)
     if accumulate:
         if dweight is None or not d.dw_f32:
             raise ValueError("accumulate: adds to a float32 dweight only")
@@ -524,7 +528,7 @@ def distill_topk(logits, labels, top_vals, top_idx, *, row_loss, loss, nvalid, t
         d.dlogits = dlogits.data_ptr()
         if d.dlogits != d.logits or d.lddz != d.ldz:
             size = logits.element_size()
-            _apart("dlogits", d.dlogits, _extent(rows, vocab, d.lddz, size), ("logits", d.logits, _extent(rows, vocab, d.ldz, size)))
+            _apart("dlogits", _area(d.dlogits or 0, rows, vocab, d.lddz, size), ("logits", _area(d.logits or 0, rows, vocab, d.ldz, size)))
     dev = _one_gpu(logits, labels, top_vals, top_idx, row_loss, loss, nvalid, dlogits, loss_scale)
     if STEP_PROFILE is not None:
         _work("distill_topk", 0.0, logits.element_size() * rows * vocab * (2.0 if dlogits is not None else 1.0) + 8.0 * rows * d.k)
@@ -546,11 +550,11 @@ def topk_logits(logits, k, *, vals, idx, lse=None):
         raise ValueError(f"vals and idx: different row strides ({d.ldo}, {ldi})")
     if lse is not None:
         d.lse = _vector("lse", lse, rows, torch.float32)
-    dev = _one_gpu(logits, vals, idx, lse)
     d.logits, d.vals, d.idx = logits.data_ptr(), vals.data_ptr(), idx.data_ptr()
-    z = ("logits", d.logits, _extent(rows, vocab, d.ldz, logits.element_size()))
-    _apart("vals", d.vals, _extent(rows, k, d.ldo, 4), z)
-    _apart("idx", d.idx, _extent(rows, k, d.ldo, 4), z)
+    z = ("logits", _area(d.logits or 0, rows, vocab, d.ldz, logits.element_size()))
+    _apart("vals", _area(d.vals or 0, rows, k, d.ldo, 4), z)
+    _apart("idx", _area(d.idx or 0, rows, k, d.ldo, 4), z)
+    dev = _one_gpu(logits, vals, idx, lse)
     d.rows, d.vocab, d.k, d.dtype = rows, vocab, k, _DTYPES[logits.dtype]
     if STEP_PROFILE is not None:
         _work("topk_logits", 0.0, logits.element_size() * rows * vocab + 8.0 * rows * k)

@@ -29,3 +29,24 @@ def test_no_rows_with_gradients_asked_for(dev, dtype, code, with_dw):
     assert so.ns_linear_cross_entropy(C.byref(d), torch.cuda.current_stream().cuda_stream) == 0, so.ns_last_error()
     torch.cuda.synchronize()
     assert float(loss) == 0 and int(nvalid) == 0 and (dh == 3.0).all() and (dw == (0.0 if with_dw else 3.0)).all()
+
+
+def test_gradients_beside_their_operands_in_one_buffer(dev):
+    """h | dh and logits | dlogits as columns of one buffer: the same values as apart, and nothing else of the buffer is written"""
+    from neuspeech1_amd import ops
+    from tests.test_vocab_loss_gpu import make_linear, make_logits, outputs
+    for rows in (30, 200):
+        h, w, labels, _ = make_linear(dev, rows, 64, 300, torch.float16, seed=61)
+        buf = torch.full((rows, 160), 5.0, device=dev, dtype=torch.float16)
+        buf[:, :64] = h
+        want = torch.empty_like(h)
+        ops.linear_cross_entropy(h, w, labels, dh=want, **outputs(dev, rows))
+        ops.linear_cross_entropy(buf[:, :64], w, labels, dh=buf[:, 80:144], **outputs(dev, rows))
+        assert torch.equal(buf[:, 80:144], want) and torch.equal(buf[:, :64], h) and (buf[:, 64:80] == 5.0).all() and (buf[:, 144:] == 5.0).all()
+        _, z, labels, (tv, ti) = make_logits(dev, rows, 301, torch.float32, 62)
+        buf = torch.full((rows, 700), 5.0, device=dev)
+        buf[:, :301] = z
+        want = torch.empty_like(z)
+        ops.distill_topk(z, labels, tv, ti, alpha=0.5, dlogits=want, **outputs(dev, rows))
+        ops.distill_topk(buf[:, :301], labels, tv, ti, alpha=0.5, dlogits=buf[:, 303:604], **outputs(dev, rows))
+        assert torch.equal(buf[:, 303:604], want) and torch.equal(buf[:, :301], z) and (buf[:, 301:303] == 5.0).all() and (buf[:, 604:] == 5.0).all()
