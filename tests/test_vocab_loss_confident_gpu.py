@@ -140,6 +140,16 @@ def test_two_candidates_and_a_tail_far_below(ops, dev, dtype, rows, d, v, rival)
     check_confident(ops, dev, h, w, labels, "h", scale=2.0 ** 18, certain=False)
 
 
+@pytest.mark.parametrize("rows,d,v,sharp", [(65, 136, 511, 1.0), (257, 264, 1001, 1.0), (300, 512, 2600, 2.0), (700, 776, 513, 0.0), (130, 64, 60001, 3.0), (2049, 64, 60001, 1.5)])
+def test_fp16_cells_kept_relative_to_labels_of_every_kind(ops, dev, rows, d, v, sharp):
+    """labels from the likeliest token to one among thousands, by the bounds that are relative to what a strip and a row hold"""
+    g = gen(rows + v, dev)
+    w = (torch.randn(v, d, generator=g, device=dev) * 2.0 * d ** -0.5).to(F16)
+    labels = torch.randint(0, v, (rows,), generator=g, device=dev)
+    h = (torch.randn(rows, d, generator=g, device=dev) + sharp * torch.rand(rows, 1, generator=g, device=dev) * w[labels].float()).to(F16)
+    check_confident(ops, dev, h, w, labels, "h", scale=2.0 ** 14, certain=False)
+
+
 # ------------------------------------------------------------------------------------------------ over logits
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("rows,v,first", [(40, 9, 0), (40, 1001, 3), (64, 5000, 0), (33, 51865, 1), (20, 70001, 0)])
