@@ -21,26 +21,47 @@ class NeuSpeechHipError(RuntimeError):
 # package around its GPU API calls (the data feed's loader thread: device synchronize, pinned / device allocations, copies).
 # HIP invalidates an open capture when another thread synchronizes the device or allocates meanwhile, thread-local capture
 # mode notwithstanding (seen on ROCm 7.0/7.2: hipErrorStreamCaptureInvalidated at the first captured launch).
+import collections  # noqa: E402
 import contextlib  # noqa: E402
 import gc  # noqa: E402
 import threading  # noqa: E402
+import time  # noqa: E402
 GPU_CAPTURE_LOCK = threading.RLock()
+
+# "start" stands last while a collection runs, "stop" otherwise.  The callback is a C method, so that it has run when the interpreter lock first changes hands within a
+# collection: a Python function can be interrupted before its first line.  (The collector passes (phase, info); info, a dict with entries, is move_to_end's true `last`.)
+_COLLECTION = collections.OrderedDict(start=None, stop=None)
+gc.callbacks.insert(0, _COLLECTION.move_to_end)
+COLLECTION_WAIT_S = 60.0
 
 
 @contextlib.contextmanager
 def capture_section():
-    """Everything between begin and end of a hipGraph capture runs inside this: GPU_CAPTURE_LOCK held, Python's cyclic collector off.
+    """Everything between begin and end of a hipGraph capture runs inside this: GPU_CAPTURE_LOCK held, Python's cyclic collector off, and no collection that another
+    thread began earlier still running (turning the collector off does not end one, and its finalizers may let this thread get ahead of it).
     torch's ~CUDAGraph synchronizes the device on ROCm, which fails while this thread captures; the check throws inside a destructor and
     ends the process.  A graph that only a reference cycle kept alive is destroyed whenever the collector happens to run -- the Python
     allocations of a capture are enough to start it -- so collection waits until the capture is closed."""
-    with GPU_CAPTURE_LOCK:
+    until = time.monotonic() + COLLECTION_WAIT_S
+    while True:
+        GPU_CAPTURE_LOCK.acquire()
         was = gc.isenabled()
         gc.disable()
-        try:
-            yield
-        finally:
-            if was:
-                gc.enable()
+        if next(reversed(_COLLECTION)) == "stop":
+            break
+        if was:
+            gc.enable()
+        GPU_CAPTURE_LOCK.release()          # (a finalizer may need it)
+        if time.monotonic() > until:
+            raise NeuSpeechHipError("no capture can begin: a garbage collection does not end (a finalizer that captures waits for its own)")
+        time.sleep(0.0005)
+    try:
+        yield
+    finally:
+        if was:
+            gc.enable()
+        GPU_CAPTURE_LOCK.release()
+
 
 ABI_VERSION = 3      # ns_version() of the library this binding was written against (3: ns_zero_spans / ns_add_i32)
 
